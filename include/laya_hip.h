@@ -34,6 +34,8 @@ enum {
 
 /* Element types of host weights and of the 16-bit MFMA operand type. */
 enum { LAYA_F32 = 0, LAYA_F16 = 1, LAYA_BF16 = 2 };
+/* Output type of the 8-bit operators below (codes with scales; no host weights of this type). */
+enum { LAYA_E4M3 = 3 };
 
 /* Encoder variants (the reference's executor is pre-LN/RoPE/GeGLU, laya_cuda/laya.py:59-79). */
 enum { LAYA_NORM_POST = 0, LAYA_NORM_PRE = 1 };
@@ -262,6 +264,62 @@ int laya_op_head_gather(const float* src, const int32_t* src_rows, const int32_t
                         const int32_t* question_kind, const int32_t* n_live, const float* type_rows,
                         const float* gamma, const float* beta, float eps, float* selected, float* normed,
                         int rows, int width, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit rows and the operators on them (no counterpart in the reference, whose operands are 16-bit).
+ *
+ * A matrix of `rows` x `width` values in 8-bit rows is two device arrays, rows back to back:
+ *   codes  [rows][laya_width8(width)]       e4m3 (OCP, no infinities), 16-byte aligned
+ *   scales [rows][laya_width8(width) / 32]  uint8, 4-byte aligned
+ * laya_width8 rounds the width up to a multiple of 128; the codes past the width are zeros.  Code i of a row
+ * stands for e4m3(code) * 2^(scale[i / 32] - 127).  A writer takes the smallest scale with which the block's largest
+ * magnitude is at most 448 (2^-127 at the least; 0 for a block of zeros) and rounds each value once, to nearest
+ * with ties to even.  A block that holds a NaN or an infinity gets the scale 255 and reads back as NaNs.
+ *
+ * Every operator runs on the current device, which owns the pointers and the stream; it makes no allocation, no
+ * host synchronisation and keeps nothing between calls, so calls may be captured, replayed and run side by side.
+ * Zero rows are a call that does nothing.  Bad sizes, types, missing or misaligned pointers: LAYA_EINVAL.
+ * ------------------------------------------------------------------------------------------ */
+
+enum { LAYA_LAYER_NORM = 0, LAYA_RMS_NORM = 1 };
+enum { LAYA_ACT_NONE = 0, LAYA_ACT_GELU = 1, LAYA_ACT_RELU = 2, LAYA_ACT_GEGLU = 3, LAYA_ACT_SWIGLU = 4 };
+
+/* Codes per 8-bit row of `width` values; -1 for a width below 1 or above 2^30.  Host-only. */
+int laya_width8(int width);
+
+/* 8-bit rows of x (LAYA_F32/F16/BF16), whose rows of `width` values start `stride` elements apart (stride >=
+ * width): weights once at load, or activations.  x needs its own element's alignment only; rows that start
+ * on whole quads (4 elements) are read fastest. */
+int laya_op_quantize8(const void* x, int dtype, int64_t stride, void* codes, void* scales, int64_t rows, int width,
+                      void* stream);
+
+/* The values 8-bit rows stand for, as dtype with rows `stride` elements apart; what lies between the rows is left as it
+ * was.  Exact in LAYA_F32, and in LAYA_BF16 but for blocks of scales below 2^-117; LAYA_F16 rounds once
+ * (infinity past its range). */
+int laya_op_dequantize8(const void* codes, const void* scales, void* out, int dtype, int64_t stride, int64_t rows,
+                        int width, void* stream);
+
+/* laya_op_norm with 8-bit output: v = residual + (sum of `splits` branch partials + bias); sum_out = v; then
+ *   kind LAYA_LAYER_NORM  y = (v - mean(v)) / sqrt(var(v) + eps) * gamma + beta
+ *   kind LAYA_RMS_NORM    y = v / sqrt(mean(v^2) + eps) * gamma + beta
+ * in fp32, out32 = y, and codes, scales = the 8-bit rows of y.  branch (partials part_stride elements apart) is of
+ * branch_dtype LAYA_F32/F16/BF16, or NULL (v = residual; bias must be NULL).  beta, bias, sum_out and
+ * out32 may be NULL; either one of sum_out and out32 may be residual itself.  1 <= width <= 8192. */
+int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, int splits, int64_t part_stride,
+                  const float* bias, const float* gamma, const float* beta, float eps, int kind, float* sum_out,
+                  float* out32, void* codes, void* scales, int rows, int width, void* stream);
+
+/* out = act(x w^T + bias) + residual: x [M][K] and w [N][K] in 8-bit rows, bias fp32 [N] or NULL, residual
+ * [M][cols] of residual_dtype LAYA_F32/F16/BF16 or NULL, out [M][cols] of out_dtype LAYA_F32/F16/BF16, or 8-bit rows
+ * (LAYA_E4M3: out takes the codes, out_scales the scales; out_scales is NULL otherwise).  cols is N, or N / 2
+ * for the gated activations, whose w (and bias) come in groups of 32 rows: 16 gate rows, then their 16 value rows
+ * (act(gate) * value; N a multiple of 32).  GELU is the exact-erf one, SWIGLU's gate x / (1 + exp(-x)).  The residual
+ * is added in fp32 before the one rounding; it may be out itself when both have the same type, and
+ * nothing else may overlap out.
+ * Sums are fp32.  tile -1 lets the planner choose; others name a tile (0 .. ), refused where it cannot make the output. */
+int laya_op_linear8(const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias,
+                    const void* residual, int residual_dtype, void* out, void* out_scales, int out_dtype,
+                    int activation, int M, int N, int K, int tile, void* stream);
 
 #ifdef __cplusplus
 }

@@ -213,4 +213,70 @@ hipError_t launch_head_tail(const HeadTailArgs& a, int width, hipStream_t stream
 // Once per device before the first tail launch: the tail kernels' dynamic LDS limit.
 hipError_t head_prepare();
 
+// ---- 8-bit rows (rows8.hpp): e4m3 codes, padded to a multiple of 128 a row, and a scale byte per 32 ----
+struct Quantize8Args {
+  const void* x;      // [rows] of `width` values, `stride` elements apart
+  long long stride;
+  uint8_t* codes;     // [rows][padded8(width)]
+  uint8_t* scales;    // [rows][padded8(width) / 32]
+  long long rows;
+  int width;
+};
+hipError_t launch_quantize8(const Quantize8Args& a, DType t, hipStream_t stream);
+
+struct Dequantize8Args {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  void* out;          // [rows] of `width` values, `stride` elements apart
+  long long stride;
+  long long rows;
+  int width;
+};
+hipError_t launch_dequantize8(const Dequantize8Args& a, DType t, hipStream_t stream);
+
+constexpr int kMaxNorm8Width = 8192;  // four waves of eight quads a lane
+struct Norm8Args {
+  const float* residual;  // [rows][width]
+  const void* branch;     // [splits] partials of [rows][width], part_stride elements apart, or null
+  int splits;
+  long long part_stride;
+  const float* bias;      // [width] added to the branch, or null
+  const float* gamma;
+  const float* beta;      // or null
+  float eps;
+  bool rms;               // root-mean-square norm; else LayerNorm
+  float* sum_out;         // residual + branch, or null; may alias residual
+  float* out32;           // the normalised rows, or null; may alias residual
+  uint8_t* codes;
+  uint8_t* scales;
+  int rows, width;
+};
+hipError_t launch_norm8(const Norm8Args& a, DType branch, hipStream_t stream);
+
+enum class Act8 : int { None = 0, Gelu = 1, Relu = 2, Geglu = 3, Swiglu = 4 };
+// out = act(x w^T + bias) + residual, both operands 8-bit rows; gated activations take w's rows in groups of 16 gate
+// rows and their 16 value rows and leave N / 2 columns.
+struct Linear8Args {
+  const uint8_t *x, *xs;  // [M][ld] codes, [M][ld / 32] scales
+  const uint8_t *w, *ws;  // [N][ld], [N][ld / 32]
+  const float* bias;      // [N] or null
+  const void* residual;   // [M][cols] or null
+  int residual_type;      // DType
+  void* out;              // [M][cols], or 8-bit rows [M][padded8(cols)]
+  uint8_t* out_scales;
+  int out_type;           // DType or kE4M3
+  Act8 act;
+  int M, N, ld;           // ld = padded8(K)
+  int cols;               // output columns: N, or N / 2 when gated
+  bool vec;               // rows of out and residual start on whole quads
+};
+constexpr int kE4M3 = 3;
+int linear8_tile_count();
+// Whether tile `id` can make this output: 8-bit blocks and gate/value groups lie inside a tile's columns, and fp32
+// outputs take a tile with exact products.
+bool linear8_tile_valid(int id, const Linear8Args& a);
+int linear8_plan(const Linear8Args& a, int cus);
+hipError_t linear8_prepare();
+hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream);
+
 }  // namespace laya

@@ -1,0 +1,58 @@
+// 8-bit rows: e4m3 codes with one power-of-two scale per 32 of them.
+//
+// A row of `width` values is stored as padded8(width) codes, a multiple of 128 (the codes past the width are
+// zeros), and one scale byte s per 32 codes; code c of the block stands for e4m3(c) * 2^(s - 127).  The scale is
+// the smallest one that leaves the whole block within the largest code, 448; a block of zeros has s = 0, and
+// a block that holds a NaN or an infinity has s = 255 and reads back as NaNs.  128 codes are what one
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes of a row, and their four scale bytes are one aligned dword.
+//
+// Power-of-two scales cost up to one bit of the codes' range against a scale of amax / 448, but no rounding:
+// reading back is exact, and a producer whose amax moves by one unit in the last place changes no value by more
+// than a code's rounding.
+#pragma once
+
+#include "common.hpp"
+
+namespace laya {
+
+constexpr int kBlock8 = 32;      // codes that share a scale
+constexpr int kPad8 = 128;       // codes per row are a multiple of this
+constexpr unsigned kInf = 0x7f800000u;
+__host__ __device__ constexpr long long padded8(long long width) { return (width + kPad8 - 1) / kPad8 * kPad8; }
+
+// Magnitude bits: as unsigned integers they order like the magnitudes, with NaNs above infinity (fmaxf drops NaNs).
+__device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+
+// Scale byte of a block whose largest magnitude has the bits `top`.  448 is 1.75 * 2^8: adding 0x1fffff carries
+// into the exponent exactly where the significand is above 1.75.
+__device__ __forceinline__ unsigned scale8(unsigned top) {
+  if (top >= kInf) return 255u;
+  const int s = static_cast<int>((top + 0x1fffffu) >> 23) - 8;
+  return s < 0 ? 0u : static_cast<unsigned>(s);
+}
+// What the block's values are multiplied by before they are rounded to codes: 2^(127 - s), exact (s <= 247).
+__device__ __forceinline__ float inverse_scale8(unsigned s) { return __builtin_bit_cast(float, (254u - s) << 23); }
+// 2^(s - 127); NaN for s = 255.
+__device__ __forceinline__ float scale_value8(unsigned s) {
+  return __builtin_bit_cast(float, s == 0 ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23);
+}
+
+// Four values of a block of scale byte s as four codes, each rounded once (to nearest, ties to even).
+__device__ __forceinline__ unsigned encode8(float a, float b, float c, float d, unsigned s) {
+  if (s == 255u) return 0x7f7f7f7fu;
+  const float m = inverse_scale8(s);
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a * m, b * m, 0, false);
+  return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(c * m, d * m, r, true));
+}
+
+// Largest magnitude bits over the 8 lanes of a 32-value block (4 values a lane, lanes 8 j .. 8 j + 7).
+__device__ __forceinline__ unsigned block_top8(unsigned top) {
+#pragma unroll
+  for (int d = 1; d <= 4; d <<= 1) {
+    const unsigned o = __shfl_xor(top, d, kWave);
+    top = top > o ? top : o;
+  }
+  return top;
+}
+
+}  // namespace laya

@@ -22,6 +22,7 @@
 #include "kernels.hpp"
 #include "laya_hip.h"
 #include "packing.hpp"
+#include "rows8.hpp"
 #include "scope.hpp"
 
 // Device scratch of laya_predict_static: the whole shape-slot arena of one forward (packed block,
@@ -869,6 +870,7 @@ void prepare_device() {
   LAYA_REQUIRE(dev >= 0 && dev < kMaxDevices, "device index beyond the library's device table");
   LAYA_HIP(gemm_prepare());
   LAYA_HIP(head_prepare());
+  LAYA_HIP(linear8_prepare());
   void* ptr = nullptr;
   LAYA_HIP(hipGetSymbolAddress(&ptr, HIP_SYMBOL(scratch)));
   LAYA_REQUIRE(ptr != nullptr, "no device address for the scratch array");
@@ -1489,6 +1491,111 @@ int laya_op_head_gather(const float* src, const int32_t* src_rows, const int32_t
     HeadGatherArgs a{src, src_rows, row_question, question_kind, n_live, type_rows, gamma, beta, eps, selected,
                      normed, rows};
     check_launch(launch_head_gather(a, width, DType::F16, static_cast<hipStream_t>(stream)), "head gather");
+  });
+}
+
+// ---------------- 8-bit rows ----------------
+
+static bool float_type(int dtype) { return dtype == LAYA_F32 || dtype == LAYA_F16 || dtype == LAYA_BF16; }
+static size_t type_size(int dtype) { return dtype == LAYA_F32 ? 4 : 2; }
+static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+constexpr int kMaxWidth8 = 1 << 30;
+constexpr int kMaxLinear8 = 1 << 20;  // a tile's rows then span fewer than 2^32 bytes
+
+// The checks that every 8-bit operand shares.
+static void require_rows8(const void* codes, const void* scales, const char* what) {
+  LAYA_REQUIRE(codes && scales, std::string(what) + ": codes and scales are required");
+  LAYA_REQUIRE(aligned_to(codes, 16) && aligned_to(scales, 4),
+               std::string(what) + ": codes must be 16-byte and scales 4-byte aligned");
+}
+
+int laya_width8(int width) {
+  return width < 1 || width > kMaxWidth8 ? -1 : static_cast<int>(padded8(width));
+}
+
+int laya_op_quantize8(const void* x, int dtype, int64_t stride, void* codes, void* scales, int64_t rows, int width,
+                      void* stream) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(float_type(dtype), "dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
+    LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxWidth8 && stride >= width, "bad rows, width or stride");
+    if (rows == 0) return;
+    require_rows8(codes, scales, "output");
+    LAYA_REQUIRE(x && aligned_to(x, type_size(dtype)), "x must be aligned to its elements");
+    Quantize8Args a{x, stride, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, width};
+    check_launch(launch_quantize8(a, static_cast<DType>(dtype), static_cast<hipStream_t>(stream)), "quantize8");
+  });
+}
+
+int laya_op_dequantize8(const void* codes, const void* scales, void* out, int dtype, int64_t stride, int64_t rows,
+                        int width, void* stream) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(float_type(dtype), "dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
+    LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxWidth8 && stride >= width, "bad rows, width or stride");
+    if (rows == 0) return;
+    require_rows8(codes, scales, "input");
+    LAYA_REQUIRE(out && aligned_to(out, type_size(dtype)), "out must be aligned to its elements");
+    Dequantize8Args a{static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), out, stride, rows, width};
+    check_launch(launch_dequantize8(a, static_cast<DType>(dtype), static_cast<hipStream_t>(stream)), "dequantize8");
+  });
+}
+
+int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, int splits, int64_t part_stride,
+                  const float* bias, const float* gamma, const float* beta, float eps, int kind, float* sum_out,
+                  float* out32, void* codes, void* scales, int rows, int width, void* stream) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(kind == LAYA_LAYER_NORM || kind == LAYA_RMS_NORM, "kind must be LAYA_LAYER_NORM or LAYA_RMS_NORM");
+    LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxNorm8Width, "rows must not be negative and width 1 to 8192");
+    LAYA_REQUIRE(eps >= 0.f, "eps must not be negative");
+    LAYA_REQUIRE(!branch || float_type(branch_dtype), "branch_dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
+    LAYA_REQUIRE(!branch || (splits >= 1 && (splits == 1 || part_stride >= static_cast<int64_t>(rows) * width)),
+                 "a branch has at least one partial, and partials do not overlap");
+    LAYA_REQUIRE(branch || !bias, "a bias needs its branch");
+    if (rows == 0) return;
+    require_rows8(codes, scales, "output");
+    LAYA_REQUIRE(residual && gamma, "residual and gamma are required");
+    LAYA_REQUIRE(aligned_to(residual, 4) && aligned_to(gamma, 4) && aligned_to(beta, 4) && aligned_to(bias, 4) &&
+                     aligned_to(sum_out, 4) && aligned_to(out32, 4) && aligned_to(branch, branch ? type_size(branch_dtype) : 1),
+                 "pointers must be aligned to their elements");
+    LAYA_REQUIRE(!sum_out || sum_out != out32, "sum_out and out32 must be different arrays");
+    Norm8Args a{residual, branch, splits, part_stride, bias, gamma, beta, eps, kind == LAYA_RMS_NORM, sum_out, out32,
+                static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, width};
+    check_launch(launch_norm8(a, branch ? static_cast<DType>(branch_dtype) : DType::F32, static_cast<hipStream_t>(stream)),
+                 "norm8");
+  });
+}
+
+int laya_op_linear8(const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias,
+                    const void* residual, int residual_dtype, void* out, void* out_scales, int out_dtype, int activation,
+                    int M, int N, int K, int tile, void* stream) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(activation >= LAYA_ACT_NONE && activation <= LAYA_ACT_SWIGLU, "activation must be a LAYA_ACT_* value");
+    LAYA_REQUIRE(float_type(out_dtype) || out_dtype == LAYA_E4M3, "out_dtype must be LAYA_F32, F16, BF16 or E4M3");
+    LAYA_REQUIRE(!residual || float_type(residual_dtype), "residual_dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
+    LAYA_REQUIRE(M >= 0 && N >= 1 && K >= 1 && N <= kMaxLinear8 && K <= kMaxLinear8,
+                 "M must not be negative, N and K between 1 and 2^20");
+    const bool glu = activation == LAYA_ACT_GEGLU || activation == LAYA_ACT_SWIGLU;
+    LAYA_REQUIRE(!glu || N % 32 == 0, "gated activations take N in groups of 32 rows");
+    if (M == 0) return;
+    require_rows8(x, x_scales, "x");
+    require_rows8(w, w_scales, "w");
+    LAYA_REQUIRE(out && (out_dtype == LAYA_E4M3) == (out_scales != nullptr), "out_scales belong to LAYA_E4M3 outputs");
+    if (out_dtype == LAYA_E4M3) require_rows8(out, out_scales, "output");
+    LAYA_REQUIRE(aligned_to(bias, 4) && (out_dtype == LAYA_E4M3 || aligned_to(out, type_size(out_dtype))) &&
+                     (!residual || aligned_to(residual, type_size(residual_dtype))),
+                 "pointers must be aligned to their elements");
+    Linear8Args a{};
+    a.x = static_cast<const uint8_t*>(x); a.xs = static_cast<const uint8_t*>(x_scales);
+    a.w = static_cast<const uint8_t*>(w); a.ws = static_cast<const uint8_t*>(w_scales);
+    a.bias = bias; a.residual = residual; a.residual_type = residual_dtype;
+    a.out = out; a.out_scales = static_cast<uint8_t*>(out_scales); a.out_type = out_dtype;
+    a.act = static_cast<Act8>(activation);
+    a.M = M; a.N = N; a.ld = static_cast<int>(padded8(K)); a.cols = glu ? N / 2 : N;
+    a.vec = a.cols % 4 == 0 && (out_dtype == LAYA_E4M3 || aligned_to(out, 4 * type_size(out_dtype))) &&
+            (!residual || aligned_to(residual, 4 * type_size(residual_dtype)));
+    prepare_device();
+    if (tile == -1) tile = linear8_plan(a, 256);
+    LAYA_REQUIRE(linear8_tile_valid(tile, a), "no such tile, or one that cannot make this output");
+    check_launch(launch_linear8(a, tile, static_cast<hipStream_t>(stream)), "linear8");
   });
 }
 

@@ -10,10 +10,12 @@ LIBRARY = Path(__file__).with_name("liblaya_hip.so")
 
 OK, EINVAL, EDEVICE, ENOMEM, ESTATE = range(5)
 ABI_VERSION = 2  # LAYA_ABI_VERSION of the struct layouts mirrored below
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 NORM_POST, NORM_PRE = 0, 1
 POS_LEARNED, POS_ROPE = 0, 1
 FFN_GELU, FFN_GEGLU = 0, 1
+LAYER_NORM, RMS_NORM = 0, 1  # laya_op_norm8 kinds
+ACT_NONE, ACT_GELU, ACT_RELU, ACT_GEGLU, ACT_SWIGLU = range(5)  # laya_op_linear8 activations
 
 
 class LayaConfig(ct.Structure):
@@ -70,6 +72,11 @@ SIGNATURES = {
     "laya_op_qkv": ([_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p], _i),
     "laya_op_attention": ([_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p], _i),
     "laya_op_gather_rows": ([_p, _p, _p, _p, _i, _p, _p, _i, _i, _p], _i),
+    "laya_width8": ([_i], _i),
+    "laya_op_quantize8": ([_p, _i, _i64, _p, _p, _i64, _i, _p], _i),
+    "laya_op_dequantize8": ([_p, _p, _p, _i, _i64, _i64, _i, _p], _i),
+    "laya_op_norm8": ([_p, _p, _i, _i, _i64, _p, _p, _p, _f, _i, _p, _p, _p, _p, _i, _i, _p], _i),
+    "laya_op_linear8": ([_p, _p, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p], _i),
     "laya_op_head_gather": ([_p, _p, _p, _p, _p, _p, _p, _p, _f, _p, _p, _i, _i, _p], _i),
 }
 

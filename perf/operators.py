@@ -226,7 +226,7 @@ def _own(s):
         check(lib.laya_op_linear8(
             _at(s["x"]), _at(s["xs"]), _at(s["w"]), _at(s["ws"]), _at(s["bias"]), _at(s["residual"]),
             CODES[case["residual"] or "f32"], _at(s["codes"] if eight else s["out"]), _at(s["scales"]) if eight else None,
-            CODES[case["out"]], ACTIVATIONS[case["act"]], case["M"], case["N"], case["K"], stream))
+            CODES[case["out"]], ACTIVATIONS[case["act"]], case["M"], case["N"], case["K"], -1, stream))
         if not eight:
             return {"out": s["out"]}
         rows, width = case["M"], _features(case)
