@@ -43,6 +43,13 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+// D = A(16x128) * B(128x16) + C of e4m3 codes with a scale per 32: lane l supplies row/column l % 16, its codes 16 (l / 16)
+// .. +15 and 64 + 16 (l / 16) .. +15, and in the low byte of its scale that of codes 32 (l / 16) .. +31 of the row.
+__device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, unsigned sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+
 // Activations.  NaNs stay NaNs and +infinity stays itself.  kFine: for fp32 outputs (libm); else accurate to
 // 3e-7 absolute, far inside a 16-bit rounding (see gelu16, whose argument is capped where its q has reached 0).
 template <bool kFine>
@@ -57,36 +64,61 @@ __device__ __forceinline__ float silu8(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
-__host__ __device__ __forceinline__ bool gated(Act8 act) { return act == Act8::Geglu || act == Act8::Swiglu; }
+__host__ __device__ constexpr bool gated(Act8 act) { return act == Act8::Geglu || act == Act8::Swiglu; }
+
+template <typename T> struct Vec { typedef T type __attribute__((ext_vector_type(4))); };
+
+// Whole quad `at` of a tensor of `type`, added to v.
+__device__ __forceinline__ void add_quad(const void* p, int type, size_t at, float (&v)[4]) {
+  auto add = [&](auto zero) {
+    typedef decltype(zero) T;
+    const typename Vec<T>::type t = *reinterpret_cast<const typename Vec<T>::type*>(static_cast<const T*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = v[i] + static_cast<float>(t[i]);
+  };
+  if (type == static_cast<int>(DType::F32)) add(0.f);
+  else if (type == static_cast<int>(DType::F16)) add(f16());
+  else add(bf16());
+}
+// Residual columns n .. n + 3 of row `row` (< M), added in fp32.
+__device__ __forceinline__ void add_residual4(const Linear8Args& a, long long row, int n, float (&v)[4]) {
+  const size_t at = static_cast<size_t>(row) * a.cols + n;
+  if (a.vec && n < a.cols) return add_quad(a.residual, a.residual_type, at, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= a.cols) continue;
+    v[i] = v[i] + (a.residual_type == static_cast<int>(DType::F32)   ? static_cast<const float*>(a.residual)[at + i]
+                   : a.residual_type == static_cast<int>(DType::F16) ? static_cast<float>(static_cast<const f16*>(a.residual)[at + i])
+                                                                     : static_cast<float>(static_cast<const bf16*>(a.residual)[at + i]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(const Linear8Args& a, long long row, int n, const float (&v)[4]) {
+  T* const dst = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.cols + n;
+  if (a.vec && n < a.cols) {
+    *reinterpret_cast<typename Vec<T>::type*>(dst) =
+        typename Vec<T>::type{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.cols) dst[i] = static_cast<T>(v[i]);
+  }
+}
+// Two values as two 16-bit ones of `type`.
+__device__ __forceinline__ unsigned pack16(int type, float x, float y) {
+  if (type == static_cast<int>(DType::F16)) {
+    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, f16x2{static_cast<f16>(x), static_cast<f16>(y)});
+  }
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, bf16x2{static_cast<bf16>(x), static_cast<bf16>(y)});
+}
 
 // Output columns n .. n + 3 of row `row` after bias and activation: adds the residual, rounds once and stores.
 // 8-bit outputs are made by 8 lanes with consecutive quads of the same row (a whole block), all of them
 // calling; columns past `cols` come in as zeros and only an 8-bit row's padding is stored from them.
 __device__ __forceinline__ void finish4(const Linear8Args& a, long long row, int n, float (&v)[4]) {
-  const size_t at = static_cast<size_t>(row) * a.cols + n;
-  const bool whole = a.vec && n < a.cols;
-  if (a.residual) {
-    float r[4] = {0.f, 0.f, 0.f, 0.f};
-    auto take = [&](auto zero) {
-      typedef decltype(zero) T;
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      const T* src = static_cast<const T*>(a.residual) + at;
-      if (whole) {
-        const T4 t = *reinterpret_cast<const T4*>(src);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = static_cast<float>(t[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < a.cols) r[i] = static_cast<float>(src[i]);
-      }
-    };
-    if (a.residual_type == static_cast<int>(DType::F32)) take(0.f);
-    else if (a.residual_type == static_cast<int>(DType::F16)) take(f16());
-    else take(bf16());
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] + r[i];
-  }
+  if (a.residual) add_residual4(a, row, n, v);
   if (a.out_type == kE4M3) {
     unsigned top = 0;
 #pragma unroll
@@ -98,23 +130,13 @@ __device__ __forceinline__ void finish4(const Linear8Args& a, long long row, int
     const size_t ld = static_cast<size_t>(padded8(a.cols));
     *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.out) + row * ld + n) = encode8(v[0], v[1], v[2], v[3], s);
     if (n % kBlock8 == 0) a.out_scales[row * (ld / kBlock8) + n / kBlock8] = static_cast<uint8_t>(s);
-    return;
+  } else if (a.out_type == static_cast<int>(DType::F32)) {
+    store4<float>(a, row, n, v);
+  } else if (a.out_type == static_cast<int>(DType::F16)) {
+    store4<f16>(a, row, n, v);
+  } else {
+    store4<bf16>(a, row, n, v);
   }
-  auto put = [&](auto zero) {
-    typedef decltype(zero) T;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T* dst = static_cast<T*>(a.out) + at;
-    if (whole) {
-      *reinterpret_cast<T4*>(dst) = T4{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.cols) dst[i] = static_cast<T>(v[i]);
-    }
-  };
-  if (a.out_type == static_cast<int>(DType::F32)) put(0.f);
-  else if (a.out_type == static_cast<int>(DType::F16)) put(f16());
-  else put(bf16());
 }
 
 // Dwords of a slab's scales in LDS: x's rows, then w's, each in whole 64-row loads.
@@ -127,7 +149,7 @@ template <int BM, int BN, int KG, int SL, int S> constexpr int lds8() {
   return stages > parts ? stages : parts;
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int SL, int S>
+template <int BM, int BN, int WM, int WN, int KG, int SL, int S, bool kFast>
 __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args a) {
   constexpr int NW = WM * WN * KG, NT = 64 * NW;
   constexpr int WTM = BM / WM, WTN = BN / WN, MB = WTM / 16, NB = WTN / 16;
@@ -137,7 +159,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
   constexpr int STAGE = stage_bytes8<BM, BN, SL>(), CODES = SL * (BM + BN) * 128;
   constexpr int GROUPS = SL * (RG + SG);
   constexpr int NLD = (GROUPS + NW - 1) / NW;  // loads per wave and stage; past the last, the last again
-  static_assert((S - 1) * NLD < 64, "vmcnt range");
+  static_assert((S - 1) * NLD < 64 && lds8<BM, BN, KG, SL, S>() <= 160 * 1024, "vmcnt range and LDS of a CU");
   extern __shared__ __align__(16) unsigned char smem_raw[];
   float* const red = reinterpret_cast<float*>(smem_raw);  // [KG][BM][PITCH], after the main loop
 
@@ -189,8 +211,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // A slab's products in two halves of 64 codes: lane group kq takes the 16 codes at 16 kq of the half, which lie
-  // in its block kq / 2, as two MFMA operands of 8 (any order of k will do that x and w share).
   auto compute = [&](int buf, int count) {
     constexpr int PS = (SL + KG - 1) / KG;
 #pragma unroll
@@ -199,30 +219,58 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
       if (slab < count) {
         const unsigned char* const codes = smem_raw + buf * STAGE + slab * (BM + BN) * 128;
         const unsigned* const sc = reinterpret_cast<const unsigned*>(smem_raw + buf * STAGE + CODES) + slab * SG * 64;
+        // Lane group kq takes the 16 codes at 16 kq of each half of the slab.
+        auto chunk = [&](int r, int h) {
+          return *reinterpret_cast<const i32x4*>(codes + r * 128 + (((4 * h + kq) ^ ((r >> 1) & 7)) << 4));
+        };
         unsigned sx[MB], sw[NB];
+        if constexpr (kFast) {
+          // One MFMA per slab and 16x16 block: the instruction takes the scale of its lane's own 32 codes in k order,
+          // block kq of the row.
 #pragma unroll
-        for (int i = 0; i < MB; ++i) sx[i] = sc[wm0 + i * 16 + r16] >> (8 * (kq >> 1));
+          for (int i = 0; i < MB; ++i) sx[i] = sc[wm0 + i * 16 + r16] >> (8 * kq);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) sw[j] = sc[SX + wn0 + j * 16 + r16] >> (8 * (kq >> 1));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          auto fragment = [&](int r, unsigned s, bf16x8 (&f)[2]) {
-            const i32x4 c = *reinterpret_cast<const i32x4*>(codes + r * 128 + (((4 * h + kq) ^ ((r >> 1) & 7)) << 4));
-            const float scale = __builtin_bit_cast(float, ((s >> (16 * h)) & 255u) << 23);
-            f[0] = widen8(c[0], c[1], scale);
-            f[1] = widen8(c[2], c[3], scale);
+          for (int j = 0; j < NB; ++j) sw[j] = sc[SX + wn0 + j * 16 + r16] >> (8 * kq);
+          i32x8 fx[MB], fw[NB];
+          auto fragment = [&](int r) {
+            const i32x4 lo = chunk(r, 0), hi = chunk(r, 1);
+            return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
           };
-          bf16x8 fx[MB][2], fw[NB][2];
 #pragma unroll
-          for (int i = 0; i < MB; ++i) fragment(wm0 + i * 16 + r16, sx[i], fx[i]);
+          for (int i = 0; i < MB; ++i) fx[i] = fragment(wm0 + i * 16 + r16);
 #pragma unroll
-          for (int j = 0; j < NB; ++j) fragment(BM + wn0 + j * 16 + r16, sw[j], fw[j]);
+          for (int j = 0; j < NB; ++j) fw[j] = fragment(BM + wn0 + j * 16 + r16);
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
+            for (int j = 0; j < NB; ++j) acc[i][j] = mfma8(fw[j], fx[i], acc[i][j], sw[j], sx[i]);
+        } else {
+          // Each half's 16 codes lie in block kq / 2 of it: two bf16 operands of 8 (any order of k will do that x
+          // and w share).
 #pragma unroll
-              for (int j = 0; j < NB; ++j) acc[i][j] = mfma16(fw[j][e], fx[i][e], acc[i][j]);
+          for (int i = 0; i < MB; ++i) sx[i] = sc[wm0 + i * 16 + r16] >> (8 * (kq >> 1));
+#pragma unroll
+          for (int j = 0; j < NB; ++j) sw[j] = sc[SX + wn0 + j * 16 + r16] >> (8 * (kq >> 1));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            auto fragment = [&](int r, unsigned s, bf16x8 (&f)[2]) {
+              const i32x4 c = chunk(r, h);
+              const float scale = __builtin_bit_cast(float, ((s >> (16 * h)) & 255u) << 23);
+              f[0] = widen8(c[0], c[1], scale);
+              f[1] = widen8(c[2], c[3], scale);
+            };
+            bf16x8 fx[MB][2], fw[NB][2];
+#pragma unroll
+            for (int i = 0; i < MB; ++i) fragment(wm0 + i * 16 + r16, sx[i], fx[i]);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fragment(BM + wn0 + j * 16 + r16, sw[j], fw[j]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = mfma16(fw[j][e], fx[i][e], acc[i][j]);
+          }
         }
       }
     }
@@ -302,56 +350,400 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
   }
 }
 
-// Tile menu: BM, BN, WM, WN, KG, SL, S.
-#define LAYA_LINEAR8_TILES        \
-  LAYA_T(0, 16, 64, 1, 2, 4, 4, 2) \
-  LAYA_T(1, 128, 128, 2, 4, 1, 1, 3)
+// ---- the batched product: a persistent ring of 256 x 256 tiles on the 8-bit matrix unit ----
+
+constexpr int kUnit8 = 64 * 128;   // bytes of a ring unit: 64 rows of one slab
+constexpr int kUnits8 = 19, kScaleStages8 = 3;
+constexpr int kScales8 = kUnits8 * kUnit8, kScaleStage8 = 512 * 4;
+constexpr int kRing8Lds = kScales8 + kScaleStages8 * kScaleStage8;
+static_assert(kRing8Lds <= 160 * 1024, "LDS of a CU");
+
+// Four dwords a lane, v[j] of lane group kq: afterwards v[k] of lane group j holds what was v[j] of group k.
+__device__ __forceinline__ void transpose4(unsigned (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v[j], v[j + 2], false, false);
+    v[j] = r[0];
+    v[j + 2] = r[1];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v[j], v[j + 1], false, false);
+    v[j] = r[0];
+    v[j + 1] = r[1];
+  }
+}
+// Maximum over the four lane groups.
+__device__ __forceinline__ unsigned group_max(unsigned m) {
+  const auto a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = a[0] > a[1] ? a[0] : a[1];
+  const auto b = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return b[0] > b[1] ? b[0] : b[1];
+}
+
+// Eight waves on a 2 x 4 grid of 128 x 64 outputs; a grid of at most one workgroup per CU walks the tiles, and the
+// operand stream runs on across tile boundaries.  LDS holds a ring of 19 units of 64 rows x 128 codes (a slab is
+// eight: four of x, four of w; every wave loads 8 rows of each unit) and three stages of scales, so up to 1.4
+// slabs are in flight behind the one consumed.  A wave's slab is eight rows of four MFMAs (a 16-row block of x
+// against its four 16-column blocks of w): w's fragments stay in registers for the slab, x's go through four
+// register sets, read two rows ahead.  The slab's one barrier sits two rows before its end, when its last fragment
+// has been read: it frees the slab's units and publishes the next slab, whose first fragments the last two rows
+// cover.
+//
+// The epilogue needs no LDS: lane (r, kq) = (lane % 16, lane / 16) holds columns 4 kq .. +3 of row r of each 16 x 16
+// block, and four lane groups exchange packed dwords so that each stores 16 consecutive columns.
+template <Act8 A, bool kE4m3>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+void linear8_ring_kernel(Linear8Args a) {
+  constexpr bool kGlu = gated(A);
+  constexpr int BM = 256, BN = 256, MB = 8, NB = 4, OC = kGlu ? BN / 2 : BN;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;  // 128 rows, 64 columns
+  const int r16 = lane & 15, kq = lane >> 4;
+
+  const int span = kE4m3 ? static_cast<int>(padded8(a.cols)) : a.cols;
+  const int nx = (span + OC - 1) / OC, ny = (a.M + BM - 1) / BM, total = nx * ny, G = gridDim.x;
+  const int n = a.ld / 128;  // slabs of a tile (the launcher checks n >= 2)
+  const int sld = a.ld / kBlock8;
+  const bool rows_major = a.M >= a.N;
+  int id = blockIdx.x;
+  if (id >= total) return;
+
+  struct Tile {
+    long long m0, n0;
+    i32x4 x, w, s;  // codes, and the scales of this wave's load
+  };
+  auto open = [&](int t) {
+    int tx, ty, tz;
+    tile_of(t, nx, ny, 1, rows_major, &tx, &ty, &tz);
+    Tile k;
+    k.m0 = static_cast<long long>(ty) * BM;
+    k.n0 = static_cast<long long>(tx) * BN;
+    k.x = rows_resource(a.x, k.m0, a.M, BM, a.ld);
+    k.w = rows_resource(a.w, k.n0, a.N, BN, a.ld);
+    k.s = wave < 4 ? rows_resource(a.xs, k.m0, a.M, BM, sld) : rows_resource(a.ws, k.n0, a.N, BN, sld);
+    return k;
+  };
+  Tile cur = open(id), nxt = cur;
+  int nid = id + G;
+  bool has_next = nid < total;
+  if (has_next) nxt = open(nid);
+
+  const unsigned lds_base = lds_address(smem_raw);
+  unsigned src[4];  // byte offset of this lane's 16 codes in each 64-row unit of an operand
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = u * 64 + wave * 8 + (lane >> 3);
+    src[u] = static_cast<unsigned>(r) * static_cast<unsigned>(a.ld) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
+  }
+  const unsigned src_scale = static_cast<unsigned>((wave & 3) * 64 + lane) * static_cast<unsigned>(sld);
+
+  // Unit u of a slab that starts at ring position `at`.
+  auto unit = [](int at, int u) { return at + u >= kUnits8 ? at + u - kUnits8 : at + u; };
+  auto after = [&](int at) { return unit(at, 8); };
+  // Loads of stream slab `s` counted from this tile's first: this tile's, the next one's, or (last tile) this
+  // tile's last again, never read.
+  auto issue = [&](int u, int s, int at) {
+    const bool next = s >= n && has_next;
+    const int kt = next ? s - n : min(s, n - 1);
+    lds_load16_buffer(u < 4 ? (next ? nxt.x : cur.x) : (next ? nxt.w : cur.w), src[u & 3], static_cast<unsigned>(kt) * 128u,
+                      lds_base + static_cast<unsigned>(unit(at, u) * kUnit8 + wave * 1024));
+  };
+  auto issue_scales = [&](int s, int stage) {
+    const bool next = s >= n && has_next;
+    const int kt = next ? s - n : min(s, n - 1);
+    lds_load4_buffer(next ? nxt.s : cur.s, src_scale, static_cast<unsigned>(kt) * 4u,
+                     lds_base + static_cast<unsigned>(kScales8 + stage * kScaleStage8 + wave * 256));
+  };
+
+  // Fragment addresses: a lane's two chunks, kq and 4 + kq, lie 64 bytes apart under the swizzle of its row.
+  const int frag = r16 * 128 + ((kq ^ (r16 >> 1)) << 4);
+  i32x8 fx[4], fw[NB];
+  unsigned sx[4], sw[NB];
+  auto read = [&](int byte) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(smem_raw + byte);
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(smem_raw + (byte ^ 64));
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto read_x = [&](int at, int stage, int i) {
+    fx[i & 3] = read(unit(at, 2 * wm + (i >> 2)) * kUnit8 + (i & 3) * 2048 + frag);
+    sx[i & 3] = smem_raw[kScales8 + stage * kScaleStage8 + (wm * 128 + i * 16 + r16) * 4 + kq];
+  };
+  auto read_w = [&](int at, int stage, int j) {
+    fw[j] = read(unit(at, 4 + wn) * kUnit8 + j * 2048 + frag);
+    sw[j] = smem_raw[kScales8 + stage * kScaleStage8 + (256 + wn * 64 + j * 16 + r16) * 4 + kq];
+  };
+  f32x4 acc[MB][NB];
+  auto row = [&](int i) {  // weights as the MFMA's A operand: the accumulator holds C^T
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = mfma8(fw[j], fx[i & 3], acc[i][j], sw[j], sx[i & 3]);
+  };
+  auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+
+  float4 bias[NB];
+  auto load_bias = [&] {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const long long c = cur.n0 + wn * 64 + j * 16 + 4 * kq;
+      bias[j] = a.bias && c < a.N ? *reinterpret_cast<const float4*>(a.bias + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  load_bias();
+
+  // Prologue: slabs 0 and 1.
+  int at = 0, stage = 0;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) issue(u, s, 8 * s);
+    issue_scales(s, s);
+  }
+  publish_stage<waitcnt_vm(9)>();
+  auto next_stage = [](int s) { return s == kScaleStages8 - 1 ? 0 : s + 1; };
+  auto read_first = [&](int at, int stage) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) read_w(at, stage, j);
+    read_x(at, stage, 0);
+    read_x(at, stage, 1);
+  };
+  read_first(0, 0);
+
+  // Rows 0 .. 5 of slab `it`, in which units 0 .. 2 of slab it + 2 go where the ring has room, and the barrier.
+  auto first_rows = [&](int it) {
+    const int to = after(after(at));
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      if (i < 3) issue(i, it + 2, to);
+      read_x(at, stage, i + 2);
+      pin();
+      row(i);
+      pin();
+    }
+    publish_stage<waitcnt_vm(3)>();
+    pin();
+  };
+  // The loads of slab s that go into the units its barrier has freed, in two parts.
+  auto rest = [&](int part, int s) {
+    const int to = after(after(at));
+    issue(part ? 5 : 3, s, to);
+    issue(part ? 6 : 4, s, to);
+    if (part) issue(7, s, to);
+    else issue_scales(s, next_stage(next_stage(stage)));
+  };
+
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int it = 0; it < n - 1; ++it) {
+      const int nat = after(at), nstage = next_stage(stage);
+      first_rows(it);
+      // The slab's units are free: the rest of slab it + 2; slab it + 1 is visible.
+      rest(0, it + 2);
+      read_x(nat, nstage, 0);
+      pin();
+      row(6);
+      pin();
+      rest(1, it + 2);
+      read_x(nat, nstage, 1);
+      pin();
+      row(7);
+      pin();
+#pragma unroll
+      for (int j = 0; j < NB; ++j) read_w(nat, nstage, j);
+      at = nat;
+      stage = nstage;
+    }
+    // The tile's last slab: the next tile's first fragments are read after the epilogue.
+    first_rows(n - 1);
+    rest(0, n + 1);
+    pin();
+    row(6);
+    pin();
+    rest(1, n + 1);
+    pin();
+    row(7);
+    at = after(at);
+    stage = next_stage(stage);
+
+    // Epilogue, four 16 x 16 output blocks at a time: block t is row block `ib` and column block `jb` of the wave
+    // (gated: a pair of row blocks, two columns blocks each).
+    int elane = lane;  // an opaque copy: the epilogue's addresses stay out of the main loop's registers
+    asm volatile("" : "+v"(elane));
+    const int er = elane & 15, eq = elane >> 4;
+    constexpr int STEPS = kGlu ? MB / 2 : MB;
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) {
+      float v[4][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if constexpr (kGlu) {
+          const int i = 2 * step + (t >> 1), j = 2 * (t & 1);
+          const float4 bg = bias[j], bv = bias[j + 1];
+          const float g[4] = {acc[i][j][0] + bg.x, acc[i][j][1] + bg.y, acc[i][j][2] + bg.z, acc[i][j][3] + bg.w};
+          const float u[4] = {acc[i][j + 1][0] + bv.x, acc[i][j + 1][1] + bv.y, acc[i][j + 1][2] + bv.z,
+                              acc[i][j + 1][3] + bv.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[t][e] = (A == Act8::Geglu ? gelu8<false>(g[e]) : silu8<false>(g[e])) * u[e];
+        } else {
+          const float4 b = bias[t];
+          v[t][0] = acc[step][t][0] + b.x; v[t][1] = acc[step][t][1] + b.y;
+          v[t][2] = acc[step][t][2] + b.z; v[t][3] = acc[step][t][3] + b.w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[t][e] = A == Act8::Gelu ? gelu8<false>(v[t][e]) : A == Act8::Relu && v[t][e] < 0.f ? 0.f : v[t][e];
+        }
+      }
+      // Row and first column of block t.
+      auto block_row = [&](int t) { return cur.m0 + wm * 128 + (kGlu ? 2 * step + (t >> 1) : step) * 16 + er; };
+      auto block_col = [&](int t) { return static_cast<int>(cur.n0 / BN) * OC + (kGlu ? wn * 32 + (t & 1) * 16 : wn * 64 + t * 16); };
+      if (a.residual) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (block_row(t) < a.M && block_col(t) < a.cols)
+            add_quad(a.residual, a.residual_type, static_cast<size_t>(block_row(t)) * a.cols + block_col(t) + 4 * eq, v[t]);
+      }
+      // After the exchange a lane holds the 16 columns of block eq.
+      const long long row_ = block_row(0) + (kGlu ? (eq >> 1) * 16 : 0);
+      const int col = block_col(0) + (kGlu ? eq & 1 : eq) * 16;
+      if constexpr (kE4m3) {
+        unsigned s[2], q[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          unsigned top = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned m = magnitude(v[2 * h + (e >> 2)][e & 3]);
+            top = top > m ? top : m;
+          }
+          s[h] = scale8(group_max(top));
+          q[2 * h] = encode8(v[2 * h][0], v[2 * h][1], v[2 * h][2], v[2 * h][3], s[h]);
+          q[2 * h + 1] = encode8(v[2 * h + 1][0], v[2 * h + 1][1], v[2 * h + 1][2], v[2 * h + 1][3], s[h]);
+        }
+        transpose4(q);
+        if (row_ < a.M && col < span) {
+          const size_t old = static_cast<size_t>(span);
+          *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(a.out) + row_ * old + col) =
+              i32x4{static_cast<int>(q[0]), static_cast<int>(q[1]), static_cast<int>(q[2]), static_cast<int>(q[3])};
+          if (!(eq & 1)) a.out_scales[row_ * (old / kBlock8) + col / kBlock8] = static_cast<uint8_t>(eq ? s[1] : s[0]);
+        }
+      } else {
+        unsigned lo[4], hi[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          lo[t] = pack16(a.out_type, v[t][0], v[t][1]);
+          hi[t] = pack16(a.out_type, v[t][2], v[t][3]);
+        }
+        transpose4(lo);
+        transpose4(hi);
+        if (row_ < a.M && col < a.cols) {
+          uint16_t* const dst = static_cast<uint16_t*>(a.out) + static_cast<size_t>(row_) * a.cols + col;
+          *reinterpret_cast<i32x4*>(dst) = i32x4{static_cast<int>(lo[0]), static_cast<int>(hi[0]), static_cast<int>(lo[1]), static_cast<int>(hi[1])};
+          *reinterpret_cast<i32x4*>(dst + 8) = i32x4{static_cast<int>(lo[2]), static_cast<int>(hi[2]), static_cast<int>(lo[3]), static_cast<int>(hi[3])};
+        }
+      }
+    }
+    if (!has_next) break;
+    cur = nxt;
+    nid += G;
+    has_next = nid < total;
+    if (has_next) nxt = open(nid);
+    load_bias();
+    read_first(at, stage);
+  }
+  // The last slabs' clamped loads may still be landing in this workgroup's LDS.
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+}
+
+// Tile menu: BM, BN, WM, WN, KG, SL, S, 8-bit matrix unit.
+#define LAYA_LINEAR8_TILES                  \
+  LAYA_T(0, 16, 16, 1, 1, 8, 8, 4, false)   \
+  LAYA_T(1, 16, 32, 1, 1, 8, 8, 3, false)   \
+  LAYA_T(2, 16, 64, 1, 2, 4, 4, 3, false)   \
+  LAYA_T(3, 32, 32, 1, 1, 8, 8, 2, false)   \
+  LAYA_T(4, 32, 64, 1, 2, 4, 4, 3, false)   \
+  LAYA_T(5, 64, 32, 2, 1, 4, 4, 3, false)   \
+  LAYA_T(6, 64, 64, 2, 2, 2, 2, 4, false)   \
+  LAYA_T(7, 64, 64, 2, 2, 4, 4, 2, false)   \
+  LAYA_T(8, 64, 128, 2, 4, 1, 1, 4, false)  \
+  LAYA_T(9, 128, 128, 2, 4, 1, 1, 4, false) \
+  LAYA_T(10, 64, 64, 2, 2, 2, 2, 4, true)   \
+  LAYA_T(11, 64, 128, 2, 4, 1, 1, 4, true)  \
+  LAYA_T(12, 128, 128, 2, 4, 1, 1, 4, true) \
+  LAYA_T(13, 128, 256, 2, 4, 1, 1, 3, true) \
+  LAYA_T(14, 64, 128, 2, 2, 2, 2, 3, false) \
+  LAYA_T(15, 32, 128, 1, 4, 2, 2, 3, false)
 
 struct Tile8 {
   int bm, bn, lds, threads;
+  bool fast;
 };
 constexpr Tile8 kTiles8[] = {
-#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S) {BM, BN, lds8<BM, BN, KG, SL, S>(), 64 * WM * WN * KG},
+#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST) {BM, BN, lds8<BM, BN, KG, SL, S>(), 64 * WM * WN * KG, FAST},
     LAYA_LINEAR8_TILES
 #undef LAYA_T
 };
-constexpr int kTiles8Count = sizeof(kTiles8) / sizeof(kTiles8[0]);
+constexpr int kTiles8Count = sizeof(kTiles8) / sizeof(kTiles8[0]), kRing8 = kTiles8Count;
+
+typedef void (*RingKernel)(Linear8Args);
+RingKernel ring_kernel(Act8 act, bool out8) {
+  switch (act) {
+#define LAYA_A(A) case Act8::A: return out8 ? linear8_ring_kernel<Act8::A, true> : linear8_ring_kernel<Act8::A, false>;
+    LAYA_A(Gelu) LAYA_A(Relu) LAYA_A(Geglu) LAYA_A(Swiglu)
+    default: LAYA_A(None)
+#undef LAYA_A
+  }
+}
+constexpr Tile8 kRingTile8 = {256, 256, kRing8Lds, 512, true};
 
 int columns8(const Linear8Args& a, int bn) { return gated(a.act) ? bn / 2 : bn; }
 
 }  // namespace
 
-int linear8_tile_count() { return kTiles8Count; }
+int linear8_tile_count() { return kTiles8Count + 1; }
 
 bool linear8_tile_valid(int id, const Linear8Args& a) {
+  if (id == kRing8) return a.out_type != static_cast<int>(DType::F32) && a.ld >= 256 && a.wide;
   // A block of 32 output codes, and a group of 16 gate and 16 value rows, lie inside one tile.
   return id >= 0 && id < kTiles8Count && (a.out_type != kE4M3 || columns8(a, kTiles8[id].bn) % kBlock8 == 0) &&
-         (!gated(a.act) || kTiles8[id].bn % 32 == 0);
+         (!gated(a.act) || kTiles8[id].bn % 32 == 0) && (a.out_type != static_cast<int>(DType::F32) || !kTiles8[id].fast);
 }
 
-int linear8_plan(const Linear8Args& a, int) { return a.M <= 64 ? 0 : 1; }
+int linear8_plan(const Linear8Args& a, int) { return a.M <= 64 ? 2 : 9; }
 
 hipError_t linear8_prepare() {
   hipError_t e = hipSuccess;
-#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S)                                                            \
+#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST)                                                            \
   if (e == hipSuccess)                                                                                   \
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear8_kernel<BM, BN, WM, WN, KG, SL, S>),   \
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>),   \
                             hipFuncAttributeMaxDynamicSharedMemorySize, kTiles8[ID].lds);
   LAYA_LINEAR8_TILES
 #undef LAYA_T
+  for (int act = 0; act < 5 && e == hipSuccess; ++act)
+    for (bool out8 : {false, true})
+      if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out8)),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
   return e;
 }
 
 hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (a.M <= 0) return hipSuccess;
-  const Tile8& t = kTiles8[tile];
+  const Tile8& t = tile == kRing8 ? kRingTile8 : kTiles8[tile];
   const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = columns8(a, t.bn);
   const long long groups = (span + oc - 1) / oc * ((static_cast<long long>(a.M) + t.bm - 1) / t.bm);
   if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(groups)), block(t.threads);
+  if (tile == kRing8) {
+    const dim3 some(static_cast<unsigned>(std::min(groups, 256LL)));
+    LAYA_LAUNCH(ring_kernel(a.act, a.out_type == kE4M3), some, block, t.lds, stream, a);
+    return hipGetLastError();
+  }
   switch (tile) {
-#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S) \
-  case ID: LAYA_LAUNCH((linear8_kernel<BM, BN, WM, WN, KG, SL, S>), grid, block, t.lds, stream, a); break;
+#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST) \
+  case ID: LAYA_LAUNCH((linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>), grid, block, t.lds, stream, a); break;
     LAYA_LINEAR8_TILES
 #undef LAYA_T
     default: return hipErrorInvalidValue;
