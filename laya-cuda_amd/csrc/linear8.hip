@@ -10,6 +10,7 @@
 // owns BM x BN outputs, WM x WN waves of it times KG groups that split the slabs; S stages of SL slabs are in
 // flight.  The groups' fp32 tiles are added in group order through LDS, so results do not depend on timing.
 #include "kernels.hpp"
+#include "ring_walk.hpp"
 #include "rows8.hpp"
 #include "tiles.hpp"
 
@@ -43,6 +44,7 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 // D = A(16x128) * B(128x16) + C of e4m3 codes with a scale per 32: lane l supplies row/column l % 16, its codes 16 (l / 16)
 // .. +15 and 64 + 16 (l / 16) .. +15, and in the low byte of its scale that of codes 32 (l / 16) .. +31 of the row.
@@ -175,6 +177,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
   const int sld = a.ld / kBlock8;  // scale bytes of a row
   const i32x4 rsX = rows_resource(a.x, m0, a.M, BM, a.ld), rsXs = rows_resource(a.xs, m0, a.M, BM, sld);
   const i32x4 rsW = rows_resource(a.w, n0, a.N, BN, a.ld), rsWs = rows_resource(a.ws, n0, a.N, BN, sld);
+  const bool live = n0 < a.N;
   const unsigned lds_base = lds_address(smem_raw);
   const int n = a.ld / 128, stages = (n + SL - 1) / SL;
 
@@ -188,16 +191,17 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
       if (g < SL * RG) {
         const int rg = g % RG, r = rg * 8 + (lane >> 3);
         const unsigned k = static_cast<unsigned>(min(stage * SL + g / RG, n - 1)) * 128u;
-        const bool isx = rg * 8 < BM;
+        const bool isx = rg * 8 < BM;  // a scalar offset has to stay inside its resource: 0 where w has no rows
         const unsigned row = static_cast<unsigned>(isx ? r : r - BM);
-        lds_load16_buffer(isx ? rsX : rsW, row * static_cast<unsigned>(a.ld) + (((lane & 7) ^ ((r >> 1) & 7)) << 4), k,
+        lds_load16_buffer(isx ? rsX : rsW, row * static_cast<unsigned>(a.ld) + (((lane & 7) ^ ((r >> 1) & 7)) << 4),
+                          isx || live ? k : 0u,
                           base + static_cast<unsigned>(g * 1024));
       } else {
         const int sg = (g - SL * RG) % SG, r = sg * 64 + lane;
         const unsigned k = static_cast<unsigned>(min(stage * SL + (g - SL * RG) / SG, n - 1)) * 4u;
         const bool isx = sg * 64 < SX;
         const unsigned row = static_cast<unsigned>(isx ? r : r - SX);
-        lds_load4_buffer(isx ? rsXs : rsWs, row * static_cast<unsigned>(sld), k,
+        lds_load4_buffer(isx ? rsXs : rsWs, row * static_cast<unsigned>(sld), isx || live ? k : 0u,
                          base + static_cast<unsigned>(CODES + (g - SL * RG) * 256));
       }
     }
@@ -355,7 +359,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
 constexpr int kUnit8 = 64 * 128;   // bytes of a ring unit: 64 rows of one slab
 constexpr int kUnits8 = 19, kScaleStages8 = 3;
 constexpr int kScales8 = kUnits8 * kUnit8, kScaleStage8 = 512 * 4;
-constexpr int kRing8Lds = kScales8 + kScaleStages8 * kScaleStage8;
+constexpr int kBias8 = kScales8 + kScaleStages8 * kScaleStage8;  // two tiles' bias, 256 floats each
+constexpr int kRing8Lds = kBias8 + 2 * 1024;
 static_assert(kRing8Lds <= 160 * 1024, "LDS of a CU");
 
 // Four dwords a lane, v[j] of lane group kq: afterwards v[k] of lane group j holds what was v[j] of group k.
@@ -394,9 +399,9 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // block, and four lane groups exchange packed dwords so that each stores 16 consecutive columns.
 template <Act8 A, bool kE4m3>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
-void linear8_ring_kernel(Linear8Args a) {
+void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   constexpr bool kGlu = gated(A);
-  constexpr int BM = 256, BN = 256, MB = 8, NB = 4, OC = kGlu ? BN / 2 : BN;
+  constexpr int BM = 256, BN = 256, MB = 8, NB = 4;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -404,26 +409,29 @@ void linear8_ring_kernel(Linear8Args a) {
   const int r16 = lane & 15, kq = lane >> 4;
 
   const int span = kE4m3 ? static_cast<int>(padded8(a.cols)) : a.cols;
-  const int nx = (span + OC - 1) / OC, ny = (a.M + BM - 1) / BM, total = nx * ny, G = gridDim.x;
+  const int total = walk.total, G = gridDim.x;
   const int n = a.ld / 128;  // slabs of a tile (the launcher checks n >= 2)
   const int sld = a.ld / kBlock8;
-  const bool rows_major = a.M >= a.N;
   int id = blockIdx.x;
   if (id >= total) return;
 
   struct Tile {
-    long long m0, n0;
+    int m0, n0;
     i32x4 x, w, s;  // codes, and the scales of this wave's load
+    bool live;      // holds rows of w (a tile of an 8-bit output's padding need not)
   };
   auto open = [&](int t) {
-    int tx, ty, tz;
-    tile_of(t, nx, ny, 1, rows_major, &tx, &ty, &tz);
+    int tx, ty;
+    ring_tile(walk, t, &tx, &ty);
     Tile k;
-    k.m0 = static_cast<long long>(ty) * BM;
-    k.n0 = static_cast<long long>(tx) * BN;
-    k.x = rows_resource(a.x, k.m0, a.M, BM, a.ld);
-    k.w = rows_resource(a.w, k.n0, a.N, BN, a.ld);
-    k.s = wave < 4 ? rows_resource(a.xs, k.m0, a.M, BM, sld) : rows_resource(a.ws, k.n0, a.N, BN, sld);
+    k.m0 = ty * BM;
+    k.n0 = tx * BN;
+    const int mr = max(min(a.M - k.m0, BM), 0), nr = max(min(a.N - k.n0, BN), 0), nf = min(k.n0, a.N);
+    k.live = nr > 0;
+    k.x = buffer_resource(a.x + static_cast<size_t>(k.m0) * a.ld, mr * a.ld);
+    k.w = buffer_resource(a.w + static_cast<size_t>(nf) * a.ld, nr * a.ld);
+    k.s = wave < 4 ? buffer_resource(a.xs + static_cast<size_t>(k.m0) * sld, mr * sld)
+                   : buffer_resource(a.ws + static_cast<size_t>(nf) * sld, nr * sld);
     return k;
   };
   Tile cur = open(id), nxt = cur;
@@ -438,22 +446,25 @@ void linear8_ring_kernel(Linear8Args a) {
     const int r = u * 64 + wave * 8 + (lane >> 3);
     src[u] = static_cast<unsigned>(r) * static_cast<unsigned>(a.ld) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
   }
-  const unsigned src_scale = static_cast<unsigned>((wave & 3) * 64 + lane) * static_cast<unsigned>(sld);
+  // Scales of 64 rows: dword 4 r + j of the load is row 16 j + r, so that a lane reads those of its row of four
+  // 16-row blocks at once.
+  const unsigned src_scale = static_cast<unsigned>((wave & 3) * 64 + (lane & 3) * 16 + (lane >> 2)) * static_cast<unsigned>(sld);
 
   // Unit u of a slab that starts at ring position `at`.
   auto unit = [](int at, int u) { return at + u >= kUnits8 ? at + u - kUnits8 : at + u; };
   auto after = [&](int at) { return unit(at, 8); };
+  // A scalar offset has to stay inside its resource (ranges.hpp): where w has no rows it is 0, and the loads read zeros.
   // Loads of stream slab `s` counted from this tile's first: this tile's, the next one's, or (last tile) this
   // tile's last again, never read.
   auto issue = [&](int u, int s, int at) {
     const bool next = s >= n && has_next;
-    const int kt = next ? s - n : min(s, n - 1);
+    const int kt = (u < 4 || (next ? nxt.live : cur.live)) ? (next ? s - n : min(s, n - 1)) : 0;
     lds_load16_buffer(u < 4 ? (next ? nxt.x : cur.x) : (next ? nxt.w : cur.w), src[u & 3], static_cast<unsigned>(kt) * 128u,
                       lds_base + static_cast<unsigned>(unit(at, u) * kUnit8 + wave * 1024));
   };
   auto issue_scales = [&](int s, int stage) {
     const bool next = s >= n && has_next;
-    const int kt = next ? s - n : min(s, n - 1);
+    const int kt = (wave < 4 || (next ? nxt.live : cur.live)) ? (next ? s - n : min(s, n - 1)) : 0;
     lds_load4_buffer(next ? nxt.s : cur.s, src_scale, static_cast<unsigned>(kt) * 4u,
                      lds_base + static_cast<unsigned>(kScales8 + stage * kScaleStage8 + wave * 256));
   };
@@ -461,39 +472,36 @@ void linear8_ring_kernel(Linear8Args a) {
   // Fragment addresses: a lane's two chunks, kq and 4 + kq, lie 64 bytes apart under the swizzle of its row.
   const int frag = r16 * 128 + ((kq ^ (r16 >> 1)) << 4);
   i32x8 fx[4], fw[NB];
-  unsigned sx[4], sw[NB];
+  unsigned sx[MB], sw[NB];
   auto read = [&](int byte) {
     const i32x4 lo = *reinterpret_cast<const i32x4*>(smem_raw + byte);
     const i32x4 hi = *reinterpret_cast<const i32x4*>(smem_raw + (byte ^ 64));
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto read_x = [&](int at, int stage, int i) {
-    fx[i & 3] = read(unit(at, 2 * wm + (i >> 2)) * kUnit8 + (i & 3) * 2048 + frag);
-    sx[i & 3] = smem_raw[kScales8 + stage * kScaleStage8 + (wm * 128 + i * 16 + r16) * 4 + kq];
-  };
-  auto read_w = [&](int at, int stage, int j) {
-    fw[j] = read(unit(at, 4 + wn) * kUnit8 + j * 2048 + frag);
-    sw[j] = smem_raw[kScales8 + stage * kScaleStage8 + (256 + wn * 64 + j * 16 + r16) * 4 + kq];
+  auto read_x = [&](int at, int i) { fx[i & 3] = read(unit(at, 2 * wm + (i >> 2)) * kUnit8 + (i & 3) * 2048 + frag); };
+  auto read_w = [&](int at, int j) { fw[j] = read(unit(at, 4 + wn) * kUnit8 + j * 2048 + frag); };
+  // Scale bytes of four 16-row blocks, moved down to the one of the lane's 32 codes.
+  auto read_scales = [&](int stage, int group, unsigned* s) {
+    const i32x4 v = *reinterpret_cast<const i32x4*>(smem_raw + kScales8 + stage * kScaleStage8 + group * 256 + r16 * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = static_cast<unsigned>(v[j]) >> (8 * kq);
   };
   f32x4 acc[MB][NB];
-  auto row = [&](int i) {  // weights as the MFMA's A operand: the accumulator holds C^T
-#pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = mfma8(fw[j], fx[i & 3], acc[i][j], sw[j], sx[i & 3]);
+  auto mma = [&](int i, int j) {  // weights as the MFMA's A operand: the accumulator holds C^T
+    acc[i][j] = mfma8(fw[j], fx[i & 3], acc[i][j], sw[j], sx[i]);
   };
   auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
 
-  float4 bias[NB];
-  auto load_bias = [&] {
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const long long c = cur.n0 + wn * 64 + j * 16 + 4 * kq;
-      bias[j] = a.bias && c < a.N ? *reinterpret_cast<const float4*>(a.bias + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+  // The tile's bias, zeros past N, into its half of the bias area (every wave loads 64 columns, twice over).
+  auto issue_bias = [&](int half) {
+    const int nr = a.bias ? max(min(a.N - cur.n0, BN), 0) : 0;
+    lds_load4_buffer(buffer_resource(a.bias + (nr ? cur.n0 : 0), nr * 4), static_cast<unsigned>((wave & 3) * 256 + lane * 4), 0,
+                     lds_base + static_cast<unsigned>(kBias8 + half * 1024 + (wave & 3) * 256));
   };
-  load_bias();
+  issue_bias(0);
 
   // Prologue: slabs 0 and 1.
-  int at = 0, stage = 0;
+  int at = 0, stage = 0, half = 0;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -502,35 +510,63 @@ void linear8_ring_kernel(Linear8Args a) {
   }
   publish_stage<waitcnt_vm(9)>();
   auto next_stage = [](int s) { return s == kScaleStages8 - 1 ? 0 : s + 1; };
+  // What rows 0 and 1 of a slab need.
   auto read_first = [&](int at, int stage) {
+    read_scales(stage, 2 * wm, sx);
+    read_scales(stage, 4 + wn, sw);
+    read_x(at, 0);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) read_w(at, stage, j);
-    read_x(at, stage, 0);
-    read_x(at, stage, 1);
+    for (int j = 0; j < NB; ++j) read_w(at, j);
+    read_x(at, 1);
   };
   read_first(0, 0);
 
-  // Rows 0 .. 5 of slab `it`, in which units 0 .. 2 of slab it + 2 go where the ring has room, and the barrier.
-  auto first_rows = [&](int it) {
+  // Rows 0 .. 5 of slab `it`, in which units 0 .. 2 of slab it + 2 go where the ring has room, and the barrier, which
+  // waits for slab it + 1.  In a tile's first slab after an epilogue (`stores`) that slab's loads are older than the
+  // epilogue's stores and the bias load, which stay in flight: waiting for the stores cost 2-3 us a tile.
+  constexpr int kStores = kGlu ? MB : 2 * MB;
+  auto first_rows = [&](int it, bool stores) {
     const int to = after(after(at));
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
       if (i < 3) issue(i, it + 2, to);
-      read_x(at, stage, i + 2);
+      if (i == 1) read_scales(stage, 2 * wm + 1, sx + 4);
+      read_x(at, i + 2);
       pin();
-      row(i);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) mma(i, j);
       pin();
     }
-    publish_stage<waitcnt_vm(3)>();
+    if (stores) publish_stage<waitcnt_vm(3 + 1 + kStores)>();
+    else publish_stage<waitcnt_vm(3)>();
     pin();
   };
-  // The loads of slab s that go into the units its barrier has freed, in two parts.
-  auto rest = [&](int part, int s) {
-    const int to = after(after(at));
-    issue(part ? 5 : 3, s, to);
-    issue(part ? 6 : 4, s, to);
-    if (part) issue(7, s, to);
-    else issue_scales(s, next_stage(next_stage(stage)));
+  // Rows 6 and 7, column by column, so that each of w's fragments is free for the next slab's (kNext) early; the
+  // units freed by the barrier take the rest of slab s.
+  auto last_rows = [&](int s, auto next) {
+    constexpr bool kNext = decltype(next)::value;
+    const int nat = after(at), to = after(nat), nstage = next_stage(stage), tostage = next_stage(nstage);
+    if constexpr (kNext) {
+      read_scales(nstage, 2 * wm, sx);
+      read_x(nat, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      if (j == 0) issue_scales(s, tostage);
+      issue(3 + j, s, to);
+      if (j == 3) issue(7, s, to);
+      pin();
+      mma(6, j);
+      mma(7, j);
+      pin();
+      if constexpr (kNext) {
+        read_w(nat, j);
+        if (j == 1) read_x(nat, 1);
+        if (j == 3) read_scales(nstage, 4 + wn, sw);
+      }
+    }
+    at = nat;
+    stage = nstage;
   };
 
   for (;;) {
@@ -538,77 +574,61 @@ void linear8_ring_kernel(Linear8Args a) {
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int it = 0; it < n - 1; ++it) {
-      const int nat = after(at), nstage = next_stage(stage);
-      first_rows(it);
-      // The slab's units are free: the rest of slab it + 2; slab it + 1 is visible.
-      rest(0, it + 2);
-      read_x(nat, nstage, 0);
-      pin();
-      row(6);
-      pin();
-      rest(1, it + 2);
-      read_x(nat, nstage, 1);
-      pin();
-      row(7);
-      pin();
-#pragma unroll
-      for (int j = 0; j < NB; ++j) read_w(nat, nstage, j);
-      at = nat;
-      stage = nstage;
+    first_rows(0, id != static_cast<int>(blockIdx.x));
+    for (int it = 1; it < n; ++it) {
+      last_rows(it + 1, std::true_type());
+      first_rows(it, false);
     }
     // The tile's last slab: the next tile's first fragments are read after the epilogue.
-    first_rows(n - 1);
-    rest(0, n + 1);
-    pin();
-    row(6);
-    pin();
-    rest(1, n + 1);
-    pin();
-    row(7);
-    at = after(at);
-    stage = next_stage(stage);
+    last_rows(n + 1, std::false_type());
 
-    // Epilogue, four 16 x 16 output blocks at a time: block t is row block `ib` and column block `jb` of the wave
-    // (gated: a pair of row blocks, two columns blocks each).
+    // Epilogue, four 16 x 16 output blocks at a time: block t is a row block of the wave and its column block t
+    // (gated: a pair of row blocks with two column blocks each).  Stores go through a resource over the tile's rows:
+    // rows past M and columns past the row's end are dropped, and every wave issues the same number of them.
     int elane = lane;  // an opaque copy: the epilogue's addresses stay out of the main loop's registers
     asm volatile("" : "+v"(elane));
     const int er = elane & 15, eq = elane >> 4;
     constexpr int STEPS = kGlu ? MB / 2 : MB;
+    constexpr unsigned kNowhere = 0x80000000u;  // past every resource
+    const int col0 = (kGlu ? cur.n0 / 2 + wn * 32 : cur.n0 + wn * 64);
+    const int rows = min(a.M - cur.m0, BM);
+    const int pitch = kE4m3 ? span : a.cols * 2;  // bytes of an output row
+    const __amdgpu_buffer_rsrc_t dst = __builtin_amdgcn_make_buffer_rsrc(
+        static_cast<uint8_t*>(a.out) + static_cast<size_t>(cur.m0) * pitch, 0, rows * pitch, 0x00020000);
+    const __amdgpu_buffer_rsrc_t dst_scales = __builtin_amdgcn_make_buffer_rsrc(
+        kE4m3 ? a.out_scales + static_cast<size_t>(cur.m0) * (span / kBlock8) : nullptr, 0, kE4m3 ? rows * (span / kBlock8) : 0,
+        0x00020000);
+    const float* const bias = reinterpret_cast<const float*>(smem_raw + kBias8 + half * 1024) + wn * 64 + 4 * eq;
+    f32x4 b[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) b[j] = *reinterpret_cast<const f32x4*>(bias + 16 * j);
 #pragma unroll
     for (int step = 0; step < STEPS; ++step) {
       float v[4][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if constexpr (kGlu) {
-          const int i = 2 * step + (t >> 1), j = 2 * (t & 1);
-          const float4 bg = bias[j], bv = bias[j + 1];
-          const float g[4] = {acc[i][j][0] + bg.x, acc[i][j][1] + bg.y, acc[i][j][2] + bg.z, acc[i][j][3] + bg.w};
-          const float u[4] = {acc[i][j + 1][0] + bv.x, acc[i][j + 1][1] + bv.y, acc[i][j + 1][2] + bv.z,
-                              acc[i][j + 1][3] + bv.w};
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[t][e] = (A == Act8::Geglu ? gelu8<false>(g[e]) : silu8<false>(g[e])) * u[e];
-        } else {
-          const float4 b = bias[t];
-          v[t][0] = acc[step][t][0] + b.x; v[t][1] = acc[step][t][1] + b.y;
-          v[t][2] = acc[step][t][2] + b.z; v[t][3] = acc[step][t][3] + b.w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[t][e] = A == Act8::Gelu ? gelu8<false>(v[t][e]) : A == Act8::Relu && v[t][e] < 0.f ? 0.f : v[t][e];
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (kGlu) {
+            const int i = 2 * step + (t >> 1), j = 2 * (t & 1);
+            const float g = acc[i][j][e] + b[j][e], u = acc[i][j + 1][e] + b[j + 1][e];
+            v[t][e] = (A == Act8::Geglu ? gelu8<false>(g) : silu8<false>(g)) * u;
+          } else {
+            const float x = acc[step][t][e] + b[t][e];
+            v[t][e] = A == Act8::Gelu ? gelu8<false>(x) : A == Act8::Relu && x < 0.f ? 0.f : x;
+          }
         }
-      }
-      // Row and first column of block t.
-      auto block_row = [&](int t) { return cur.m0 + wm * 128 + (kGlu ? 2 * step + (t >> 1) : step) * 16 + er; };
-      auto block_col = [&](int t) { return static_cast<int>(cur.n0 / BN) * OC + (kGlu ? wn * 32 + (t & 1) * 16 : wn * 64 + t * 16); };
+      // Row in the tile and first column of block t.
+      auto block_row = [&](int t) { return wm * 128 + (kGlu ? 2 * step + (t >> 1) : step) * 16 + er; };
+      auto block_col = [&](int t) { return col0 + (kGlu ? t & 1 : t) * 16; };
       if (a.residual) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-          if (block_row(t) < a.M && block_col(t) < a.cols)
-            add_quad(a.residual, a.residual_type, static_cast<size_t>(block_row(t)) * a.cols + block_col(t) + 4 * eq, v[t]);
+          if (block_row(t) < rows && block_col(t) < a.cols)
+            add_quad(a.residual, a.residual_type, static_cast<size_t>(cur.m0 + block_row(t)) * a.cols + block_col(t) + 4 * eq, v[t]);
       }
       // After the exchange a lane holds the 16 columns of block eq.
-      const long long row_ = block_row(0) + (kGlu ? (eq >> 1) * 16 : 0);
-      const int col = block_col(0) + (kGlu ? eq & 1 : eq) * 16;
+      const int row = block_row(0) + (kGlu ? (eq >> 1) * 16 : 0), col = col0 + (kGlu ? eq & 1 : eq) * 16;
       if constexpr (kE4m3) {
         unsigned s[2], q[4];
 #pragma unroll
@@ -624,12 +644,10 @@ void linear8_ring_kernel(Linear8Args a) {
           q[2 * h + 1] = encode8(v[2 * h + 1][0], v[2 * h + 1][1], v[2 * h + 1][2], v[2 * h + 1][3], s[h]);
         }
         transpose4(q);
-        if (row_ < a.M && col < span) {
-          const size_t old = static_cast<size_t>(span);
-          *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(a.out) + row_ * old + col) =
-              i32x4{static_cast<int>(q[0]), static_cast<int>(q[1]), static_cast<int>(q[2]), static_cast<int>(q[3])};
-          if (!(eq & 1)) a.out_scales[row_ * (old / kBlock8) + col / kBlock8] = static_cast<uint8_t>(eq ? s[1] : s[0]);
-        }
+        const bool in = col < span;
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{q[0], q[1], q[2], q[3]}, dst, in ? row * pitch + col : kNowhere, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b8(static_cast<unsigned char>(eq & 2 ? s[1] : s[0]), dst_scales,
+                                             in && !(eq & 1) ? row * (span / kBlock8) + col / kBlock8 : kNowhere, 0, 0);
       } else {
         unsigned lo[4], hi[4];
 #pragma unroll
@@ -639,19 +657,19 @@ void linear8_ring_kernel(Linear8Args a) {
         }
         transpose4(lo);
         transpose4(hi);
-        if (row_ < a.M && col < a.cols) {
-          uint16_t* const dst = static_cast<uint16_t*>(a.out) + static_cast<size_t>(row_) * a.cols + col;
-          *reinterpret_cast<i32x4*>(dst) = i32x4{static_cast<int>(lo[0]), static_cast<int>(hi[0]), static_cast<int>(lo[1]), static_cast<int>(hi[1])};
-          *reinterpret_cast<i32x4*>(dst + 8) = i32x4{static_cast<int>(lo[2]), static_cast<int>(hi[2]), static_cast<int>(lo[3]), static_cast<int>(hi[3])};
-        }
+        const unsigned to = col < a.cols ? row * pitch + col * 2 : kNowhere;
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[0], hi[0], lo[1], hi[1]}, dst, to, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[2], hi[2], lo[3], hi[3]}, dst, to == kNowhere ? to : to + 16, 0, 0);
       }
     }
     if (!has_next) break;
-    cur = nxt;
+    id = nid;
     nid += G;
+    cur = nxt;
     has_next = nid < total;
     if (has_next) nxt = open(nid);
-    load_bias();
+    half ^= 1;
+    issue_bias(half);
     read_first(at, stage);
   }
   // The last slabs' clamped loads may still be landing in this workgroup's LDS.
@@ -688,7 +706,7 @@ constexpr Tile8 kTiles8[] = {
 };
 constexpr int kTiles8Count = sizeof(kTiles8) / sizeof(kTiles8[0]), kRing8 = kTiles8Count;
 
-typedef void (*RingKernel)(Linear8Args);
+typedef void (*RingKernel)(Linear8Args, RingWalk);
 RingKernel ring_kernel(Act8 act, bool out8) {
   switch (act) {
 #define LAYA_A(A) case Act8::A: return out8 ? linear8_ring_kernel<Act8::A, true> : linear8_ring_kernel<Act8::A, false>;
@@ -696,6 +714,10 @@ RingKernel ring_kernel(Act8 act, bool out8) {
     default: LAYA_A(None)
 #undef LAYA_A
   }
+}
+RingWalk walk_of(const Linear8Args& a) {
+  const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = gated(a.act) ? 128 : 256;
+  return ring_walk((span + oc - 1) / oc, (static_cast<long long>(a.M) + 255) / 256, a.M >= a.N);
 }
 constexpr Tile8 kRingTile8 = {256, 256, kRing8Lds, 512, true};
 
@@ -706,7 +728,7 @@ int columns8(const Linear8Args& a, int bn) { return gated(a.act) ? bn / 2 : bn; 
 int linear8_tile_count() { return kTiles8Count + 1; }
 
 bool linear8_tile_valid(int id, const Linear8Args& a) {
-  if (id == kRing8) return a.out_type != static_cast<int>(DType::F32) && a.ld >= 256 && a.wide;
+  if (id == kRing8) return a.out_type != static_cast<int>(DType::F32) && a.ld >= 256 && a.wide && walk_of(a).total > 0;
   // A block of 32 output codes, and a group of 16 gate and 16 value rows, lie inside one tile.
   return id >= 0 && id < kTiles8Count && (a.out_type != kE4M3 || columns8(a, kTiles8[id].bn) % kBlock8 == 0) &&
          (!gated(a.act) || kTiles8[id].bn % 32 == 0) && (a.out_type != static_cast<int>(DType::F32) || !kTiles8[id].fast);
@@ -737,8 +759,8 @@ hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(groups)), block(t.threads);
   if (tile == kRing8) {
-    const dim3 some(static_cast<unsigned>(std::min(groups, 256LL)));
-    LAYA_LAUNCH(ring_kernel(a.act, a.out_type == kE4M3), some, block, t.lds, stream, a);
+    const RingWalk walk = walk_of(a);
+    LAYA_LAUNCH(ring_kernel(a.act, a.out_type == kE4M3), dim3(std::min(walk.total, 256)), block, t.lds, stream, a, walk);
     return hipGetLastError();
   }
   switch (tile) {
