@@ -82,9 +82,12 @@ __device__ __forceinline__ void lds_load16(const void* g, unsigned lds) {
 // lds + 16 l (lds wave-uniform, in M0).  Loads past the resource's byte range return zeros.
 // soffset must be wave-uniform; readfirstlane puts it in an SGPR where the compiler computed it with
 // vector instructions (integer division of uniform values), and folds away where it already is one.
+// A vector-memory instruction may read an SGPR that a vector instruction wrote (readfirstlane; the readlane of a
+// spilled one) only five wait states later, which the hardware does not check and, for a load inside inline
+// assembly, the compiler does not either: s_nop 4 is those five.
 __device__ __forceinline__ void lds_load16_buffer(i32x4 rsrc, unsigned voffset, unsigned soffset, unsigned lds) {
   soffset = __builtin_amdgcn_readfirstlane(soffset);
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset),
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset),
                "{m0}"(lds));
 }
 // 128-bit buffer resource of `bytes` bytes at `base` (raw buffer: stride 0, byte offsets), wave-uniform.

@@ -24,7 +24,7 @@ namespace {
 // lds_load16_buffer's form for 4 bytes a lane: lane l's dword goes to LDS byte address lds + 4 l.
 __device__ __forceinline__ void lds_load4_buffer(i32x4 rsrc, unsigned voffset, unsigned soffset, unsigned lds) {
   soffset = __builtin_amdgcn_readfirstlane(soffset);
-  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds));
+  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds));
 }
 
 // Resource over `rows` rows of `pitch` bytes from row `first`: rows past the last read as zeros.
@@ -480,11 +480,16 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   };
   auto read_x = [&](int at, int i) { fx[i & 3] = read(unit(at, 2 * wm + (i >> 2)) * kUnit8 + (i & 3) * 2048 + frag); };
   auto read_w = [&](int at, int j) { fw[j] = read(unit(at, 4 + wn) * kUnit8 + j * 2048 + frag); };
-  // Scale bytes of four 16-row blocks, moved down to the one of the lane's 32 codes.
+  // Scale dwords of four 16-row blocks; `settle` moves the byte of the lane's 32 codes down.  It comes two rows after
+  // the read: the schedule's pins keep it where it is written, and it waits for the read.
   auto read_scales = [&](int stage, int group, unsigned* s) {
     const i32x4 v = *reinterpret_cast<const i32x4*>(smem_raw + kScales8 + stage * kScaleStage8 + group * 256 + r16 * 16);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = static_cast<unsigned>(v[j]) >> (8 * kq);
+    for (int j = 0; j < 4; ++j) s[j] = static_cast<unsigned>(v[j]);
+  };
+  auto settle = [&](unsigned* s, const unsigned* raw) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = raw[j] >> (8 * kq);
   };
   f32x4 acc[MB][NB];
   auto mma = [&](int i, int j) {  // weights as the MFMA's A operand: the accumulator holds C^T
@@ -518,6 +523,8 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) read_w(at, j);
     read_x(at, 1);
+    settle(sx, sx);
+    settle(sw, sw);
   };
   read_first(0, 0);
 
@@ -531,6 +538,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     for (int i = 0; i < 6; ++i) {
       if (i < 3) issue(i, it + 2, to);
       if (i == 1) read_scales(stage, 2 * wm + 1, sx + 4);
+      if (i == 3) settle(sx + 4, sx + 4);
       read_x(at, i + 2);
       pin();
 #pragma unroll
@@ -546,8 +554,10 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   auto last_rows = [&](int s, auto next) {
     constexpr bool kNext = decltype(next)::value;
     const int nat = after(at), to = after(nat), nstage = next_stage(stage), tostage = next_stage(nstage);
+    unsigned nw[4];
     if constexpr (kNext) {
       read_scales(nstage, 2 * wm, sx);
+      read_scales(nstage, 4 + wn, nw);
       read_x(nat, 0);
     }
 #pragma unroll
@@ -562,7 +572,8 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
       if constexpr (kNext) {
         read_w(nat, j);
         if (j == 1) read_x(nat, 1);
-        if (j == 3) read_scales(nstage, 4 + wn, sw);
+        if (j == 2) settle(sx, sx);
+        if (j == 3) settle(sw, nw);
       }
     }
     at = nat;
