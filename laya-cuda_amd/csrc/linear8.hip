@@ -357,8 +357,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
 // ---- the batched product: a persistent ring of 256 x 256 tiles on the 8-bit matrix unit ----
 
 constexpr int kUnit8 = 64 * 128;   // bytes of a ring unit: 64 rows of one slab
-constexpr int kUnits8 = 19, kScaleStages8 = 3;
-constexpr int kScales8 = kUnits8 * kUnit8, kScaleStage8 = 512 * 4;
+constexpr int kSlab8 = 8 * kUnit8;  // four units of x, four of w
+constexpr int kScaleStages8 = 3;
+constexpr int kScales8 = 2 * kSlab8, kScaleStage8 = 512 * 4;
 constexpr int kBias8 = kScales8 + kScaleStages8 * kScaleStage8;  // two tiles' bias, 256 floats each
 constexpr int kRing8Lds = kBias8 + 2 * 1024;
 static_assert(kRing8Lds <= 160 * 1024, "LDS of a CU");
@@ -387,13 +388,14 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 }
 
 // Eight waves on a 2 x 4 grid of 128 x 64 outputs; a grid of at most one workgroup per CU walks the tiles, and the
-// operand stream runs on across tile boundaries.  LDS holds a ring of 19 units of 64 rows x 128 codes (a slab is
-// eight: four of x, four of w; every wave loads 8 rows of each unit) and three stages of scales, so up to 1.4
-// slabs are in flight behind the one consumed.  A wave's slab is eight rows of four MFMAs (a 16-row block of x
-// against its four 16-column blocks of w): w's fragments stay in registers for the slab, x's go through four
-// register sets, read two rows ahead.  The slab's one barrier sits two rows before its end, when its last fragment
-// has been read: it frees the slab's units and publishes the next slab, whose first fragments the last two rows
-// cover.
+// operand stream runs on across tile boundaries.  LDS holds two slabs as units of 64 rows x 128 codes (of each of
+// which every wave loads 8 rows) and three stages of scales.  A wave's slab is eight rows of four MFMAs (a 16-row
+// block of x against its four 16-column blocks of w): w's fragments stay in registers for the slab, x's go through
+// four register sets, read two rows ahead.  Two barriers a slab, each some rows after the reads it waits for:
+//   before row 2: w's units and the first half of x's have been read and take the slab after the next;
+//   before row 6: the second half of x's; the next slab's first fragments are read under rows 6 and 7.
+// What a barrier publishes was issued three barriers earlier, one and a half slabs: with one barrier a slab (one
+// slab for most loads) the loads' latency bounded the loop.
 //
 // The epilogue needs no LDS: lane (r, kq) = (lane % 16, lane / 16) holds columns 4 kq .. +3 of row r of each 16 x 16
 // block, and four lane groups exchange packed dwords so that each stores 16 consecutive columns.
@@ -450,17 +452,14 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   // 16-row blocks at once.
   const unsigned src_scale = static_cast<unsigned>((wave & 3) * 64 + (lane & 3) * 16 + (lane >> 2)) * static_cast<unsigned>(sld);
 
-  // Unit u of a slab that starts at ring position `at`.
-  auto unit = [](int at, int u) { return at + u >= kUnits8 ? at + u - kUnits8 : at + u; };
-  auto after = [&](int at) { return unit(at, 8); };
   // A scalar offset has to stay inside its resource (ranges.hpp): where w has no rows it is 0, and the loads read zeros.
   // Loads of stream slab `s` counted from this tile's first: this tile's, the next one's, or (last tile) this
   // tile's last again, never read.
-  auto issue = [&](int u, int s, int at) {
+  auto issue = [&](int u, int s, int buf) {
     const bool next = s >= n && has_next;
     const int kt = (u < 4 || (next ? nxt.live : cur.live)) ? (next ? s - n : min(s, n - 1)) : 0;
     lds_load16_buffer(u < 4 ? (next ? nxt.x : cur.x) : (next ? nxt.w : cur.w), src[u & 3], static_cast<unsigned>(kt) * 128u,
-                      lds_base + static_cast<unsigned>(unit(at, u) * kUnit8 + wave * 1024));
+                      lds_base + static_cast<unsigned>(buf * kSlab8 + u * kUnit8 + wave * 1024));
   };
   auto issue_scales = [&](int s, int stage) {
     const bool next = s >= n && has_next;
@@ -473,13 +472,25 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   const int frag = r16 * 128 + ((kq ^ (r16 >> 1)) << 4);
   i32x8 fx[4], fw[NB];
   unsigned sx[MB], sw[NB];
-  auto read = [&](int byte) {
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(smem_raw + byte);
-    const i32x4 hi = *reinterpret_cast<const i32x4*>(smem_raw + (byte ^ 64));
+  // A slab's addresses: one register pair per operand, the blocks at constant offsets from it.  Opaque to the compiler,
+  // which kept a pair per buffer and block otherwise, and spilled.
+  struct Place {
+    int lo, hi;
+  };
+  auto place = [&](int base) {
+    Place p{base + frag, (base + frag) ^ 64};
+    asm volatile("" : "+v"(p.lo), "+v"(p.hi));
+    return p;
+  };
+  auto read = [&](const Place& p, int offset) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(smem_raw + p.lo + offset);
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(smem_raw + p.hi + offset);
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto read_x = [&](int at, int i) { fx[i & 3] = read(unit(at, 2 * wm + (i >> 2)) * kUnit8 + (i & 3) * 2048 + frag); };
-  auto read_w = [&](int at, int j) { fw[j] = read(unit(at, 4 + wn) * kUnit8 + j * 2048 + frag); };
+  auto place_x = [&](int buf) { return place(buf * kSlab8 + wm * 2 * kUnit8); };
+  auto place_w = [&](int buf) { return place(buf * kSlab8 + (4 + wn) * kUnit8); };
+  auto read_x = [&](const Place& p, int i) { fx[i & 3] = read(p, i * 2048); };
+  auto read_w = [&](const Place& p, int j) { fw[j] = read(p, j * 2048); };
   // Scale dwords of four 16-row blocks; `settle` moves the byte of the lane's 32 codes down.  It comes two rows after
   // the read: the schedule's pins keep it where it is written, and it waits for the read.
   auto read_scales = [&](int stage, int group, unsigned* s) {
@@ -494,6 +505,8 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   f32x4 acc[MB][NB];
   auto mma = [&](int i, int j) {  // weights as the MFMA's A operand: the accumulator holds C^T
     acc[i][j] = mfma8(fw[j], fx[i & 3], acc[i][j], sw[j], sx[i]);
+    // Emits nothing; as MFMAs have no side effects, the compiler moved them past barriers, holding all their fragments.
+    asm volatile("" : "+v"(acc[i][j]));
   };
   auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
 
@@ -505,78 +518,102 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   };
   issue_bias(0);
 
+  // The two groups of a slab's loads: those that go out before row 2 (scales, w, first half of x), and before row 6.
+  auto issue_first = [&](int part, int s, int buf, int stage) {
+    if (part == 0) issue_scales(s, stage), issue(4, s, buf);
+    else if (part == 1) issue(5, s, buf), issue(0, s, buf);
+    else if (part == 2) issue(6, s, buf), issue(2, s, buf);
+    else issue(7, s, buf);
+  };
+  constexpr int kFirst = 7, kSecond = 2;
+  auto issue_second = [&](int part, int s, int buf) { issue(part ? 3 : 1, s, buf); };
+
   // Prologue: slabs 0 and 1.
-  int at = 0, stage = 0, half = 0;
+  int buf = 0, stage = 0, half = 0;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) issue(u, s, 8 * s);
-    issue_scales(s, s);
+    for (int q = 0; q < 4; ++q) issue_first(q, s, s, s);
+    issue_second(0, s, s);
+    issue_second(1, s, s);
   }
-  publish_stage<waitcnt_vm(9)>();
+  publish_stage<waitcnt_vm(0)>();  // both slabs: the first tile's first slab waits as the later tiles' do
   auto next_stage = [](int s) { return s == kScaleStages8 - 1 ? 0 : s + 1; };
   // What rows 0 and 1 of a slab need.
-  auto read_first = [&](int at, int stage) {
+  auto read_first = [&] {
     read_scales(stage, 2 * wm, sx);
     read_scales(stage, 4 + wn, sw);
-    read_x(at, 0);
+    const Place px = place_x(buf), pw = place_w(buf);
+    read_x(px, 0);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) read_w(at, j);
-    read_x(at, 1);
+    for (int j = 0; j < NB; ++j) read_w(pw, j);
+    read_x(px, 1);
     settle(sx, sx);
     settle(sw, sw);
   };
-  read_first(0, 0);
+  read_first();
 
-  // Rows 0 .. 5 of slab `it`, in which units 0 .. 2 of slab it + 2 go where the ring has room, and the barrier, which
-  // waits for slab it + 1.  In a tile's first slab after an epilogue (`stores`) that slab's loads are older than the
-  // epilogue's stores and the bias load, which stay in flight: waiting for the stores cost 2-3 us a tile.
+  // The waits leave what is younger than the loads that the barrier publishes in flight: a group of each kind, and in a
+  // tile's first slab (kLate) the epilogue stores and the bias load, which come between the two tiles' loads.  Waiting
+  // for the stores there cost 2-3 us a tile.  (No wait is chosen at run time: across the branch the compiler moved
+  // the MFMAs behind the barrier.)
   constexpr int kStores = kGlu ? MB : 2 * MB;
-  auto first_rows = [&](int it, bool stores) {
-    const int to = after(after(at));
+  constexpr int kWait = kFirst + kSecond, kWaitLate = kWait + kStores + 1;
+  auto four = [&](int i) {
+    pin();
 #pragma unroll
-    for (int i = 0; i < 6; ++i) {
-      if (i < 3) issue(i, it + 2, to);
-      if (i == 1) read_scales(stage, 2 * wm + 1, sx + 4);
-      if (i == 3) settle(sx + 4, sx + 4);
-      read_x(at, i + 2);
-      pin();
-#pragma unroll
-      for (int j = 0; j < NB; ++j) mma(i, j);
-      pin();
-    }
-    if (stores) publish_stage<waitcnt_vm(3 + 1 + kStores)>();
-    else publish_stage<waitcnt_vm(3)>();
+    for (int j = 0; j < NB; ++j) mma(i, j);
     pin();
   };
-  // Rows 6 and 7, column by column, so that each of w's fragments is free for the next slab's (kNext) early; the
-  // units freed by the barrier take the rest of slab s.
-  auto last_rows = [&](int s, auto next) {
+  // Rows 0 .. 5 of the slab in `buf`; `to`: the stream slab whose loads go out.
+  auto first_rows = [&](int to, auto late) {
+    constexpr int kVm = decltype(late)::value ? kWaitLate : kWait;
+    const int tostage = next_stage(next_stage(stage));
+    const Place px = place_x(buf);
+    read_x(px, 2);
+    four(0);
+    read_scales(stage, 2 * wm + 1, sx + 4);
+    read_x(px, 3);
+    four(1);
+    publish_stage<waitcnt_vm(kVm)>();
+    pin();
+#pragma unroll
+    for (int i = 2; i < 6; ++i) {
+      issue_first(i - 2, to, buf, tostage);
+      if (i == 3) settle(sx + 4, sx + 4);
+      read_x(px, i + 2);
+      four(i);
+    }
+    publish_stage<waitcnt_vm(kVm)>();
+    pin();
+  };
+  // Rows 6 and 7, column by column, so that each of w's fragments is free for the next slab's (kNext) early.
+  auto last_rows = [&](int to, auto next) {
     constexpr bool kNext = decltype(next)::value;
-    const int nat = after(at), to = after(nat), nstage = next_stage(stage), tostage = next_stage(nstage);
+    const int nstage = next_stage(stage);
     unsigned nw[4];
     if constexpr (kNext) {
       read_scales(nstage, 2 * wm, sx);
       read_scales(nstage, 4 + wn, nw);
-      read_x(nat, 0);
     }
+    const Place px = place_x(buf ^ 1), pw = place_w(buf ^ 1);
+    if constexpr (kNext) read_x(px, 0);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      if (j == 0) issue_scales(s, tostage);
-      issue(3 + j, s, to);
-      if (j == 3) issue(7, s, to);
+      if (j == 0) issue_second(0, to, buf);
+      if (j == 2) issue_second(1, to, buf);
       pin();
       mma(6, j);
       mma(7, j);
       pin();
       if constexpr (kNext) {
-        read_w(nat, j);
-        if (j == 1) read_x(nat, 1);
+        read_w(pw, j);
+        if (j == 1) read_x(px, 1);
         if (j == 2) settle(sx, sx);
         if (j == 3) settle(sw, nw);
       }
     }
-    at = nat;
+    buf ^= 1;
     stage = nstage;
   };
 
@@ -585,10 +622,10 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    first_rows(0, id != static_cast<int>(blockIdx.x));
+    first_rows(2, std::true_type());
     for (int it = 1; it < n; ++it) {
       last_rows(it + 1, std::true_type());
-      first_rows(it, false);
+      first_rows(it + 2, std::false_type());
     }
     // The tile's last slab: the next tile's first fragments are read after the epilogue.
     last_rows(n + 1, std::false_type());
@@ -681,7 +718,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     if (has_next) nxt = open(nid);
     half ^= 1;
     issue_bias(half);
-    read_first(at, stage);
+    read_first();
   }
   // The last slabs' clamped loads may still be landing in this workgroup's LDS.
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
