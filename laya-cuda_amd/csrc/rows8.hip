@@ -66,33 +66,121 @@ __device__ __forceinline__ void store_codes(uint8_t* codes, uint8_t* scales, int
   }
 }
 
-// One quad of a row per thread; a wave's 64 quads are 8 whole blocks of one row or of neighbouring rows (rows hold
-// whole multiples of 128 codes, 32 quads).
-template <typename T, bool kVec>
-__global__ __launch_bounds__(256) void quantize8_kernel(Quantize8Args a) {
-  const int ld = static_cast<int>(padded8(a.width)), per_row = ld / 4;
-  const long long quads = a.rows * per_row, step = static_cast<long long>(gridDim.x) * 256;
-  for (long long q = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; q < quads; q += step) {
-    const long long row = q / per_row;
-    const int idx = static_cast<int>(q - row * per_row) * 4;
-    float v[4];
-    load4<T, kVec>(static_cast<const T*>(a.x) + row * a.stride, idx, a.width, v);
-    store_codes(a.codes + row * ld, a.scales + row * (ld / kBlock8), idx, ld, v);
+// Quantising and reading back work on pieces of 16 bytes of values: kPiece<T> of them a thread, 4 or 8, so that a block
+// is 8 or 4 lanes.  A workgroup owns 256 U pieces, all loaded before the first is used.  Piece q of the matrix is
+// piece q % per_row of row q / per_row; the workgroup's first one is divided in 64 bits, once, the others by a
+// multiplication.
+template <typename T> constexpr int kPiece = 16 / sizeof(T);
+struct Place8 {
+  long long row;
+  int piece;
+};
+__device__ __forceinline__ Place8 place8(long long row0, int in, int per_row, unsigned magic) {
+  // in < per_row + 1024: at most one row further for long rows, else divided exactly (in and per_row are under 2^11).
+  const int rows = per_row >= 1024 ? (in >= per_row) : static_cast<int>(__umulhi(static_cast<unsigned>(in), magic));
+  return Place8{row0 + rows, in - rows * per_row};
+}
+// Pieces a thread: one of up to 2^21 pieces (their workgroups run in few rounds: 5,003 x 1,000 fp32 values take 6.3 us,
+// and 6.9 with four), four of more (65,536 x 1,024 fp16 values: 57 us with one, 42 with four).
+int pieces_a_thread(long long pieces) { return pieces <= 1 << 21 ? 1 : 4; }
+unsigned piece_magic(int per_row) {  // ceil(2^32 / per_row); rows hold 16 pieces at least
+  return static_cast<unsigned>(((1ULL << 32) + per_row - 1) / per_row);
+}
+
+template <typename T, bool kVec, int U>
+__global__ __launch_bounds__(256) void quantize8_kernel(Quantize8Args a, unsigned magic) {
+  constexpr int E = kPiece<T>;
+  typedef T TE __attribute__((ext_vector_type(E)));
+  const int ld = static_cast<int>(padded8(a.width)), per_row = ld / E;
+  const long long total = a.rows * per_row, first = static_cast<long long>(blockIdx.x) * (256 * U);
+  const long long row0 = first / per_row;
+  const int in0 = static_cast<int>(first - row0 * per_row) + threadIdx.x;
+  float v[U][E];
+  Place8 o[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    o[u] = place8(row0, in0 + u * 256, per_row, magic);
+    if (first + u * 256 + threadIdx.x >= total) continue;
+    const T* const src = static_cast<const T*>(a.x) + o[u].row * a.stride + o[u].piece * E;
+    const int left = a.width - o[u].piece * E;
+    if constexpr (kVec) {
+      TE t;
+      if (left > 0) t = *reinterpret_cast<const TE*>(src);
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[u][i] = left > 0 ? static_cast<float>(t[i]) : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[u][i] = i < left ? static_cast<float>(src[i]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (first + u * 256 + threadIdx.x >= total) return;  // rows are whole blocks: alike in a block's lanes
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const unsigned m = magnitude(v[u][i]);
+      top = top > m ? top : m;
+    }
+#pragma unroll
+    for (int d = 1; d < kBlock8 / E; d <<= 1) {
+      const unsigned m = __shfl_xor(top, d, kWave);
+      top = top > m ? top : m;
+    }
+    const unsigned s = scale8(top);
+    typedef unsigned Codes __attribute__((ext_vector_type(E / 4)));
+    Codes c;
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) c[i] = encode8(v[u][4 * i], v[u][4 * i + 1], v[u][4 * i + 2], v[u][4 * i + 3], s);
+    *reinterpret_cast<Codes*>(a.codes + o[u].row * ld + o[u].piece * E) = c;
+    if ((threadIdx.x & (kBlock8 / E - 1)) == 0)
+      a.scales[o[u].row * (ld / kBlock8) + o[u].piece / (kBlock8 / E)] = static_cast<uint8_t>(s);
   }
 }
 
-template <typename T, bool kVec>
-__global__ __launch_bounds__(256) void dequantize8_kernel(Dequantize8Args a) {
-  const int ld = static_cast<int>(padded8(a.width)), per_row = (a.width + 3) / 4;
-  const long long quads = a.rows * per_row, step = static_cast<long long>(gridDim.x) * 256;
-  for (long long q = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; q < quads; q += step) {
-    const long long row = q / per_row;
-    const int idx = static_cast<int>(q - row * per_row) * 4;
-    const int c = *reinterpret_cast<const int*>(a.codes + row * ld + idx);
-    const float s = scale_value8(a.scales[row * (ld / kBlock8) + idx / kBlock8]);
-    const float v[4] = {__builtin_amdgcn_cvt_f32_fp8(c, 0) * s, __builtin_amdgcn_cvt_f32_fp8(c, 1) * s,
-                        __builtin_amdgcn_cvt_f32_fp8(c, 2) * s, __builtin_amdgcn_cvt_f32_fp8(c, 3) * s};
-    store4<T, kVec>(static_cast<T*>(a.out) + row * a.stride, idx, a.width, v);
+template <typename T, bool kVec, int U>
+__global__ __launch_bounds__(256) void dequantize8_kernel(Dequantize8Args a, unsigned magic) {
+  constexpr int E = kPiece<T>;
+  typedef int Codes __attribute__((ext_vector_type(E / 4)));
+  typedef T TE __attribute__((ext_vector_type(E)));
+  const int ld = static_cast<int>(padded8(a.width)), per_row = ld / E;
+  const long long total = a.rows * per_row, first = static_cast<long long>(blockIdx.x) * (256 * U);
+  const long long row0 = first / per_row;
+  const int in0 = static_cast<int>(first - row0 * per_row) + threadIdx.x;
+  Codes c[U];
+  unsigned s[U];
+  Place8 o[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    o[u] = place8(row0, in0 + u * 256, per_row, magic);
+    if (first + u * 256 + threadIdx.x >= total) continue;
+    c[u] = *reinterpret_cast<const Codes*>(a.codes + o[u].row * ld + o[u].piece * E);
+    s[u] = a.scales[o[u].row * (ld / kBlock8) + o[u].piece / (kBlock8 / E)];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (first + u * 256 + threadIdx.x >= total) return;
+    const float f = scale_value8(s[u]);
+    float v[E];
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+      v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(c[u][i], 0) * f;
+      v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(c[u][i], 1) * f;
+      v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(c[u][i], 2) * f;
+      v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(c[u][i], 3) * f;
+    }
+    T* const dst = static_cast<T*>(a.out) + o[u].row * a.stride + o[u].piece * E;
+    const int left = a.width - o[u].piece * E;
+    if constexpr (kVec) {
+      TE t;
+#pragma unroll
+      for (int i = 0; i < E; ++i) t[i] = static_cast<T>(v[i]);
+      if (left > 0) *reinterpret_cast<TE*>(dst) = t;
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i < left) dst[i] = static_cast<T>(v[i]);
+    }
   }
 }
 
@@ -101,13 +189,14 @@ __global__ __launch_bounds__(256) void dequantize8_kernel(Dequantize8Args a) {
 // rounded, to 8-bit rows.  W waves own a row and keep it in registers, C quads a lane: quad c of a lane holds
 // elements 256 W c + 256 wave + 4 lane .. +3, so a wave's loads are contiguous and 8 lanes are one block.
 // The variance is the centred one, in a second pass over the registers.
-template <typename B, int C, int W, bool kVec>
+// NS: the branch's partials when they are known at launch, so that they, the residual and the parameters are loaded
+// before the first addition (one memory round trip); -1: any number, in a loop.
+template <typename B, int C, int W, bool kVec, int NS, bool kEarly>
 __global__ __launch_bounds__(64 * (W == 1 ? 4 : W)) void norm8_kernel(Norm8Args a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = W == 1 ? blockIdx.x * (blockDim.x >> 6) + wave : blockIdx.x;
   if (row >= a.rows) return;
   const int first = (W == 1 ? 0 : wave * 256) + lane * 4;
-  const size_t at = static_cast<size_t>(row) * a.width;
   auto quad = [&](int c) { return first + c * 256 * W; };
   __shared__ float part[W];
   auto row_sum = [&](float v) {
@@ -122,17 +211,46 @@ __global__ __launch_bounds__(64 * (W == 1 ? 4 : W)) void norm8_kernel(Norm8Args 
     }
     return v;
   };
-
-  float v[C][4], t[4];
+  const float n = static_cast<float>(a.width);
+  const int ld = static_cast<int>(padded8(a.width));
+  float gamma[kEarly ? C : 1][4], beta[kEarly ? C : 1][4];
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      load4<float, kVec>(a.gamma, quad(c), a.width, gamma[c]);
+      if (a.beta) load4<float, kVec>(a.beta, quad(c), a.width, beta[c]);
+    }
+  }
+  const size_t at = static_cast<size_t>(row) * a.width;
+  float v[C][4], t[4], res[kEarly ? C : 1][4];
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) load4<float, kVec>(a.residual + at, quad(c), a.width, res[c]);
+  }
   if (a.branch) {
 #pragma unroll
     for (int c = 0; c < C; ++c) load4<B, kVec>(static_cast<const B*>(a.branch) + at, quad(c), a.width, v[c]);
-    for (int s = 1; s < a.splits; ++s) {
+    if constexpr (NS > 1) {
+      float p[NS - 1][C][4];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        load4<B, kVec>(static_cast<const B*>(a.branch) + s * a.part_stride + at, quad(c), a.width, t);
+      for (int s = 1; s < NS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] + t[i];
+        for (int c = 0; c < C; ++c)
+          load4<B, kVec>(static_cast<const B*>(a.branch) + s * a.part_stride + at, quad(c), a.width, p[s - 1][c]);
+#pragma unroll
+      for (int s = 1; s < NS; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] + p[s - 1][c][i];
+    } else if constexpr (NS < 0) {
+      for (int s = 1; s < a.splits; ++s) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          load4<B, kVec>(static_cast<const B*>(a.branch) + s * a.part_stride + at, quad(c), a.width, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[c][i] = v[c][i] + t[i];
+        }
       }
     }
     if (a.bias) {
@@ -146,13 +264,13 @@ __global__ __launch_bounds__(64 * (W == 1 ? 4 : W)) void norm8_kernel(Norm8Args 
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    load4<float, kVec>(a.residual + at, quad(c), a.width, t);
+    const int r = kEarly ? c : 0;
+    if constexpr (!kEarly) load4<float, kVec>(a.residual + at, quad(c), a.width, res[0]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[c][i] = a.branch ? t[i] + v[c][i] : t[i];
+    for (int i = 0; i < 4; ++i) v[c][i] = a.branch ? res[r][i] + v[c][i] : res[r][i];
     if (a.sum_out) store4<float, kVec>(a.sum_out + at, quad(c), a.width, v[c]);
   }
 
-  const float n = static_cast<float>(a.width);
   if (!a.rms) {
     float s = 0.f;
 #pragma unroll
@@ -171,14 +289,18 @@ __global__ __launch_bounds__(64 * (W == 1 ? 4 : W)) void norm8_kernel(Norm8Args 
 #pragma unroll
     for (int i = 0; i < 4; ++i) sq += v[c][i] * v[c][i];
   const float inv = 1.0f / sqrtf(row_sum(sq) / n + a.eps);
-  const int ld = static_cast<int>(padded8(a.width));
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    float g[4], b[4] = {0.f, 0.f, 0.f, 0.f};
-    load4<float, kVec>(a.gamma, quad(c), a.width, g);
-    if (a.beta) load4<float, kVec>(a.beta, quad(c), a.width, b);
+    const int p = kEarly ? c : 0;
+    if constexpr (!kEarly) {
+      load4<float, kVec>(a.gamma, quad(c), a.width, gamma[0]);
+      if (a.beta) load4<float, kVec>(a.beta, quad(c), a.width, beta[0]);
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[c][i] = quad(c) + i < a.width ? v[c][i] * inv * g[i] + b[i] : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const float y = v[c][i] * inv * gamma[p][i];
+      v[c][i] = quad(c) + i >= a.width ? 0.f : a.beta ? y + beta[p][i] : y;
+    }
     if (a.out32) store4<float, kVec>(a.out32 + at, quad(c), a.width, v[c]);
     store_codes(a.codes + static_cast<size_t>(row) * ld, a.scales + static_cast<size_t>(row) * (ld / kBlock8), quad(c), ld, v[c]);
   }
@@ -195,58 +317,66 @@ hipError_t for_type(DType t, F&& f) {
   }
 }
 
-constexpr long long kMaxGrid = 1 << 20;  // of the elementwise kernels; larger problems loop
-
 }  // namespace
 
 hipError_t launch_quantize8(const Quantize8Args& a, DType t, hipStream_t stream) {
   if (a.rows <= 0) return hipSuccess;
-  const long long quads = a.rows * (padded8(a.width) / 4);
-  const dim3 grid(static_cast<unsigned>(std::min((quads + 255) / 256, kMaxGrid)));
   return for_type(t, [&](auto v) {
     typedef decltype(v) T;
-    const bool vec = a.width % 4 == 0 && a.stride % 4 == 0 && aligned(a.x, 4 * sizeof(T));
-    if (vec) LAYA_LAUNCH((quantize8_kernel<T, true>), grid, dim3(256), 0, stream, a);
-    else LAYA_LAUNCH((quantize8_kernel<T, false>), grid, dim3(256), 0, stream, a);
+    const int per_row = static_cast<int>(padded8(a.width) / kPiece<T>), u = pieces_a_thread(a.rows * per_row);
+    const long long groups = (a.rows * per_row + 256 * u - 1) / (256 * u);
+    if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(groups));
+    const unsigned magic = piece_magic(per_row);
+    const bool vec = a.width % kPiece<T> == 0 && a.stride % kPiece<T> == 0 && aligned(a.x, 16);
+    if (vec && u == 4) LAYA_LAUNCH((quantize8_kernel<T, true, 4>), grid, dim3(256), 0, stream, a, magic);
+    else if (vec) LAYA_LAUNCH((quantize8_kernel<T, true, 1>), grid, dim3(256), 0, stream, a, magic);
+    else if (u == 4) LAYA_LAUNCH((quantize8_kernel<T, false, 4>), grid, dim3(256), 0, stream, a, magic);
+    else LAYA_LAUNCH((quantize8_kernel<T, false, 1>), grid, dim3(256), 0, stream, a, magic);
     return hipGetLastError();
   });
 }
 
 hipError_t launch_dequantize8(const Dequantize8Args& a, DType t, hipStream_t stream) {
   if (a.rows <= 0) return hipSuccess;
-  const long long quads = a.rows * ((a.width + 3) / 4);
-  const dim3 grid(static_cast<unsigned>(std::min((quads + 255) / 256, kMaxGrid)));
   return for_type(t, [&](auto v) {
     typedef decltype(v) T;
-    const bool vec = a.width % 4 == 0 && a.stride % 4 == 0 && aligned(a.out, 4 * sizeof(T));
-    if (vec) LAYA_LAUNCH((dequantize8_kernel<T, true>), grid, dim3(256), 0, stream, a);
-    else LAYA_LAUNCH((dequantize8_kernel<T, false>), grid, dim3(256), 0, stream, a);
+    const int per_row = static_cast<int>(padded8(a.width) / kPiece<T>), u = pieces_a_thread(a.rows * per_row);
+    const long long groups = (a.rows * per_row + 256 * u - 1) / (256 * u);
+    if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(groups));
+    const unsigned magic = piece_magic(per_row);
+    const bool vec = a.width % kPiece<T> == 0 && a.stride % kPiece<T> == 0 && aligned(a.out, 16);
+    if (vec && u == 4) LAYA_LAUNCH((dequantize8_kernel<T, true, 4>), grid, dim3(256), 0, stream, a, magic);
+    else if (vec) LAYA_LAUNCH((dequantize8_kernel<T, true, 1>), grid, dim3(256), 0, stream, a, magic);
+    else if (u == 4) LAYA_LAUNCH((dequantize8_kernel<T, false, 4>), grid, dim3(256), 0, stream, a, magic);
+    else LAYA_LAUNCH((dequantize8_kernel<T, false, 1>), grid, dim3(256), 0, stream, a, magic);
     return hipGetLastError();
   });
 }
 
 namespace {
 
-template <typename B, bool kVec>
+constexpr int kFewRows8 = 4096;
+
+template <typename B, bool kVec, int NS, bool kEarly>
 hipError_t launch_norm8_t(const Norm8Args& a, hipStream_t stream) {
   if (a.width <= 2048) {
-    const int wpb = a.rows <= 4096 ? 1 : 4;  // few rows: one-wave workgroups, spread over every CU
-    const dim3 grid((a.rows + wpb - 1) / wpb), block(64 * wpb);
-    switch ((a.width + 255) / 256) {
-#define LAYA_CASE(C) case C: LAYA_LAUNCH((norm8_kernel<B, C, 1, kVec>), grid, block, 0, stream, a); break;
-      LAYA_CASE(1) LAYA_CASE(2) LAYA_CASE(3) LAYA_CASE(4) LAYA_CASE(5) LAYA_CASE(6) LAYA_CASE(7) LAYA_CASE(8)
+    const int wpb = a.rows <= kFewRows8 ? 1 : 4;  // few rows: one-wave workgroups, spread over every CU
+    const dim3 grid((a.rows - 1) / wpb + 1), block(64 * wpb);
+    const int c = (a.width + 255) / 256;
+#define LAYA_CASE(C) \
+  if (c <= C) { LAYA_LAUNCH((norm8_kernel<B, C, 1, kVec, NS, kEarly>), grid, block, 0, stream, a); return hipGetLastError(); }
+    LAYA_CASE(1) LAYA_CASE(2) LAYA_CASE(3) LAYA_CASE(4) LAYA_CASE(5) LAYA_CASE(6) LAYA_CASE(8)
 #undef LAYA_CASE
-    }
-  } else {
-    const dim3 grid(a.rows), block(256);
-    switch ((a.width + 1023) / 1024) {
-#define LAYA_CASE(C) case C: LAYA_LAUNCH((norm8_kernel<B, C, 4, kVec>), grid, block, 0, stream, a); break;
-      LAYA_CASE(3) LAYA_CASE(4) LAYA_CASE(5) LAYA_CASE(6) LAYA_CASE(7) LAYA_CASE(8)
-#undef LAYA_CASE
-      default: return hipErrorInvalidValue;
-    }
   }
-  return hipGetLastError();
+  const dim3 grid(a.rows), block(256);
+  const int c = (a.width + 1023) / 1024;
+#define LAYA_CASE(C) \
+  if (c <= C) { LAYA_LAUNCH((norm8_kernel<B, C, 4, kVec, NS, kEarly>), grid, block, 0, stream, a); return hipGetLastError(); }
+  LAYA_CASE(3) LAYA_CASE(4) LAYA_CASE(6) LAYA_CASE(8)
+#undef LAYA_CASE
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
@@ -258,7 +388,15 @@ hipError_t launch_norm8(const Norm8Args& a, DType branch, hipStream_t stream) {
     const bool vec = a.width % 4 == 0 && aligned(a.residual, 16) && aligned(a.branch, 4 * sizeof(B)) &&
                      (a.splits <= 1 || a.part_stride % 4 == 0) && aligned(a.bias, 16) && aligned(a.gamma, 16) &&
                      aligned(a.beta, 16) && aligned(a.sum_out, 16) && aligned(a.out32, 16);
-    return vec ? launch_norm8_t<B, true>(a, stream) : launch_norm8_t<B, false>(a, stream);
+    const int splits = a.branch ? a.splits : 1;
+    if (!vec) return launch_norm8_t<B, false, -1, false>(a, stream);
+    const bool few = a.rows <= kFewRows8;
+    if (splits == 1) return few ? launch_norm8_t<B, true, 1, true>(a, stream) : launch_norm8_t<B, true, 1, false>(a, stream);
+    if constexpr (sizeof(B) == 4) {  // split-K partials are fp32, and of few rows
+      if (few && splits == 2) return launch_norm8_t<B, true, 2, true>(a, stream);
+      if (few && splits <= 4) return splits == 3 ? launch_norm8_t<B, true, 3, true>(a, stream) : launch_norm8_t<B, true, 4, true>(a, stream);
+    }
+    return launch_norm8_t<B, true, -1, false>(a, stream);
   });
 }
 
