@@ -173,8 +173,8 @@ __device__ __forceinline__ float gelu(float v) { return 0.5f * v * (1.0f + erff(
 // |GELU| = 1e-5, against 3.3e-7, 5.4e-8 and 1e-3 for the rational form below.  An exponential and ten
 // VALU operations where that takes a reciprocal more: the epilogue of a 65536 x 4096 GEMM runs this
 // 268M times (585 -> 551 us).
-__device__ __forceinline__ float gelu16(float x) {
-  const float ax = fabsf(x);
+// gelu16_tail: that q for ax = |x|.
+__device__ __forceinline__ float gelu16_tail(float ax) {
   float p = __builtin_fmaf(ax, 8.8822900e-07f, -1.4745427506568376e-05f);
   p = __builtin_fmaf(ax, p, 6.223141099326313e-05f);
   p = __builtin_fmaf(ax, p, 4.555389459710568e-04f);
@@ -183,7 +183,11 @@ __device__ __forceinline__ float gelu16(float x) {
   p = __builtin_fmaf(ax, p, 4.590853750705719e-01f);
   p = __builtin_fmaf(ax, p, 1.1511214971542358f);
   p = __builtin_fmaf(ax, p, 1.0f);
-  return __builtin_fmaf(-ax, __builtin_amdgcn_exp2f(-p), fmaxf(x, 0.f));
+  return __builtin_amdgcn_exp2f(-p);
+}
+__device__ __forceinline__ float gelu16(float x) {
+  const float ax = fabsf(x);
+  return __builtin_fmaf(-ax, gelu16_tail(ax), fmaxf(x, 0.f));
 }
 
 // The same function by a rational approximation: less exact and dearer, kept for the GeGLU epilogues because

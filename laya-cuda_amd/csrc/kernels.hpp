@@ -272,9 +272,7 @@ struct Linear8Args {
   bool wide;              // whole 16-column blocks: rows of out start on 16 of its bytes, bias and residual on whole quads
 };
 constexpr int kE4M3 = 3;
-int linear8_tile_count();
-// Whether tile `id` can make this output: 8-bit blocks and gate/value groups lie inside a tile's columns, and fp32
-// outputs take a tile with exact products.
+// Tiles and the planner's choice among them: linear8_plan.hpp.
 bool linear8_tile_valid(int id, const Linear8Args& a);
 int linear8_plan(const Linear8Args& a, int cus);
 hipError_t linear8_prepare();

@@ -10,6 +10,7 @@
 // owns BM x BN outputs, WM x WN waves of it times KG groups that split the slabs; S stages of SL slabs are in
 // flight.  The groups' fp32 tiles are added in group order through LDS, so results do not depend on timing.
 #include "kernels.hpp"
+#include "linear8_plan.hpp"
 #include "ring_walk.hpp"
 #include "rows8.hpp"
 #include "tiles.hpp"
@@ -52,13 +53,14 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, u
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
-// Activations.  NaNs stay NaNs and +infinity stays itself.  kFine: for fp32 outputs (libm); else accurate to
-// 3e-7 absolute, far inside a 16-bit rounding (see gelu16, whose argument is capped where its q has reached 0).
+// Activations.  NaNs stay NaNs (the maximum is IEEE 754-2019's) and +infinity stays itself.  kFine: for fp32
+// outputs (libm); else accurate to 3e-7 absolute, far inside a 16-bit rounding: gelu16 with its argument capped
+// where its tail has reached 0.
 template <bool kFine>
 __device__ __forceinline__ float gelu8(float x) {
   if constexpr (kFine) return 0.5f * x * (1.0f + erff(x * 0.7071067811865475f));
-  const float t = fminf(fabsf(x), 16.f);
-  return x != x ? x : gelu16(-t) + (x > 0.f ? x : 0.f);
+  const float ax = fminf(fabsf(x), 16.f);
+  return __builtin_fmaf(-ax, gelu16_tail(ax), __builtin_elementwise_maximum(x, 0.f));
 }
 template <bool kFine>
 __device__ __forceinline__ float silu8(float x) {
@@ -148,7 +150,7 @@ template <int BM, int BN, int SL> constexpr int stage_bytes8() {
 }
 template <int BM, int BN, int KG, int SL, int S> constexpr int lds8() {
   const int stages = S * stage_bytes8<BM, BN, SL>(), parts = KG * BM * (BN + 4) * 4;
-  return stages > parts ? stages : parts;
+  return (stages > parts ? stages : parts) + BN * 4;  // and the tile's bias
 }
 
 template <int BM, int BN, int WM, int WN, int KG, int SL, int S, bool kFast>
@@ -164,6 +166,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
   static_assert((S - 1) * NLD < 64 && lds8<BM, BN, KG, SL, S>() <= 160 * 1024, "vmcnt range and LDS of a CU");
   extern __shared__ __align__(16) unsigned char smem_raw[];
   float* const red = reinterpret_cast<float*>(smem_raw);  // [KG][BM][PITCH], after the main loop
+  float* const sbias = reinterpret_cast<float*>(smem_raw + lds8<BM, BN, KG, SL, S>() - BN * 4);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -206,6 +209,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
       }
     }
   };
+
+  static_assert(NT >= BN, "a thread per bias column");
+  const float early_bias = a.bias && tid < BN && n0 + tid < a.N ? a.bias[n0 + tid] : 0.f;
 
   const int kg = wave / (WM * WN), wm0 = (wave % (WM * WN)) / WN * WTM, wn0 = wave % WN * WTN;
   const int r16 = lane & 15, kq = lane >> 4;
@@ -298,6 +304,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
   }
   __syncthreads();  // the partial tiles reuse the stages
 
+  if (tid < BN) sbias[tid] = early_bias;
   float* const mine = red + kg * BM * PITCH;
 #pragma unroll
   for (int i = 0; i < MB; ++i)
@@ -306,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
       *reinterpret_cast<f32x4*>(mine + (wm0 + i * 16 + r16) * PITCH + wn0 + j * 16 + 4 * kq) = acc[i][j];
   __syncthreads();
 
-  // Four columns n .. n + 3 of tile row r: the groups' sum in group order, and the bias; zeros past N.
+  // Four columns n .. n + 3 of tile row r: the groups' sum in group order, and the bias (zeros past N).
   auto total4 = [&](int r, int n, float (&v)[4]) {
     f32x4 t = *reinterpret_cast<const f32x4*>(red + r * PITCH + n);
 #pragma unroll
@@ -315,42 +322,43 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[e] = t[e] + o[e];
     }
+    const f32x4 b = *reinterpret_cast<const f32x4*>(sbias + n);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = t[e];
-      if (a.bias && n0 + n + e < a.N) v[e] = v[e] + a.bias[n0 + n + e];
+    for (int e = 0; e < 4; ++e) v[e] = t[e] + b[e];
+  };
+  auto write = [&](auto glu_c, auto fine_c) {
+    constexpr bool kGlu = decltype(glu_c)::value, kFine = decltype(fine_c)::value;
+    constexpr int OC = kGlu ? BN / 2 : BN, Q = OC / 4;
+#pragma unroll 1
+    for (int c = tid; c < BM * Q; c += NT) {
+      const int r = c / Q, f = (c % Q) * 4, col = tx * OC + f;
+      if (m0 + r >= a.M || col >= span) continue;  // alike in the 8 lanes of a block
+      float v[4];
+      if constexpr (kGlu) {
+        float g[4];
+        const int n = (f / 16) * 32 + f % 16;
+        total4(r, n, g);
+        total4(r, n + 16, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (a.act == Act8::Geglu ? gelu8<kFine>(g[e]) : silu8<kFine>(g[e])) * v[e];
+      } else {
+        total4(r, f, v);
+        if (a.act == Act8::Gelu) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = gelu8<kFine>(v[e]);
+        } else if (a.act == Act8::Relu) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+        }
+      }
+      finish4(a, m0 + r, col, v);
     }
   };
   const bool fine = a.out_type == static_cast<int>(DType::F32);
-  const int quads = oc / 4;
-  for (int c = tid; c < BM * quads; c += NT) {
-    const int r = c / quads, f = (c % quads) * 4;
-    const long long row = m0 + r;
-    const int col = static_cast<int>(n0 / BN) * oc + f;
-    if (row >= a.M || col >= span) continue;  // alike in the 8 lanes of a block
-    float v[4];
-    if (glu) {
-      float g[4];
-      const int n = (f / 16) * 32 + f % 16;
-      total4(r, n, g);
-      total4(r, n + 16, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y = a.act == Act8::Geglu ? (fine ? gelu8<true>(g[e]) : gelu8<false>(g[e]))
-                                             : (fine ? silu8<true>(g[e]) : silu8<false>(g[e]));
-        v[e] = y * v[e];
-      }
-    } else {
-      total4(r, f, v);
-      if (a.act == Act8::Gelu) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fine ? gelu8<true>(v[e]) : gelu8<false>(v[e]);
-      } else if (a.act == Act8::Relu) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
-      }
-    }
-    finish4(a, row, col, v);
+  if (BN % 32 == 0 && glu) {
+    if constexpr (BN % 32 == 0) fine ? write(std::true_type(), std::true_type()) : write(std::true_type(), std::false_type());
+  } else {
+    fine ? write(std::false_type(), std::true_type()) : write(std::false_type(), std::false_type());
   }
 }
 
@@ -724,35 +732,11 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
 }
 
-// Tile menu: BM, BN, WM, WN, KG, SL, S, 8-bit matrix unit.
-#define LAYA_LINEAR8_TILES                  \
-  LAYA_T(0, 16, 16, 1, 1, 8, 8, 4, false)   \
-  LAYA_T(1, 16, 32, 1, 1, 8, 8, 3, false)   \
-  LAYA_T(2, 16, 64, 1, 2, 4, 4, 3, false)   \
-  LAYA_T(3, 32, 32, 1, 1, 8, 8, 2, false)   \
-  LAYA_T(4, 32, 64, 1, 2, 4, 4, 3, false)   \
-  LAYA_T(5, 64, 32, 2, 1, 4, 4, 3, false)   \
-  LAYA_T(6, 64, 64, 2, 2, 2, 2, 4, false)   \
-  LAYA_T(7, 64, 64, 2, 2, 4, 4, 2, false)   \
-  LAYA_T(8, 64, 128, 2, 4, 1, 1, 4, false)  \
-  LAYA_T(9, 128, 128, 2, 4, 1, 1, 4, false) \
-  LAYA_T(10, 64, 64, 2, 2, 2, 2, 4, true)   \
-  LAYA_T(11, 64, 128, 2, 4, 1, 1, 4, true)  \
-  LAYA_T(12, 128, 128, 2, 4, 1, 1, 4, true) \
-  LAYA_T(13, 128, 256, 2, 4, 1, 1, 3, true) \
-  LAYA_T(14, 64, 128, 2, 2, 2, 2, 3, false) \
-  LAYA_T(15, 32, 128, 1, 4, 2, 2, 3, false)
-
-struct Tile8 {
-  int bm, bn, lds, threads;
-  bool fast;
-};
-constexpr Tile8 kTiles8[] = {
-#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST) {BM, BN, lds8<BM, BN, KG, SL, S>(), 64 * WM * WN * KG, FAST},
+constexpr int kTileLds8[] = {
+#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST, OCC, L, B, C) lds8<BM, BN, KG, SL, S>(),
     LAYA_LINEAR8_TILES
 #undef LAYA_T
 };
-constexpr int kTiles8Count = sizeof(kTiles8) / sizeof(kTiles8[0]), kRing8 = kTiles8Count;
 
 typedef void (*RingKernel)(Linear8Args, RingWalk);
 RingKernel ring_kernel(Act8 act, bool out8) {
@@ -767,32 +751,27 @@ RingWalk walk_of(const Linear8Args& a) {
   const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = gated(a.act) ? 128 : 256;
   return ring_walk((span + oc - 1) / oc, (static_cast<long long>(a.M) + 255) / 256, a.M >= a.N);
 }
-constexpr Tile8 kRingTile8 = {256, 256, kRing8Lds, 512, true};
-
-int columns8(const Linear8Args& a, int bn) { return gated(a.act) ? bn / 2 : bn; }
+Problem8 problem_of(const Linear8Args& a) {
+  const bool out8 = a.out_type == kE4M3;
+  return Problem8{a.M, out8 ? padded8(a.cols) : a.cols, a.ld / 128, gated(a.act), out8,
+                  a.out_type == static_cast<int>(DType::F32), a.wide && walk_of(a).total > 0};
+}
 
 }  // namespace
 
-int linear8_tile_count() { return kTiles8Count + 1; }
+bool linear8_tile_valid(int id, const Linear8Args& a) { return tile8_valid(id, problem_of(a)); }
 
-bool linear8_tile_valid(int id, const Linear8Args& a) {
-  if (id == kRing8) return a.out_type != static_cast<int>(DType::F32) && a.ld >= 256 && a.wide && walk_of(a).total > 0;
-  // A block of 32 output codes, and a group of 16 gate and 16 value rows, lie inside one tile.
-  return id >= 0 && id < kTiles8Count && (a.out_type != kE4M3 || columns8(a, kTiles8[id].bn) % kBlock8 == 0) &&
-         (!gated(a.act) || kTiles8[id].bn % 32 == 0) && (a.out_type != static_cast<int>(DType::F32) || !kTiles8[id].fast);
-}
-
-int linear8_plan(const Linear8Args& a, int) { return a.M <= 64 ? 2 : 9; }
+int linear8_plan(const Linear8Args& a, int cus) { return linear8_plan(problem_of(a), cus); }
 
 hipError_t linear8_prepare() {
   hipError_t e = hipSuccess;
-#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST)                                                            \
-  if (e == hipSuccess)                                                                                   \
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>),   \
-                            hipFuncAttributeMaxDynamicSharedMemorySize, kTiles8[ID].lds);
+#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST, OCC, L, B, C)                                            \
+  if (e == hipSuccess)                                                                                       \
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>), \
+                            hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds8[ID]);
   LAYA_LINEAR8_TILES
 #undef LAYA_T
-  for (int act = 0; act < 5 && e == hipSuccess; ++act)
+  for (int act = 0; act < 5; ++act)
     for (bool out8 : {false, true})
       if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out8)),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
@@ -801,19 +780,25 @@ hipError_t linear8_prepare() {
 
 hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (a.M <= 0) return hipSuccess;
-  const Tile8& t = tile == kRing8 ? kRingTile8 : kTiles8[tile];
-  const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = columns8(a, t.bn);
-  const long long groups = (span + oc - 1) / oc * ((static_cast<long long>(a.M) + t.bm - 1) / t.bm);
-  if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(groups)), block(t.threads);
   if (tile == kRing8) {
     const RingWalk walk = walk_of(a);
-    LAYA_LAUNCH(ring_kernel(a.act, a.out_type == kE4M3), dim3(std::min(walk.total, 256)), block, t.lds, stream, a, walk);
+    LAYA_LAUNCH(ring_kernel(a.act, a.out_type == kE4M3), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
     return hipGetLastError();
   }
+  const long long span = problem_of(a).span;
+  auto grid = [&](int bm, int bn) {
+    const long long oc = gated(a.act) ? bn / 2 : bn;
+    return (span + oc - 1) / oc * ((static_cast<long long>(a.M) + bm - 1) / bm);
+  };
   switch (tile) {
-#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST) \
-  case ID: LAYA_LAUNCH((linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>), grid, block, t.lds, stream, a); break;
+#define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST, OCC, L, B, C)                                            \
+  case ID: {                                                                                                 \
+    const long long groups = grid(BM, BN);                                                                   \
+    if (groups > 0x7fffffffLL) return hipErrorInvalidValue;                                                  \
+    LAYA_LAUNCH((linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>), dim3(static_cast<unsigned>(groups)),      \
+                dim3(64 * WM * WN * KG), kTileLds8[ID], stream, a);                                          \
+    break;                                                                                                   \
+  }
     LAYA_LINEAR8_TILES
 #undef LAYA_T
     default: return hipErrorInvalidValue;
