@@ -372,7 +372,8 @@ constexpr int kBias8 = kScales8 + kScaleStages8 * kScaleStage8;  // two tiles' b
 constexpr int kRing8Lds = kBias8 + 2 * 1024;
 static_assert(kRing8Lds <= 160 * 1024, "LDS of a CU");
 
-// Four dwords a lane, v[j] of lane group kq: afterwards v[k] of lane group j holds what was v[j] of group k.
+// Exchanges between the four lane groups (lanes 16 q .. 16 q + 15).
+// v[j] of group q: afterwards v[k] of group j holds what was v[j] of group k.
 __device__ __forceinline__ void transpose4(unsigned (&v)[4]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -386,6 +387,14 @@ __device__ __forceinline__ void transpose4(unsigned (&v)[4]) {
     v[j] = r[0];
     v[j + 1] = r[1];
   }
+}
+// x and y of group q are chunks q of two runs of four: afterwards groups 0 and 1 hold x's chunks (0, 1) and (2, 3) in x and
+// y, groups 2 and 3 y's.
+__device__ __forceinline__ void pair_chunks(unsigned& x, unsigned& y) {
+  const auto a = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap(a[0], a[1], false, false);
+  x = b[0];
+  y = b[1];
 }
 // Maximum over the four lane groups.
 __device__ __forceinline__ unsigned group_max(unsigned m) {
@@ -646,6 +655,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     const int er = elane & 15, eq = elane >> 4;
     constexpr int STEPS = kGlu ? MB / 2 : MB;
     constexpr unsigned kNowhere = 0x80000000u;  // past every resource
+    constexpr int kStream = kE4m3 ? 2 : 0;
     const int col0 = (kGlu ? cur.n0 / 2 + wn * 32 : cur.n0 + wn * 64);
     const int rows = min(a.M - cur.m0, BM);
     const int pitch = kE4m3 ? span : a.cols * 2;  // bytes of an output row
@@ -683,9 +693,9 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
           if (block_row(t) < rows && block_col(t) < a.cols)
             add_quad(a.residual, a.residual_type, static_cast<size_t>(cur.m0 + block_row(t)) * a.cols + block_col(t) + 4 * eq, v[t]);
       }
-      // After the exchange a lane holds the 16 columns of block eq.
-      const int row = block_row(0) + (kGlu ? (eq >> 1) * 16 : 0), col = col0 + (kGlu ? eq & 1 : eq) * 16;
       if constexpr (kE4m3) {
+        // After the exchange a lane holds the 16 codes of block eq.
+        const int row = block_row(0) + (kGlu ? (eq >> 1) * 16 : 0), col = col0 + (kGlu ? eq & 1 : eq) * 16;
         unsigned s[2], q[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -701,21 +711,22 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
         }
         transpose4(q);
         const bool in = col < span;
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{q[0], q[1], q[2], q[3]}, dst, in ? row * pitch + col : kNowhere, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{q[0], q[1], q[2], q[3]}, dst, in ? row * pitch + col : kNowhere, 0, kStream);
         __builtin_amdgcn_raw_buffer_store_b8(static_cast<unsigned char>(eq & 2 ? s[1] : s[0]), dst_scales,
                                              in && !(eq & 1) ? row * (span / kBlock8) + col / kBlock8 : kNowhere, 0, 0);
       } else {
-        unsigned lo[4], hi[4];
+        // Two neighbouring blocks a store: after the exchange a lane holds 8 consecutive columns of the 32, and a row's
+        // four lanes 64 bytes.
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          lo[t] = pack16(a.out_type, v[t][0], v[t][1]);
-          hi[t] = pack16(a.out_type, v[t][2], v[t][3]);
+        for (int h = 0; h < 2; ++h) {
+          unsigned x[2] = {pack16(a.out_type, v[2 * h][0], v[2 * h][1]), pack16(a.out_type, v[2 * h][2], v[2 * h][3])};
+          unsigned y[2] = {pack16(a.out_type, v[2 * h + 1][0], v[2 * h + 1][1]), pack16(a.out_type, v[2 * h + 1][2], v[2 * h + 1][3])};
+          pair_chunks(x[0], y[0]);
+          pair_chunks(x[1], y[1]);
+          const int row = block_row(2 * h), col = block_col(2 * h) + eq * 8;
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], x[1], y[0], y[1]}, dst, col < a.cols ? row * pitch + col * 2 : kNowhere, 0,
+                                                 kStream);
         }
-        transpose4(lo);
-        transpose4(hi);
-        const unsigned to = col < a.cols ? row * pitch + col * 2 : kNowhere;
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[0], hi[0], lo[1], hi[1]}, dst, to, 0, 0);
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[2], hi[2], lo[3], hi[3]}, dst, to == kNowhere ? to : to + 16, 0, 0);
       }
     }
     if (!has_next) break;
