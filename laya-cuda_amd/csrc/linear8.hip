@@ -53,18 +53,14 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c, unsigned sa, u
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
-// Activations.  NaNs stay NaNs (the maximum is IEEE 754-2019's) and +infinity stays itself.  kFine: for fp32
-// outputs (libm); else accurate to 3e-7 absolute, far inside a 16-bit rounding: gelu16 with its argument capped
-// where its tail has reached 0.
-template <bool kFine>
+// Activations, accurate to 3e-7 absolute (gelu16 with its argument capped where its tail has reached 0; SiLU by the
+// hardware's exponential and reciprocal, a few units in the last place).  NaNs stay NaNs (the maximum is IEEE 754-2019's)
+// and +infinity stays itself.
 __device__ __forceinline__ float gelu8(float x) {
-  if constexpr (kFine) return 0.5f * x * (1.0f + erff(x * 0.7071067811865475f));
   const float ax = fminf(fabsf(x), 16.f);
   return __builtin_fmaf(-ax, gelu16_tail(ax), __builtin_elementwise_maximum(x, 0.f));
 }
-template <bool kFine>
 __device__ __forceinline__ float silu8(float x) {
-  if constexpr (kFine) return x / (1.0f + expf(-x));
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
@@ -326,8 +322,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = t[e] + b[e];
   };
-  auto write = [&](auto glu_c, auto fine_c) {
-    constexpr bool kGlu = decltype(glu_c)::value, kFine = decltype(fine_c)::value;
+  auto write = [&](auto glu_c) {
+    constexpr bool kGlu = decltype(glu_c)::value;
     constexpr int OC = kGlu ? BN / 2 : BN, Q = OC / 4;
 #pragma unroll 1
     for (int c = tid; c < BM * Q; c += NT) {
@@ -340,12 +336,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
         total4(r, n, g);
         total4(r, n + 16, v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (a.act == Act8::Geglu ? gelu8<kFine>(g[e]) : silu8<kFine>(g[e])) * v[e];
+        for (int e = 0; e < 4; ++e) v[e] = (a.act == Act8::Geglu ? gelu8(g[e]) : silu8(g[e])) * v[e];
       } else {
         total4(r, f, v);
         if (a.act == Act8::Gelu) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = gelu8<kFine>(v[e]);
+          for (int e = 0; e < 4; ++e) v[e] = gelu8(v[e]);
         } else if (a.act == Act8::Relu) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
@@ -354,12 +350,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
       finish4(a, m0 + r, col, v);
     }
   };
-  const bool fine = a.out_type == static_cast<int>(DType::F32);
-  if (BN % 32 == 0 && glu) {
-    if constexpr (BN % 32 == 0) fine ? write(std::true_type(), std::true_type()) : write(std::true_type(), std::false_type());
-  } else {
-    fine ? write(std::false_type(), std::true_type()) : write(std::false_type(), std::false_type());
+  if constexpr (BN % 32 == 0) {
+    if (glu) return write(std::true_type());
   }
+  write(std::false_type());
 }
 
 // ---- the batched product: a persistent ring of 256 x 256 tiles on the 8-bit matrix unit ----
@@ -416,10 +410,15 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 //
 // The epilogue needs no LDS: lane (r, kq) = (lane % 16, lane / 16) holds columns 4 kq .. +3 of row r of each 16 x 16
 // block, and four lane groups exchange packed dwords so that each stores 16 consecutive columns.
-template <Act8 A, bool kE4m3>
+//
+// fp32 outputs take the same walk and stream with exact products (kExact): a slab is two passes, one per 64-code half,
+// over the eight row blocks, with w's half widened for the pass and x's next row block widened between the MFMAs of
+// the present one.  Its MFMAs take twice as long, so a barrier frees all of x's units, another all of w's.
+enum class Out8 { Half, E4m3, F32 };
+template <Act8 A, Out8 O>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
-  constexpr bool kGlu = gated(A);
+  constexpr bool kGlu = gated(A), kE4m3 = O == Out8::E4m3, kExact = O == Out8::F32;
   constexpr int BM = 256, BN = 256, MB = 8, NB = 4;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 63;
@@ -535,15 +534,18 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   };
   issue_bias(0);
 
-  // The two groups of a slab's loads: those that go out before row 2 (scales, w, first half of x), and before row 6.
+  // The two groups of a slab's loads, and what each barrier leaves in flight beside the stores (below).
+  // Before row 2: scales, w and the first half of x; before row 6: the rest of x.  kExact: scales and w; x.
   auto issue_first = [&](int part, int s, int buf, int stage) {
-    if (part == 0) issue_scales(s, stage), issue(4, s, buf);
-    else if (part == 1) issue(5, s, buf), issue(0, s, buf);
-    else if (part == 2) issue(6, s, buf), issue(2, s, buf);
-    else issue(7, s, buf);
+    if (part == 0) issue_scales(s, stage);
+    issue(4 + part, s, buf);
+    if (!kExact && (part == 1 || part == 2)) issue(part == 1 ? 0 : 2, s, buf);
   };
-  constexpr int kFirst = 7, kSecond = 2;
-  auto issue_second = [&](int part, int s, int buf) { issue(part ? 3 : 1, s, buf); };
+  auto issue_second = [&](int part, int s, int buf) {
+    issue(kExact ? 2 * part : 2 * part + 1, s, buf);
+    if (kExact) issue(2 * part + 1, s, buf);
+  };
+  constexpr int kFirst = kExact ? 5 : 7, kSecond = 9 - kFirst;
 
   // Prologue: slabs 0 and 1.
   int buf = 0, stage = 0, half = 0;
@@ -556,8 +558,58 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   }
   publish_stage<waitcnt_vm(0)>();  // both slabs: the first tile's first slab waits as the later tiles' do
   auto next_stage = [](int s) { return s == kScaleStages8 - 1 ? 0 : s + 1; };
+
+  // kExact: a lane's half (h) of a 16-row block is 16 codes of block kq / 2 of the half, two bf16 operands of 8.
+  i32x4 cx[4], cw[NB], xa[2], xb[2];
+  bf16x8 ww[NB][2];
+  auto read_cx = [&](const Place& p, int h, int i) {
+    cx[i & 3] = *reinterpret_cast<const i32x4*>(smem_raw + (h ? p.hi : p.lo) + i * 2048);
+  };
+  auto read_cw = [&](const Place& p, int h, int j) {
+    cw[j] = *reinterpret_cast<const i32x4*>(smem_raw + (h ? p.hi : p.lo) + j * 2048);
+  };
+  auto half_scale = [&](unsigned s, int h) {
+    return __builtin_bit_cast(float, ((s >> (8 * (kq >> 1) + 16 * h)) & 255u) << 23);
+  };
+  auto widen_w = [&](int h, int j) {
+    const float f = half_scale(sw[j], h);
+    ww[j][0] = widen8(cw[j][0], cw[j][1], f);
+    ww[j][1] = widen8(cw[j][2], cw[j][3], f);
+  };
+  // Two of the 16 codes of x's row block i into xb.
+  auto widen_x = [&](float f, int i, int k) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const int c = cx[i & 3][k >> 1];
+    const bf16x2 v = k & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, f, false);
+    int d = __builtin_bit_cast(int, v);
+    asm volatile("" : "+v"(d));  // stays between the MFMAs
+    xb[k >> 2][k & 3] = d;
+  };
+  auto mma_exact = [&](int i, int j, int e) {
+    acc[i][j] = mfma16(ww[j][e], __builtin_bit_cast(bf16x8, xa[e]), acc[i][j]);
+    asm volatile("" : "+v"(acc[i][j]));
+  };
+
   // What rows 0 and 1 of a slab need.
   auto read_first = [&] {
+    if constexpr (kExact) {
+      read_scales(stage, 2 * wm, sx);
+      read_scales(stage, 2 * wm + 1, sx + 4);
+      read_scales(stage, 4 + wn, sw);
+      const Place px = place_x(buf), pw = place_w(buf);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) read_cw(pw, 0, j);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) read_cx(px, 0, i);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) widen_w(0, j);
+      const float f = half_scale(sx[0], 0);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) widen_x(f, 0, k);
+      xa[0] = xb[0];
+      xa[1] = xb[1];
+      return;
+    }
     read_scales(stage, 2 * wm, sx);
     read_scales(stage, 4 + wn, sw);
     const Place px = place_x(buf), pw = place_w(buf);
@@ -574,8 +626,8 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   // tile's first slab (kLate) the epilogue stores and the bias load, which come between the two tiles' loads.  Waiting
   // for the stores there cost 2-3 us a tile.  (No wait is chosen at run time: across the branch the compiler moved
   // the MFMAs behind the barrier.)
-  constexpr int kStores = kGlu ? MB : 2 * MB;
-  constexpr int kWait = kFirst + kSecond, kWaitLate = kWait + kStores + 1;
+  constexpr int kStores = (kGlu ? MB : 2 * MB) * (kExact ? 2 : 1);
+  constexpr int kWait = kExact ? kFirst : kFirst + kSecond, kWaitLate = kWait + kStores + 1;
   auto four = [&](int i) {
     pin();
 #pragma unroll
@@ -634,18 +686,89 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     stage = nstage;
   };
 
+  // kExact: a slab, its row blocks numbered t = 8 h + i.  Row block t + 1 is widened under t's MFMAs, t + 3 read; at
+  // the end of a pass w's next half is widened column by column as its registers come free.
+  auto exact_slab = [&](int to, auto late, auto next) {
+    constexpr bool kNext = decltype(next)::value;
+    constexpr int kVm = decltype(late)::value ? kWaitLate : kWait;
+    const int nstage = next_stage(stage), tostage = next_stage(nstage);
+    const Place px = place_x(buf), pw = place_w(buf);
+    Place qx = px;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      const int i = t & 7, u = t + 1;
+      if (t == 3) {  // w has been read
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0_keep_vm());
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        pin();
+      }
+      if (t == 13) {  // x has been read, and the next slab is there
+        publish_stage<waitcnt_vm(kVm)>();
+        pin();
+        if constexpr (kNext) {
+          qx = place_x(buf ^ 1);
+          const Place qw = place_w(buf ^ 1);
+          read_scales(nstage, 2 * wm, sx);
+          read_scales(nstage, 4 + wn, sw);
+#pragma unroll
+          for (int j = 0; j < NB; ++j) read_cw(qw, 0, j);
+        }
+      }
+      if (t >= 3 && t < 7) issue_first(t - 3, to, buf, tostage);
+      if (t == 13 || t == 14) issue_second(t - 13, to, buf);
+      if (t == 0) read_scales(stage, 2 * wm + 1, sx + 4);
+      if (t < 2) {
+        read_cw(pw, 1, 2 * t);
+        read_cw(pw, 1, 2 * t + 1);
+      }
+      if (t < 13) read_cx(px, (t + 3) >> 3, (t + 3) & 7);
+      else if (kNext) read_cx(qx, 0, t - 13);
+      pin();
+      const bool more = t < 15 || kNext;
+      const float f = more ? half_scale(sx[u & 7], (u >> 3) & 1) : 0.f;
+      if (i < 7) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          mma_exact(i, k & 3, k >> 2);
+          widen_x(f, u & 7, k);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          mma_exact(i, j, 0);
+          if (more) widen_x(f, u & 7, 2 * j);
+          mma_exact(i, j, 1);
+          if (more) widen_x(f, u & 7, 2 * j + 1);
+          if (more) widen_w((u >> 3) & 1, j);
+        }
+      }
+      pin();
+      xa[0] = xb[0];
+      xa[1] = xb[1];
+    }
+    buf ^= 1;
+    stage = nstage;
+  };
+
   for (;;) {
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    first_rows(2, std::true_type());
+    if constexpr (kExact) {
+      exact_slab(2, std::true_type(), std::true_type());
+      for (int it = 1; it < n - 1; ++it) exact_slab(it + 2, std::false_type(), std::true_type());
+      exact_slab(n + 1, std::false_type(), std::false_type());
+    } else {
+      first_rows(2, std::true_type());
     for (int it = 1; it < n; ++it) {
       last_rows(it + 1, std::true_type());
       first_rows(it + 2, std::false_type());
     }
     // The tile's last slab: the next tile's first fragments are read after the epilogue.
     last_rows(n + 1, std::false_type());
+    }
 
     // Epilogue, four 16 x 16 output blocks at a time: block t is a row block of the wave and its column block t
     // (gated: a pair of row blocks with two column blocks each).  Stores go through a resource over the tile's rows:
@@ -658,7 +781,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     constexpr int kStream = kE4m3 ? 2 : 0;
     const int col0 = (kGlu ? cur.n0 / 2 + wn * 32 : cur.n0 + wn * 64);
     const int rows = min(a.M - cur.m0, BM);
-    const int pitch = kE4m3 ? span : a.cols * 2;  // bytes of an output row
+    const int pitch = kE4m3 ? span : a.cols * (kExact ? 4 : 2);  // bytes of an output row
     const __amdgpu_buffer_rsrc_t dst = __builtin_amdgcn_make_buffer_rsrc(
         static_cast<uint8_t*>(a.out) + static_cast<size_t>(cur.m0) * pitch, 0, rows * pitch, 0x00020000);
     const __amdgpu_buffer_rsrc_t dst_scales = __builtin_amdgcn_make_buffer_rsrc(
@@ -678,10 +801,10 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
           if constexpr (kGlu) {
             const int i = 2 * step + (t >> 1), j = 2 * (t & 1);
             const float g = acc[i][j][e] + b[j][e], u = acc[i][j + 1][e] + b[j + 1][e];
-            v[t][e] = (A == Act8::Geglu ? gelu8<false>(g) : silu8<false>(g)) * u;
+            v[t][e] = (A == Act8::Geglu ? gelu8(g) : silu8(g)) * u;
           } else {
             const float x = acc[step][t][e] + b[t][e];
-            v[t][e] = A == Act8::Gelu ? gelu8<false>(x) : A == Act8::Relu && x < 0.f ? 0.f : x;
+            v[t][e] = A == Act8::Gelu ? gelu8(x) : A == Act8::Relu && x < 0.f ? 0.f : x;
           }
         }
       // Row in the tile and first column of block t.
@@ -693,7 +816,15 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
           if (block_row(t) < rows && block_col(t) < a.cols)
             add_quad(a.residual, a.residual_type, static_cast<size_t>(cur.m0 + block_row(t)) * a.cols + block_col(t) + 4 * eq, v[t]);
       }
-      if constexpr (kE4m3) {
+      if constexpr (kExact) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int col = block_col(t) + 4 * eq;
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(u32x4, f32x4{v[t][0], v[t][1], v[t][2], v[t][3]}), dst,
+              col < a.cols ? block_row(t) * pitch + col * 4 : kNowhere, 0, kStream);
+        }
+      } else if constexpr (kE4m3) {
         // After the exchange a lane holds the 16 codes of block eq.
         const int row = block_row(0) + (kGlu ? (eq >> 1) * 16 : 0), col = col0 + (kGlu ? eq & 1 : eq) * 16;
         unsigned s[2], q[4];
@@ -750,13 +881,21 @@ constexpr int kTileLds8[] = {
 };
 
 typedef void (*RingKernel)(Linear8Args, RingWalk);
-RingKernel ring_kernel(Act8 act, bool out8) {
+RingKernel ring_kernel(Act8 act, Out8 out) {
+  auto of = [out](auto act_c) -> RingKernel {
+    constexpr Act8 A = decltype(act_c)::value;
+    return out == Out8::Half ? linear8_ring_kernel<A, Out8::Half> : out == Out8::E4m3 ? linear8_ring_kernel<A, Out8::E4m3>
+                                                                                     : linear8_ring_kernel<A, Out8::F32>;
+  };
   switch (act) {
-#define LAYA_A(A) case Act8::A: return out8 ? linear8_ring_kernel<Act8::A, true> : linear8_ring_kernel<Act8::A, false>;
+#define LAYA_A(A) case Act8::A: return of(std::integral_constant<Act8, Act8::A>());
     LAYA_A(Gelu) LAYA_A(Relu) LAYA_A(Geglu) LAYA_A(Swiglu)
     default: LAYA_A(None)
 #undef LAYA_A
   }
+}
+Out8 out_of(const Linear8Args& a) {
+  return a.out_type == kE4M3 ? Out8::E4m3 : a.out_type == static_cast<int>(DType::F32) ? Out8::F32 : Out8::Half;
 }
 RingWalk walk_of(const Linear8Args& a) {
   const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = gated(a.act) ? 128 : 256;
@@ -783,8 +922,8 @@ hipError_t linear8_prepare() {
   LAYA_LINEAR8_TILES
 #undef LAYA_T
   for (int act = 0; act < 5; ++act)
-    for (bool out8 : {false, true})
-      if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out8)),
+    for (Out8 out : {Out8::Half, Out8::E4m3, Out8::F32})
+      if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out)),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
   return e;
 }
@@ -793,7 +932,7 @@ hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (a.M <= 0) return hipSuccess;
   if (tile == kRing8) {
     const RingWalk walk = walk_of(a);
-    LAYA_LAUNCH(ring_kernel(a.act, a.out_type == kE4M3), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
+    LAYA_LAUNCH(ring_kernel(a.act, out_of(a)), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
     return hipGetLastError();
   }
   const long long span = problem_of(a).span;

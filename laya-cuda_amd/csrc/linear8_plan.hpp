@@ -47,7 +47,7 @@ struct Problem8 {
 // Whether tile `id` can make this output: a block of 32 output codes and a group of 16 gate and 16 value rows lie
 // inside one tile, and fp32 outputs are made from exact products.
 constexpr bool tile8_valid(int id, const Problem8& p) {
-  if (id == kRing8) return p.ring && !p.fine && p.slabs >= 2;
+  if (id == kRing8) return p.ring && p.slabs >= 2;
   if (id < 0 || id >= kLinear8Tiles) return false;
   const Tile8Cost& t = kTile8Costs[id];
   return !(p.fine && t.fast) && !(p.gated && t.bn % 32) && !(p.out8 && (p.gated ? t.bn / 2 : t.bn) % 32);
@@ -68,7 +68,8 @@ constexpr int linear8_plan(const Problem8& p, int cus) {
       // Its first round depends on how many CUs fetch and store at once.
       const float full = tiles < cus ? static_cast<float>(tiles) / static_cast<float>(cus) : 1.f;
       const long long rounds = (tiles + cus - 1) / cus;
-      time = 6.6f + 5.5f * full + n * (1.34f + 0.36f * full) + static_cast<float>(rounds - 1) * (5.4f + 1.7f * n);
+      time = p.fine ? 12.4f + full + n * (2.56f + 0.5f * full) + static_cast<float>(rounds - 1) * (15.3f + 3.27f * n)
+                    : 6.6f + 5.5f * full + n * (1.34f + 0.36f * full) + static_cast<float>(rounds - 1) * (5.4f + 1.7f * n);
     } else {
       const Tile8Cost& t = kTile8Costs[id];
       const long long round = static_cast<long long>(cus) * t.occ, rounds = (tiles + round - 1) / round;
