@@ -84,11 +84,19 @@ __device__ __forceinline__ void lds_load16(const void* g, unsigned lds) {
 // vector instructions (integer division of uniform values), and folds away where it already is one.
 // A vector-memory instruction may read an SGPR that a vector instruction wrote (readfirstlane; the readlane of a
 // spilled one) only five wait states later, which the hardware does not check and, for a load inside inline
-// assembly, the compiler does not either: s_nop 4 is those five.
+// assembly, the compiler does not either.  kVectorOffset: soffset may be such a one, and goes through a scalar copy,
+// a read that the hardware does check.  (Everywhere, the copies cost the 24-layer batch 1.3%, and five wait
+// states 1.5%.)  The resource's words have to be older.
+template <bool kVectorOffset = false>
 __device__ __forceinline__ void lds_load16_buffer(i32x4 rsrc, unsigned voffset, unsigned soffset, unsigned lds) {
   soffset = __builtin_amdgcn_readfirstlane(soffset);
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset),
-               "{m0}"(lds));
+  if constexpr (kVectorOffset) {
+    unsigned copy;
+    asm volatile("s_mov_b32 %0, %3\n\tbuffer_load_dwordx4 %1, %2, %0 offen lds" : "=&s"(copy) : "v"(voffset), "s"(rsrc), "s"(soffset),
+                 "{m0}"(lds));
+  } else {
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds));
+  }
 }
 // 128-bit buffer resource of `bytes` bytes at `base` (raw buffer: stride 0, byte offsets), wave-uniform.
 __device__ __forceinline__ i32x4 buffer_resource(const void* base, unsigned bytes) {

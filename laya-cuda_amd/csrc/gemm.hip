@@ -585,7 +585,8 @@ void gemm_pipe_kernel(GemmArgs a) {
   if constexpr (!M16) load_early_pos<TM, E>(a, m0 + wm0 + (lane & 31), early_pos);
   const unsigned lds_base = lds_address(smem_raw);
   auto issue_at = [&](int q, int kt, int base) {  // base: element offset of the load's LDS destination
-    lds_load16_buffer(q < AG ? rsA : rsB, src[q], static_cast<unsigned>(kt) * BKS * 2,
+    // fp32 outputs: kt starts at a split's first slab, a quotient that may have been made by vector instructions.
+    lds_load16_buffer<E == Epi::F32>(q < AG ? rsA : rsB, src[q], static_cast<unsigned>(kt) * BKS * 2,
                       lds_base + static_cast<unsigned>(base + dst[q]) * 2);
   };
   auto issue = [&](int q, int kt, int st) { issue_at(q, kt, st * SLAB); };

@@ -89,7 +89,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void gemm_burst_kernel(GemmArgs 
     for (int q = 0; q < NLD; ++q) {
       const int g = min(wave + NW * q, GROUPS - 1), rg = g % RG, slab = g / RG;
       const unsigned k = static_cast<unsigned>(kb + min(stage * SL + slab, n - 1)) * 128u;
-      lds_load16_buffer(rg * 8 < BM ? rsA : rsB, src[q], k, lds_base + static_cast<unsigned>(buf * STAGE + g * 1024));
+      // Where a slab's groups are no power of two, g / RG, and with it k, is made by vector instructions.
+      lds_load16_buffer<(RG & (RG - 1)) != 0>(rg * 8 < BM ? rsA : rsB, src[q], k, lds_base + static_cast<unsigned>(buf * STAGE + g * 1024));
     }
   };
 

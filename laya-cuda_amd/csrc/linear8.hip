@@ -22,8 +22,14 @@ namespace laya {
 
 namespace {
 
-// lds_load16_buffer's form for 4 bytes a lane: lane l's dword goes to LDS byte address lds + 4 l.
-__device__ __forceinline__ void lds_load4_buffer(i32x4 rsrc, unsigned voffset, unsigned soffset, unsigned lds) {
+// Direct loads as lds_load16_buffer, 16 bytes and 4 bytes a lane (lane l's go to LDS byte address lds + 16 l or 4 l), for
+// resources that vector instructions may just have written (readfirstlane, the readlane of a spilled one): s_nop 4
+// is the five wait states that such an SGPR needs before a vector-memory instruction reads it.
+__device__ __forceinline__ void load_lds16(i32x4 rsrc, unsigned voffset, unsigned soffset, unsigned lds) {
+  soffset = __builtin_amdgcn_readfirstlane(soffset);
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds));
+}
+__device__ __forceinline__ void load_lds4(i32x4 rsrc, unsigned voffset, unsigned soffset, unsigned lds) {
   soffset = __builtin_amdgcn_readfirstlane(soffset);
   asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(lds));
 }
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
         const unsigned k = static_cast<unsigned>(min(stage * SL + g / RG, n - 1)) * 128u;
         const bool isx = rg * 8 < BM;  // a scalar offset has to stay inside its resource: 0 where w has no rows
         const unsigned row = static_cast<unsigned>(isx ? r : r - BM);
-        lds_load16_buffer(isx ? rsX : rsW, row * static_cast<unsigned>(a.ld) + (((lane & 7) ^ ((r >> 1) & 7)) << 4),
+        load_lds16(isx ? rsX : rsW, row * static_cast<unsigned>(a.ld) + (((lane & 7) ^ ((r >> 1) & 7)) << 4),
                           isx || live ? k : 0u,
                           base + static_cast<unsigned>(g * 1024));
       } else {
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void linear8_kernel(Linear8Args 
         const unsigned k = static_cast<unsigned>(min(stage * SL + (g - SL * RG) / SG, n - 1)) * 4u;
         const bool isx = sg * 64 < SX;
         const unsigned row = static_cast<unsigned>(isx ? r : r - SX);
-        lds_load4_buffer(isx ? rsXs : rsWs, row * static_cast<unsigned>(sld), isx || live ? k : 0u,
+        load_lds4(isx ? rsXs : rsWs, row * static_cast<unsigned>(sld), isx || live ? k : 0u,
                          base + static_cast<unsigned>(CODES + (g - SL * RG) * 256));
       }
     }
@@ -474,13 +480,13 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   auto issue = [&](int u, int s, int buf) {
     const bool next = s >= n && has_next;
     const int kt = (u < 4 || (next ? nxt.live : cur.live)) ? (next ? s - n : min(s, n - 1)) : 0;
-    lds_load16_buffer(u < 4 ? (next ? nxt.x : cur.x) : (next ? nxt.w : cur.w), src[u & 3], static_cast<unsigned>(kt) * 128u,
+    load_lds16(u < 4 ? (next ? nxt.x : cur.x) : (next ? nxt.w : cur.w), src[u & 3], static_cast<unsigned>(kt) * 128u,
                       lds_base + static_cast<unsigned>(buf * kSlab8 + u * kUnit8 + wave * 1024));
   };
   auto issue_scales = [&](int s, int stage) {
     const bool next = s >= n && has_next;
     const int kt = (wave < 4 || (next ? nxt.live : cur.live)) ? (next ? s - n : min(s, n - 1)) : 0;
-    lds_load4_buffer(next ? nxt.s : cur.s, src_scale, static_cast<unsigned>(kt) * 4u,
+    load_lds4(next ? nxt.s : cur.s, src_scale, static_cast<unsigned>(kt) * 4u,
                      lds_base + static_cast<unsigned>(kScales8 + stage * kScaleStage8 + wave * 256));
   };
 
@@ -529,7 +535,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   // The tile's bias, zeros past N, into its half of the bias area (every wave loads 64 columns, twice over).
   auto issue_bias = [&](int half) {
     const int nr = a.bias ? max(min(a.N - cur.n0, BN), 0) : 0;
-    lds_load4_buffer(buffer_resource(a.bias + (nr ? cur.n0 : 0), nr * 4), static_cast<unsigned>((wave & 3) * 256 + lane * 4), 0,
+    load_lds4(buffer_resource(a.bias + (nr ? cur.n0 : 0), nr * 4), static_cast<unsigned>((wave & 3) * 256 + lane * 4), 0,
                      lds_base + static_cast<unsigned>(kBias8 + half * 1024 + (wave & 3) * 256));
   };
   issue_bias(0);
