@@ -539,6 +539,9 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
                      lds_base + static_cast<unsigned>(kBias8 + half * 1024 + (wave & 3) * 256));
   };
   issue_bias(0);
+  // Of the two waves of a SIMD the second goes first where both could: apart, one's MFMAs cover the other's reads (up to
+  // 2% of a batched product, 4% of a one-round one).
+  if (wm) __builtin_amdgcn_s_setprio(1);
 
   // The two groups of a slab's loads, and what each barrier leaves in flight beside the stores (below).
   // Before row 2: scales, w and the first half of x; before row 6: the rest of x.  kExact: scales and w; x.

@@ -357,6 +357,70 @@ def test_linear_epilogues(gpu, act, out, rtype):
                    residual=rng.normal(0, 1, (M, cols)).astype(np.float32) if rtype else None, rtype=rtype or "f32")
 
 
+@pytest.mark.parametrize("M,N,K", [(4200, 4352, 256), (4333, 4416, 384), (65, 66048, 640)])
+@pytest.mark.parametrize("out,act,rtype", [("bf16", "none", "bf16"), ("f16", "gelu", ""), ("e4m3", "relu", ""), ("f32", "none", "f32"),
+                                           ("f32", "swiglu", ""), ("e4m3", "geglu", ""), ("bf16", "swiglu", "f32")])
+def test_linear_more_tiles_than_compute_units(gpu, M, N, K, out, act, rtype):
+    """The tile with the highest number (the persistent one) walks several tiles a workgroup: every output against 64 bits."""
+    t, lib = torch(), _lib.load()
+    gen = t.Generator(device=gpu).manual_seed(M)
+    normal = lambda *s: t.randn(*s, device=gpu, generator=gen)  # noqa: E731
+
+    def rows8(n, k, std):
+        held = Rows8(gpu, n, k)
+        v = normal(n, k) * std
+        check(lib.laya_op_quantize8(p(v), _lib.F32, k, p(held.codes), p(held.scales), n, k, stream()))
+        back = t.empty(n, k, device=gpu)
+        check(lib.laya_op_dequantize8(p(held.codes), p(held.scales), p(back), _lib.F32, k, n, k, stream()))
+        return held, back.double()
+
+    (x, xv), (w, wv) = rows8(M, K, 1.0), rows8(N, K, K ** -.5)
+    gated = act in ("geglu", "swiglu")
+    cols = N // 2 if gated else N
+    bias = normal(N) * .5
+    res = normal(M, cols).to(dtype(rtype)) if rtype else None
+    o = Rows8(gpu, M, cols) if out == "e4m3" else t.full((M + 1, cols), 9.0, dtype=dtype(out), device=gpu)
+    args = (p(x.codes), p(x.scales), p(w.codes), p(w.scales), p(bias), p(res), CODE[rtype or "f32"],
+            *((p(o.codes), p(o.scales)) if out == "e4m3" else (p(o), None)), CODE[out], ACT[act], M, N, K)
+    for tile in range(63, -1, -1):
+        if lib.laya_op_linear8(*args, tile, stream()) == _lib.OK:
+            break
+    assert tile > 0
+    wt = wv.t().contiguous()
+    v = xv @ wt + bias.double()
+    # As the small cases': (steps + 6) 2 u of the magnitudes, and 2^-11 of the products' root sum of squares on the 8-bit unit.
+    tol = (R.width8(K) // 32 + 6) * 2 * U * (xv.abs() @ wt.abs() + bias.abs().double())
+    if out != "f32":
+        tol += 2.0 ** -11 * ((xv ** 2) @ (wt ** 2)).sqrt()
+    gelu = lambda g: g * t.special.ndtr(g)  # noqa: E731
+    if gated:
+        g, e = v.view(M, -1, 2, 16), tol.view(M, -1, 2, 16)
+        a = gelu(g[:, :, 0]) if act == "geglu" else g[:, :, 0] * t.sigmoid(g[:, :, 0])
+        want = (a * g[:, :, 1]).reshape(M, -1)
+        tol = (1.13 * e[:, :, 0] * g[:, :, 1].abs() + e[:, :, 1] * (g[:, :, 0].abs() + e[:, :, 0]) + 1e-6 * g[:, :, 1].abs()).reshape(M, -1)
+        tol += 4 * U * want.abs()
+    else:
+        want = gelu(v) if act == "gelu" else v.clamp(min=0) if act == "relu" else v
+        if act != "none":
+            tol = 1.13 * tol + 1e-6
+    if res is not None:
+        want = want + res.double()
+        tol += U * want.abs()
+    if out == "e4m3":
+        assert (o.codes[-1] == GUARD).all() and (o.scales[-1] == GUARD).all()
+        back = t.empty(M, cols, device=gpu)
+        check(lib.laya_op_dequantize8(p(o.codes), p(o.scales), p(back), _lib.F32, cols, M, cols, stream()))
+        pad = R.width8(cols) - cols
+        assert not pad or not o.codes[:-1, cols:].any()
+        top = t.nn.functional.pad(want.abs(), (0, pad)).view(M, -1, 32).amax(-1).repeat_interleave(32, 1)[:, :cols]
+        got, tol = back.double(), tol + 2.0 ** -4 * (want.abs() + tol) + 2.0 ** -10 * (top + tol.max()) / 224
+    else:
+        assert (o[M:] == 9).all()
+        got, tol = o[:M].double(), tol + HALF[out] * (want.abs() + tol)
+    off = (got - want).abs() - tol
+    assert (off <= 0).all(), f"{int((off > 0).sum())} beyond, worst by {float(off.max())}"
+
+
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N", [(7, 64), (7, 67), (400, 640)])
 def test_linear_onto_its_own_residual(gpu, out, M, N):
