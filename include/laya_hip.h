@@ -271,14 +271,15 @@ int laya_op_head_gather(const float* src, const int32_t* src_rows, const int32_t
  * A matrix of `rows` x `width` values in 8-bit rows is two device arrays, rows back to back:
  *   codes  [rows][laya_width8(width)]       e4m3 (OCP, no infinities), 16-byte aligned
  *   scales [rows][laya_width8(width) / 32]  uint8, 4-byte aligned
- * laya_width8 rounds the width up to a multiple of 128; the codes past the width are zeros.  Code i of a row
- * stands for e4m3(code) * 2^(scale[i / 32] - 127).  A writer takes the smallest scale with which the block's largest
+ * laya_width8 rounds the width up to a multiple of 128; the codes past the width are zeros (NaN codes where
+ * a block, or for laya_op_linear8 a row, holds a NaN).  Code i of a row stands for e4m3(code) * 2^(scale[i / 32] - 127).  A writer takes the smallest scale with which the block's largest
  * magnitude is at most 448 (2^-127 at the least; 0 for a block of zeros) and rounds each value once, to nearest
  * with ties to even.  A block that holds a NaN or an infinity gets the scale 255 and reads back as NaNs.
  *
  * Every operator runs on the current device, which owns the pointers and the stream; it makes no allocation, no
  * host synchronisation and keeps nothing between calls, so calls may be captured, replayed and run side by side.
- * Zero rows are a call that does nothing.  Bad sizes, types, missing or misaligned pointers: LAYA_EINVAL.
+ * An output overlaps no input and no other output unless its operator says so.  Zero rows are a call that does
+ * nothing.  Bad sizes, types, missing or misaligned pointers: LAYA_EINVAL.
  * ------------------------------------------------------------------------------------------ */
 
 enum { LAYA_LAYER_NORM = 0, LAYA_RMS_NORM = 1 };
@@ -289,7 +290,7 @@ int laya_width8(int width);
 
 /* 8-bit rows of x (LAYA_F32/F16/BF16), whose rows of `width` values start `stride` elements apart (stride >=
  * width): weights once at load, or activations.  x needs its own element's alignment only; rows that start
- * on whole quads (4 elements) are read fastest. */
+ * and end on whole 16 bytes are read fastest.  At most 2^36 codes, from values that span at most 2^50 elements. */
 int laya_op_quantize8(const void* x, int dtype, int64_t stride, void* codes, void* scales, int64_t rows, int width,
                       void* stream);
 
@@ -304,7 +305,8 @@ int laya_op_dequantize8(const void* codes, const void* scales, void* out, int dt
  *   kind LAYA_RMS_NORM    y = v / sqrt(mean(v^2) + eps) * gamma + beta
  * in fp32, out32 = y, and codes, scales = the 8-bit rows of y.  branch (partials part_stride elements apart) is of
  * branch_dtype LAYA_F32/F16/BF16, or NULL (v = residual; bias must be NULL).  beta, bias, sum_out and
- * out32 may be NULL; either one of sum_out and out32 may be residual itself.  1 <= width <= 8192. */
+ * out32 may be NULL; either one of sum_out and out32 may be residual itself.  1 <= width <= 8192; fewer than 2^26 rows,
+ * 2^24 of widths above 2048. */
 int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, int splits, int64_t part_stride,
                   const float* bias, const float* gamma, const float* beta, float eps, int kind, float* sum_out,
                   float* out32, void* codes, void* scales, int rows, int width, void* stream);
@@ -316,7 +318,10 @@ int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, i
  * (act(gate) * value; N a multiple of 32).  GELU is the exact-erf one, SWIGLU's gate x / (1 + exp(-x)).  The residual
  * is added in fp32 before the one rounding; it may be out itself when both have the same type, and
  * nothing else may overlap out.
- * Sums are fp32.  tile -1 lets the planner choose; others name a tile (0 .. ), refused where it cannot make the output. */
+ * Sums are fp32.  fp32 outputs are made from exact products (of values of at least 2^-126, smaller ones count as
+ * zero); the others may be summed by the 8-bit matrix unit, whose additions were off by up to 6e-5 of the root of the
+ * products' sum of squares, under half a bf16 or fp16 step of results of that size.  Activations are
+ * accurate to 1e-6.  tile -1 lets the planner choose; others name a tile (0 .. ), refused where it cannot make the output. */
 int laya_op_linear8(const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias,
                     const void* residual, int residual_dtype, void* out, void* out_scales, int out_dtype,
                     int activation, int M, int N, int K, int tile, void* stream);

@@ -415,7 +415,7 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // slab for most loads) the loads' latency bounded the loop.
 //
 // The epilogue needs no LDS: lane (r, kq) = (lane % 16, lane / 16) holds columns 4 kq .. +3 of row r of each 16 x 16
-// block, and four lane groups exchange packed dwords so that each stores 16 consecutive columns.
+// block, and the four lane groups exchange packed dwords so that each stores 16 bytes of consecutive columns.
 //
 // fp32 outputs take the same walk and stream with exact products (kExact): a slab is two passes, one per 64-code half,
 // over the eight row blocks, with w's half widened for the pass and x's next row block widened between the MFMAs of
@@ -771,12 +771,12 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
       exact_slab(n + 1, std::false_type(), std::false_type());
     } else {
       first_rows(2, std::true_type());
-    for (int it = 1; it < n; ++it) {
-      last_rows(it + 1, std::true_type());
-      first_rows(it + 2, std::false_type());
-    }
-    // The tile's last slab: the next tile's first fragments are read after the epilogue.
-    last_rows(n + 1, std::false_type());
+      for (int it = 1; it < n; ++it) {
+        last_rows(it + 1, std::true_type());
+        first_rows(it + 2, std::false_type());
+      }
+      // The tile's last slab: the next tile's first fragments are read after the epilogue.
+      last_rows(n + 1, std::false_type());
     }
 
     // Epilogue, four 16 x 16 output blocks at a time: block t is a row block of the wave and its column block t
@@ -787,7 +787,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     const int er = elane & 15, eq = elane >> 4;
     constexpr int STEPS = kGlu ? MB / 2 : MB;
     constexpr unsigned kNowhere = 0x80000000u;  // past every resource
-    constexpr int kStream = kE4m3 ? 2 : 0;
+    constexpr int kStream = kE4m3 ? 2 : 0;  // 8-bit codes past the caches (nontemporal); other types lost by it
     const int col0 = (kGlu ? cur.n0 / 2 + wn * 32 : cur.n0 + wn * 64);
     const int rows = min(a.M - cur.m0, BM);
     const int pitch = kE4m3 ? span : a.cols * (kExact ? 4 : 2);  // bytes of an output row
@@ -908,7 +908,7 @@ Out8 out_of(const Linear8Args& a) {
 }
 RingWalk walk_of(const Linear8Args& a) {
   const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = gated(a.act) ? 128 : 256;
-  return ring_walk((span + oc - 1) / oc, (static_cast<long long>(a.M) + 255) / 256, a.M >= a.N);
+  return ring_walk((span + oc - 1) / oc, (static_cast<long long>(a.M) + 255) / 256);
 }
 Problem8 problem_of(const Linear8Args& a) {
   const bool out8 = a.out_type == kE4M3;
@@ -947,17 +947,14 @@ hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   const long long span = problem_of(a).span;
   auto grid = [&](int bm, int bn) {
     const long long oc = gated(a.act) ? bn / 2 : bn;
-    return (span + oc - 1) / oc * ((static_cast<long long>(a.M) + bm - 1) / bm);
+    return dim3(static_cast<unsigned>((span + oc - 1) / oc * ((static_cast<long long>(a.M) + bm - 1) / bm)));
   };
   switch (tile) {
 #define LAYA_T(ID, BM, BN, WM, WN, KG, SL, S, FAST, OCC, L, B, C)                                            \
-  case ID: {                                                                                                 \
-    const long long groups = grid(BM, BN);                                                                   \
-    if (groups > 0x7fffffffLL) return hipErrorInvalidValue;                                                  \
-    LAYA_LAUNCH((linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>), dim3(static_cast<unsigned>(groups)),      \
-                dim3(64 * WM * WN * KG), kTileLds8[ID], stream, a);                                          \
-    break;                                                                                                   \
-  }
+  case ID:                                                                                                   \
+    LAYA_LAUNCH((linear8_kernel<BM, BN, WM, WN, KG, SL, S, FAST>), grid(BM, BN), dim3(64 * WM * WN * KG),    \
+                kTileLds8[ID], stream, a);                                                                   \
+    break;
     LAYA_LINEAR8_TILES
 #undef LAYA_T
     default: return hipErrorInvalidValue;

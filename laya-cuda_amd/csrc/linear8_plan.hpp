@@ -44,13 +44,20 @@ struct Problem8 {
   bool gated, out8, fine, ring;  // 8-bit and fp32 outputs; `ring`: the ring kernel takes this call
 };
 
+// Workgroups of BM x BN tiles.
+constexpr long long tiles8(const Problem8& p, long long bm, long long bn) {
+  const long long oc = p.gated ? bn / 2 : bn;
+  return (p.span + oc - 1) / oc * ((p.rows + bm - 1) / bm);
+}
+
 // Whether tile `id` can make this output: a block of 32 output codes and a group of 16 gate and 16 value rows lie
-// inside one tile, and fp32 outputs are made from exact products.
+// inside one tile, fp32 outputs are made from exact products, and a launch has fewer than 2^32 threads.
 constexpr bool tile8_valid(int id, const Problem8& p) {
   if (id == kRing8) return p.ring && p.slabs >= 2;
   if (id < 0 || id >= kLinear8Tiles) return false;
   const Tile8Cost& t = kTile8Costs[id];
-  return !(p.fine && t.fast) && !(p.gated && t.bn % 32) && !(p.out8 && (p.gated ? t.bn / 2 : t.bn) % 32);
+  return !(p.fine && t.fast) && !(p.gated && t.bn % 32) && !(p.out8 && (p.gated ? t.bn / 2 : t.bn) % 32) &&
+         tiles8(p, t.bm, t.bn) < (1LL << 32) / 512;
 }
 
 // The valid tile with the least estimated time on `cus` compute units.
@@ -60,8 +67,7 @@ constexpr int linear8_plan(const Problem8& p, int cus) {
   for (int id = 0; id <= kLinear8Tiles; ++id) {
     if (!tile8_valid(id, p)) continue;
     const bool ring = id == kRing8;
-    const long long bm = ring ? 256 : kTile8Costs[id].bm, bn = ring ? 256 : kTile8Costs[id].bn, oc = p.gated ? bn / 2 : bn;
-    const long long tiles = (p.span + oc - 1) / oc * ((p.rows + bm - 1) / bm);
+    const long long tiles = ring ? tiles8(p, 256, 256) : tiles8(p, kTile8Costs[id].bm, kTile8Costs[id].bn);
     const float n = static_cast<float>(p.slabs);
     float time = 0.f;
     if (ring) {

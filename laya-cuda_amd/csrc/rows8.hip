@@ -191,15 +191,17 @@ __global__ __launch_bounds__(256) void dequantize8_kernel(Dequantize8Args a, uns
 // LayerNorm, y = v / sqrt(mean of v^2 + eps) * gamma for the root-mean-square norm; v goes to sum_out, y to out32 and,
 // rounded, to 8-bit rows.  W waves own a row and keep it in registers, C quads a lane: quad c of a lane holds
 // elements 256 W c + 256 wave + 4 lane .. +3, so a wave's loads are contiguous and 8 lanes are one block.
-// The variance is the centred one, in a second pass over the registers.
+// The variance is the centred one, in a second pass over the registers.  A workgroup is one row: four rows a workgroup
+// took up to 7% longer.
 // NS: the branch's partials when they are known at launch, so that they, the residual and the parameters are loaded
-// before the first addition (one memory round trip); -1: any number, in a loop.
-template <typename B, int C, int W, bool kVec, int NS, bool kEarly>
-__global__ __launch_bounds__(64 * (W == 1 ? 4 : W)) void norm8_kernel(Norm8Args a) {
+// before the first addition (one memory round trip); -1: any number, in a loop, and the rest where it is used.  An fp32
+// residual of 512 x 1,024 with a bf16 branch: 4.1 us early, 5.0 late; 65,536 x 1,024: 127 and 132.
+template <typename B, int C, int W, bool kVec, int NS>
+__global__ __launch_bounds__(64 * W) void norm8_kernel(Norm8Args a) {
+  constexpr bool kEarly = NS > 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = W == 1 ? blockIdx.x * (blockDim.x >> 6) + wave : blockIdx.x;
-  if (row >= a.rows) return;
-  const int first = (W == 1 ? 0 : wave * 256) + lane * 4;
+  const int row = blockIdx.x;
+  const int first = wave * 256 + lane * 4;
   auto quad = [&](int c) { return first + c * 256 * W; };
   __shared__ float part[W];
   auto row_sum = [&](float v) {
@@ -328,7 +330,6 @@ hipError_t launch_quantize8(const Quantize8Args& a, DType t, hipStream_t stream)
     typedef decltype(v) T;
     const int per_row = static_cast<int>(padded8(a.width) / kPiece<T>), u = pieces_a_thread(a.rows * per_row);
     const long long groups = (a.rows * per_row + 256 * u - 1) / (256 * u);
-    if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(groups));
     const unsigned magic = piece_magic(per_row);
     const bool vec = a.width % kPiece<T> == 0 && a.stride % kPiece<T> == 0 && aligned(a.x, 16);
@@ -346,7 +347,6 @@ hipError_t launch_dequantize8(const Dequantize8Args& a, DType t, hipStream_t str
     typedef decltype(v) T;
     const int per_row = static_cast<int>(padded8(a.width) / kPiece<T>), u = pieces_a_thread(a.rows * per_row);
     const long long groups = (a.rows * per_row + 256 * u - 1) / (256 * u);
-    if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(groups));
     const unsigned magic = piece_magic(per_row);
     const bool vec = a.width % kPiece<T> == 0 && a.stride % kPiece<T> == 0 && aligned(a.out, 16);
@@ -360,24 +360,13 @@ hipError_t launch_dequantize8(const Dequantize8Args& a, DType t, hipStream_t str
 
 namespace {
 
-constexpr int kFewRows8 = 4096;
-
-template <typename B, bool kVec, int NS, bool kEarly>
+template <typename B, bool kVec, int NS>
 hipError_t launch_norm8_t(const Norm8Args& a, hipStream_t stream) {
-  if (a.width <= 2048) {
-    const int wpb = a.rows <= kFewRows8 ? 1 : 4;  // few rows: one-wave workgroups, spread over every CU
-    const dim3 grid((a.rows - 1) / wpb + 1), block(64 * wpb);
-    const int c = (a.width + 255) / 256;
-#define LAYA_CASE(C) \
-  if (c <= C) { LAYA_LAUNCH((norm8_kernel<B, C, 1, kVec, NS, kEarly>), grid, block, 0, stream, a); return hipGetLastError(); }
-    LAYA_CASE(1) LAYA_CASE(2) LAYA_CASE(3) LAYA_CASE(4) LAYA_CASE(5) LAYA_CASE(6) LAYA_CASE(8)
-#undef LAYA_CASE
-  }
-  const dim3 grid(a.rows), block(256);
-  const int c = (a.width + 1023) / 1024;
-#define LAYA_CASE(C) \
-  if (c <= C) { LAYA_LAUNCH((norm8_kernel<B, C, 4, kVec, NS, kEarly>), grid, block, 0, stream, a); return hipGetLastError(); }
-  LAYA_CASE(3) LAYA_CASE(4) LAYA_CASE(6) LAYA_CASE(8)
+  const dim3 grid(a.rows);
+#define LAYA_CASE(C, W) \
+  if (a.width <= 256 * W * C) { LAYA_LAUNCH((norm8_kernel<B, C, W, kVec, NS>), grid, dim3(64 * W), 0, stream, a); return hipGetLastError(); }
+  LAYA_CASE(1, 1) LAYA_CASE(2, 1) LAYA_CASE(3, 1) LAYA_CASE(4, 1) LAYA_CASE(5, 1) LAYA_CASE(6, 1) LAYA_CASE(8, 1)
+  LAYA_CASE(3, 4) LAYA_CASE(4, 4) LAYA_CASE(6, 4) LAYA_CASE(8, 4)
 #undef LAYA_CASE
   return hipErrorInvalidValue;
 }
@@ -392,14 +381,17 @@ hipError_t launch_norm8(const Norm8Args& a, DType branch, hipStream_t stream) {
                      (a.splits <= 1 || a.part_stride % 4 == 0) && aligned(a.bias, 16) && aligned(a.gamma, 16) &&
                      aligned(a.beta, 16) && aligned(a.sum_out, 16) && aligned(a.out32, 16);
     const int splits = a.branch ? a.splits : 1;
-    if (!vec) return launch_norm8_t<B, false, -1, false>(a, stream);
-    const bool few = a.rows <= kFewRows8;
-    if (splits == 1) return few ? launch_norm8_t<B, true, 1, true>(a, stream) : launch_norm8_t<B, true, 1, false>(a, stream);
-    if constexpr (sizeof(B) == 4) {  // split-K partials are fp32, and of few rows
-      if (few && splits == 2) return launch_norm8_t<B, true, 2, true>(a, stream);
-      if (few && splits <= 4) return splits == 3 ? launch_norm8_t<B, true, 3, true>(a, stream) : launch_norm8_t<B, true, 4, true>(a, stream);
+    if (!vec) return launch_norm8_t<B, false, -1>(a, stream);
+    // Eight quads a lane of everything are registers that many rows' waves miss, unless fp32 partials keep HBM busy
+    // anyhow: 8,192 x 8,192 with a bf16 branch 177 us early, 154 late (fp32: 199 and 209), 512 rows 11.4 and 12.9.
+    const bool early = a.width <= 6144 || sizeof(B) == 4 || a.rows <= 512;
+    if (early && splits == 1) return launch_norm8_t<B, true, 1>(a, stream);
+    if constexpr (sizeof(B) == 4) {  // split-K partials are fp32: 16,384 x 2,048 with four 152 us, in the loop 160
+      if (early && splits == 2) return launch_norm8_t<B, true, 2>(a, stream);
+      if (early && splits == 3) return launch_norm8_t<B, true, 3>(a, stream);
+      if (early && splits == 4) return launch_norm8_t<B, true, 4>(a, stream);
     }
-    return launch_norm8_t<B, true, -1, false>(a, stream);
+    return launch_norm8_t<B, true, -1>(a, stream);
   });
 }
 

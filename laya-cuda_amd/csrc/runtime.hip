@@ -1501,12 +1501,21 @@ static size_t type_size(int dtype) { return dtype == LAYA_F32 ? 4 : 2; }
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 constexpr int kMaxWidth8 = 1 << 30;
 constexpr int kMaxLinear8 = 1 << 20;  // a tile's rows then span fewer than 2^32 bytes
+// Codes of a matrix, and elements from its first value to its last row's: a launch then has fewer than 2^32 threads, and
+// offsets fit 64 bits.
+constexpr int64_t kMaxCodes8 = (1LL << 36) - 1, kMaxSpan8 = 1LL << 50;
 
 // The checks that every 8-bit operand shares.
 static void require_rows8(const void* codes, const void* scales, const char* what) {
   LAYA_REQUIRE(codes && scales, std::string(what) + ": codes and scales are required");
   LAYA_REQUIRE(aligned_to(codes, 16) && aligned_to(scales, 4),
                std::string(what) + ": codes must be 16-byte and scales 4-byte aligned");
+}
+
+static void require_extent8(int64_t rows, int width, int64_t stride) {
+  LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxWidth8 && stride >= width, "bad rows, width or stride");
+  LAYA_REQUIRE(rows <= kMaxCodes8 / padded8(width) && (rows == 0 || stride <= kMaxSpan8 / rows),
+               "rows: at most 2^36 codes, from values that span at most 2^50 elements");
 }
 
 int laya_width8(int width) {
@@ -1517,7 +1526,7 @@ int laya_op_quantize8(const void* x, int dtype, int64_t stride, void* codes, voi
                       void* stream) {
   return guarded(nullptr, [&] {
     LAYA_REQUIRE(float_type(dtype), "dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
-    LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxWidth8 && stride >= width, "bad rows, width or stride");
+    require_extent8(rows, width, stride);
     if (rows == 0) return;
     require_rows8(codes, scales, "output");
     LAYA_REQUIRE(x && aligned_to(x, type_size(dtype)), "x must be aligned to its elements");
@@ -1530,7 +1539,7 @@ int laya_op_dequantize8(const void* codes, const void* scales, void* out, int dt
                         int width, void* stream) {
   return guarded(nullptr, [&] {
     LAYA_REQUIRE(float_type(dtype), "dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
-    LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxWidth8 && stride >= width, "bad rows, width or stride");
+    require_extent8(rows, width, stride);
     if (rows == 0) return;
     require_rows8(codes, scales, "input");
     LAYA_REQUIRE(out && aligned_to(out, type_size(dtype)), "out must be aligned to its elements");
@@ -1545,6 +1554,7 @@ int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, i
   return guarded(nullptr, [&] {
     LAYA_REQUIRE(kind == LAYA_LAYER_NORM || kind == LAYA_RMS_NORM, "kind must be LAYA_LAYER_NORM or LAYA_RMS_NORM");
     LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxNorm8Width, "rows must not be negative and width 1 to 8192");
+    LAYA_REQUIRE(rows < (width <= 2048 ? 1 << 26 : 1 << 24), "rows: fewer than 2^26, 2^24 of widths above 2048");
     LAYA_REQUIRE(eps >= 0.f, "eps must not be negative");
     LAYA_REQUIRE(!branch || float_type(branch_dtype), "branch_dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
     LAYA_REQUIRE(!branch || (splits >= 1 && (splits == 1 || part_stride >= static_cast<int64_t>(rows) * width)),

@@ -17,6 +17,9 @@ int main() {
           ++chosen[id];
           ++checked;
         }
+  // 2^30 rows: 2^26 of the smallest tiles, more workgroups than a launch takes, and 2^23 of the largest.
+  const Problem8 many{1LL << 30, 16, 1, false, false, true, false}, fewer{(1LL << 30) - 128, 16, 1, false, false, true, false};
+  if (tile8_valid(0, many) || linear8_plan(many, 256) != -1 || linear8_plan(fewer, 256) < 11) return std::fprintf(stderr, "2^30 rows\n"), 1;
   for (int id = 0; id <= kRing8; ++id)
     if (!chosen[id]) return std::fprintf(stderr, "tile %d is never chosen\n", id), 1;
   std::printf("checked %lld\n", checked);

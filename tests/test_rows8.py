@@ -145,3 +145,16 @@ def test_nothing_is_wrapped_in_ctypes_structures():
     """The new operators add no structure: the binding's ABI version stays."""
     assert _lib.load().laya_abi_version() == _lib.ABI_VERSION == 2
     assert _lib.SIGNATURES["laya_op_linear8"][1] is ct.c_int
+
+
+def test_extents_past_a_launch_are_refused():
+    """Codes and spans that no launch covers, and offsets that would not fit 64 bits."""
+    refused("laya_op_quantize8", P, _lib.F32, 1, P, P, 1 << 29, 1, None, match="2^36 codes")
+    refused("laya_op_quantize8", P, _lib.F32, 1 << 62, P, P, 2, 100, None, match="2^50 elements")
+    refused("laya_op_quantize8", P, _lib.F32, 100, P, P, (1 << 63) - 1, 100, None, match="2^36 codes")
+    refused("laya_op_dequantize8", P, P, P, _lib.F32, 1 << 62, 2, 100, None, match="2^50 elements")
+    refused("laya_op_dequantize8", P, P, P, _lib.F32, 1 << 20, 1 << 17, 1 << 20, None, match="2^36 codes")
+    norm = dict(residual=P, branch=None, branch_dtype=0, splits=1, part_stride=0, bias=None, gamma=P, beta=None, eps=1e-5,
+                kind=_lib.RMS_NORM, sum_out=None, out32=None, codes=P, scales=P, rows=1 << 26, width=4, stream=None)
+    refused("laya_op_norm8", *norm.values(), match="fewer than 2^26")
+    refused("laya_op_norm8", *{**norm, "rows": 1 << 24, "width": 2052}.values(), match="fewer than 2^26")
