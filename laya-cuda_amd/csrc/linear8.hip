@@ -126,13 +126,7 @@ __device__ __forceinline__ unsigned pack16(int type, float x, float y) {
 __device__ __forceinline__ void finish4(const Linear8Args& a, long long row, int n, float (&v)[4]) {
   if (a.residual) add_residual4(a, row, n, v);
   if (a.out_type == kE4M3) {
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned m = magnitude(v[i]);
-      top = top > m ? top : m;
-    }
-    const unsigned s = scale8(block_top8(top));
+    const unsigned s = scale8(block_top8(magnitude(largest(largest(0.f, v[0], v[1]), v[2], v[3]))));
     const size_t ld = static_cast<size_t>(padded8(a.cols));
     *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.out) + row * ld + n) = encode8(v[0], v[1], v[2], v[3], s);
     if (n % kBlock8 == 0) a.out_scales[row * (ld / kBlock8) + n / kBlock8] = static_cast<uint8_t>(s);
@@ -839,13 +833,10 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
         unsigned s[2], q[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          unsigned top = 0;
+          float top = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const unsigned m = magnitude(v[2 * h + (e >> 2)][e & 3]);
-            top = top > m ? top : m;
-          }
-          s[h] = scale8(group_max(top));
+          for (int e = 0; e < 8; e += 2) top = largest(top, v[2 * h + (e >> 2)][e & 3], v[2 * h + (e >> 2)][(e & 3) + 1]);
+          s[h] = scale8(group_max(magnitude(top)));
           q[2 * h] = encode8(v[2 * h][0], v[2 * h][1], v[2 * h][2], v[2 * h][3], s[h]);
           q[2 * h + 1] = encode8(v[2 * h + 1][0], v[2 * h + 1][1], v[2 * h + 1][2], v[2 * h + 1][3], s[h]);
         }

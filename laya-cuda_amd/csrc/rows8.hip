@@ -55,13 +55,7 @@ __device__ __forceinline__ void store4(T* row, int idx, int width, const float (
 
 // Writes the codes of quad `idx` (of ld codes a row) and, from a block's first lane, its scale byte.
 __device__ __forceinline__ void store_codes(uint8_t* codes, uint8_t* scales, int idx, int ld, const float (&v)[4]) {
-  unsigned top = magnitude(v[0]);
-#pragma unroll
-  for (int i = 1; i < 4; ++i) {
-    const unsigned m = magnitude(v[i]);
-    top = top > m ? top : m;
-  }
-  const unsigned s = scale8(block_top8(top));
+  const unsigned s = scale8(block_top8(magnitude(largest(largest(0.f, v[0], v[1]), v[2], v[3]))));
   if (idx < ld) {
     *reinterpret_cast<unsigned*>(codes + idx) = encode8(v[0], v[1], v[2], v[3], s);
     if ((idx & (kBlock8 - 1)) == 0) scales[idx / kBlock8] = static_cast<uint8_t>(s);
@@ -119,12 +113,10 @@ __global__ __launch_bounds__(256) void quantize8_kernel(Quantize8Args a, unsigne
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (first + u * 256 + threadIdx.x >= total) return;  // rows are whole blocks: alike in a block's lanes
-    unsigned top = 0;
+    float widest = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const unsigned m = magnitude(v[u][i]);
-      top = top > m ? top : m;
-    }
+    for (int i = 0; i < E; i += 2) widest = largest(widest, v[u][i], v[u][i + 1]);
+    unsigned top = magnitude(widest);
 #pragma unroll
     for (int d = 1; d < kBlock8 / E; d <<= 1) {
       const unsigned m = __shfl_xor(top, d, kWave);

@@ -20,8 +20,12 @@ constexpr int kPad8 = 128;       // codes per row are a multiple of this
 constexpr unsigned kInf = 0x7f800000u;
 __host__ __device__ constexpr long long padded8(long long width) { return (width + kPad8 - 1) / kPad8 * kPad8; }
 
-// Magnitude bits: as unsigned integers they order like the magnitudes, with NaNs above infinity (fmaxf drops NaNs).
+// Magnitude bits: as unsigned integers they order like the magnitudes, with NaNs above infinity.
 __device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+// The largest of top (>= 0 or NaN), |a| and |b|: one v_maximum3_f32, which keeps NaNs (fmaxf drops them).
+__device__ __forceinline__ float largest(float top, float a, float b) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(a)), __builtin_fabsf(b));
+}
 
 // Scale byte of a block whose largest magnitude has the bits `top`.  448 is 1.75 * 2^8: adding 0x1fffff carries
 // into the exponent exactly where the significand is above 1.75.
@@ -30,19 +34,20 @@ __device__ __forceinline__ unsigned scale8(unsigned top) {
   const int s = static_cast<int>((top + 0x1fffffu) >> 23) - 8;
   return s < 0 ? 0u : static_cast<unsigned>(s);
 }
-// What the block's values are multiplied by before they are rounded to codes: 2^(127 - s), exact (s <= 247).
-__device__ __forceinline__ float inverse_scale8(unsigned s) { return __builtin_bit_cast(float, (254u - s) << 23); }
 // 2^(s - 127); NaN for s = 255.
 __device__ __forceinline__ float scale_value8(unsigned s) {
   return __builtin_bit_cast(float, s == 0 ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23);
 }
 
-// Four values of a block of scale byte s as four codes, each rounded once (to nearest, ties to even).
+// Four values of a block of scale byte s as four codes, each rounded once (to nearest, ties to even): the conversion
+// divides by its scale operand's power of two (exponent 0 is 2^-127).  With it and the maximum of three above, a
+// product of 65,536 x 4,096 x 1,024 into 8-bit rows takes 287 instead of 293 us, and with GELU 386 instead of 398.
 __device__ __forceinline__ unsigned encode8(float a, float b, float c, float d, unsigned s) {
-  if (s == 255u) return 0x7f7f7f7fu;
-  const float m = inverse_scale8(s);
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a * m, b * m, 0, false);
-  return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(c * m, d * m, r, true));
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  const float scale = __builtin_bit_cast(float, s << 23);
+  i16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, a, b, scale, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+  return s == 255u ? 0x7f7f7f7fu : __builtin_bit_cast(unsigned, r);
 }
 
 // Largest magnitude bits over the 8 lanes of a 32-value block (4 values a lane, lanes 8 j .. 8 j + 7).
