@@ -1,9 +1,13 @@
 // Matrix product of 8-bit rows: out = act(x w^T + bias) + residual, x [M][K] and w [N][K] in the form of rows8.hpp.
 //
-// linear8_kernel keeps every product exact: a code times its scale is a bf16 value (4 significant bits), so the codes
-// are widened in registers, with their scales, by v_cvt_scalef32_pk_bf16_fp8 and multiplied by v_mfma_f32_16x16x32_bf16,
-// whose sums are fp32 (measured: 8e-8 of the result's norm at K = 4,096).  It moves half the bytes of the 16-bit
-// product, which is what few rows are bound by.
+// Exact products: a code times its scale is a bf16 value (4 significant bits), so the codes are widened in
+// registers, with their scales, by v_cvt_scalef32_pk_bf16_fp8 and multiplied by v_mfma_f32_16x16x32_bf16, whose sums
+// are fp32 (measured: 8e-8 of the result's norm at K = 4,096).  It moves half the bytes of the 16-bit product, which is
+// what few rows are bound by (1 x 4,096 x 1,024 4.9 us, 96 x 2,304 x 768 6.2, both a launch and one or two memory round
+// trips; 512 x 1,024 x 4,096 with fp32 output 14.8, operand stream and widening).
+// The 8-bit unit (kFast): v_mfma_scale_f32_16x16x128_f8f6f4 takes codes and scales as they are, at twice the rate, but its
+// own additions drop bits: 1.4e-5 of the root of the products' sum of squares, at most 6e-5, however a sum is cut.
+// That is below the rounding of 16- and 8-bit outputs, which may take it; fp32 outputs do not.
 //
 // Layout: whole 128-code slabs go straight from global memory into LDS, 16-byte chunk c of row r at position
 // c ^ (r / 2) % 8, so that 16 lanes reading one chunk of 16 consecutive rows touch all banks once.  A workgroup
@@ -414,6 +418,11 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // fp32 outputs take the same walk and stream with exact products (kExact): a slab is two passes, one per 64-code half,
 // over the eight row blocks, with w's half widened for the pass and x's next row block widened between the MFMAs of
 // the present one.  Its MFMAs take twice as long, so a barrier frees all of x's units, another all of w's.
+//
+// Measured: 65,536 x 1,024 x 4,096 into bf16 305-320 us (1.72-1.8 PFLOP/s), into fp32 with an fp32 residual 499 (1.10); 65,536
+// x 4,096 x 1,024 into bf16 320-335, into 8-bit rows 287, with GELU 371-386.  MFMAs alone take 145 us, operand loads alone
+// 202 (K = 4,096) and 109 (K = 1,024); a row of MFMAs under which loads go out takes 1.5 to 1.9 times as long, and the
+// epilogue 8,200 clocks a tile, 17,400 with GELU into 8-bit rows.
 enum class Out8 { Half, E4m3, F32 };
 template <Act8 A, Out8 O>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
