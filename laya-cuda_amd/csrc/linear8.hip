@@ -78,20 +78,10 @@ __host__ __device__ constexpr bool gated(Act8 act) { return act == Act8::Geglu |
 
 template <typename T> struct Vec { typedef T type __attribute__((ext_vector_type(4))); };
 
-// Whole quad `at` of a tensor of `type`, added to v.
+// Whole quad `at` of a tensor.
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::type quad_at(const void* p, size_t at) {
   return *reinterpret_cast<const typename Vec<T>::type*>(static_cast<const T*>(p) + at);
-}
-__device__ __forceinline__ void add_quad(const void* p, int type, size_t at, float (&v)[4]) {
-  auto add = [&](auto zero) {
-    const auto t = quad_at<decltype(zero)>(p, at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] + static_cast<float>(t[i]);
-  };
-  if (type == static_cast<int>(DType::F32)) add(0.f);
-  else if (type == static_cast<int>(DType::F16)) add(f16());
-  else add(bf16());
 }
 // Residual columns n .. n + 3 of U places, zeros past the columns; every load goes out before the first is used.
 template <int U>
@@ -468,12 +458,12 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // over the eight row blocks, with w's half widened for the pass and x's next row block widened between the MFMAs of
 // the present one.  Its MFMAs take twice as long, so a barrier frees all of x's units, another all of w's.
 //
-// Measured: 65,536 x 1,024 x 4,096 into bf16 305-320 us (1.72-1.8 PFLOP/s), into fp32 with an fp32 residual 499 (1.10); 65,536
-// x 4,096 x 1,024 into bf16 320-335, into 8-bit rows 287, with GELU 371-386.  MFMAs alone take 145 us, operand loads alone
+// Measured: 65,536 x 1,024 x 4,096 into bf16 270-320 us by the card's clock (2.0-1.7 PFLOP/s), into fp32 460, with an fp32
+// residual 500-545; 65,536 x 4,096 x 1,024 into bf16 305-335, into 8-bit rows 287, with GELU 343-386.  MFMAs alone take 145 us, operand loads alone
 // 202 (K = 4,096) and 109 (K = 1,024); a row of MFMAs under which loads go out takes 1.5 to 1.9 times as long, and the
 // epilogue 8,200 clocks a tile, 17,400 with GELU into 8-bit rows.
 enum class Out8 { Half, E4m3, F32 };
-template <Act8 A, Out8 O>
+template <Act8 A, Out8 O, bool kResidual>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   constexpr bool kGlu = gated(A), kE4m3 = O == Out8::E4m3, kExact = O == Out8::F32;
@@ -849,12 +839,60 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
         kE4m3 ? a.out_scales + static_cast<size_t>(cur.m0) * (span / kBlock8) : nullptr, 0, kE4m3 ? rows * (span / kBlock8) : 0,
         0x00020000);
     const float* const bias = reinterpret_cast<const float*>(smem_raw + kBias8 + half * 1024) + wn * 64 + 4 * eq;
+    // Row in the tile and first column of block t of a step.
+    auto row_of = [&](int step, int t) { return wm * 128 + (kGlu ? 2 * step + (t >> 1) : step) * 16 + er; };
+    auto block_col = [&](int t) { return col0 + (kGlu ? t & 1 : t) * 16; };
+    // The residual's quads of a step, as they lie in memory (16-bit ones in the low half): all four loads go out before the
+    // first is used (bf16 to bf16, 15,088 x 1,024 x 1,024 32.4 -> 28.3 us against one at a time, 65,536 x 1,024 x 4,096 307 -> 295;
+    // fp32 551 -> 545, where the tile ends of all CUs meet at HBM).  A step ahead they spilled.
+    const int rsize = a.residual_type == static_cast<int>(DType::F32) ? 4 : 2;
+    auto fetch_residual = [&](int step, u32x4 (&to)[4]) {
+      pin();
+      const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(static_cast<const uint8_t*>(a.residual)) + static_cast<size_t>(cur.m0) * a.cols * rsize, 0,
+          rows * a.cols * rsize, 0x00020000);
+      unsigned at[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int col = block_col(t) + 4 * eq;
+        at[t] = col < a.cols ? static_cast<unsigned>((row_of(step, t) * a.cols + col) * rsize) : kNowhere;
+      }
+      if (rsize == 4) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) to[t] = __builtin_amdgcn_raw_buffer_load_b128(src, at[t], 0, 0);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const auto q = __builtin_amdgcn_raw_buffer_load_b64(src, at[t], 0, 0);
+          to[t][0] = q[0];
+          to[t][1] = q[1];
+        }
+      }
+    };
+    auto add_residual = [&](const u32x4 (&from)[4], float (&v)[4][4]) {
+      auto add = [&](auto zero) {
+        typedef typename Vec<decltype(zero)>::type Q;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          Q q;
+          __builtin_memcpy(&q, &from[t], sizeof(Q));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[t][e] = v[t][e] + static_cast<float>(q[e]);
+        }
+      };
+      if (rsize == 4) add(0.f);
+      else if (a.residual_type == static_cast<int>(DType::F16)) add(f16());
+      else add(bf16());
+    };
+
     f32x4 b[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) b[j] = *reinterpret_cast<const f32x4*>(bias + 16 * j);
 #pragma unroll
     for (int step = 0; step < STEPS; ++step) {
       float v[4][4];
+      u32x4 raw[4];
+      if constexpr (kResidual) fetch_residual(step, raw);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -868,15 +906,8 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
             v[t][e] = A == Act8::Gelu ? gelu8(x) : A == Act8::Relu && x < 0.f ? 0.f : x;
           }
         }
-      // Row in the tile and first column of block t.
-      auto block_row = [&](int t) { return wm * 128 + (kGlu ? 2 * step + (t >> 1) : step) * 16 + er; };
-      auto block_col = [&](int t) { return col0 + (kGlu ? t & 1 : t) * 16; };
-      if (a.residual) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (block_row(t) < rows && block_col(t) < a.cols)
-            add_quad(a.residual, a.residual_type, static_cast<size_t>(cur.m0 + block_row(t)) * a.cols + block_col(t) + 4 * eq, v[t]);
-      }
+      auto block_row = [&](int t) { return row_of(step, t); };
+      if constexpr (kResidual) add_residual(raw, v);
       if constexpr (kExact) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -939,11 +970,16 @@ constexpr int kTileLds8[] = {
 };
 
 typedef void (*RingKernel)(Linear8Args, RingWalk);
-RingKernel ring_kernel(Act8 act, Out8 out) {
-  auto of = [out](auto act_c) -> RingKernel {
+RingKernel ring_kernel(Act8 act, Out8 out, bool residual) {
+  auto with = [residual](auto act_c, auto out_c) -> RingKernel {
     constexpr Act8 A = decltype(act_c)::value;
-    return out == Out8::Half ? linear8_ring_kernel<A, Out8::Half> : out == Out8::E4m3 ? linear8_ring_kernel<A, Out8::E4m3>
-                                                                                     : linear8_ring_kernel<A, Out8::F32>;
+    constexpr Out8 O = decltype(out_c)::value;
+    return residual ? linear8_ring_kernel<A, O, true> : linear8_ring_kernel<A, O, false>;
+  };
+  auto of = [&](auto act_c) -> RingKernel {
+    return out == Out8::Half   ? with(act_c, std::integral_constant<Out8, Out8::Half>())
+           : out == Out8::E4m3 ? with(act_c, std::integral_constant<Out8, Out8::E4m3>())
+                               : with(act_c, std::integral_constant<Out8, Out8::F32>());
   };
   switch (act) {
 #define LAYA_A(A) case Act8::A: return of(std::integral_constant<Act8, Act8::A>());
@@ -981,8 +1017,9 @@ hipError_t linear8_prepare() {
 #undef LAYA_T
   for (int act = 0; act < 5; ++act)
     for (Out8 out : {Out8::Half, Out8::E4m3, Out8::F32})
-      if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out)),
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
+      for (bool residual : {false, true})
+        if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out, residual)),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
   return e;
 }
 
@@ -990,7 +1027,7 @@ hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (a.M <= 0) return hipSuccess;
   if (tile == kRing8) {
     const RingWalk walk = walk_of(a);
-    LAYA_LAUNCH(ring_kernel(a.act, out_of(a)), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
+    LAYA_LAUNCH(ring_kernel(a.act, out_of(a), a.residual != nullptr), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
     return hipGetLastError();
   }
   const long long span = problem_of(a).span;
