@@ -3,7 +3,7 @@
 //
 // All three are bound by HBM: every value is read once and every code written once, and the arithmetic between
 // (a maximum over 32 values and a conversion each) hides behind the loads.  65,536 rows of 1,024: quantised from fp16
-// in 37 us (5.5 TB/s) and read back to bf16 in 36, fp32 residual plus bf16 branch normalised in 126 (5.9 TB/s; a copy on this
+// in 37-39 us (5.3 TB/s) and read back to bf16 in 36, fp32 residual plus bf16 branch normalised in 127 (5.8 TB/s; a copy on this
 // card reaches 4.8 past the last-level cache).
 #include "rows8.hpp"
 #include "kernels.hpp"
