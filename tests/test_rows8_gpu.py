@@ -429,6 +429,16 @@ def test_linear_onto_its_own_residual(gpu, out, M, N):
     close(*linear(gpu, x, w, out=out, rtype=out, residual=rng.normal(0, 1, (M, N)).astype(np.float32), inplace=True))
 
 
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+def test_linear_onto_its_own_residual_on_every_tile(gpu, out, act):
+    """Rows and columns that end inside every tile: each reads a residual place before any lane writes it."""
+    rng = np.random.default_rng(31)
+    x, w = operands(gpu, rng, 300, 1184, 384)
+    every_tile(gpu, x, w, act=act, out=out, rtype=out, inplace=True, bias=rng.normal(0, .5, 1184).astype(np.float32),
+               residual=rng.normal(0, 1, (300, 592 if act == "swiglu" else 1184)).astype(np.float32))
+
+
 def test_linear_nan_blocks_and_the_largest_codes(gpu):
     """A NaN block spoils its row (of x) or column (of w) alone, on every tile and in 8-bit outputs its whole block."""
     rng = np.random.default_rng(9)
