@@ -284,6 +284,7 @@ int laya_op_head_gather(const float* src, const int32_t* src_rows, const int32_t
 
 enum { LAYA_LAYER_NORM = 0, LAYA_RMS_NORM = 1 };
 enum { LAYA_ACT_NONE = 0, LAYA_ACT_GELU = 1, LAYA_ACT_RELU = 2, LAYA_ACT_GEGLU = 3, LAYA_ACT_SWIGLU = 4 };
+enum { LAYA_TILE_EXACT = -1, LAYA_TILE_FAST = -2 };  /* planned tiles of laya_op_linear8 */
 
 /* Codes per 8-bit row of `width` values; -1 for a width below 1 or above 2^30.  Host-only. */
 int laya_width8(int width);
@@ -318,10 +319,15 @@ int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, i
  * (act(gate) * value; N a multiple of 32).  GELU is the exact-erf one, SWIGLU's gate x / (1 + exp(-x)).  The residual
  * is added in fp32 before the one rounding; it may be out itself when both have the same type, and
  * nothing else may overlap out.
- * Sums are fp32.  fp32 outputs are made from exact products (of values of at least 2^-126, smaller ones count as
- * zero); the others may be summed by the 8-bit matrix unit, whose additions were off by up to 6e-5 of the root of the
- * products' sum of squares, under half a bf16 or fp16 step of results of that size.  Activations are
- * accurate to 1e-6.  tile -1 lets the planner choose; others name a tile (0 .. ), refused where it cannot make the output. */
+ * tile says how the sums are made:
+ *   LAYA_TILE_EXACT  exact products (of values of at least 2^-126, smaller ones count as zero) and fp32 sums, whatever the
+ *                    output's type; the planner chooses the tile, and with it the order of a sum.
+ *   LAYA_TILE_FAST   16- and 8-bit outputs may take the 8-bit matrix unit, at up to twice the rate.  It cuts the products
+ *                    of each group of 8 neighbours off, towards zero, 2^13 below the largest sum of two codes' exponents: a
+ *                    sum loses up to 2^-10 of its products' magnitudes (2^-7 where the largest have a subnormal code),
+ *                    one-sidedly where they have one sign.
+ *   0 .. 14          that tile, refused where it cannot make the output; 5, 7 to 10 and 13 are of the 8-bit unit.
+ * Activations are accurate to 1e-6, a gated one's times its value. */
 int laya_op_linear8(const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias,
                     const void* residual, int residual_dtype, void* out, void* out_scales, int out_dtype,
                     int activation, int M, int N, int K, int tile, void* stream);

@@ -272,9 +272,9 @@ struct Linear8Args {
   bool wide;              // whole 16-column blocks: rows of out start on 16 of its bytes, bias and residual on whole quads
 };
 constexpr int kE4M3 = 3;
-// Tiles and the planner's choice among them: linear8_plan.hpp.
+// Tiles and the planner's choice among them: linear8_plan.hpp; `exact`: among those of exact products.
 bool linear8_tile_valid(int id, const Linear8Args& a);
-int linear8_plan(const Linear8Args& a, int cus);
+int linear8_plan(const Linear8Args& a, bool exact, int cus);
 hipError_t linear8_prepare();
 hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream);
 

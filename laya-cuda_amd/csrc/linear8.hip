@@ -5,9 +5,13 @@
 // are fp32 (measured: 8e-8 of the result's norm at K = 4,096).  It moves half the bytes of the 16-bit product, which is
 // what few rows are bound by (1 x 4,096 x 1,024 4.9 us, 96 x 2,304 x 768 6.2, both a launch and one or two memory round
 // trips; 512 x 1,024 x 4,096 with fp32 output 14.8, operand stream and widening).
-// The 8-bit unit (kFast): v_mfma_scale_f32_16x16x128_f8f6f4 takes codes and scales as they are, at twice the rate, but its
-// own additions drop bits: 1.4e-5 of the root of the products' sum of squares, at most 6e-5, however a sum is cut.
-// That is below the rounding of 16- and 8-bit outputs, which may take it; fp32 outputs do not.
+// The 8-bit unit (kFast): v_mfma_scale_f32_16x16x128_f8f6f4 takes codes and scales as they are, at twice the rate, but
+// aligns each 8 neighbouring products to their largest sum of exponents (a subnormal code's is its type's least) and cuts
+// them off 2^13 below it, towards zero (measured with one large product and one small, normal and subnormal, and with
+// significands of 1.125 to 1.875; the groups' sums are then added to 24 bits).
+// Normal operands lose 2e-5 of the root of the products' sum of squares (1e-4 at most), where a channel in 128 is a
+// thousand times the others and the products have one sign 1.6e-4 of their magnitudes (6e-4 at most): no sum in 32 bits. So
+// a product takes it only where its caller says so, and never for fp32 outputs.
 //
 // Layout: whole 128-code slabs go straight from global memory into LDS, 16-byte chunk c of row r at position
 // c ^ (r / 2) % 8, so that 16 lanes reading one chunk of 16 consecutive rows touch all banks once.  A workgroup
@@ -454,7 +458,7 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // The epilogue needs no LDS: lane (r, kq) = (lane % 16, lane / 16) holds columns 4 kq .. +3 of row r of each 16 x 16
 // block, and the four lane groups exchange packed dwords so that each stores 16 bytes of consecutive columns.
 //
-// fp32 outputs take the same walk and stream with exact products (kExact): a slab is two passes, one per 64-code half,
+// Exact products (kExact) take the same walk and stream: a slab is two passes, one per 64-code half,
 // over the eight row blocks, with w's half widened for the pass and x's next row block widened between the MFMAs of
 // the present one.  Its MFMAs take twice as long, so a barrier frees all of x's units, another all of w's.
 //
@@ -463,10 +467,11 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // 202 (K = 4,096) and 109 (K = 1,024); a row of MFMAs under which loads go out takes 1.5 to 1.9 times as long, and the
 // epilogue 8,200 clocks a tile, 17,400 with GELU into 8-bit rows.
 enum class Out8 { Half, E4m3, F32 };
-template <Act8 A, Out8 O, bool kResidual>
+template <Act8 A, Out8 O, bool kExact, bool kResidual>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
-  constexpr bool kGlu = gated(A), kE4m3 = O == Out8::E4m3, kExact = O == Out8::F32;
+  constexpr bool kGlu = gated(A), kE4m3 = O == Out8::E4m3, kF32 = O == Out8::F32;
+  static_assert(kExact || !kF32, "fp32 outputs are made from exact products");
   constexpr int BM = 256, BN = 256, MB = 8, NB = 4;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 63;
@@ -677,7 +682,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
   // tile's first slab (kLate) the epilogue stores and the bias load, which come between the two tiles' loads.  Waiting
   // for the stores there cost 2-3 us a tile.  (No wait is chosen at run time: across the branch the compiler moved
   // the MFMAs behind the barrier.)
-  constexpr int kStores = (kGlu ? MB : 2 * MB) * (kExact ? 2 : 1);
+  constexpr int kStores = (kGlu ? MB : 2 * MB) * (kF32 ? 2 : 1);
   constexpr int kWait = kExact ? kFirst : kFirst + kSecond, kWaitLate = kWait + kStores + 1;
   auto four = [&](int i) {
     pin();
@@ -832,7 +837,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     constexpr int kStream = kE4m3 ? 2 : 0;  // 8-bit codes past the caches (nontemporal); other types lost by it
     const int col0 = (kGlu ? cur.n0 / 2 + wn * 32 : cur.n0 + wn * 64);
     const int rows = min(a.M - cur.m0, BM);
-    const int pitch = kE4m3 ? span : a.cols * (kExact ? 4 : 2);  // bytes of an output row
+    const int pitch = kE4m3 ? span : a.cols * (kF32 ? 4 : 2);  // bytes of an output row
     const __amdgpu_buffer_rsrc_t dst = __builtin_amdgcn_make_buffer_rsrc(
         static_cast<uint8_t*>(a.out) + static_cast<size_t>(cur.m0) * pitch, 0, rows * pitch, 0x00020000);
     const __amdgpu_buffer_rsrc_t dst_scales = __builtin_amdgcn_make_buffer_rsrc(
@@ -908,7 +913,7 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
         }
       auto block_row = [&](int t) { return row_of(step, t); };
       if constexpr (kResidual) add_residual(raw, v);
-      if constexpr (kExact) {
+      if constexpr (kF32) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int col = block_col(t) + 4 * eq;
@@ -970,11 +975,13 @@ constexpr int kTileLds8[] = {
 };
 
 typedef void (*RingKernel)(Linear8Args, RingWalk);
-RingKernel ring_kernel(Act8 act, Out8 out, bool residual) {
-  auto with = [residual](auto act_c, auto out_c) -> RingKernel {
+RingKernel ring_kernel(Act8 act, Out8 out, bool exact, bool residual) {
+  auto with = [exact, residual](auto act_c, auto out_c) -> RingKernel {
     constexpr Act8 A = decltype(act_c)::value;
     constexpr Out8 O = decltype(out_c)::value;
-    return residual ? linear8_ring_kernel<A, O, true> : linear8_ring_kernel<A, O, false>;
+    if constexpr (O != Out8::F32)
+      if (!exact) return residual ? linear8_ring_kernel<A, O, false, true> : linear8_ring_kernel<A, O, false, false>;
+    return residual ? linear8_ring_kernel<A, O, true, true> : linear8_ring_kernel<A, O, true, false>;
   };
   auto of = [&](auto act_c) -> RingKernel {
     return out == Out8::Half   ? with(act_c, std::integral_constant<Out8, Out8::Half>())
@@ -995,17 +1002,17 @@ RingWalk walk_of(const Linear8Args& a) {
   const long long span = a.out_type == kE4M3 ? padded8(a.cols) : a.cols, oc = gated(a.act) ? 128 : 256;
   return ring_walk((span + oc - 1) / oc, (static_cast<long long>(a.M) + 255) / 256);
 }
-Problem8 problem_of(const Linear8Args& a) {
+Problem8 problem_of(const Linear8Args& a, bool exact) {
   const bool out8 = a.out_type == kE4M3;
   return Problem8{a.M, out8 ? padded8(a.cols) : a.cols, a.ld / 128, gated(a.act), out8,
-                  a.out_type == static_cast<int>(DType::F32), a.wide && walk_of(a).total > 0};
+                  exact || a.out_type == static_cast<int>(DType::F32), a.wide && walk_of(a).total > 0};
 }
 
 }  // namespace
 
-bool linear8_tile_valid(int id, const Linear8Args& a) { return tile8_valid(id, problem_of(a)); }
+bool linear8_tile_valid(int id, const Linear8Args& a) { return tile8_valid(id, problem_of(a, false)); }
 
-int linear8_plan(const Linear8Args& a, int cus) { return linear8_plan(problem_of(a), cus); }
+int linear8_plan(const Linear8Args& a, bool exact, int cus) { return linear8_plan(problem_of(a, exact), cus); }
 
 hipError_t linear8_prepare() {
   hipError_t e = hipSuccess;
@@ -1017,20 +1024,22 @@ hipError_t linear8_prepare() {
 #undef LAYA_T
   for (int act = 0; act < 5; ++act)
     for (Out8 out : {Out8::Half, Out8::E4m3, Out8::F32})
-      for (bool residual : {false, true})
-        if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out, residual)),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
+      for (bool exact : {false, true})
+        for (bool residual : {false, true})
+          if (e == hipSuccess && (exact || out != Out8::F32))
+            e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out, exact, residual)),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
   return e;
 }
 
 hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (a.M <= 0) return hipSuccess;
-  if (tile == kRing8) {
+  if (tile == kFastRing8 || tile == kRing8) {
     const RingWalk walk = walk_of(a);
-    LAYA_LAUNCH(ring_kernel(a.act, out_of(a), a.residual != nullptr), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
+    LAYA_LAUNCH(ring_kernel(a.act, out_of(a), tile == kRing8, a.residual != nullptr), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
     return hipGetLastError();
   }
-  const long long span = problem_of(a).span;
+  const long long span = problem_of(a, false).span;
   auto grid = [&](int bm, int bn) {
     const long long oc = gated(a.act) ? bn / 2 : bn;
     return dim3(static_cast<unsigned>((span + oc - 1) / oc * ((static_cast<long long>(a.M) + bm - 1) / bm)));

@@ -23,7 +23,8 @@ namespace laya {
   LAYA_T(10, 128, 128, 2, 4, 1, 1, 2, true, 2, 4.4f, 3.70f, 1.400f)    \
   LAYA_T(11, 128, 128, 2, 4, 1, 1, 4, false, 1, 2.8f, 4.44f, 1.229f)   \
   LAYA_T(12, 128, 128, 2, 2, 1, 1, 2, false, 2, 4.0f, 6.20f, 2.280f)
-constexpr int kLinear8Tiles = 13, kRing8 = kLinear8Tiles;  // the persistent ring comes last
+// The persistent rings come last: on the 8-bit matrix unit, and with exact products.
+constexpr int kLinear8Tiles = 13, kFastRing8 = kLinear8Tiles, kRing8 = kLinear8Tiles + 1;
 
 struct Tile8Cost {
   int bm, bn;
@@ -41,7 +42,7 @@ static_assert(sizeof(kTile8Costs) / sizeof(kTile8Costs[0]) == kLinear8Tiles, "a 
 struct Problem8 {
   long long rows, span;  // output rows, and columns with an 8-bit row's padding
   int slabs;             // of 128 codes
-  bool gated, out8, fine, ring;  // 8-bit and fp32 outputs; `ring`: the ring kernel takes this call
+  bool gated, out8, fine, ring;  // 8-bit outputs; `fine`: exact products alone; `ring`: the ring kernels take this call
 };
 
 // Workgroups of BM x BN tiles.
@@ -51,9 +52,9 @@ constexpr long long tiles8(const Problem8& p, long long bm, long long bn) {
 }
 
 // Whether tile `id` can make this output: a block of 32 output codes and a group of 16 gate and 16 value rows lie
-// inside one tile, fp32 outputs are made from exact products, and a launch has fewer than 2^32 threads.
+// inside one tile, exact products are made where they are asked for, and a launch has fewer than 2^32 threads.
 constexpr bool tile8_valid(int id, const Problem8& p) {
-  if (id == kRing8) return p.ring && p.slabs >= 2;
+  if (id == kFastRing8 || id == kRing8) return p.ring && p.slabs >= 2 && !(p.fine && id == kFastRing8);
   if (id < 0 || id >= kLinear8Tiles) return false;
   const Tile8Cost& t = kTile8Costs[id];
   return !(p.fine && t.fast) && !(p.gated && t.bn % 32) && !(p.out8 && (p.gated ? t.bn / 2 : t.bn) % 32) &&
@@ -64,9 +65,9 @@ constexpr bool tile8_valid(int id, const Problem8& p) {
 constexpr int linear8_plan(const Problem8& p, int cus) {
   int best = -1;
   float least = 0.f;
-  for (int id = 0; id <= kLinear8Tiles; ++id) {
+  for (int id = 0; id <= kRing8; ++id) {
     if (!tile8_valid(id, p)) continue;
-    const bool ring = id == kRing8;
+    const bool ring = id >= kLinear8Tiles;
     const long long tiles = ring ? tiles8(p, 256, 256) : tiles8(p, kTile8Costs[id].bm, kTile8Costs[id].bn);
     const float n = static_cast<float>(p.slabs);
     float time = 0.f;
@@ -74,8 +75,8 @@ constexpr int linear8_plan(const Problem8& p, int cus) {
       // Its first round depends on how many CUs fetch and store at once.
       const float full = tiles < cus ? static_cast<float>(tiles) / static_cast<float>(cus) : 1.f;
       const long long rounds = (tiles + cus - 1) / cus;
-      time = p.fine ? 12.4f + full + n * (2.56f + 0.5f * full) + static_cast<float>(rounds - 1) * (15.3f + 3.27f * n)
-                    : 6.6f + 5.5f * full + n * (1.34f + 0.36f * full) + static_cast<float>(rounds - 1) * (5.4f + 1.7f * n);
+      time = id == kRing8 ? 12.4f + full + n * (2.56f + 0.5f * full) + static_cast<float>(rounds - 1) * (15.3f + 3.27f * n)
+                          : 6.6f + 5.5f * full + n * (1.34f + 0.36f * full) + static_cast<float>(rounds - 1) * (5.4f + 1.7f * n);
     } else {
       const Tile8Cost& t = kTile8Costs[id];
       const long long round = static_cast<long long>(cus) * t.occ, rounds = (tiles + round - 1) / round;

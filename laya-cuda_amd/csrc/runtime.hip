@@ -1604,7 +1604,7 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
             (!residual || aligned_to(residual, 4 * type_size(residual_dtype)));
     a.wide = a.vec && a.cols % 16 == 0 && aligned_to(out, 16) && aligned_to(bias, 16);
     prepare_device();
-    if (tile == -1) tile = linear8_plan(a, 256);
+    if (tile == LAYA_TILE_EXACT || tile == LAYA_TILE_FAST) tile = linear8_plan(a, tile == LAYA_TILE_EXACT, 256);
     LAYA_REQUIRE(linear8_tile_valid(tile, a), "no such tile, or one that cannot make this output");
     check_launch(launch_linear8(a, tile, static_cast<hipStream_t>(stream)), "linear8");
   });

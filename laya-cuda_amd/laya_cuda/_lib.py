@@ -16,6 +16,7 @@ POS_LEARNED, POS_ROPE = 0, 1
 FFN_GELU, FFN_GEGLU = 0, 1
 LAYER_NORM, RMS_NORM = 0, 1  # laya_op_norm8 kinds
 ACT_NONE, ACT_GELU, ACT_RELU, ACT_GEGLU, ACT_SWIGLU = range(5)  # laya_op_linear8 activations
+TILE_EXACT, TILE_FAST = -1, -2  # and its planned tiles
 
 
 class LayaConfig(ct.Structure):
