@@ -272,9 +272,12 @@ int laya_op_head_gather(const float* src, const int32_t* src_rows, const int32_t
  *   codes  [rows][laya_width8(width)]       e4m3 (OCP, no infinities), 16-byte aligned
  *   scales [rows][laya_width8(width) / 32]  uint8, 4-byte aligned
  * laya_width8 rounds the width up to a multiple of 128; the codes past the width are zeros (NaN codes where
- * a block, or for laya_op_linear8 a row, holds a NaN).  Code i of a row stands for e4m3(code) * 2^(scale[i / 32] - 127).  A writer takes the smallest scale with which the block's largest
+ * a block, or for laya_op_linear8 a row, holds a NaN).  Code i of a row stands for
+ * e4m3(code) * 2^(scale[i / 32] - 127).  A writer takes the smallest scale with which the block's largest
  * magnitude is at most 448 (2^-127 at the least; 0 for a block of zeros) and rounds each value once, to nearest
- * with ties to even.  A block that holds a NaN or an infinity gets the scale 255 and reads back as NaNs.
+ * with ties to even; finite values stay finite (what would round to 2^128 goes to 240 * 2^120).  A block that holds
+ * a NaN or an infinity gets the scale 255 and reads back as NaNs.  Codes that no writer makes, of 2^128 or more (scales
+ * 247 to 254), read back as infinities, and exact products take them as such.
  *
  * Every operator runs on the current device, which owns the pointers and the stream; it makes no allocation, no
  * host synchronisation and keeps nothing between calls, so calls may be captured, replayed and run side by side.

@@ -2,7 +2,7 @@
 //
 // A row of `width` values is stored as padded8(width) codes, a multiple of 128 (the codes past the width are
 // zeros), and one scale byte s per 32 codes; code c of the block stands for e4m3(c) * 2^(s - 127).  The scale is
-// the smallest one that leaves the whole block within the largest code, 448; a block of zeros has s = 0, and
+// the smallest one that leaves the whole block within the largest code, 448 (at most 247); a block of zeros has s = 0, and
 // a block that holds a NaN or an infinity has s = 255 and reads back as NaNs.  128 codes are what one
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes of a row, and their four scale bytes are one aligned dword.
 //
@@ -39,7 +39,8 @@ __device__ __forceinline__ float scale_value8(unsigned s) {
   return __builtin_bit_cast(float, s == 0 ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23);
 }
 
-// Four values of a block of scale byte s as four codes, each rounded once (to nearest, ties to even): the conversion
+// Four values of a block of scale byte s as four codes, each rounded once (to nearest, ties to even; what rounds to 2^128,
+// the code 256 of the largest scale 247, goes to 240 there, so that finite values stay finite): the conversion
 // divides by its scale operand's power of two (exponent 0 is 2^-127).  With it and the maximum of three above, a
 // product of 65,536 x 4,096 x 1,024 into 8-bit rows takes 287 instead of 293 us, and with GELU 386 instead of 398.
 __device__ __forceinline__ unsigned encode8(float a, float b, float c, float d, unsigned s) {
@@ -47,7 +48,12 @@ __device__ __forceinline__ unsigned encode8(float a, float b, float c, float d, 
   const float scale = __builtin_bit_cast(float, s << 23);
   i16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(i16x2{0, 0}, a, b, scale, false);
   r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
-  return s == 255u ? 0x7f7f7f7fu : __builtin_bit_cast(unsigned, r);
+  unsigned codes = __builtin_bit_cast(unsigned, r);
+  if (__builtin_amdgcn_ballot_w64(s >= 247u)) {  // a branch that few waves take
+    const unsigned over = s == 247u ? ((codes & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u : 0u;  // 0x78 (256) is the only code past 0x77
+    codes = s == 255u ? 0x7f7f7f7fu : codes - (over >> 7);
+  }
+  return codes;
 }
 
 // Largest magnitude bits over the 8 lanes of a 32-value block (4 values a lane, lanes 8 j .. 8 j + 7).
