@@ -294,7 +294,8 @@ int laya_width8(int width);
 
 /* 8-bit rows of x (LAYA_F32/F16/BF16), whose rows of `width` values start `stride` elements apart (stride >=
  * width): weights once at load, or activations.  x needs its own element's alignment only; rows that start
- * and end on whole 16 bytes are read fastest.  At most 2^36 codes, from values that span at most 2^50 elements. */
+ * and end on whole 16 bytes are read fastest.  At most 2^36 - 4096 codes, from values that span at
+ * most 2^50 elements. */
 int laya_op_quantize8(const void* x, int dtype, int64_t stride, void* codes, void* scales, int64_t rows, int width,
                       void* stream);
 

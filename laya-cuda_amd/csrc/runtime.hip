@@ -1501,9 +1501,9 @@ static size_t type_size(int dtype) { return dtype == LAYA_F32 ? 4 : 2; }
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 constexpr int kMaxWidth8 = 1 << 30;
 constexpr int kMaxLinear8 = 1 << 20;  // a tile's rows then span fewer than 2^32 bytes
-// Codes of a matrix, and elements from its first value to its last row's: a launch then has fewer than 2^32 threads, and
-// offsets fit 64 bits.
-constexpr int64_t kMaxCodes8 = (1LL << 36) - 1, kMaxSpan8 = 1LL << 50;
+// Codes of a matrix, and elements from its first value to its last row's: a launch (4,096 fp32 values' codes a workgroup of
+// 256 threads) then has fewer than 2^32 threads, and offsets fit 64 bits.
+constexpr int64_t kMaxCodes8 = (1LL << 36) - 4096, kMaxSpan8 = 1LL << 50;
 
 // The checks that every 8-bit operand shares.
 static void require_rows8(const void* codes, const void* scales, const char* what) {
@@ -1515,7 +1515,7 @@ static void require_rows8(const void* codes, const void* scales, const char* wha
 static void require_extent8(int64_t rows, int width, int64_t stride) {
   LAYA_REQUIRE(rows >= 0 && width >= 1 && width <= kMaxWidth8 && stride >= width, "bad rows, width or stride");
   LAYA_REQUIRE(rows <= kMaxCodes8 / padded8(width) && (rows == 0 || stride <= kMaxSpan8 / rows),
-               "rows: at most 2^36 codes, from values that span at most 2^50 elements");
+               "rows: at most 2^36 codes less 4096, from values that span at most 2^50 elements");
 }
 
 int laya_width8(int width) {
