@@ -269,7 +269,7 @@ struct Linear8Args {
   int M, N, ld;           // ld = padded8(K)
   int cols;               // output columns: N, or N / 2 when gated
   bool vec;               // rows of out and residual start on whole quads
-  bool wide;              // whole 16-column blocks: rows of out start on 16 of its bytes, bias and residual on whole quads
+  bool wide;              // the ring kernels' whole stores and residual quads lie inside the rows of out and residual
 };
 constexpr int kE4M3 = 3;
 // Tiles and the planner's choice among them: linear8_plan.hpp; `exact`: among those of exact products.

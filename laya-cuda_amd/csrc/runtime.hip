@@ -1602,7 +1602,9 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
     a.M = M; a.N = N; a.ld = static_cast<int>(padded8(K)); a.cols = glu ? N / 2 : N;
     a.vec = a.cols % 4 == 0 && (out_dtype == LAYA_E4M3 || aligned_to(out, 4 * type_size(out_dtype))) &&
             (!residual || aligned_to(residual, 4 * type_size(residual_dtype)));
-    a.wide = a.vec && a.cols % 16 == 0 && aligned_to(out, 16) && aligned_to(bias, 16);
+    // What the ring kernels' epilogues touch at once: a residual's quads, four fp32 or eight 16-bit outputs, 16 codes of a padded row.
+    a.wide = aligned_to(out, 16) && (a.vec || (out_dtype == LAYA_E4M3 && !residual)) &&
+             (out_dtype == LAYA_F32 || out_dtype == LAYA_E4M3 || a.cols % 8 == 0);
     prepare_device();
     if (tile == LAYA_TILE_EXACT || tile == LAYA_TILE_FAST) tile = linear8_plan(a, tile == LAYA_TILE_EXACT, 256);
     LAYA_REQUIRE(linear8_tile_valid(tile, a), "no such tile, or one that cannot make this output");

@@ -103,8 +103,7 @@ def test_the_8_bit_unit_s_bound(gpu, out, M, N, K):
             try:
                 off, mag, own = error_of(gpu, a, b, out, tile)
             except RuntimeError as e:
-                # The ring takes whole 16-column blocks and two slabs at least.
-                assert "no such tile" in str(e) and tile == 13 and (N % 16 or K <= 128)
+                assert "no such tile" in str(e) and tile == 13 and K <= 128  # the ring takes two slabs at least
                 continue
             worst = ((off - own) / mag).max().item()
             assert worst <= 2.0 ** -10 + exact_bound(K), f"{kind}, tile {tile}: {worst:.3g}"
@@ -147,7 +146,28 @@ def test_fp32_outputs_ignore_the_8_bit_unit(gpu):
                                            ("e4m3", "geglu", ""), ("f16", "swiglu", "")])
 @pytest.mark.parametrize("M,N,K", [(4200, 4352, 256), (4333, 4416, 384), (65, 66048, 640)])
 def test_both_rings_over_more_tiles_than_compute_units(gpu, M, N, K, out, act, rtype):
-    """Every output of both persistent kernels, several tiles a workgroup, beside the exact tile of 128 x 128."""
+    rings(gpu, M, N, K, out, act, rtype)
+
+
+@pytest.mark.parametrize("out,act,rtype,rest", [
+    ("f32", "none", "", 4), ("f32", "gelu", "f32", 8), ("f32", "none", "bf16", 12), ("f32", "relu", "f16", 4), ("bf16", "none", "", 8),
+    ("f16", "gelu", "f32", 8), ("bf16", "relu", "bf16", 8), ("e4m3", "none", "", 1), ("e4m3", "gelu", "", 7), ("e4m3", "relu", "", 14),
+    ("e4m3", "none", "f32", 4), ("e4m3", "gelu", "bf16", 12), ("e4m3", "relu", "f16", 8)])
+@pytest.mark.parametrize("M,N,K", [(4333, 4400, 384), (300, 512, 256), (70, 66048, 640)])
+def test_rings_of_columns_that_end_inside_a_block(gpu, M, N, K, out, act, rtype, rest):
+    """Columns past a multiple of 16: the persistent kernels take every number whose stores and residual quads are whole."""
+    rings(gpu, M, N + rest, K, out, act, rtype)
+
+
+@pytest.mark.parametrize("out,rtype,N", [("f32", "", 1001), ("f32", "", 1002), ("bf16", "", 1004), ("f16", "", 1003), ("e4m3", "f32", 1002),
+                                         ("e4m3", "bf16", 1001)])
+def test_rings_refuse_columns_that_end_inside_a_store(gpu, out, rtype, N):
+    """Such calls take the other tiles, by the planner's choice, and get the same sums."""
+    rings(gpu, 700, N, 256, out, "none", rtype, refused=True)
+
+
+def rings(gpu, M, N, K, out, act, rtype, refused=False):
+    """Every output of both persistent kernels beside the exact tile of 128 x 128."""
     t, lib = torch(), _lib.load()
     (x, xv), (w, wv) = made(gpu, "normal", M, N, K)
     gen = t.Generator(device=gpu).manual_seed(5)
@@ -171,6 +191,10 @@ def test_both_rings_over_more_tiles_than_compute_units(gpu, M, N, K, out, act, r
     want, mag = run(11), xv.abs() @ wv.abs().t().contiguous() + bias.abs()
     step = 2.0 ** -4 if out == "e4m3" else HALF[out]
     for tile, share in ((14, 2 * exact_bound(K)), (13, 2.0 ** -10 + 2 * exact_bound(K))):
+        if refused or (tile == 13 and out == "f32"):
+            with pytest.raises(RuntimeError, match="no such tile"):
+                run(tile)
+            tile, share = -1, 2 * exact_bound(K)
         got = run(tile)
         if act in ("geglu", "swiglu"):  # |act'| <= 1.13 and |act(g)| <= |g|
             m = mag.view(M, -1, 2, 16)
