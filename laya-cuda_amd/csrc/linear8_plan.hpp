@@ -4,25 +4,25 @@
 namespace laya {
 
 // BM x BN outputs a workgroup, WM x WN waves times KG groups that split the slabs, S stages of SL slabs; FAST: the 8-bit
-// matrix unit, else widened codes.  Then the fit that linear8_plan uses, in microseconds, from products of 64 to 1,024
-// tiles and K = 512 to 4,096 with operands that alternate between three sets (out of L2): a launch takes
-// L + rounds (B + C slabs), a round being OCC tiles a CU.  Tiles of two a CU hide one workgroup's fill and epilogue
-// behind the other's slabs, which pays from the second round on.
+// matrix unit, else widened codes.  Then the fit that linear8_plan uses, in microseconds (tune_linear8_costs.py sweeps, fits and
+// checks it): a launch takes L + rounds (B + C slabs), a round being OCC tiles a CU.  On 120 held-out products the choice
+// takes at most 1.04 times the best tile of exact products, at most 1.16 times the best of all, and on average under 1.005.
+// Tiles of two a CU hide one workgroup's fill and epilogue behind the other's slabs, which pays from the second round on.
 //            ID   BM   BN WM WN KG SL  S  FAST  OCC  L     B     C
 #define LAYA_LINEAR8_TILES                                             \
-  LAYA_T(0, 16, 16, 1, 1, 8, 8, 4, false, 1, 1.4f, 2.45f, 0.086f)      \
-  LAYA_T(1, 16, 32, 1, 1, 8, 8, 3, false, 1, 1.4f, 3.09f, 0.108f)      \
-  LAYA_T(2, 16, 64, 1, 2, 4, 4, 3, false, 1, 1.6f, 2.56f, 0.202f)      \
-  LAYA_T(3, 64, 32, 2, 1, 4, 4, 3, false, 1, 1.6f, 2.90f, 0.275f)      \
-  LAYA_T(4, 64, 64, 2, 2, 2, 2, 4, false, 1, 1.6f, 2.91f, 0.471f)      \
-  LAYA_T(5, 64, 64, 2, 2, 2, 2, 4, true, 1, 1.4f, 3.02f, 0.334f)       \
-  LAYA_T(6, 64, 64, 2, 2, 1, 1, 4, false, 2, 1.7f, 3.10f, 0.810f)      \
-  LAYA_T(7, 64, 64, 2, 2, 1, 1, 4, true, 2, 1.7f, 2.40f, 0.690f)       \
-  LAYA_T(8, 64, 128, 2, 4, 1, 1, 4, true, 1, 1.7f, 3.02f, 0.565f)      \
-  LAYA_T(9, 128, 128, 2, 4, 1, 1, 4, true, 1, 2.3f, 4.53f, 0.791f)     \
-  LAYA_T(10, 128, 128, 2, 4, 1, 1, 2, true, 2, 4.4f, 3.70f, 1.400f)    \
-  LAYA_T(11, 128, 128, 2, 4, 1, 1, 4, false, 1, 2.8f, 4.44f, 1.229f)   \
-  LAYA_T(12, 128, 128, 2, 2, 1, 1, 2, false, 2, 4.0f, 6.20f, 2.280f)
+  LAYA_T(0, 16, 16, 1, 1, 8, 8, 4, false, 1, 1.13f, 2.77f, 0.083f)     \
+  LAYA_T(1, 16, 32, 1, 1, 8, 8, 3, false, 1, 1.20f, 3.34f, 0.119f)     \
+  LAYA_T(2, 16, 64, 1, 2, 4, 4, 3, false, 1, 1.21f, 3.17f, 0.198f)     \
+  LAYA_T(3, 64, 32, 2, 1, 4, 4, 3, false, 1, 0.68f, 4.06f, 0.256f)     \
+  LAYA_T(4, 64, 64, 2, 2, 2, 2, 4, false, 1, 0.32f, 3.85f, 0.439f)     \
+  LAYA_T(5, 64, 64, 2, 2, 2, 2, 4, true, 1, 0.24f, 3.90f, 0.270f)      \
+  LAYA_T(6, 64, 64, 2, 2, 1, 1, 4, false, 2, 1.56f, 3.15f, 0.798f)     \
+  LAYA_T(7, 64, 64, 2, 2, 1, 1, 4, true, 2, 1.53f, 3.04f, 0.553f)      \
+  LAYA_T(8, 64, 128, 2, 4, 1, 1, 4, true, 1, 0.17f, 4.01f, 0.492f)     \
+  LAYA_T(9, 128, 128, 2, 4, 1, 1, 4, true, 1, 0.00f, 5.79f, 0.717f)    \
+  LAYA_T(10, 128, 128, 2, 4, 1, 1, 2, true, 2, 0.00f, 6.95f, 1.097f)   \
+  LAYA_T(11, 128, 128, 2, 4, 1, 1, 4, false, 1, 0.00f, 5.52f, 1.233f)  \
+  LAYA_T(12, 128, 128, 2, 2, 1, 1, 2, false, 2, 1.48f, 8.39f, 1.900f)
 // The persistent rings come last: on the 8-bit matrix unit, and with exact products.
 constexpr int kLinear8Tiles = 13, kFastRing8 = kLinear8Tiles, kRing8 = kLinear8Tiles + 1;
 
@@ -38,6 +38,11 @@ constexpr Tile8Cost kTile8Costs[] = {
 #undef LAYA_T
 };
 static_assert(sizeof(kTile8Costs) / sizeof(kTile8Costs[0]) == kLinear8Tiles, "a row per tile");
+
+// The rings': start, what every CU's fetching and storing at once adds to it, a slab of the first round, a further round, its
+// slabs.
+constexpr float kFastRingCost[] = {6.72f, 3.51f, 1.48f, 6.74f, 1.55f};
+constexpr float kRingCost[] = {8.84f, 1.97f, 2.71f, 9.65f, 2.62f};
 
 struct Problem8 {
   long long rows, span;  // output rows, and columns with an 8-bit row's padding
@@ -72,11 +77,10 @@ constexpr int linear8_plan(const Problem8& p, int cus) {
     const float n = static_cast<float>(p.slabs);
     float time = 0.f;
     if (ring) {
-      // Its first round depends on how many CUs fetch and store at once.
       const float full = tiles < cus ? static_cast<float>(tiles) / static_cast<float>(cus) : 1.f;
       const long long rounds = (tiles + cus - 1) / cus;
-      time = id == kRing8 ? 12.4f + full + n * (2.56f + 0.5f * full) + static_cast<float>(rounds - 1) * (15.3f + 3.27f * n)
-                          : 6.6f + 5.5f * full + n * (1.34f + 0.36f * full) + static_cast<float>(rounds - 1) * (5.4f + 1.7f * n);
+      const float* const k = id == kRing8 ? kRingCost : kFastRingCost;
+      time = k[0] + k[1] * full + k[2] * n + static_cast<float>(rounds - 1) * (k[3] + k[4] * n);
     } else {
       const Tile8Cost& t = kTile8Costs[id];
       const long long round = static_cast<long long>(cus) * t.occ, rounds = (tiles + round - 1) / round;
