@@ -855,7 +855,7 @@ int guarded(Engine* E, F&& body) {
 }
 
 std::mutex g_prepare_mutex;
-std::vector<int> g_prepared;
+std::vector<int> g_prepared, g_prepared8;  // devices set up for everything but the 8-bit product, and for it
 // Per device: the device address of `scratch` (each device holds its own copy of the array).
 constexpr int kMaxDevices = 64;
 void* g_scratch[kMaxDevices] = {};
@@ -870,12 +870,21 @@ void prepare_device() {
   LAYA_REQUIRE(dev >= 0 && dev < kMaxDevices, "device index beyond the library's device table");
   LAYA_HIP(gemm_prepare());
   LAYA_HIP(head_prepare());
-  LAYA_HIP(linear8_prepare());
   void* ptr = nullptr;
   LAYA_HIP(hipGetSymbolAddress(&ptr, HIP_SYMBOL(scratch)));
   LAYA_REQUIRE(ptr != nullptr, "no device address for the scratch array");
   g_scratch[dev] = ptr;
   g_prepared.push_back(dev);
+}
+// The 8-bit product's kernel attributes, which no engine needs: set by its first call on a device.
+void prepare_linear8() {
+  int dev = 0;
+  LAYA_HIP(hipGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(g_prepare_mutex);
+  for (int d : g_prepared8)
+    if (d == dev) return;
+  LAYA_HIP(linear8_prepare());
+  g_prepared8.push_back(dev);
 }
 
 // laya_predict_static: host staging of the packed block (pageable, process-wide) and the lock
@@ -1605,7 +1614,7 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
     // What the ring kernels' epilogues touch at once: a residual's quads, four fp32 or eight 16-bit outputs, 16 codes of a padded row.
     a.wide = aligned_to(out, 16) && (a.vec || (out_dtype == LAYA_E4M3 && !residual)) &&
              (out_dtype == LAYA_F32 || out_dtype == LAYA_E4M3 || a.cols % 8 == 0);
-    prepare_device();
+    prepare_linear8();
     if (tile == LAYA_TILE_EXACT || tile == LAYA_TILE_FAST) tile = linear8_plan(a, tile == LAYA_TILE_EXACT, 256);
     LAYA_REQUIRE(linear8_tile_valid(tile, a), "no such tile, or one that cannot make this output");
     check_launch(launch_linear8(a, tile, static_cast<hipStream_t>(stream)), "linear8");
