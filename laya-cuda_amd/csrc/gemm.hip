@@ -1378,7 +1378,6 @@ template <typename T, Epi E>
 hipError_t gemm_launch_t(const GemmArgs& a, int tile, hipStream_t stream);
 template <typename T, Epi E>
 hipError_t gemm_prepare_t();
-int gemm_device_cus();  // compute units of the current device (the persistent tiles' grid)
 
 #ifdef LAYA_GEMM_EPI
 

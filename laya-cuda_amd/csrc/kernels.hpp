@@ -89,6 +89,7 @@ enum class GemmCosts { None, Replay, Forward };
 void gemm_plan(int M, int N, int K, Epi epi, DType t, int cus, int* tile, int* splits, bool rope, bool measured,
                GemmCosts costs, int max_splits = 8);
 hipError_t gemm_prepare();  // sets LDS attributes of the large-tile kernels (call once per device)
+int gemm_device_cus();      // compute units of the current device (plans, and the persistent kernels' grids); 0 on failure
 // Pipelined tiles read their operands through buffer resources with 32-bit byte offsets: true when
 // both operands ([M][lda] and [N][ldb] 16-bit) span fewer than 2^32 bytes.
 bool gemm_operands_addressable(long long M, long long lda, long long N, long long ldb);

@@ -1029,6 +1029,7 @@ hipError_t linear8_prepare() {
           if (e == hipSuccess && (exact || out != Out8::F32))
             e = hipFuncSetAttribute(reinterpret_cast<const void*>(ring_kernel(static_cast<Act8>(act), out, exact, residual)),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, kRing8Lds);
+  if (e == hipSuccess && gemm_device_cus() <= 0) e = hipErrorInvalidDevice;  // read by plans and launches, kept from here on
   return e;
 }
 
@@ -1036,7 +1037,7 @@ hipError_t launch_linear8(const Linear8Args& a, int tile, hipStream_t stream) {
   if (a.M <= 0) return hipSuccess;
   if (tile == kFastRing8 || tile == kRing8) {
     const RingWalk walk = walk_of(a);
-    LAYA_LAUNCH(ring_kernel(a.act, out_of(a), tile == kRing8, a.residual != nullptr), dim3(std::min(walk.total, 256)), dim3(512), kRing8Lds, stream, a, walk);
+    LAYA_LAUNCH(ring_kernel(a.act, out_of(a), tile == kRing8, a.residual != nullptr), dim3(std::min(walk.total, gemm_device_cus())), dim3(512), kRing8Lds, stream, a, walk);
     return hipGetLastError();
   }
   const long long span = problem_of(a, false).span;

@@ -1615,7 +1615,7 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
     a.wide = aligned_to(out, 16) && (a.vec || (out_dtype == LAYA_E4M3 && !residual)) &&
              (out_dtype == LAYA_F32 || out_dtype == LAYA_E4M3 || a.cols % 8 == 0);
     prepare_linear8();
-    if (tile == LAYA_TILE_EXACT || tile == LAYA_TILE_FAST) tile = linear8_plan(a, tile == LAYA_TILE_EXACT, 256);
+    if (tile == LAYA_TILE_EXACT || tile == LAYA_TILE_FAST) tile = linear8_plan(a, tile == LAYA_TILE_EXACT, gemm_device_cus());
     LAYA_REQUIRE(linear8_tile_valid(tile, a), "no such tile, or one that cannot make this output");
     check_launch(launch_linear8(a, tile, static_cast<hipStream_t>(stream)), "linear8");
   });
