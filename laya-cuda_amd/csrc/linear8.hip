@@ -834,7 +834,9 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     const int er = elane & 15, eq = elane >> 4;
     constexpr int STEPS = kGlu ? MB / 2 : MB;
     constexpr unsigned kNowhere = 0x80000000u;  // past every resource
-    constexpr int kStream = kE4m3 ? 2 : 0;  // 8-bit codes past the caches (nontemporal); other types lost by it
+    // 8-bit codes past the caches (nontemporal): with the down projection behind it an FFN of 65,536 x 4,096 x 1,024 on the 8-bit
+    // unit takes 716 instead of 723 us, of 4,096 rows 69.8 and 70.4, with exact products the same; other types lost by it.
+    constexpr int kStream = kE4m3 ? 2 : 0;
     const int col0 = (kGlu ? cur.n0 / 2 + wn * 32 : cur.n0 + wn * 64);
     const int rows = min(a.M - cur.m0, BM);
     const int pitch = kE4m3 ? span : a.cols * (kF32 ? 4 : 2);  // bytes of an output row
