@@ -1602,6 +1602,7 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
     LAYA_REQUIRE(aligned_to(bias, 4) && (out_dtype == LAYA_E4M3 || aligned_to(out, type_size(out_dtype))) &&
                      (!residual || aligned_to(residual, type_size(residual_dtype))),
                  "pointers must be aligned to their elements");
+    LAYA_REQUIRE(!residual || residual != out || residual_dtype == out_dtype, "a residual that is out itself has its type");
     Linear8Args a{};
     a.x = static_cast<const uint8_t*>(x); a.xs = static_cast<const uint8_t*>(x_scales);
     a.w = static_cast<const uint8_t*>(w); a.ws = static_cast<const uint8_t*>(w_scales);
