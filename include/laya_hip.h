@@ -301,7 +301,7 @@ int laya_op_quantize8(const void* x, int dtype, int64_t stride, void* codes, voi
 
 /* The values 8-bit rows stand for, as dtype with rows `stride` elements apart; what lies between the rows is left as it
  * was.  Exact in LAYA_F32, and in LAYA_BF16 but for blocks of scales below 2^-117; LAYA_F16 rounds once
- * (infinity past its range). */
+ * (infinity past its range).  Extents as laya_op_quantize8's. */
 int laya_op_dequantize8(const void* codes, const void* scales, void* out, int dtype, int64_t stride, int64_t rows,
                         int width, void* stream);
 
@@ -321,8 +321,8 @@ int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, i
  * (LAYA_E4M3: out takes the codes, out_scales the scales; out_scales is NULL otherwise).  cols is N, or N / 2
  * for the gated activations, whose w (and bias) come in groups of 32 rows: 16 gate rows, then their 16 value rows
  * (act(gate) * value; N a multiple of 32).  GELU is the exact-erf one, SWIGLU's gate x / (1 + exp(-x)).  The residual
- * is added in fp32 before the one rounding; it may be out itself when both have the same type, and
- * nothing else may overlap out.
+ * is added in fp32 before the one rounding; it may be out itself when both have the same type (with another
+ * it is refused), and nothing else may overlap out.
  * tile says how the sums are made:
  *   LAYA_TILE_EXACT  exact products (of values of at least 2^-126, smaller ones count as zero) and fp32 sums, whatever the
  *                    output's type; the planner chooses the tile, and with it the order of a sum.
@@ -331,7 +331,7 @@ int laya_op_norm8(const float* residual, const void* branch, int branch_dtype, i
  *                    sum loses up to 2^-10 of its products' magnitudes (2^-7 where the largest have a subnormal code),
  *                    one-sidedly where they have one sign.
  *   0 .. 14          that tile, refused where it cannot make the output; 5, 7 to 10 and 13 are of the 8-bit unit.
- * Activations are accurate to 1e-6, a gated one's times its value. */
+ * Activations are accurate to 1e-6 of the larger of 1 and their magnitude, a gated one's times its value. */
 int laya_op_linear8(const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias,
                     const void* residual, int residual_dtype, void* out, void* out_scales, int out_dtype,
                     int activation, int M, int N, int K, int tile, void* stream);

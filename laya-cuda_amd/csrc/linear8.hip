@@ -4,7 +4,7 @@
 // registers, with their scales, by v_cvt_scalef32_pk_bf16_fp8 and multiplied by v_mfma_f32_16x16x32_bf16, whose sums
 // are fp32 (measured: 8e-8 of the result's norm at K = 4,096).  It moves half the bytes of the 16-bit product, which is
 // what few rows are bound by (1 x 4,096 x 1,024 4.9 us, 96 x 2,304 x 768 6.2, both a launch and one or two memory round
-// trips; 512 x 1,024 x 4,096 with fp32 output 14.8, operand stream and widening).
+// trips; 512 x 1,024 x 4,096 with fp32 output 14.4, operand stream and widening).
 // The 8-bit unit (kFast): v_mfma_scale_f32_16x16x128_f8f6f4 takes codes and scales as they are, at twice the rate, but
 // aligns each 8 neighbouring products to their largest sum of exponents (a subnormal code's is its type's least) and cuts
 // them off 2^13 below it, towards zero (measured with one large product and one small, normal and subnormal, and with
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, waves8<64 * WM * WN * KG>(lds8<B
   write(std::false_type());
 }
 
-// ---- the batched product: a persistent ring of 256 x 256 tiles on the 8-bit matrix unit ----
+// ---- the batched product: a persistent ring of 256 x 256 tiles ----
 
 constexpr int kUnit8 = 64 * 128;   // bytes of a ring unit: 64 rows of one slab
 constexpr int kSlab8 = 8 * kUnit8;  // four units of x, four of w
@@ -462,9 +462,10 @@ __device__ __forceinline__ unsigned group_max(unsigned m) {
 // over the eight row blocks, with w's half widened for the pass and x's next row block widened between the MFMAs of
 // the present one.  Its MFMAs take twice as long, so a barrier frees all of x's units, another all of w's.
 //
-// Measured: 65,536 x 1,024 x 4,096 into bf16 270-320 us by the card's clock (2.0-1.7 PFLOP/s), into fp32 460, with an fp32
-// residual 500-545; 65,536 x 4,096 x 1,024 into bf16 305-335, into 8-bit rows 287, with GELU 343-386.  MFMAs alone take 145 us, operand loads alone
-// 202 (K = 4,096) and 109 (K = 1,024); a row of MFMAs under which loads go out takes 1.5 to 1.9 times as long, and the
+// Measured, us by the card's clock: 65,536 x 1,024 x 4,096 on the 8-bit unit into bf16 262-320 (2.1-1.7 PFLOP/s); exact into
+// bf16 430-455, fp32 445-460, with an fp32 residual 480-545.  65,536 x 4,096 x 1,024 on the unit into bf16 305-335, 8-bit rows
+// 280-287, with GELU 343-386; exact 465-475, 450-465, 510-549.  The unit's MFMAs alone take 145 us, operand loads alone
+// 202 (K = 4,096) and 109 (K = 1,024); a row of its MFMAs under which loads go out takes 1.5 to 1.9 times as long, and the
 // epilogue 8,200 clocks a tile, 17,400 with GELU into 8-bit rows.
 enum class Out8 { Half, E4m3, F32 };
 template <Act8 A, Out8 O, bool kExact, bool kResidual>
@@ -851,7 +852,9 @@ void linear8_ring_kernel(Linear8Args a, RingWalk walk) {
     auto block_col = [&](int t) { return col0 + (kGlu ? t & 1 : t) * 16; };
     // The residual's quads of a step, as they lie in memory (16-bit ones in the low half): all four loads go out before the
     // first is used (bf16 to bf16, 15,088 x 1,024 x 1,024 32.4 -> 28.3 us against one at a time, 65,536 x 1,024 x 4,096 307 -> 295;
-    // fp32 551 -> 545, where the tile ends of all CUs meet at HBM).  A step ahead they spilled.
+    // fp32 551 -> 545, where the tile ends of all CUs meet at HBM).  The last of them waits for the step before's stores too, as
+    // both share one in-order counter.  These kernels spill: 10 to 15 registers with exact products, 1 on the unit ungated; a step's
+    // loads a whole step earlier spilled 55 and more.
     const int rsize = a.residual_type == static_cast<int>(DType::F32) ? 4 : 2;
     auto fetch_residual = [&](int step, u32x4 (&to)[4]) {
       pin();
