@@ -336,6 +336,95 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
                     const void* residual, int residual_dtype, void* out, void* out_scales, int out_dtype,
                     int activation, int M, int N, int K, int tile, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions, and attention over packed sequences with masks, capped scores and distance biases (no counterpart in
+ * the reference, whose rotation is part of its layout kernel and whose attention is bidirectional or windowed, of heads of 64).
+ *
+ * As above: the current device owns the pointers and the stream, no allocation, no host synchronisation, nothing kept
+ * between calls, LAYA_EINVAL for bad arguments.  Rows of heads lie `row` elements apart and a row's heads `head` elements
+ * apart, so that a projection's packed rows, caches and head-major planes are read and written where they are.
+ * ------------------------------------------------------------------------------------------ */
+
+enum { LAYA_ROTARY_HALF = 0, LAYA_ROTARY_INTERLEAVED = 1 };  /* pairs (i, i + rotated / 2), or (2 i, 2 i + 1) */
+enum {
+  LAYA_FREQ_PLAIN = 0,   /* theta^(-2 i / rotated) radians a position */
+  LAYA_FREQ_LINEAR = 1,  /* that over factor: positions are squeezed */
+  LAYA_FREQ_BASE = 2,    /* theta times factor^(rotated / (rotated - 2)) (times factor for rotated 2): the slowest pair
+                            slows down by factor, the fastest stays */
+  LAYA_FREQ_PARTS = 3    /* by the turns n that a pair makes over `original` positions: kept where n >= high, over factor
+                            where n <= low, and between them mixed in proportion */
+};
+
+/* Frequencies of the rotated / 2 pairs in turns (2 pi) a position, 64 bits, for laya_op_rotary (copied to the device by the
+ * caller).  original, low and high belong to LAYA_FREQ_PARTS.  theta > 0, factor >= 1, rotated even and from 2 to 8192,
+ * original > 0, 0 <= low < high.  Host-only. */
+int laya_rotary_frequencies(int kind, double theta, int rotated, double factor, double original, double low,
+                            double high, double* host_turns);
+
+/* out = x with each head's first `rotated` values turned by their row's position: with the angle 2 pi positions[row] turns[i]
+ * of pair i, (a, b) -> amplitude (a cos - b sin, a sin + b cos); direction -1 turns back (the gradient of direction 1, and
+ * its inverse where amplitude is 1).  Values rotated .. dim - 1 are copied.  dtype LAYA_F32/F16/BF16; positions
+ * int32, of either sign; turns as laya_rotary_frequencies makes them.  Angles are exact to 2^-27 of a turn at any position,
+ * arithmetic is fp32 with one rounding.  out may be x itself with the same strides, else it overlaps nothing; what lies
+ * between rows and heads is left as it was.  rotated even, 2 <= rotated <= dim <= 8192, heads * dim <= 2^20, rows <= 2^23,
+ * strides not negative and below 2^40 in magnitude.  Whole 16 bytes of halves, strides and addresses are fastest. */
+int laya_op_rotary(const void* x, int64_t x_row, int64_t x_head, void* out, int64_t out_row, int64_t out_head,
+                   int dtype, const int32_t* positions, const double* turns, float amplitude, int layout,
+                   int direction, int64_t rows, int heads, int dim, int rotated, void* stream);
+
+/* Ranges of a document mask: bounds[row] = (first, end) of the run of equal neighbouring ids that holds the row, counted from
+ * its sequence's start.  documents [rows], bounds [rows][2], starts and lengths [n_seq] are device memory; a
+ * sequence's rows are starts[s] .. starts[s] + lengths[s] - 1, cut to the array and to max_length; rows of no sequence are left
+ * as they were.  One call serves every layer and head of a batch. */
+int laya_op_document_bounds(const int32_t* documents, const int32_t* starts, const int32_t* lengths, int n_seq,
+                            int64_t rows, int max_length, int32_t* bounds, void* stream);
+
+/* A call of laya_op_attend.  Sequence s has the queries of rows q_starts[s] .. + q_lengths[s] - 1 of q and the keys and values of
+ * rows k_starts[s] .. + k_lengths[s] - 1 of k and v (device arrays, cut to the row counts and to max_q and max_k); its query i
+ * stands at position p = i + k_lengths[s] - q_lengths[s].  Query head h reads key head h / (heads / kv_heads).  The query sees key j if
+ *   j < prefix[s], or  bounds[row][0] <= j < bounds[row][1]  and  p - before <= j <= p + after
+ * (prefix and bounds may be NULL: no prefix, no bounds; row counts q's rows; -1: no limit).  before = -1, after = 0 is causal, a prefix beside
+ * it a prefix mask, bounds of laya_op_document_bounds a document mask.  Then
+ *   t = scale q . k;  t = cap tanh(t / cap) if cap > 0;  t -= slopes[h] |j - p|  or  t += table[h][clamp(j - p, -span, span) + span];
+ *   out = sum of softmax(t) v over the keys seen.
+ * A query that sees no key, or whose scores are all below -1e30 (biases of a type's lowest value hide keys), gets zeros; what lies in
+ * hidden keys, NaNs and infinities too, does not matter.  out's rows of no query are left as they were. */
+typedef struct LayaAttend {
+  uint32_t struct_bytes;  /* sizeof(LayaAttend) */
+  int32_t dtype;          /* LAYA_F16 or LAYA_BF16: q, k, v, out */
+  const void* q;          /* [q_rows][heads][dim] */
+  const void* k;          /* [k_rows][kv_heads][dim] */
+  const void* v;          /* [k_rows][kv_heads][dim] */
+  void* out;              /* [q_rows][heads][dim]; overlaps nothing */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  /* strides in elements */
+  int32_t heads, kv_heads, dim;
+  int32_t q_rows, k_rows;
+  int32_t n_seq, max_q, max_k;  /* sequences, and the most queries and keys that one has */
+  const int32_t* q_starts;
+  const int32_t* q_lengths;
+  const int32_t* k_starts;
+  const int32_t* k_lengths;
+  float scale, cap;       /* cap 0: none */
+  const float* slopes;    /* [heads], or NULL */
+  const float* table;     /* [heads][2 span + 1], or NULL; not both */
+  int32_t span;
+  int32_t before, after;
+  const int32_t* prefix;  /* [n_seq], or NULL */
+  const int32_t* bounds;  /* [q_rows][2], or NULL */
+} LayaAttend;
+
+/* Bytes of workspace that laya_op_attend needs for this call: 0 unless long keys of few queries are shared by several
+ * workgroups.  Depends on the sizes, before, and whether there is a prefix, not on pointers; -1 for sizes that are refused.  Host-only. */
+int64_t laya_attend_workspace(const LayaAttend* call);
+
+/* The attention described above, sums and softmax in fp32, weights rounded to dtype for the matrix unit, one rounding of the
+ * output.  Lengths of zero are fine.  dim a multiple of 8 up to 256, heads a multiple of kv_heads; q, k, v and out and
+ * their strides on whole 16 bytes, row strides of k and v at least dim and below 2^23; scale >= 0, cap >= 0, both finite, cap a normal number;
+ * span 0 to 1024 with a table; rows, max_q, max_k, before and after below 2^30.  workspace: device memory, 16-byte
+ * aligned, of the bytes that laya_attend_workspace tells (NULL for 0), written before it is read; calls that may run at
+ * the same time, captured ones too, take different ones.  Equal calls give equal bits. */
+int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,576 @@
+// Attention over packed sequences: prompts, single tokens and what lies between (attend_core.hpp has what they share).
+//
+// Compiled once for each head width (LAYA_ATTEND_DIM), and once without for what is no kernel of a width.
+#include "attend_core.hpp"
+
+#include <type_traits>
+
+namespace laya {
+
+#ifdef LAYA_ATTEND_DIM
+
+namespace {
+
+// Prompts: a workgroup of four waves owns 128 queries of one head, and blocks of 64 keys pass through LDS, shared by the waves.
+// While the softmax of block j runs, the wave's matrix instructions are the products of block j - 1 with V and the scores of
+// block j + 1, which do not depend on it.  Step j waits for K(j + 1) and V(j - 1), loaded during the step before, and starts
+// K(j + 2) and V(j) into the buffers of K(j) and V(j - 2), whose reads the barrier has ended.
+template <typename T, int D, bool kCap, DistanceBias kBias>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void attend_kernel(
+    AttendArgs a, int tiles, int unit, int units) {
+  constexpr int KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
+  typedef Rows<T, D, KB, kCap, kBias> R;
+  typedef typename R::T8 T8;
+  typedef typename Vec4<T>::type T4;
+  // Workgroup -> (sequence, head, tile).  Workgroups go round the 8 XCDs by their number: a unit (the tiles of one head, or of
+  // the heads that share keys) stays on one XCD, so that its keys come into one L2 once; tiles with the most keys first.
+  int pair, tile;
+  {
+    const int id = blockIdx.x;
+    if (unit) {
+      const int y = id >> 3, at = y / (tiles * unit), w = y - at * tiles * unit;
+      const int u = (id & 7) + 8 * at;
+      if (u >= units) return;
+      const int t = w / unit;
+      tile = tiles - 1 - t;
+      pair = u * unit + (w - t * unit);
+    } else {
+      const int t = id / units;
+      tile = tiles - 1 - t;
+      pair = id - t * units;
+    }
+  }
+  const int s = pair / a.heads, head = pair - s * a.heads, kv = head / a.group;
+  const Sequence sq = sequence(a, s);
+  const int row0 = tile * 128;
+  if (row0 >= sq.nq) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = row0 + wave * 32 + (lane & 31);
+  const bool valid = i < sq.nq;
+  const bool active = row0 + wave * 32 < sq.nq;  // waves past the last query only stage keys
+  const Seen me = valid ? seen(a, sq, i) : Seen{i + sq.nk - sq.nq, 0, 0};
+
+  __shared__ __align__(16) T sk[2][KB * P];
+  __shared__ __align__(16) T sv[2][KB * P];
+  __shared__ int wg_lo[4], wg_hi[4];
+  constexpr int kPad = KB + 32;  // distances past the span that a block near its ends reaches
+  __shared__ float stable[kBias == DistanceBias::Table ? 2 * (kMaxSpan + kPad) + 1 : 1];
+
+  const Range range = wave_range(me, valid);
+  if (lane == 0) {
+    wg_lo[wave] = range.lo;
+    wg_hi[wave] = range.hi;
+  }
+  if constexpr (kBias == DistanceBias::Table) {
+    const float* from = a.table + static_cast<size_t>(head) * (2 * a.span + 1);
+    for (int e = tid; e < 2 * (a.span + kPad) + 1; e += 256) stable[e] = from[max(0, min(2 * a.span, e - kPad))] * kLog2e;
+  }
+  __syncthreads();
+  const int klo = __builtin_amdgcn_readfirstlane(min(min(wg_lo[0], wg_lo[1]), min(wg_lo[2], wg_lo[3])));
+  const int khi = __builtin_amdgcn_readfirstlane(max(max(wg_hi[0], wg_hi[1]), max(wg_hi[2], wg_hi[3])));
+  const Blocks<KB> blocks(sq.prefix, klo, khi);
+  const int nb = blocks.count;
+
+  const T* K = static_cast<const T*>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
+  const T* V = static_cast<const T*>(a.v) + sq.k0 * a.v_row + kv * a.v_head;
+  const T* Q = static_cast<const T*>(a.q) + (sq.q0 + (valid ? i : 0)) * a.q_row + head * a.q_head;
+
+  // This thread's 16-byte chunks of a block: row r0 + step m, chunk index swizzled by the row.
+  constexpr int CH = KB * kChunks / 256, step = 256 / kChunks;
+  const int r0 = tid / kChunks, c0 = tid % kChunks;
+  const unsigned lds_k[2] = {lds_address(sk[0]), lds_address(sk[1])}, lds_v[2] = {lds_address(sv[0]), lds_address(sv[1])};
+  auto stage = [&](const T* base, long long row, int j, unsigned lds, auto swizzle) {
+    const int key = blocks.key(j);
+    const i32x4 rs = block_resource(base, row, key, min(KB, sq.nk - key), a.dim);
+#pragma unroll
+    for (int m = 0; m < CH; ++m) {
+      const int r = r0 + m * step, c = c0 ^ swizzle(r);
+      const unsigned at = c * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(row) + 16u * c : kNoChunk;
+      lds_load16_buffer<true>(rs, at, 0u, lds + (wave + 4u * m) * 1024u);
+    }
+  };
+  auto load_k = [&](int j, int buf) { stage(K, a.k_row, j, lds_k[buf], [](int r) { return Block<D>::k_swizzle(r); }); };
+  auto load_v = [&](int j, int buf) { stage(V, a.v_row, j, lds_v[buf], [](int r) { return Block<D>::v_swizzle(r); }); };
+
+  R rows;
+  rows.start(lane);
+  if (nb > 0) load_k(0, 0);
+  rows.load_q(Q, a.dim, valid);
+  rows.lo = me.lo;
+  rows.hi = me.hi;
+  rows.prefix = sq.prefix;
+  rows.position = me.position;
+  rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
+  rows.table = stable + a.span + kPad;
+  if (nb > 1) load_k(1, 1);
+
+  f32x16 sc[2][2];
+  T8 p[4];
+  // Whether every key of the block is seen by every row.
+  auto whole = [&](int key) { return key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi); };
+  float far_left = 0.f, far_right = 0.f;
+  if constexpr (kBias == DistanceBias::Table) {
+    far_left = stable[0];
+    far_right = stable[2 * (a.span + kPad)];
+  }
+  const int first_position = __builtin_amdgcn_readfirstlane(me.position);
+  auto softmax = [&](f32x16 (&t)[2], int key, auto edge) {
+    if constexpr (kBias == DistanceBias::Table) {
+      // Blocks wholly past the span on one side add that end's value; the table's LDS rows reach no further than the others need.
+      const bool left = key + KB - 1 - first_position <= -a.span, right = key - (first_position + 31) >= a.span;
+      if (left || right) {
+        const float b = left ? far_left : far_right;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float x = t[kt][r];
+            if constexpr (kCap) t[kt][r] = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f), -2.0f * a.cap, a.cap) + b;
+            else t[kt][r] = __builtin_fmaf(x, a.scale, b);
+          }
+      } else {
+        rows.template change<true>(a, t, key);
+      }
+    } else {
+      rows.template change<true>(a, t, key);
+    }
+    if constexpr (decltype(edge)::value) rows.hide(t, key);
+  };
+  auto body = [&](int j, auto parity, auto edge) {
+    constexpr int X = decltype(parity)::value;
+    if (j > 0) rows.weigh((LdsBytes)(sv[X ^ 1]), p);
+    softmax(sc[X], blocks.key(j), edge);
+    float sum = rows.weights(a, sc[X], p);
+    rows.scores((LdsBytes)(sk[X ^ 1]), sc[X ^ 1]);  // past the last block: of stale keys, never used
+    rows.total += rows.move(a, sc[X], p, sum);
+  };
+  auto turn = [&](int j, auto parity) {
+    constexpr int X = decltype(parity)::value;
+    publish_stage<waitcnt_vm(0)>();
+    if (j + 2 < nb) load_k(j + 2, X);
+    load_v(j, X);
+    if (!active) return;
+    if (whole(blocks.key(j))) body(j, parity, std::false_type());
+    else body(j, parity, std::true_type());
+  };
+  publish_stage<waitcnt_vm(0)>();
+  if (nb > 0) {
+    if (active) rows.scores((LdsBytes)(sk[0]), sc[0]);
+    for (int j = 0; j < nb; j += 2) {
+      turn(j, std::integral_constant<int, 0>());
+      if (j + 1 < nb) turn(j + 1, std::integral_constant<int, 1>());
+    }
+    publish_stage<waitcnt_vm(0)>();
+    if (active) rows.weigh((LdsBytes)(sv[(nb - 1) & 1]), p);
+  }
+  if (!active) return;
+
+  T* out = static_cast<T*>(a.out) + head * a.out_head;
+  const unsigned live = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(valid));
+  unsigned bad = rows.not_numbers() & live;
+  const float total = halves_sum(rows.total);
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  if (valid && !(bad >> (lane & 31) & 1)) {
+    T* row = out + (sq.q0 + i) * a.out_row;
+#pragma unroll
+    for (int d = 0; d < R::DT; ++d)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int at = 32 * d + 8 * r4 + 4 * rows.g;
+        T4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_half<T>(rows.o[d][4 * r4 + e] * inv);
+        if (at < a.dim) *reinterpret_cast<T4*>(row + at) = v;
+      }
+  }
+  while (bad) {
+    const int b = __builtin_ctz(bad);
+    bad &= bad - 1;
+    const int ib = row0 + wave * 32 + b;
+    const Seen m = seen(a, sq, ib);
+    CarefulRow<T, D, KB, kCap, kBias> c;
+    c.run(a, static_cast<const T*>(a.q) + (sq.q0 + ib) * a.q_row + head * a.q_head, K, V, sq.nk, m.position, m.lo, m.hi, sq.prefix,
+          rows.slope, a.table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr, blocks, 0, nb, lane);
+    const float n = c.total == 0.f ? 0.f : 1.0f / c.total;
+#pragma unroll
+    for (int x = 0; x < c.ND; ++x)
+      if (lane + 64 * x < a.dim) out[(sq.q0 + ib) * a.out_row + lane + 64 * x] = to_half<T>(c.sum[x] * n);
+  }
+}
+
+// Few rows: a workgroup owns 32 rows, the (token, head) pairs of the heads that share keys, and its waves split their keys into
+// blocks of 32, each wave with two stages of its own in LDS: while it works on one, the other's loads are on their way.  Long
+// contexts are shared by a.splits workgroups, whose sums join_kernel adds.
+template <typename T, int D, bool kCap, DistanceBias kBias>
+__global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 2 : 1))) void attend_split_kernel(AttendArgs a) {
+  constexpr int KB = 32, NW = D <= 128 ? 4 : 2, NT = 64 * NW, P = Block<D>::kPitch, kChunks = P / 8;
+  typedef Rows<T, D, KB, kCap, kBias> R;
+  typedef typename R::T8 T8;
+  typedef typename Vec4<T>::type T4;
+  constexpr int kStage = 2 * KB * P;  // elements: a block of K, one of V
+  constexpr int OP = D + 1;           // pitch of a row of sums (floats)
+  static_assert(NW * 2 * kStage * sizeof(T) >= NW * 32 * OP * sizeof(float), "the waves' sums fit the stages");
+  __shared__ __align__(16) T lds[NW * 2 * kStage];
+  __shared__ float s_reference[NW][32], s_total[NW][32];
+  __shared__ int s_bad[32];
+
+  int id = blockIdx.x;
+  const int z = id % a.splits;
+  id /= a.splits;
+  const int tile = id % a.row_tiles;
+  id /= a.row_tiles;
+  const int kv = id % a.kv_heads, s = id / a.kv_heads;
+  const Sequence sq = sequence(a, s);
+  const int n_rows = sq.nq * a.group;  // below 2^31: the host's check of max_q * group
+  if (tile * 32 >= n_rows) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = tile * 32 + (lane & 31);
+  const bool valid = row < n_rows;
+  const int i = valid ? row / a.group : 0, head = kv * a.group + (valid ? row - i * a.group : 0);
+  const Seen me = valid ? seen(a, sq, i) : Seen{0, 0, 0};
+  const Range range = wave_range(me, valid);
+  const Blocks<KB> blocks(sq.prefix, range.lo, range.hi);
+  const int each = (blocks.count + a.splits - 1) / a.splits;
+  const int j0 = min(blocks.count, z * each), j1 = min(blocks.count, j0 + each);
+
+  const T* K = static_cast<const T*>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
+  const T* V = static_cast<const T*>(a.v) + sq.k0 * a.v_row + kv * a.v_head;
+
+  constexpr int CH = KB * kChunks / 64, step = 64 / kChunks;
+  const int r0 = lane / kChunks, c0 = lane % kChunks;
+  const unsigned stage0 = lds_address(lds + wave * 2 * kStage);
+  auto stage = [&](int j, int buf) {
+    const int key = blocks.key(j), left = min(KB, sq.nk - key);
+    const i32x4 rk = block_resource(K, a.k_row, key, left, a.dim), rv = block_resource(V, a.v_row, key, left, a.dim);
+    const unsigned to = stage0 + buf * static_cast<unsigned>(kStage * sizeof(T));
+#pragma unroll
+    for (int m = 0; m < CH; ++m) {
+      const int r = r0 + m * step, c = c0 ^ Block<D>::k_swizzle(r);
+      const unsigned at = c * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.k_row) + 16u * c : kNoChunk;
+      lds_load16_buffer<true>(rk, at, 0u, to + m * 1024u);
+    }
+#pragma unroll
+    for (int m = 0; m < CH; ++m) {
+      const int r = r0 + m * step, c = c0 ^ Block<D>::v_swizzle(r);
+      const unsigned at = c * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.v_row) + 16u * c : kNoChunk;
+      lds_load16_buffer<true>(rv, at, 0u, to + KB * P * 2u + m * 1024u);
+    }
+  };
+
+  R rows;
+  rows.start(lane);
+  rows.load_q(static_cast<const T*>(a.q) + (sq.q0 + i) * a.q_row + head * a.q_head, a.dim, valid);
+  rows.lo = me.lo;
+  rows.hi = me.hi;
+  rows.prefix = sq.prefix;
+  rows.position = me.position;
+  rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
+  rows.table = kBias == DistanceBias::Table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr;
+
+  int j = j0 + wave;
+  if (j < j1) stage(j, 0);
+  auto body = [&](int jj, int buf, auto edge) {
+    const LdsBytes k = (LdsBytes)(lds + (wave * 2 + buf) * kStage);
+    f32x16 sc[1];
+    T8 p[2];
+    rows.scores(k, sc);
+    rows.template change<false>(a, sc, blocks.key(jj));
+    if constexpr (decltype(edge)::value) rows.hide(sc, blocks.key(jj));
+    const float sum = rows.weights(a, sc, p);
+    rows.total += rows.move(a, sc, p, sum);
+    rows.weigh(k + KB * P * 2, p);
+  };
+  for (int buf = 0; j < j1; j += NW, buf ^= 1) {
+    const int key = blocks.key(j);
+    // The other stage's reads ended before its loads start: LDS answers a wave in order, and this waits for them.
+    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0_keep_vm());
+    asm volatile("" ::: "memory");
+    if (j + NW < j1) {
+      stage(j + NW, buf ^ 1);
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(2 * CH));  // all but the loads just issued
+    } else {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));
+    }
+    asm volatile("" ::: "memory");
+    if (key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi)) body(j, buf, std::false_type());
+    else body(j, buf, std::true_type());
+  }
+
+  // The waves' sums join: sum_w 2^(m_w - M) O_w and sum_w 2^(m_w - M) l_w.
+  if (tid < 32) s_bad[tid] = 0;
+  __syncthreads();  // every wave is done with its stages
+  float* so = reinterpret_cast<float*>(lds);
+  {
+    const unsigned bad = rows.not_numbers();
+    const float total = halves_sum(rows.total);
+    if (rows.g == 0) {
+      s_reference[wave][lane & 31] = rows.reference;
+      s_total[wave][lane & 31] = total;
+      if (valid && (bad >> lane & 1)) s_bad[lane] = 1;  // every writer writes 1
+    }
+    float* mine = so + (wave * 32 + (lane & 31)) * OP;
+#pragma unroll
+    for (int d = 0; d < R::DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[32 * d + 8 * (r >> 2) + 4 * rows.g + (r & 3)] = rows.o[d][r];
+  }
+  __syncthreads();
+  constexpr int DPT = D * 32 / NT;
+  static_assert(DPT % 4 == 0, "whole quads a thread");
+  const long long slot = ((static_cast<long long>(s) * a.kv_heads + kv) * a.row_tiles + tile) * a.splits + z;
+  float* part = a.parts + slot * 32 * a.dim;
+  float* ml = a.parts + static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * a.splits * 32 * a.dim + slot * 64;
+  T* out = static_cast<T*>(a.out);
+  {
+    const int mr = tid % 32, d0 = tid / 32 * DPT;
+    const int orow = tile * 32 + mr;
+    if (orow < n_rows && !s_bad[mr]) {
+      float m = kNothing;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, s_reference[w][mr]);
+      float wt[NW], total = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        wt[w] = __builtin_amdgcn_exp2f(s_reference[w][mr] - m);
+        total += wt[w] * s_total[w][mr];
+      }
+      const int oi = orow / a.group, oh = kv * a.group + orow - oi * a.group;
+      T* to = out + (sq.q0 + oi) * a.out_row + oh * a.out_head;
+      const float inv = a.splits > 1 ? 1.f : total == 0.f ? 0.f : 1.0f / total;
+#pragma unroll
+      for (int e = 0; e < DPT; e += 4) {
+        if (d0 + e >= a.dim) continue;
+        f32x4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < NW; ++w) sum += wt[w] * so[(w * 32 + mr) * OP + d0 + e + x];
+          v[x] = sum * inv;
+        }
+        if (a.splits > 1) {
+          *reinterpret_cast<f32x4*>(part + mr * a.dim + d0 + e) = v;
+        } else {
+          T4 h;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) h[x] = to_half<T>(v[x]);
+          *reinterpret_cast<T4*>(to + d0 + e) = h;
+        }
+      }
+      if (a.splits > 1 && d0 == 0) {
+        ml[2 * mr] = m;
+        ml[2 * mr + 1] = total;
+      }
+    }
+  }
+  for (int b = wave; b < 32; b += NW) {
+    if (!s_bad[b]) continue;
+    const int orow = tile * 32 + b, oi = orow / a.group, oh = kv * a.group + orow - oi * a.group;
+    const Seen m = seen(a, sq, oi);
+    CarefulRow<T, D, KB, kCap, kBias> c;
+    c.run(a, static_cast<const T*>(a.q) + (sq.q0 + oi) * a.q_row + oh * a.q_head, K, V, sq.nk, m.position, m.lo, m.hi, sq.prefix,
+          kBias == DistanceBias::Slopes ? a.slopes[oh] * kLog2e : 0.f,
+          a.table ? a.table + static_cast<size_t>(oh) * (2 * a.span + 1) + a.span : nullptr, blocks, j0, j1, lane);
+    const float n = c.total == 0.f ? 0.f : 1.0f / c.total;
+#pragma unroll
+    for (int x = 0; x < c.ND; ++x) {
+      const int d = lane + 64 * x;
+      if (d >= a.dim) continue;
+      if (a.splits > 1) part[b * a.dim + d] = c.sum[x];
+      else out[(sq.q0 + oi) * a.out_row + oh * a.out_head + d] = to_half<T>(c.sum[x] * n);
+    }
+    if (a.splits > 1 && lane == 0) {
+      ml[2 * b] = c.reference;
+      ml[2 * b + 1] = c.total;
+    }
+  }
+}
+
+template <typename T, int D, bool kCap, DistanceBias kBias>
+hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
+  if (split) {
+    const unsigned grid = static_cast<unsigned>(static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * a.splits);
+    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(grid), dim3(D <= 128 ? 256 : 128), 0, stream, a);
+    return hipGetLastError();
+  }
+  const int tiles = (a.max_q + 127) / 128;
+  const long long pairs = static_cast<long long>(a.n_seq) * a.heads, shared = static_cast<long long>(a.n_seq) * a.kv_heads;
+  // Heads that share keys on one XCD, or each head, where that fills the XCDs evenly; else every tile for itself.
+  int unit = shared % 8 == 0 || shared >= 64 ? a.group : pairs % 8 == 0 || pairs >= 64 ? 1 : 0;
+  const long long units = unit ? pairs / unit : pairs;
+  const long long grid = unit ? (units + 7) / 8 * 8 * unit * tiles : pairs * tiles;
+  LAYA_LAUNCH((attend_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a, tiles, unit,
+              static_cast<int>(units));
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_type(const AttendArgs& a, DistanceBias bias, bool cap, bool split, hipStream_t stream) {
+  switch (bias) {
+    case DistanceBias::None:
+      return cap ? launch_kind<T, D, true, DistanceBias::None>(a, split, stream) : launch_kind<T, D, false, DistanceBias::None>(a, split, stream);
+    case DistanceBias::Slopes:
+      return cap ? launch_kind<T, D, true, DistanceBias::Slopes>(a, split, stream)
+                 : launch_kind<T, D, false, DistanceBias::Slopes>(a, split, stream);
+    default:
+      return cap ? launch_kind<T, D, true, DistanceBias::Table>(a, split, stream)
+                 : launch_kind<T, D, false, DistanceBias::Table>(a, split, stream);
+  }
+}
+
+}  // namespace
+
+template <>
+hipError_t launch_attend_dim<LAYA_ATTEND_DIM>(const AttendArgs& a, DType t, DistanceBias bias, bool cap, bool split, hipStream_t stream) {
+  return t == DType::F16 ? launch_type<f16, LAYA_ATTEND_DIM>(a, bias, cap, split, stream)
+                         : launch_type<bf16, LAYA_ATTEND_DIM>(a, bias, cap, split, stream);
+}
+
+#else  // what is no kernel of a width
+
+template <> hipError_t launch_attend_dim<64>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
+template <> hipError_t launch_attend_dim<96>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
+template <> hipError_t launch_attend_dim<128>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
+template <> hipError_t launch_attend_dim<256>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
+
+namespace {
+
+// A row's sums over the splits: weights 2^(m_z - M), then one division.  A wave a row; a lane a split, then a lane a dim.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long long at = static_cast<long long>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long tiles = static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles;
+  const long long tile = at / 32;
+  const int r = static_cast<int>(at % 32);
+  if (tile >= tiles) return;
+  const int s = static_cast<int>(tile / (a.kv_heads * a.row_tiles)), w = static_cast<int>(tile % (a.kv_heads * a.row_tiles));
+  const int kv = w / a.row_tiles, row = w % a.row_tiles * 32 + r;
+  const int q0 = a.q_starts[s];
+  const int nq = q0 < 0 || q0 >= a.q_rows ? 0 : min(min(a.q_lengths[s], a.max_q), a.q_rows - q0);
+  const int i = row / a.group;
+  if (i >= nq) return;
+  const float* parts = a.parts + tile * a.splits * 32 * a.dim + r * a.dim;
+  const float2* ml = reinterpret_cast<const float2*>(a.parts + tiles * a.splits * 32 * a.dim) + tile * a.splits * 32 + r;
+  float m = kNothing, l = 0.f;
+  if (lane < a.splits) {
+    const float2 x = ml[lane * 32];
+    m = x.x;
+    l = x.y;
+  }
+  const float top = wave_max(m);
+  const float weight = __builtin_amdgcn_exp2f(m - top);
+  const float total = wave_sum(weight * l);
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  float sum[kMaxAttendDim / 64] = {0.f, 0.f, 0.f, 0.f};
+  for (int z = 0; z < a.splits; ++z) {
+    const float f = __shfl(weight, z, kWave);
+#pragma unroll
+    for (int x = 0; x < kMaxAttendDim / 64; ++x)
+      if (lane + 64 * x < a.dim) sum[x] += f * parts[static_cast<long long>(z) * 32 * a.dim + lane + 64 * x];
+  }
+  T* out = static_cast<T*>(a.out) + (q0 + i) * a.out_row + (kv * a.group + row - i * a.group) * a.out_head;
+#pragma unroll
+  for (int x = 0; x < kMaxAttendDim / 64; ++x)
+    if (lane + 64 * x < a.dim) out[lane + 64 * x] = to_half<T>(sum[x] * inv);
+}
+
+// The run of equal ids around each row of a sequence.  A wave takes 64 rows: where ids change comes from one ballot, and what
+// begins before or ends behind them is looked for 512 rows at a time.
+__global__ __launch_bounds__(256) void document_bounds_kernel(BoundsArgs a, int groups) {
+  const int s = blockIdx.x / groups, lane = threadIdx.x & 63;
+  const int start = __builtin_amdgcn_readfirstlane(a.starts[s]);
+  int n = __builtin_amdgcn_readfirstlane(a.lengths[s]);
+  n = start < 0 || start >= a.rows ? 0 : max(0, min(min(n, a.max_length), a.rows - start));
+  const int i0 = (static_cast<int>(blockIdx.x % groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64;
+  if (i0 >= n) return;
+  const int32_t* ids = a.documents + start;
+  const int i = i0 + lane, last = min(n, i0 + 64) - 1;
+  const int mine = ids[min(i, n - 1)], before = ids[max(0, min(i, n - 1) - 1)];
+  const unsigned long long begins = __builtin_amdgcn_ballot_w64(i < n && (i == 0 || mine != before));
+  // First row of the run that row i0 lies in, and the end of the one that row `last` lies in.
+  int first = i0, end = last + 1;
+  if (!(begins & 1)) {
+    const int id = __builtin_amdgcn_readfirstlane(mine);
+    for (first = 0;;) {  // ends where a row differs, or before row 0
+      int found = -1;
+      const int from = i0 - 1 - first;  // rows above it are of the run
+      for (int c = 7; c >= 0; --c) {
+        const int at = from - 64 * c - lane;
+        const unsigned long long other = __builtin_amdgcn_ballot_w64(at < 0 || ids[max(at, 0)] != id);
+        if (other) found = 64 * c + __builtin_ctzll(other);
+      }
+      if (found >= 0) {
+        first = from - found + 1;
+        break;
+      }
+      first += 512;
+    }
+  }
+  {
+    const int id = __builtin_amdgcn_readfirstlane(ids[last]);
+    for (int gone = 0;; gone += 512) {
+      int found = -1;
+      for (int c = 7; c >= 0; --c) {
+        const int at = last + 1 + gone + 64 * c + lane;
+        const unsigned long long other = __builtin_amdgcn_ballot_w64(at >= n || ids[min(at, n - 1)] != id);
+        if (other) found = 64 * c + __builtin_ctzll(other);
+      }
+      if (found >= 0) {
+        end = last + 1 + gone + found;
+        break;
+      }
+    }
+  }
+  if (i >= n) return;
+  const unsigned long long upto = begins & (~0ull >> (63 - lane)), behind = lane == 63 ? 0 : begins >> (lane + 1);
+  const int lo = upto ? i0 + 63 - __builtin_clzll(upto) : first;
+  const int hi = behind ? i + 1 + __builtin_ctzll(behind) : end;
+  a.bounds[start + i] = make_int2(lo, hi);
+}
+
+}  // namespace
+
+AttendPlan attend_plan(const AttendArgs& a) {
+  AttendPlan p{};
+  const long long few = static_cast<long long>(a.max_q) * a.group;
+  const long long prompt = static_cast<long long>((a.max_q + 127) / 128) * a.n_seq * a.heads;
+  p.split = few <= 32 || prompt < 256;
+  p.row_tiles = static_cast<int>((few + 31) / 32);
+  p.splits = 1;
+  if (!p.split) return p;
+  long long keys = a.max_k;
+  if (a.before >= 0 && !a.prefix) keys = keys < static_cast<long long>(a.before) + a.max_q + 64 ? keys : static_cast<long long>(a.before) + a.max_q + 64;
+  const long long base = static_cast<long long>(a.n_seq) * a.kv_heads * p.row_tiles;
+  const long long wanted = 1024 / (base > 0 ? base : 1), most = keys / 512;
+  long long n = wanted < most ? wanted : most;
+  p.splits = static_cast<int>(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
+  if (p.splits > 1) p.workspace = base * p.splits * 32 * (a.dim + 2) * 4;
+  return p;
+}
+
+hipError_t launch_attend(const AttendArgs& args, DType t, DistanceBias bias, bool cap, const AttendPlan& plan, hipStream_t stream) {
+  AttendArgs a = args;
+  a.row_tiles = plan.row_tiles;
+  a.splits = plan.splits;
+  const hipError_t e = a.dim <= 64    ? launch_attend_dim<64>(a, t, bias, cap, plan.split, stream)
+                       : a.dim <= 96  ? launch_attend_dim<96>(a, t, bias, cap, plan.split, stream)
+                       : a.dim <= 128 ? launch_attend_dim<128>(a, t, bias, cap, plan.split, stream)
+                                      : launch_attend_dim<256>(a, t, bias, cap, plan.split, stream);
+  if (e != hipSuccess || plan.splits <= 1) return e;
+  const long long rows = static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * 32;
+  const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
+  if (t == DType::F16) LAYA_LAUNCH(join_kernel<f16>, grid, dim3(256), 0, stream, a);
+  else LAYA_LAUNCH(join_kernel<bf16>, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_document_bounds(const BoundsArgs& a, hipStream_t stream) {
+  const int groups = (a.max_length + 255) / 256;
+  LAYA_LAUNCH(document_bounds_kernel, dim3(static_cast<unsigned>(static_cast<long long>(groups) * a.n_seq)), dim3(256), 0, stream, a, groups);
+  return hipGetLastError();
+}
+
+#endif
+
+}  // namespace laya

@@ -1,0 +1,68 @@
+// Attention over packed sequences with key ranges, capped scores and distance biases: arguments and plan.
+#pragma once
+
+#include "kernels.hpp"
+
+namespace laya {
+
+constexpr int kMaxSpan = 1024;     // of a bias table: its head's row lies in LDS
+constexpr int kMaxAttendDim = 256;
+constexpr int kMaxSplits = 64;     // of a sequence's keys over workgroups: one lane each when they are joined
+
+enum class DistanceBias : int { None = 0, Slopes = 1, Table = 2 };
+
+struct AttendArgs {
+  const void *q, *k, *v;
+  void* out;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
+  int heads, kv_heads, group, dim;  // group = heads / kv_heads
+  int n_seq, max_q, max_k, q_rows, k_rows;
+  const int32_t *q_starts, *q_lengths, *k_starts, *k_lengths;  // [n_seq]
+  float scale;           // of a raw product: to log2 units, or, capped, to twice the tanh's argument in log2 units
+  float cap;             // in log2 units
+  const float* slopes;   // [heads]
+  const float* table;    // [heads][2 span + 1]
+  int span;
+  int before, after;     // -1: no limit
+  const int32_t* prefix; // [n_seq] or null
+  const int2* bounds;    // [q_rows] (first, end) or null
+  // Split plan: row tiles of 32 (token, head) rows, and how many workgroups share a tile's keys.
+  int row_tiles, splits;
+  float* parts;          // [n_seq][kv_heads][row_tiles][splits][32][dim] sums, then as many [32][2] of reference and total
+};
+
+// The launch of a call: which kernel, and for the split one its row tiles and splits; workspace in bytes.
+struct AttendPlan {
+  bool split;
+  int row_tiles, splits;
+  long long workspace;
+};
+AttendPlan attend_plan(const AttendArgs& a);
+
+template <int D>  // the compiled head widths
+hipError_t launch_attend_dim(const AttendArgs& a, DType t, DistanceBias bias, bool cap, bool split, hipStream_t stream);
+hipError_t launch_attend(const AttendArgs& a, DType t, DistanceBias bias, bool cap, const AttendPlan& plan, hipStream_t stream);
+
+struct BoundsArgs {
+  const int32_t* documents;  // [rows]
+  const int32_t *starts, *lengths;
+  int n_seq, rows, max_length;
+  int2* bounds;
+};
+hipError_t launch_document_bounds(const BoundsArgs& a, hipStream_t stream);
+
+struct RotaryArgs {
+  const void* x;
+  void* out;
+  long long x_row, x_head, out_row, out_head;  // elements
+  const int32_t* positions;  // [rows]
+  const double* turns;       // [rotated / 2] turns a position
+  float amplitude, direction;
+  long long rows;
+  int heads, dim, rotated;
+  bool interleaved, in_place;
+  int rows_each;             // rows a workgroup (the launcher's)
+};
+hipError_t launch_rotary(const RotaryArgs& a, DType t, hipStream_t stream);
+
+}  // namespace laya

@@ -1,0 +1,369 @@
+// Device parts that the kernels of attend.hip share: a sequence's ranges, what a row sees, a block's scores, weights and sums.
+//
+// A wave holds 32 query rows as the columns of S^T = K Q^T (v_mfma_f32_32x32x16, keys as rows): lane (row l % 32, g = l / 32)
+// gets the scores of keys 8 (r / 4) + 4 g + r % 4 of each 32, so a row's softmax crosses lanes once (l and l ^ 32), and its 16-bit
+// weights are already the B operand of O^T = V^T P^T.  V's rows lie in LDS as they lie in memory, a key each; its transpose
+// comes from ds_read_b64_tr_b16, in which 16 lanes read four keys' 16 dims and each gets one dim's four keys.  Key slots e of a
+// group of 16 keys are 4 g + e and 8 + 4 g + e - 4: those whose weights the lane holds.
+//
+// Scores live in log2 units.  A row's reference starts at kNothing and moves to a block's largest score only when the lane's
+// weights pass 2^13 in sum (each is at most that, so fp16 holds it): most blocks need no maximum.  Weights are rounded to 16 bits
+// for the matrix unit, and the normaliser sums the rounded ones.
+#pragma once
+
+#include "attend.hpp"
+
+namespace laya {
+
+constexpr float kNothing = -1e30f;    // the reference of a row that has seen no key; scores not above it count as hidden
+constexpr float kMostWeight = 8192.f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float pair_sum(f16x2 p, float acc) {
+  return __builtin_amdgcn_fdot2(p, f16x2{1.0f16, 1.0f16}, acc, false);
+}
+__device__ __forceinline__ float pair_sum(bf16x2 p, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(p, bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}, acc, false);
+}
+// A value joined with lane l ^ 32's, without LDS.
+__device__ __forceinline__ float halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int rows_min(int v) {  // over 32 lanes; both halves of the wave hold the same rows
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v = min(v, __shfl_xor(v, d, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int rows_max(int v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v = max(v, __shfl_xor(v, d, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// LDS rows of a staged block: kPitch elements, in 16-byte chunks whose index is XORed with a function of the row.  K is read 16
+// rows at one chunk (their 256-byte windows must hold 16 different positions), V four rows at four neighbouring chunks.
+template <int D>
+struct Block {
+  static constexpr int kPitch = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  static constexpr int kChunks = kPitch / 8;
+  __device__ static __forceinline__ int k_swizzle(int row) { return kPitch == 64 ? (row >> 1) & 7 : row & 15; }
+  __device__ static __forceinline__ int v_swizzle(int row) { return kPitch == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
+};
+
+// A sequence's rows, cut to what the arrays hold.
+struct Sequence {
+  int q0, nq, k0, nk, prefix;
+};
+__device__ __forceinline__ Sequence sequence(const AttendArgs& a, int s) {
+  Sequence r;
+  r.q0 = __builtin_amdgcn_readfirstlane(a.q_starts[s]);
+  r.k0 = __builtin_amdgcn_readfirstlane(a.k_starts[s]);
+  const int nq = __builtin_amdgcn_readfirstlane(a.q_lengths[s]), nk = __builtin_amdgcn_readfirstlane(a.k_lengths[s]);
+  r.nq = r.q0 < 0 || r.q0 >= a.q_rows ? 0 : max(0, min(min(nq, a.max_q), a.q_rows - r.q0));
+  r.nk = r.k0 < 0 || r.k0 >= a.k_rows ? 0 : max(0, min(min(nk, a.max_k), a.k_rows - r.k0));
+  r.prefix = a.prefix ? max(0, min(__builtin_amdgcn_readfirstlane(a.prefix[s]), r.nk)) : 0;
+  return r;
+}
+
+// The keys that query i of a sequence sees: those below `prefix`, and [lo, hi).
+struct Seen {
+  int position, lo, hi;
+};
+__device__ __forceinline__ Seen seen(const AttendArgs& a, const Sequence& s, int i) {
+  Seen r;
+  r.position = i + s.nk - s.nq;
+  r.lo = a.before >= 0 ? max(0, r.position - a.before) : 0;
+  r.hi = a.after >= 0 ? min(s.nk, r.position + a.after + 1) : s.nk;
+  if (a.bounds) {
+    const int2 b = a.bounds[s.q0 + i];
+    r.lo = max(r.lo, b.x);
+    r.hi = min(r.hi, b.y);
+  }
+  if (r.lo >= r.hi) r.lo = r.hi = 0;
+  if (r.lo <= s.prefix) {  // one range
+    r.lo = 0;
+    r.hi = max(r.hi, s.prefix);
+  }
+  return r;
+}
+
+// What the 32 rows of a wave see together.  Rows past the sequence's last have no say.
+struct Range {
+  int lo, hi;          // every seen key behind the prefix
+  int all_lo, all_hi;  // keys that all rows see
+};
+__device__ __forceinline__ Range wave_range(const Seen& s, bool valid) {
+  Range r;
+  const bool any = valid && s.lo < s.hi;
+  r.lo = rows_min(any ? s.lo : INT_MAX);
+  r.hi = rows_max(any ? s.hi : 0);
+  r.all_lo = rows_max(valid ? s.lo : 0);
+  r.all_hi = rows_min(valid ? s.hi : INT_MAX);
+  return r;
+}
+
+// The blocks of KB keys that hold a seen key: those of the prefix, then those of a range behind it.
+template <int KB>
+struct Blocks {
+  int first, second, count;  // blocks of the prefix; the range's first block; all
+  __device__ __forceinline__ Blocks(int prefix, int lo, int hi) {
+    first = (prefix + KB - 1) / KB;
+    second = max(first, lo / KB);
+    count = first + (lo < hi ? max(0, (hi + KB - 1) / KB - second) : 0);
+  }
+  __device__ __forceinline__ int key(int j) const { return (j < first ? j : second + j - first) * KB; }
+};
+
+// Buffer resource of the rows [key, min(key + KB, nk)) of one head: what lies behind them reads as zeros.
+template <typename T>
+__device__ __forceinline__ i32x4 block_resource(const T* head, long long row, int key, int rows, int dim) {
+  const uint64_t p = reinterpret_cast<uint64_t>(head + key * row);
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(p));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32) & 0xffff);
+  r[2] = __builtin_amdgcn_readfirstlane(rows <= 0 ? 0 : static_cast<int>(((rows - 1) * row + dim) * 2));
+  r[3] = 0x00020000;
+  asm volatile("s_nop 4" : "+s"(r));  // a load may read an SGPR that a vector instruction wrote only five wait states later
+  return r;
+}
+constexpr unsigned kNoChunk = 0x80000000u;  // an offset behind every resource (they span fewer than 2^31 bytes)
+
+typedef __attribute__((address_space(3))) const char* LdsBytes;
+
+// Per-lane state of 32 rows.
+template <typename T, int D, int KB, bool kCap, DistanceBias kBias>
+struct Rows {
+  typedef typename Vec8<T>::type T8;
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  typedef Block<D> B;
+  static constexpr int KS = D / 16, DT = D / 32, KT = KB / 32;
+  static constexpr bool kRaw = !kCap && kBias == DistanceBias::None;  // scores stay raw products until they become weights
+
+  T8 q[KS];
+  f32x16 o[DT];
+  float reference, total;
+  int lo, hi, prefix, position;
+  float slope;
+  const float* table;  // of this row's head, at distance 0 (in LDS where kLdsTable)
+  int lane, g;
+  unsigned k_at, v_at;  // byte offsets of this lane's first fragments
+
+  __device__ __forceinline__ void start(int l) {
+    lane = l;
+    g = l >> 5;
+    const int ql = l & 31;
+    k_at = 2u * static_cast<unsigned>(ql * B::kPitch + ((g ^ B::k_swizzle(ql)) << 3));
+    const int row = 4 * g + ((l & 15) >> 2), chunk = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+    v_at = 2u * static_cast<unsigned>(row * B::kPitch + ((chunk ^ B::v_swizzle(row)) << 3) + (l & 1) * 4);
+    reference = kNothing;
+    total = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  }
+
+  // Q^T fragments: dims 16 ks + 8 g .. + 7 of the row; zeros behind the head's last and in rows that are none.
+  __device__ __forceinline__ void load_q(const T* row, int dim, bool valid) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int at = 16 * ks + 8 * g;
+      if (valid && at < dim) {
+        q[ks] = *reinterpret_cast<const T8*>(row + at);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[ks][e] = to_half<T>(0.f);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void scores(LdsBytes k, f32x16 (&s)[KT]) const {
+    typedef __attribute__((address_space(3))) const T8* Lds8;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[kt] = mfma32(*(Lds8)(k + (k_at ^ (ks * 32u)) + kt * 64 * B::kPitch), q[ks], s[kt]);
+    }
+  }
+
+  __device__ __forceinline__ void weigh(LdsBytes v, const T8 (&p)[2 * KT]) {  // O^T += V^T P^T
+    typedef __attribute__((address_space(3))) s16x4* Lds4;
+#pragma unroll
+    for (int c = 0; c < 2 * KT; ++c)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const LdsBytes at = v + (v_at ^ (d * 64u)) + c * 32 * B::kPitch;
+        const s16x4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(at));
+        const s16x4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(at + 16 * B::kPitch));
+        const s16x8 both = __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = mfma32(__builtin_bit_cast(T8, both), p[c], o[d]);
+      }
+  }
+
+  // Key of score r of tile kt of the block at `key`, less the lane's first.
+  static constexpr int slot(int kt, int r) { return 32 * kt + 8 * (r >> 2) + (r & 3); }
+
+  // Raw products to log2 scores: cap and bias.  kLdsTable: `table` may be read up to a block and 32 rows past the span.
+  template <bool kLdsTable>
+  __device__ __forceinline__ void change(const AttendArgs& a, f32x16 (&s)[KT], int key) const {
+    if constexpr (!kRaw) {
+      const int at = key + 4 * g - position;
+      const float from = static_cast<float>(at);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x = s[kt][r];
+          if constexpr (kCap) {  // cap tanh(x) = cap - 2 cap / (1 + exp(2 x)); exact to 2^-22 of the cap
+            const float y = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f);
+            x = __builtin_fmaf(y, -2.0f * a.cap, a.cap);
+          }
+          float b = 0.f;
+          if constexpr (kBias == DistanceBias::Slopes) b = -slope * fabsf(from + static_cast<float>(slot(kt, r)));
+          if constexpr (kBias == DistanceBias::Table) {
+            const int d = at + slot(kt, r);
+            b = kLdsTable ? table[d] : table[max(-a.span, min(a.span, d))] * kLog2e;
+          }
+          s[kt][r] = kCap ? x + b : __builtin_fmaf(x, a.scale, b);
+        }
+    }
+  }
+
+  __device__ __forceinline__ void hide(f32x16 (&s)[KT], int key) const {
+    const int at = key + 4 * g;
+    const unsigned seen_keys = static_cast<unsigned>(hi - lo);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = at + slot(kt, r);
+        s[kt][r] = (static_cast<unsigned>(j - lo) < seen_keys || j < prefix) ? s[kt][r] : -INFINITY;
+      }
+  }
+
+  __device__ __forceinline__ float block_max(const AttendArgs& a, const f32x16 (&s)[KT]) const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, s[kt][r]);
+    m = halves_max(m);
+    return kRaw ? m * a.scale : m;
+  }
+
+  __device__ __forceinline__ float weights(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT]) const {
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 2 * KT; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = s[c >> 1][8 * (c & 1) + e];
+        p[c][e] = to_half<T>(__builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x, a.scale, -reference) : x - reference));
+      }
+      sum[0] = pair_sum(__builtin_shufflevector(p[c], p[c], 0, 1), sum[0]);
+      sum[1] = pair_sum(__builtin_shufflevector(p[c], p[c], 2, 3), sum[1]);
+      sum[0] = pair_sum(__builtin_shufflevector(p[c], p[c], 4, 5), sum[0]);
+      sum[1] = pair_sum(__builtin_shufflevector(p[c], p[c], 6, 7), sum[1]);
+    }
+    return sum[0] + sum[1];
+  }
+
+  // Weights that are too large for the reference: it moves to the block's largest score.  Negative scales turn the order of raw
+  // scores round, so the caller's scale is not negative.
+  __device__ __forceinline__ float move(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], float sum) {
+    if (__builtin_amdgcn_ballot_w64(!(sum <= kMostWeight))) {
+      const float m = block_max(a, s);
+      const float to = m > reference + 8.f ? m : reference;
+      const float alpha = to == reference ? 1.f : __builtin_amdgcn_exp2f(reference - to);
+      reference = to;
+      total *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      sum = weights(a, s, p);
+    }
+    return sum;
+  }
+
+  // Rows (bits 0 to 31) whose sums are no numbers: a weight of 0 times an infinity or NaN in a hidden key's value, if nothing
+  // the row sees is one.
+  __device__ __forceinline__ unsigned not_numbers() const {
+    float x = total;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x = __builtin_fmaf(o[d][r], 0.f, x);  // NaN for a NaN or an infinity
+    const unsigned long long bad = __builtin_amdgcn_ballot_w64(x != x);
+    return static_cast<unsigned>(bad | bad >> 32);
+  }
+};
+
+// One row by itself, hidden keys never touched: what a wave does for a row whose sums are no numbers.  Blocks [j0, j1) of
+// the row's tile; lane l holds dims l, l + 64, ...
+template <typename T, int D, int KB, bool kCap, DistanceBias kBias>
+struct CarefulRow {
+  static constexpr int ND = (D + 63) / 64;
+  float sum[ND], reference, total;
+
+  __device__ __forceinline__ void run(const AttendArgs& a, const T* q, const T* k, const T* v, int nk, int position, int lo, int hi,
+                                      int prefix, float slope, const float* table, const Blocks<KB>& blocks, int j0, int j1, int lane) {
+    typedef typename Vec8<T>::type T8;
+    reference = kNothing;
+    total = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) sum[i] = 0.f;
+    for (int j = j0; j < j1; ++j) {
+      const int first = blocks.key(j), key = first + lane;
+      const bool see = lane < KB && key < nk && ((key >= lo && key < hi) || key < prefix);
+      float x = -INFINITY;
+      if (see) {
+        const T* row = k + key * a.k_row;
+        x = 0.f;
+        for (int c = 0; c < a.dim; c += 8) {
+          const T8 kc = *reinterpret_cast<const T8*>(row + c), qc = *reinterpret_cast<const T8*>(q + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = __builtin_fmaf(to_float(kc[e]), to_float(qc[e]), x);
+        }
+        x *= a.scale;
+        if constexpr (kCap) x = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f), -2.0f * a.cap, a.cap);
+        if constexpr (kBias == DistanceBias::Slopes) x -= slope * fabsf(static_cast<float>(key - position));
+        if constexpr (kBias == DistanceBias::Table) x += table[max(-a.span, min(a.span, key - position))] * kLog2e;
+      }
+      const float to = fmaxf(reference, wave_max(x));
+      const float alpha = to == reference ? 1.f : __builtin_amdgcn_exp2f(reference - to);
+      const float p = see ? __builtin_amdgcn_exp2f(x - to) : 0.f;
+      reference = to;
+      total = total * alpha + wave_sum(p);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) sum[i] *= alpha;
+      unsigned long long left = __builtin_amdgcn_ballot_w64(see);
+      while (left) {
+        const int t = __builtin_ctzll(left);
+        left &= left - 1;
+        const float w = __shfl(p, t, kWave);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          if (lane + 64 * i < a.dim) sum[i] = __builtin_fmaf(w, to_float(v[(first + t) * a.v_row + lane + 64 * i]), sum[i]);
+      }
+      if (total != total) break;  // NaN from a seen score: so is every output
+    }
+    if (total != total) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i) sum[i] = total;
+    }
+  }
+};
+
+}  // namespace laya

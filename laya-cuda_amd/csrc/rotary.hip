@@ -1,0 +1,155 @@
+// Rotary positions on strided rows of heads, and the frequencies they take.
+//
+//   angle(row, i) = 2 pi positions[row] turns[i],  (a, b) -> amplitude (a cos - b sin, a sin + b cos)
+//
+// over the pairs i of each head's leading `rotated` values; what lies behind them is copied.  A value is read and written
+// once, so HBM is the bound.  A workgroup takes a few rows: every thread loads its values first, and while they are on their way
+// the workgroup makes the rows' cosines and sines once for all heads, in LDS.  The angle is reduced to an eighth of a turn in
+// 64 bits (a position of a million at 32 bits would be off by 0.06 radians), the sine and cosine of the rest are fp32.
+#include "attend.hpp"
+
+namespace laya {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnits = 4;  // units a thread has in flight
+
+// cos and sin of 2 pi turn.  The nearest quarter turn goes first, in 64 bits: what is left, at most an eighth, rounds to fp32
+// within 2^-28 of a turn.
+__device__ __forceinline__ float2 cos_sin(double turn) {
+  const double quarter = rint(turn * 4.0);
+  const float rest = static_cast<float>(2.0 * turn - 0.5 * quarter);  // in half turns, at most 1/4
+  const float s = sinpif(rest), c = cospif(rest);
+  const int q = static_cast<int>(quarter - 4.0 * floor(quarter * 0.25));
+  const float x = q & 1 ? -s : c, y = q & 1 ? c : s;
+  return q & 2 ? make_float2(-x, -y) : make_float2(x, y);
+}
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+
+// A unit is V pairs (half layout: V values of either half) or V values in a row (interleaved pairs, or values behind the rotated
+// ones, which have no pair).  V: 16 bytes where strides, sizes and addresses allow it, else one pair or value.
+template <typename T, int V, bool kHalf>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+  extern __shared__ float2 table[];  // [rows][pairs], cosine and sine times the amplitude
+  constexpr int kSide = kHalf ? 1 : (V > 1 ? V : 2);  // values a turning unit takes at one place
+  const int pairs = a.rotated / 2;
+  const int turning = kHalf ? pairs / V : a.rotated / kSide;      // units of a head that turn
+  const int copied = a.in_place ? 0 : (a.dim - a.rotated) / V;    // and that are copied
+  const int per_head = turning + copied, per_row = per_head * a.heads;
+  const long long row0 = static_cast<long long>(blockIdx.x) * a.rows_each;
+  const int rows = static_cast<int>(min(static_cast<long long>(a.rows_each), a.rows - row0));
+  const T* x = static_cast<const T*>(a.x);
+  T* out = static_cast<T*>(a.out);
+  // Units of this workgroup: rows * per_row, shared with the other workgroups of blockIdx.y.
+  const int units = rows * per_row;
+  bool made = false;
+  for (int first = blockIdx.y * kThreads * kUnits; first < units || !made; first += gridDim.y * kThreads * kUnits) {
+    Pack<T, V> p[kUnits], q[kUnits];
+    long long to[kUnits];
+    int pair[kUnits], local[kUnits];  // pair -1: a copied unit, -2: none
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int u = first + k * kThreads + static_cast<int>(threadIdx.x);
+      pair[k] = -2;
+      if (u < units) {
+        const int r = u / per_row, w = u - r * per_row;
+        const int h = w / per_head, c = w - h * per_head;
+        const bool turns = c < turning;
+        const int at = turns ? c * (kHalf ? V : kSide) : a.rotated + (c - turning) * V;
+        const T* src = x + (row0 + r) * a.x_row + h * a.x_head + at;
+        to[k] = (row0 + r) * a.out_row + h * a.out_head + at;
+        local[k] = r * pairs;
+        pair[k] = turns ? (kHalf ? at : at / 2) : -1;
+        p[k] = *reinterpret_cast<const Pack<T, V>*>(src);
+        if (turns && (kHalf || V == 1)) q[k] = *reinterpret_cast<const Pack<T, V>*>(src + (kHalf ? pairs : 1));
+      }
+    }
+    if (!made) {
+      for (int i = threadIdx.x; i < rows * pairs; i += kThreads) {
+        const int r = i / pairs;
+        const float2 cs = cos_sin(a.positions[row0 + r] * a.turns[i - r * pairs]);
+        table[i] = make_float2(cs.x * a.amplitude, cs.y * a.amplitude * a.direction);
+      }
+      __syncthreads();
+      made = true;
+    }
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      if (pair[k] == -2) continue;
+      if (pair[k] >= 0) {
+        const float2* cs = table + local[k] + pair[k];
+        if constexpr (kHalf || V == 1) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float u = to_float(p[k].v[e]), w = to_float(q[k].v[e]);
+            p[k].v[e] = to_half<T>(__builtin_fmaf(u, cs[e].x, -(w * cs[e].y)));
+            q[k].v[e] = to_half<T>(__builtin_fmaf(u, cs[e].y, w * cs[e].x));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            const float u = to_float(p[k].v[e]), w = to_float(p[k].v[e + 1]);
+            p[k].v[e] = to_half<T>(__builtin_fmaf(u, cs[e / 2].x, -(w * cs[e / 2].y)));
+            p[k].v[e + 1] = to_half<T>(__builtin_fmaf(u, cs[e / 2].y, w * cs[e / 2].x));
+          }
+        }
+        if constexpr (kHalf || V == 1) *reinterpret_cast<Pack<T, V>*>(out + to[k] + (kHalf ? pairs : 1)) = q[k];
+      }
+      *reinterpret_cast<Pack<T, V>*>(out + to[k]) = p[k];
+    }
+  }
+}
+
+template <typename T>
+bool whole(const RotaryArgs& a) {
+  constexpr long long V = 16 / sizeof(T);
+  const auto fits = [](long long n) { return n % V == 0; };
+  return fits(a.x_row) && fits(a.x_head) && fits(a.out_row) && fits(a.out_head) && fits(a.dim) &&
+         fits(a.interleaved ? a.rotated : a.rotated / 2) && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
+         (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+}
+
+template <typename T, int V, bool kHalf>
+hipError_t launch_v(RotaryArgs a, hipStream_t stream) {
+  const int pairs = a.rotated / 2;
+  const int per_row = ((kHalf ? pairs / V : a.rotated / (V > 1 ? V : 2)) + (a.in_place ? 0 : (a.dim - a.rotated) / V)) * a.heads;
+  // Rows a workgroup: one batch of units, whose tables fit the 32 KB of LDS that leave a CU five workgroups.  With few rows
+  // one each, its units over as many workgroups as hold them (each makes the row's table again).
+  const int batch = kThreads * kUnits;
+  long long each = batch / per_row;
+  if (each > 32768 / (8 * pairs)) each = 32768 / (8 * pairs);
+  if (each > a.rows / 1024) each = a.rows / 1024;
+  if (each < 1) each = 1;
+  a.rows_each = static_cast<int>(each);
+  const long long groups = (a.rows + each - 1) / each;
+  long long parts = (each * per_row + batch - 1) / batch;
+  if (parts > (1LL << 23) / groups) parts = (1LL << 23) / groups;  // a launch of fewer than 2^32 threads; a workgroup takes several batches
+  if (parts < 1) parts = 1;
+  LAYA_LAUNCH((rotary_kernel<T, V, kHalf>), dim3(static_cast<unsigned>(groups), static_cast<unsigned>(parts)), dim3(kThreads), a.rows_each * pairs * sizeof(float2),
+              stream, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_t(const RotaryArgs& a, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  if (whole<T>(a)) return a.interleaved ? launch_v<T, V, false>(a, stream) : launch_v<T, V, true>(a, stream);
+  return a.interleaved ? launch_v<T, 1, false>(a, stream) : launch_v<T, 1, true>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_rotary(const RotaryArgs& a, DType t, hipStream_t stream) {
+  switch (t) {
+    case DType::F32: return launch_t<float>(a, stream);
+    case DType::F16: return launch_t<f16>(a, stream);
+    default: return launch_t<bf16>(a, stream);
+  }
+}
+
+}  // namespace laya

@@ -19,6 +19,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "attend.hpp"
 #include "kernels.hpp"
 #include "laya_hip.h"
 #include "packing.hpp"
@@ -1619,6 +1620,161 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
     if (tile == LAYA_TILE_EXACT || tile == LAYA_TILE_FAST) tile = linear8_plan(a, tile == LAYA_TILE_EXACT, gemm_device_cus());
     LAYA_REQUIRE(linear8_tile_valid(tile, a), "no such tile, or one that cannot make this output");
     check_launch(launch_linear8(a, tile, static_cast<hipStream_t>(stream)), "linear8");
+  });
+}
+
+// ---------------- rotary positions, attention over packed sequences ----------------
+
+constexpr int kMaxRotaryDim = 8192, kMaxRotaryRow = 1 << 20;
+constexpr int64_t kMaxRotaryRows = 1LL << 23, kMaxStride = 1LL << 40;
+static bool stride_ok(int64_t s) { return s >= 0 && s < kMaxStride; }
+
+int laya_rotary_frequencies(int kind, double theta, int rotated, double factor, double original, double low, double high,
+                            double* host_turns) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(kind >= LAYA_FREQ_PLAIN && kind <= LAYA_FREQ_PARTS, "kind must be a LAYA_FREQ_* value");
+    LAYA_REQUIRE(rotated >= 2 && rotated <= kMaxRotaryDim && rotated % 2 == 0, "rotated must be even, from 2 to 8192");
+    LAYA_REQUIRE(theta > 0 && std::isfinite(theta), "theta must be positive");
+    LAYA_REQUIRE(kind == LAYA_FREQ_PLAIN || (factor >= 1 && std::isfinite(factor)), "factor must be at least 1");
+    LAYA_REQUIRE(kind != LAYA_FREQ_PARTS || (original > 0 && std::isfinite(original) && low >= 0 && low < high && std::isfinite(high)),
+                 "original must be positive and 0 <= low < high");
+    LAYA_REQUIRE(host_turns, "host_turns is required");
+    constexpr double kTwoPi = 6.283185307179586476925286766559;
+    if (kind == LAYA_FREQ_BASE) theta *= rotated > 2 ? std::pow(factor, rotated / (rotated - 2.0)) : factor;
+    for (int i = 0; i < rotated / 2; ++i) {
+      double turns = std::pow(theta, -2.0 * i / rotated) / kTwoPi;
+      if (kind == LAYA_FREQ_LINEAR) turns /= factor;
+      if (kind == LAYA_FREQ_PARTS) {
+        const double kept = std::min(1.0, std::max(0.0, (original * turns - low) / (high - low)));
+        turns = turns * kept + turns / factor * (1.0 - kept);
+      }
+      host_turns[i] = turns;
+    }
+  });
+}
+
+int laya_op_rotary(const void* x, int64_t x_row, int64_t x_head, void* out, int64_t out_row, int64_t out_head, int dtype,
+                   const int32_t* positions, const double* turns, float amplitude, int layout, int direction, int64_t rows, int heads,
+                   int dim, int rotated, void* stream) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(float_type(dtype), "dtype must be LAYA_F32, LAYA_F16 or LAYA_BF16");
+    LAYA_REQUIRE(layout == LAYA_ROTARY_HALF || layout == LAYA_ROTARY_INTERLEAVED, "layout must be a LAYA_ROTARY_* value");
+    LAYA_REQUIRE(direction == 1 || direction == -1, "direction must be 1 or -1");
+    LAYA_REQUIRE(std::isfinite(amplitude), "amplitude must be finite");
+    LAYA_REQUIRE(dim >= 2 && dim <= kMaxRotaryDim && heads >= 1 && static_cast<int64_t>(heads) * dim <= kMaxRotaryRow,
+                 "dim must be 2 to 8192, and heads * dim at most 2^20");
+    LAYA_REQUIRE(rotated >= 2 && rotated <= dim && rotated % 2 == 0, "rotated must be even, from 2 to dim");
+    LAYA_REQUIRE(rows >= 0 && rows <= kMaxRotaryRows, "rows: 0 to 2^23");
+    LAYA_REQUIRE(stride_ok(x_row) && stride_ok(x_head) && stride_ok(out_row) && stride_ok(out_head), "strides must be 0 to 2^40");
+    LAYA_REQUIRE((heads == 1 || out_head >= dim) && (rows < 2 || out_row >= dim), "out's rows and heads must not overlap");
+    if (rows == 0) return;
+    LAYA_REQUIRE(x && out && positions && turns, "x, out, positions and turns are required");
+    LAYA_REQUIRE(aligned_to(x, type_size(dtype)) && aligned_to(out, type_size(dtype)) && aligned_to(positions, 4) && aligned_to(turns, 8),
+                 "pointers must be aligned to their elements");
+    const bool in_place = x == out;
+    LAYA_REQUIRE(!in_place || ((x_row == out_row || rows == 1) && (x_head == out_head || heads == 1)), "in place, both strides must be the same");
+    RotaryArgs a{};
+    a.x = x; a.out = out; a.x_row = x_row; a.x_head = x_head; a.out_row = out_row; a.out_head = out_head;
+    a.positions = positions; a.turns = turns; a.amplitude = amplitude; a.direction = static_cast<float>(direction);
+    a.rows = rows; a.heads = heads; a.dim = dim; a.rotated = rotated;
+    a.interleaved = layout == LAYA_ROTARY_INTERLEAVED; a.in_place = in_place;
+    check_launch(launch_rotary(a, static_cast<DType>(dtype), static_cast<hipStream_t>(stream)), "rotary");
+  });
+}
+
+constexpr int kMaxPacked = 1 << 30;
+constexpr int64_t kMaxGroups = 1 << 24;  // workgroups of 256 threads in one launch
+
+int laya_op_document_bounds(const int32_t* documents, const int32_t* starts, const int32_t* lengths, int n_seq, int64_t rows,
+                            int max_length, int32_t* bounds, void* stream) {
+  return guarded(nullptr, [&] {
+    LAYA_REQUIRE(n_seq >= 0 && rows >= 0 && rows < kMaxPacked && max_length >= 0 && max_length < kMaxPacked,
+                 "n_seq, rows and max_length must not be negative, and rows and max_length below 2^30");
+    LAYA_REQUIRE((static_cast<int64_t>(max_length) + 255) / 256 * n_seq < kMaxGroups, "n_seq * max_length: too large for one launch");
+    if (n_seq == 0 || rows == 0 || max_length == 0) return;
+    LAYA_REQUIRE(documents && starts && lengths && bounds, "documents, starts, lengths and bounds are required");
+    LAYA_REQUIRE(aligned_to(documents, 4) && aligned_to(starts, 4) && aligned_to(lengths, 4) && aligned_to(bounds, 8),
+                 "bounds must be 8-byte and the other arrays 4-byte aligned");
+    BoundsArgs a{documents, starts, lengths, n_seq, static_cast<int>(rows), max_length, reinterpret_cast<int2*>(bounds)};
+    check_launch(launch_document_bounds(a, static_cast<hipStream_t>(stream)), "document bounds");
+  });
+}
+
+// The sizes of a call, checked; its launch.
+static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
+  LAYA_REQUIRE(c && c->struct_bytes == sizeof(LayaAttend), "struct_bytes must be sizeof(LayaAttend)");
+  LAYA_REQUIRE(c->dtype == LAYA_F16 || c->dtype == LAYA_BF16, "dtype must be LAYA_F16 or LAYA_BF16");
+  LAYA_REQUIRE(c->dim >= 8 && c->dim <= kMaxAttendDim && c->dim % 8 == 0, "dim must be a multiple of 8, from 8 to 256");
+  LAYA_REQUIRE(c->heads >= 1 && c->kv_heads >= 1 && c->heads % c->kv_heads == 0 && c->heads <= 1 << 16,
+               "heads must be a multiple of kv_heads, at most 2^16");
+  LAYA_REQUIRE(c->q_rows >= 0 && c->k_rows >= 0 && c->n_seq >= 0 && c->max_q >= 0 && c->max_k >= 0 && c->q_rows < kMaxPacked &&
+                   c->k_rows < kMaxPacked && c->max_q < kMaxPacked && c->max_k < kMaxPacked,
+               "rows, n_seq, max_q and max_k must not be negative, and below 2^30");
+  LAYA_REQUIRE(c->before >= -1 && c->after >= -1 && c->before < kMaxPacked && c->after < kMaxPacked,
+               "before and after must be -1 (no limit) or 0 to 2^30");
+  LAYA_REQUIRE(!(c->slopes && c->table), "slopes or a table, not both");
+  LAYA_REQUIRE(!c->table || (c->span >= 0 && c->span <= kMaxSpan), "span must be 0 to 1024");
+  AttendArgs a{};
+  a.heads = c->heads; a.kv_heads = c->kv_heads; a.group = c->heads / c->kv_heads; a.dim = c->dim;
+  a.q_rows = c->q_rows; a.k_rows = c->k_rows; a.n_seq = c->n_seq; a.max_q = c->max_q; a.max_k = c->max_k;
+  a.before = c->before; a.after = c->after; a.span = c->table ? c->span : 0;
+  a.prefix = c->prefix;
+  const int64_t pairs = static_cast<int64_t>(c->n_seq) * c->heads;
+  LAYA_REQUIRE(pairs < kMaxGroups && (static_cast<int64_t>(c->max_q) + 127) / 128 * (pairs + 8 * a.group) < kMaxGroups &&
+                   static_cast<int64_t>(c->max_q) * a.group < (1LL << 30),
+               "n_seq * heads * max_q: too large for one launch");
+  *plan = attend_plan(a);
+  LAYA_REQUIRE(!plan->split || static_cast<int64_t>(c->n_seq) * c->kv_heads * plan->row_tiles * plan->splits < kMaxGroups,
+               "n_seq * heads * max_q: too large for one launch");
+  return a;
+}
+
+int64_t laya_attend_workspace(const LayaAttend* call) {
+  int64_t bytes = -1;
+  guarded(nullptr, [&] {
+    AttendPlan plan;
+    attend_sizes(call, &plan);
+    bytes = plan.workspace;
+  });
+  return bytes;
+}
+
+int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded(nullptr, [&] {
+    AttendPlan plan;
+    AttendArgs a = attend_sizes(call, &plan);
+    const LayaAttend& c = *call;
+    LAYA_REQUIRE(c.scale >= 0.f && std::isfinite(c.scale) && (c.cap == 0.f || (c.cap >= 1e-30f && std::isfinite(c.cap))),
+                 "scale must not be negative, cap 0 or at least 1e-30, both finite");
+    LAYA_REQUIRE(stride_ok(c.q_row) && stride_ok(c.q_head) && stride_ok(c.k_row) && stride_ok(c.k_head) && stride_ok(c.v_row) &&
+                     stride_ok(c.v_head) && stride_ok(c.out_row) && stride_ok(c.out_head) &&
+                     ((c.q_row | c.q_head | c.k_row | c.k_head | c.v_row | c.v_head | c.out_row | c.out_head) & 7) == 0,
+                 "strides must be multiples of 8 elements from 0 to 2^40");
+    LAYA_REQUIRE(c.k_row >= c.dim && c.v_row >= c.dim && c.k_row < (1 << 23) && c.v_row < (1 << 23),
+                 "rows of k and v must be dim to 2^23 elements apart");
+    LAYA_REQUIRE((c.heads == 1 || c.out_head >= c.dim) && (c.q_rows < 2 || c.out_row >= c.dim), "out's rows and heads must not overlap");
+    if (c.n_seq == 0 || c.max_q == 0 || c.q_rows == 0) return;
+    LAYA_REQUIRE(c.q && c.out && c.q_starts && c.q_lengths && c.k_starts && c.k_lengths && (c.k_rows == 0 || (c.k && c.v)),
+                 "q, k, v, out, starts and lengths are required");
+    LAYA_REQUIRE(aligned_to(c.q, 16) && aligned_to(c.k, 16) && aligned_to(c.v, 16) && aligned_to(c.out, 16),
+                 "q, k, v and out must be 16-byte aligned");
+    LAYA_REQUIRE(aligned_to(c.q_starts, 4) && aligned_to(c.q_lengths, 4) && aligned_to(c.k_starts, 4) && aligned_to(c.k_lengths, 4) &&
+                     aligned_to(c.slopes, 4) && aligned_to(c.table, 4) && aligned_to(c.prefix, 4) && aligned_to(c.bounds, 8),
+                 "bounds must be 8-byte and the other arrays 4-byte aligned");
+    LAYA_REQUIRE(plan.workspace == 0 || (workspace && aligned_to(workspace, 16) && workspace_bytes >= plan.workspace),
+                 "workspace: laya_attend_workspace's bytes, 16-byte aligned");
+    a.q = c.q; a.k = c.k; a.v = c.v; a.out = c.out;
+    a.q_row = c.q_row; a.q_head = c.q_head; a.k_row = c.k_row; a.k_head = c.k_head;
+    a.v_row = c.v_row; a.v_head = c.v_head; a.out_row = c.out_row; a.out_head = c.out_head;
+    a.q_starts = c.q_starts; a.q_lengths = c.q_lengths; a.k_starts = c.k_starts; a.k_lengths = c.k_lengths;
+    constexpr float kLog2e = 1.4426950408889634f;
+    a.scale = c.cap > 0.f ? 2.0f * kLog2e * (c.scale / c.cap) : c.scale * kLog2e;
+    a.cap = c.cap * kLog2e;
+    a.slopes = c.slopes; a.table = c.table; a.bounds = reinterpret_cast<const int2*>(c.bounds);
+    a.parts = static_cast<float*>(workspace);
+    const DistanceBias bias = c.slopes ? DistanceBias::Slopes : c.table ? DistanceBias::Table : DistanceBias::None;
+    check_launch(launch_attend(a, c.dtype == LAYA_F16 ? DType::F16 : DType::BF16, bias, c.cap > 0.f, plan, static_cast<hipStream_t>(stream)),
+                 "attend");
   });
 }
 

@@ -17,6 +17,8 @@ FFN_GELU, FFN_GEGLU = 0, 1
 LAYER_NORM, RMS_NORM = 0, 1  # laya_op_norm8 kinds
 ACT_NONE, ACT_GELU, ACT_RELU, ACT_GEGLU, ACT_SWIGLU = range(5)  # laya_op_linear8 activations
 TILE_EXACT, TILE_FAST = -1, -2  # and its planned tiles
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1  # laya_op_rotary layouts
+FREQ_PLAIN, FREQ_LINEAR, FREQ_BASE, FREQ_PARTS = range(4)  # laya_rotary_frequencies kinds
 
 
 class LayaConfig(ct.Structure):
@@ -41,7 +43,18 @@ class LayaDevice(ct.Structure):
                 ("clock_khz", ct.c_int32), ("supported", ct.c_int32)]
 
 
-_p, _i, _f, _i64 = ct.c_void_p, ct.c_int, ct.c_float, ct.c_int64
+class LayaAttend(ct.Structure):
+    _fields_ = ([("struct_bytes", ct.c_uint32), ("dtype", ct.c_int32)]
+                + [(name, ct.c_void_p) for name in ("q", "k", "v", "out")]
+                + [(name, ct.c_int64) for name in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")]
+                + [(name, ct.c_int32) for name in ("heads", "kv_heads", "dim", "q_rows", "k_rows", "n_seq", "max_q", "max_k")]
+                + [(name, ct.c_void_p) for name in ("q_starts", "q_lengths", "k_starts", "k_lengths")]
+                + [("scale", ct.c_float), ("cap", ct.c_float), ("slopes", ct.c_void_p), ("table", ct.c_void_p),
+                   ("span", ct.c_int32), ("before", ct.c_int32), ("after", ct.c_int32), ("prefix", ct.c_void_p),
+                   ("bounds", ct.c_void_p)])
+
+
+_p, _i, _f, _i64, _d = ct.c_void_p, ct.c_int, ct.c_float, ct.c_int64, ct.c_double
 _ip = ct.POINTER(ct.c_int32)
 _fp = ct.POINTER(ct.c_float)
 
@@ -78,6 +91,11 @@ SIGNATURES = {
     "laya_op_dequantize8": ([_p, _p, _p, _i, _i64, _i64, _i, _p], _i),
     "laya_op_norm8": ([_p, _p, _i, _i, _i64, _p, _p, _p, _f, _i, _p, _p, _p, _p, _i, _i, _p], _i),
     "laya_op_linear8": ([_p, _p, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p], _i),
+    "laya_rotary_frequencies": ([_i, _d, _i, _d, _d, _d, _d, ct.POINTER(_d)], _i),
+    "laya_op_rotary": ([_p, _i64, _i64, _p, _i64, _i64, _i, _p, _p, _f, _i, _i, _i64, _i, _i, _i, _p], _i),
+    "laya_op_document_bounds": ([_p, _p, _p, _i, _i64, _i, _p, _p], _i),
+    "laya_attend_workspace": ([ct.POINTER(LayaAttend)], _i64),
+    "laya_op_attend": ([ct.POINTER(LayaAttend), _p, _i64, _p], _i),
     "laya_op_head_gather": ([_p, _p, _p, _p, _p, _p, _p, _p, _f, _p, _p, _i, _i, _p], _i),
 }
 
