@@ -11,15 +11,14 @@ namespace laya {
 
 namespace {
 
-// Prompts: a workgroup of four waves owns 128 queries of one head, and blocks of 64 keys pass through LDS, shared by the waves.
-// While the softmax of block j runs, the wave's matrix instructions are the products of block j - 1 with V and the scores of
-// block j + 1, which do not depend on it.  Step j waits for K(j + 1) and V(j - 1), loaded during the step before, and starts
-// K(j + 2) and V(j) into the buffers of K(j) and V(j - 2), whose reads the barrier has ended.
+// Prompts: a workgroup of four waves owns 128 queries of one head, and blocks of 64 keys pass through LDS, shared by the waves
+// and double-buffered.  A wave works on them 32 keys at a time and skips those that none of its rows sees.
 template <typename T, int D, bool kCap, DistanceBias kBias>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void attend_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3 : D <= 128 ? 2 : 1))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
   constexpr int KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
-  typedef Rows<T, D, KB, kCap, kBias> R;
+  constexpr int SB = 32;  // keys of one step
+  typedef Rows<T, D, SB, kCap, kBias> R;
   typedef typename R::T8 T8;
   typedef typename Vec4<T>::type T4;
   // Workgroup -> (sequence, head, tile).  Workgroups go round the 8 XCDs by their number: a unit (the tiles of one head, or of
@@ -79,7 +78,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
   constexpr int CH = KB * kChunks / 256, step = 256 / kChunks;
   const int r0 = tid / kChunks, c0 = tid % kChunks;
   const unsigned lds_k[2] = {lds_address(sk[0]), lds_address(sk[1])}, lds_v[2] = {lds_address(sv[0]), lds_address(sv[1])};
-  auto stage = [&](const T* base, long long row, int j, unsigned lds, auto swizzle) {
+  auto stage = [&](const T* base, long long row, int j, unsigned lds, auto swizzle) __attribute__((always_inline)) {
     const int key = blocks.key(j);
     const i32x4 rs = block_resource(base, row, key, min(KB, sq.nk - key), a.dim);
 #pragma unroll
@@ -89,79 +88,53 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
       lds_load16_buffer<true>(rs, at, 0u, lds + (wave + 4u * m) * 1024u);
     }
   };
-  auto load_k = [&](int j, int buf) { stage(K, a.k_row, j, lds_k[buf], [](int r) { return Block<D>::k_swizzle(r); }); };
-  auto load_v = [&](int j, int buf) { stage(V, a.v_row, j, lds_v[buf], [](int r) { return Block<D>::v_swizzle(r); }); };
+  auto load = [&](int j, int buf) __attribute__((always_inline)) {
+    stage(K, a.k_row, j, lds_k[buf], [](int r) { return Block<D>::k_swizzle(r); });
+    stage(V, a.v_row, j, lds_v[buf], [](int r) { return Block<D>::v_swizzle(r); });
+  };
 
   R rows;
   rows.start(lane);
-  if (nb > 0) load_k(0, 0);
+  if (nb > 0) load(0, 0);
   rows.load_q(Q, a.dim, valid);
   rows.lo = me.lo;
   rows.hi = me.hi;
   rows.prefix = sq.prefix;
   rows.position = me.position;
   rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
-  rows.table = stable + a.span + kPad;
-  if (nb > 1) load_k(1, 1);
+  const LdsFloats table = (LdsFloats)(stable) + a.span + kPad;
 
-  f32x16 sc[2][2];
-  T8 p[4];
-  // Whether every key of the block is seen by every row.
-  auto whole = [&](int key) { return key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi); };
   float far_left = 0.f, far_right = 0.f;
   if constexpr (kBias == DistanceBias::Table) {
     far_left = stable[0];
     far_right = stable[2 * (a.span + kPad)];
   }
   const int first_position = __builtin_amdgcn_readfirstlane(me.position);
-  auto softmax = [&](f32x16 (&t)[2], int key, auto edge) {
-    if constexpr (kBias == DistanceBias::Table) {
-      // Blocks wholly past the span on one side add that end's value; the table's LDS rows reach no further than the others need.
-      const bool left = key + KB - 1 - first_position <= -a.span, right = key - (first_position + 31) >= a.span;
-      if (left || right) {
-        const float b = left ? far_left : far_right;
+  for (int j = 0; j < nb; ++j) {
+    publish_stage<waitcnt_vm(0)>();
+    if (j + 1 < nb) load(j + 1, (j + 1) & 1);
+    const unsigned buffer = (j & 1) * static_cast<unsigned>(KB * P * sizeof(T));
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float x = t[kt][r];
-            if constexpr (kCap) t[kt][r] = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f), -2.0f * a.cap, a.cap) + b;
-            else t[kt][r] = __builtin_fmaf(x, a.scale, b);
-          }
+    for (int h = 0; h < KB / SB; ++h) {
+      const int key = blocks.key(j) + SB * h;
+      const bool whole = key + SB <= sq.prefix || (key >= range.all_lo && key + SB <= range.all_hi);
+      if (!active || !(whole || key < sq.prefix || (key < range.hi && key + SB > range.lo))) continue;
+      f32x16 t[R::KT];
+      T8 p[2 * R::KT];
+      rows.scores((LdsBytes)(sk[0]) + SB * h * P * 2, buffer, t);
+      if constexpr (kBias == DistanceBias::Table) {
+        // Steps wholly past the span on one side add that end's value; the table's LDS rows reach as far as the others need.
+        const bool left = key + SB - 1 - first_position <= -a.span, right = key - (first_position + 31) >= a.span;
+        if (left || right) rows.add(a, t, left ? far_left : far_right);
+        else rows.change(a, t, key, table);
       } else {
-        rows.template change<true>(a, t, key);
+        rows.change(a, t, key, table);
       }
-    } else {
-      rows.template change<true>(a, t, key);
+      if (!whole) rows.hide(t, key);
+      const float sum = rows.weights(a, t, p);
+      rows.total += rows.move(a, t, p, sum);
+      rows.weigh((LdsBytes)(sv[0]) + SB * h * P * 2, buffer, p);
     }
-    if constexpr (decltype(edge)::value) rows.hide(t, key);
-  };
-  auto body = [&](int j, auto parity, auto edge) {
-    constexpr int X = decltype(parity)::value;
-    if (j > 0) rows.weigh((LdsBytes)(sv[X ^ 1]), p);
-    softmax(sc[X], blocks.key(j), edge);
-    float sum = rows.weights(a, sc[X], p);
-    rows.scores((LdsBytes)(sk[X ^ 1]), sc[X ^ 1]);  // past the last block: of stale keys, never used
-    rows.total += rows.move(a, sc[X], p, sum);
-  };
-  auto turn = [&](int j, auto parity) {
-    constexpr int X = decltype(parity)::value;
-    publish_stage<waitcnt_vm(0)>();
-    if (j + 2 < nb) load_k(j + 2, X);
-    load_v(j, X);
-    if (!active) return;
-    if (whole(blocks.key(j))) body(j, parity, std::false_type());
-    else body(j, parity, std::true_type());
-  };
-  publish_stage<waitcnt_vm(0)>();
-  if (nb > 0) {
-    if (active) rows.scores((LdsBytes)(sk[0]), sc[0]);
-    for (int j = 0; j < nb; j += 2) {
-      turn(j, std::integral_constant<int, 0>());
-      if (j + 1 < nb) turn(j + 1, std::integral_constant<int, 1>());
-    }
-    publish_stage<waitcnt_vm(0)>();
-    if (active) rows.weigh((LdsBytes)(sv[(nb - 1) & 1]), p);
   }
   if (!active) return;
 
@@ -239,7 +212,7 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
   constexpr int CH = KB * kChunks / 64, step = 64 / kChunks;
   const int r0 = lane / kChunks, c0 = lane % kChunks;
   const unsigned stage0 = lds_address(lds + wave * 2 * kStage);
-  auto stage = [&](int j, int buf) {
+  auto stage = [&](int j, int buf) __attribute__((always_inline)) {
     const int key = blocks.key(j), left = min(KB, sq.nk - key);
     const i32x4 rk = block_resource(K, a.k_row, key, left, a.dim), rv = block_resource(V, a.v_row, key, left, a.dim);
     const unsigned to = stage0 + buf * static_cast<unsigned>(kStage * sizeof(T));
@@ -265,23 +238,13 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
   rows.prefix = sq.prefix;
   rows.position = me.position;
   rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
-  rows.table = kBias == DistanceBias::Table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr;
+  const float* table = kBias == DistanceBias::Table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr;
 
   int j = j0 + wave;
   if (j < j1) stage(j, 0);
-  auto body = [&](int jj, int buf, auto edge) {
-    const LdsBytes k = (LdsBytes)(lds + (wave * 2 + buf) * kStage);
-    f32x16 sc[1];
-    T8 p[2];
-    rows.scores(k, sc);
-    rows.template change<false>(a, sc, blocks.key(jj));
-    if constexpr (decltype(edge)::value) rows.hide(sc, blocks.key(jj));
-    const float sum = rows.weights(a, sc, p);
-    rows.total += rows.move(a, sc, p, sum);
-    rows.weigh(k + KB * P * 2, p);
-  };
   for (int buf = 0; j < j1; j += NW, buf ^= 1) {
     const int key = blocks.key(j);
+    const unsigned mine = (wave * 2 + buf) * static_cast<unsigned>(kStage * sizeof(T));
     // The other stage's reads ended before its loads start: LDS answers a wave in order, and this waits for them.
     __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0_keep_vm());
     asm volatile("" ::: "memory");
@@ -292,8 +255,14 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));
     }
     asm volatile("" ::: "memory");
-    if (key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi)) body(j, buf, std::false_type());
-    else body(j, buf, std::true_type());
+    f32x16 t[1];
+    T8 p[2];
+    rows.scores((LdsBytes)(lds), mine, t);
+    rows.change(a, t, key, table);
+    if (!(key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi))) rows.hide(t, key);
+    const float sum = rows.weights(a, t, p);
+    rows.total += rows.move(a, t, p, sum);
+    rows.weigh((LdsBytes)(lds) + KB * P * 2, mine, p);
   }
 
   // The waves' sums join: sum_w 2^(m_w - M) O_w and sum_w 2^(m_w - M) l_w.

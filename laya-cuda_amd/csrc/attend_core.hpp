@@ -13,6 +13,8 @@
 
 #include "attend.hpp"
 
+#include <type_traits>
+
 namespace laya {
 
 constexpr float kNothing = -1e30f;    // the reference of a row that has seen no key; scores not above it count as hidden
@@ -136,6 +138,7 @@ __device__ __forceinline__ i32x4 block_resource(const T* head, long long row, in
 constexpr unsigned kNoChunk = 0x80000000u;  // an offset behind every resource (they span fewer than 2^31 bytes)
 
 typedef __attribute__((address_space(3))) const char* LdsBytes;
+typedef __attribute__((address_space(3))) const float* LdsFloats;
 
 // Per-lane state of 32 rows.
 template <typename T, int D, int KB, bool kCap, DistanceBias kBias>
@@ -152,7 +155,6 @@ struct Rows {
   float reference, total;
   int lo, hi, prefix, position;
   float slope;
-  const float* table;  // of this row's head, at distance 0 (in LDS where kLdsTable)
   int lane, g;
   unsigned k_at, v_at;  // byte offsets of this lane's first fragments
 
@@ -185,7 +187,8 @@ struct Rows {
     }
   }
 
-  __device__ __forceinline__ void scores(LdsBytes k, f32x16 (&s)[KT]) const {
+  // offset: of the block behind `k` (and of its values behind `v`), a multiple of 1 KB.
+  __device__ __forceinline__ void scores(LdsBytes k, unsigned offset, f32x16 (&s)[KT]) const {
     typedef __attribute__((address_space(3))) const T8* Lds8;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -193,17 +196,17 @@ struct Rows {
       for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        s[kt] = mfma32(*(Lds8)(k + (k_at ^ (ks * 32u)) + kt * 64 * B::kPitch), q[ks], s[kt]);
+        s[kt] = mfma32(*(Lds8)(k + ((k_at + offset) ^ (ks * 32u)) + kt * 64 * B::kPitch), q[ks], s[kt]);
     }
   }
 
-  __device__ __forceinline__ void weigh(LdsBytes v, const T8 (&p)[2 * KT]) {  // O^T += V^T P^T
+  __device__ __forceinline__ void weigh(LdsBytes v, unsigned offset, const T8 (&p)[2 * KT]) {  // O^T += V^T P^T
     typedef __attribute__((address_space(3))) s16x4* Lds4;
 #pragma unroll
     for (int c = 0; c < 2 * KT; ++c)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const LdsBytes at = v + (v_at ^ (d * 64u)) + c * 32 * B::kPitch;
+        const LdsBytes at = v + ((v_at + offset) ^ (d * 64u)) + c * 32 * B::kPitch;
         const s16x4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(at));
         const s16x4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4)(at + 16 * B::kPitch));
         const s16x8 both = __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -214,9 +217,11 @@ struct Rows {
   // Key of score r of tile kt of the block at `key`, less the lane's first.
   static constexpr int slot(int kt, int r) { return 32 * kt + 8 * (r >> 2) + (r & 3); }
 
-  // Raw products to log2 scores: cap and bias.  kLdsTable: `table` may be read up to a block and 32 rows past the span.
-  template <bool kLdsTable>
-  __device__ __forceinline__ void change(const AttendArgs& a, f32x16 (&s)[KT], int key) const {
+  // Raw products to log2 scores: cap and bias.  table: of this row's head, at distance 0; one in LDS is in log2 units and may
+  // be read up to a block and 32 rows past the span.
+  template <typename Table>
+  __device__ __forceinline__ void change(const AttendArgs& a, f32x16 (&s)[KT], int key, Table table) const {
+    constexpr bool kLdsTable = std::is_same<Table, LdsFloats>::value;
     if constexpr (!kRaw) {
       const int at = key + 4 * g - position;
       const float from = static_cast<float>(at);
@@ -238,6 +243,20 @@ struct Rows {
           s[kt][r] = kCap ? x + b : __builtin_fmaf(x, a.scale, b);
         }
     }
+  }
+
+  // The same with one bias for all keys.
+  __device__ __forceinline__ void add(const AttendArgs& a, f32x16 (&s)[KT], float b) const {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = s[kt][r];
+        if constexpr (kCap)
+          s[kt][r] = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f), -2.0f * a.cap, a.cap) + b;
+        else
+          s[kt][r] = __builtin_fmaf(x, a.scale, b);
+      }
   }
 
   __device__ __forceinline__ void hide(f32x16 (&s)[KT], int key) const {
