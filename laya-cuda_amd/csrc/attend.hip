@@ -51,23 +51,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
 
   __shared__ __align__(16) T sk[2][KB * P];
   __shared__ __align__(16) T sv[2][KB * P];
-  __shared__ int wg_lo[4], wg_hi[4];
+  __shared__ Range wg_range[4];
   constexpr int kPad = KB + 32;  // distances past the span that a block near its ends reaches
   __shared__ float stable[kBias == DistanceBias::Table ? 2 * (kMaxSpan + kPad) + 1 : 1];
 
-  const Range range = wave_range(me, valid);
-  if (lane == 0) {
-    wg_lo[wave] = range.lo;
-    wg_hi[wave] = range.hi;
-  }
+  const Range range = wave_range(a, sq, me, valid, row0 + wave * 32, min(row0 + wave * 32 + 31, sq.nq - 1));
+  if (lane == 0) wg_range[wave] = active ? range : Range{INT_MAX, 0, 0, INT_MAX};
   if constexpr (kBias == DistanceBias::Table) {
     const float* from = a.table + static_cast<size_t>(head) * (2 * a.span + 1);
     for (int e = tid; e < 2 * (a.span + kPad) + 1; e += 256) stable[e] = from[max(0, min(2 * a.span, e - kPad))] * kLog2e;
   }
   __syncthreads();
-  const int klo = __builtin_amdgcn_readfirstlane(min(min(wg_lo[0], wg_lo[1]), min(wg_lo[2], wg_lo[3])));
-  const int khi = __builtin_amdgcn_readfirstlane(max(max(wg_hi[0], wg_hi[1]), max(wg_hi[2], wg_hi[3])));
-  const Blocks<KB> blocks(sq.prefix, klo, khi);
+  Range wg = wg_range[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    wg.lo = min(wg.lo, wg_range[w].lo);
+    wg.hi = max(wg.hi, wg_range[w].hi);
+    wg.all_lo = max(wg.all_lo, wg_range[w].all_lo);
+    wg.all_hi = min(wg.all_hi, wg_range[w].all_hi);
+  }
+  // With a bias the keys next to the queries come first: their scores are the largest as a rule, and references move once.
+  const int last_position = min(row0 + 127, sq.nq - 1) + sq.nk - sq.nq;
+  const Blocks<KB> blocks(sq.prefix, __builtin_amdgcn_readfirstlane(wg.lo), __builtin_amdgcn_readfirstlane(wg.hi),
+                          kBias == DistanceBias::None ? 0 : last_position);
+  const int plain_lo = __builtin_amdgcn_readfirstlane(wg.all_lo), plain_hi = __builtin_amdgcn_readfirstlane(wg.all_hi) - KB;
   const int nb = blocks.count;
 
   const T* K = static_cast<const T*>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
@@ -77,25 +84,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
   // This thread's 16-byte chunks of a block: row r0 + step m, chunk index swizzled by the row.
   constexpr int CH = KB * kChunks / 256, step = 256 / kChunks;
   const int r0 = tid / kChunks, c0 = tid % kChunks;
-  const unsigned lds_k[2] = {lds_address(sk[0]), lds_address(sk[1])}, lds_v[2] = {lds_address(sv[0]), lds_address(sv[1])};
-  auto stage = [&](const T* base, long long row, int j, unsigned lds, auto swizzle) __attribute__((always_inline)) {
-    const int key = blocks.key(j);
-    const i32x4 rs = block_resource(base, row, key, min(KB, sq.nk - key), a.dim);
+  unsigned at_k[CH], at_v[CH];
 #pragma unroll
-    for (int m = 0; m < CH; ++m) {
-      const int r = r0 + m * step, c = c0 ^ swizzle(r);
-      const unsigned at = c * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(row) + 16u * c : kNoChunk;
-      lds_load16_buffer<true>(rs, at, 0u, lds + (wave + 4u * m) * 1024u);
-    }
-  };
-  auto load = [&](int j, int buf) __attribute__((always_inline)) {
-    stage(K, a.k_row, j, lds_k[buf], [](int r) { return Block<D>::k_swizzle(r); });
-    stage(V, a.v_row, j, lds_v[buf], [](int r) { return Block<D>::v_swizzle(r); });
+  for (int m = 0; m < CH; ++m) {
+    const int r = r0 + m * step, ck = c0 ^ Block<D>::k_swizzle(r), cv = c0 ^ Block<D>::v_swizzle(r);
+    at_k[m] = ck * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.k_row) + 16u * ck : kNoChunk;
+    at_v[m] = cv * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.v_row) + 16u * cv : kNoChunk;
+  }
+  const Source<KB> from_k(K, a.k_row, sq.nk, a.dim), from_v(V, a.v_row, sq.nk, a.dim);
+  constexpr unsigned kBuffer = KB * P * sizeof(T);
+  const unsigned lds_k = lds_address(sk[0]) + wave * 1024u, lds_v = lds_address(sv[0]) + wave * 1024u;
+  auto load = [&](int key, unsigned buffer) __attribute__((always_inline)) {
+    const i32x4 rk = from_k.resource(key, sq.nk), rv = from_v.resource(key, sq.nk);
+#pragma unroll
+    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(rk, at_k[m], 0u, lds_k + buffer + 4096u * m);
+#pragma unroll
+    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(rv, at_v[m], 0u, lds_v + buffer + 4096u * m);
   };
 
   R rows;
   rows.start(lane);
-  if (nb > 0) load(0, 0);
+  int key0 = blocks.taken(0);
+  if (nb > 0) load(key0, 0);
   rows.load_q(Q, a.dim, valid);
   rows.lo = me.lo;
   rows.hi = me.hi;
@@ -110,15 +120,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
     far_right = stable[2 * (a.span + kPad)];
   }
   const int first_position = __builtin_amdgcn_readfirstlane(me.position);
-  for (int j = 0; j < nb; ++j) {
+  unsigned buffer = 0;
+  for (int j = 0; j < nb; ++j, buffer ^= kBuffer) {
     publish_stage<waitcnt_vm(0)>();
-    if (j + 1 < nb) load(j + 1, (j + 1) & 1);
-    const unsigned buffer = (j & 1) * static_cast<unsigned>(KB * P * sizeof(T));
+    const int now = key0;
+    if (j + 1 < nb) {
+      key0 = blocks.taken(j + 1);
+      load(key0, buffer ^ kBuffer);
+    }
+    if (!active) continue;
+    const bool plain = now >= plain_lo && now <= plain_hi;  // every wave's rows see every key
 #pragma unroll
     for (int h = 0; h < KB / SB; ++h) {
-      const int key = blocks.key(j) + SB * h;
-      const bool whole = key + SB <= sq.prefix || (key >= range.all_lo && key + SB <= range.all_hi);
-      if (!active || !(whole || key < sq.prefix || (key < range.hi && key + SB > range.lo))) continue;
+      const int key = now + SB * h;
+      bool whole = true;
+      if (!plain) {
+        whole = key + SB <= sq.prefix || (key >= range.all_lo && key + SB <= range.all_hi);
+        if (!(whole || key < sq.prefix || (key < range.hi && key + SB > range.lo))) continue;
+      }
       f32x16 t[R::KT];
       T8 p[2 * R::KT];
       rows.scores((LdsBytes)(sk[0]) + SB * h * P * 2, buffer, t);
@@ -201,8 +220,9 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
   const bool valid = row < n_rows;
   const int i = valid ? row / a.group : 0, head = kv * a.group + (valid ? row - i * a.group : 0);
   const Seen me = valid ? seen(a, sq, i) : Seen{0, 0, 0};
-  const Range range = wave_range(me, valid);
-  const Blocks<KB> blocks(sq.prefix, range.lo, range.hi);
+  const int last = min(tile * 32 + 31, n_rows - 1) / a.group;
+  const Range range = wave_range(a, sq, me, valid, tile * 32 / a.group, last);
+  const Blocks<KB> blocks(sq.prefix, range.lo, range.hi, kBias == DistanceBias::None ? 0 : last + sq.nk - sq.nq);
   const int each = (blocks.count + a.splits - 1) / a.splits;
   const int j0 = min(blocks.count, z * each), j1 = min(blocks.count, j0 + each);
 
@@ -212,20 +232,20 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
   constexpr int CH = KB * kChunks / 64, step = 64 / kChunks;
   const int r0 = lane / kChunks, c0 = lane % kChunks;
   const unsigned stage0 = lds_address(lds + wave * 2 * kStage);
-  auto stage = [&](int j, int buf) __attribute__((always_inline)) {
-    const int key = blocks.key(j), left = min(KB, sq.nk - key);
-    const i32x4 rk = block_resource(K, a.k_row, key, left, a.dim), rv = block_resource(V, a.v_row, key, left, a.dim);
+  const Source<KB> from_k(K, a.k_row, sq.nk, a.dim), from_v(V, a.v_row, sq.nk, a.dim);
+  auto stage = [&](int key, int buf) __attribute__((always_inline)) {
+    const i32x4 rk = from_k.resource(key, sq.nk), rv = from_v.resource(key, sq.nk);
     const unsigned to = stage0 + buf * static_cast<unsigned>(kStage * sizeof(T));
 #pragma unroll
     for (int m = 0; m < CH; ++m) {
       const int r = r0 + m * step, c = c0 ^ Block<D>::k_swizzle(r);
-      const unsigned at = c * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.k_row) + 16u * c : kNoChunk;
+      const unsigned at = c * 8 < a.dim ? static_cast<unsigned>(r) * from_k.row + 16u * c : kNoChunk;
       lds_load16_buffer<true>(rk, at, 0u, to + m * 1024u);
     }
 #pragma unroll
     for (int m = 0; m < CH; ++m) {
       const int r = r0 + m * step, c = c0 ^ Block<D>::v_swizzle(r);
-      const unsigned at = c * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.v_row) + 16u * c : kNoChunk;
+      const unsigned at = c * 8 < a.dim ? static_cast<unsigned>(r) * from_v.row + 16u * c : kNoChunk;
       lds_load16_buffer<true>(rv, at, 0u, to + KB * P * 2u + m * 1024u);
     }
   };
@@ -241,15 +261,17 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
   const float* table = kBias == DistanceBias::Table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr;
 
   int j = j0 + wave;
-  if (j < j1) stage(j, 0);
+  int key0 = blocks.taken(j);
+  if (j < j1) stage(key0, 0);
   for (int buf = 0; j < j1; j += NW, buf ^= 1) {
-    const int key = blocks.key(j);
+    const int key = key0;
     const unsigned mine = (wave * 2 + buf) * static_cast<unsigned>(kStage * sizeof(T));
     // The other stage's reads ended before its loads start: LDS answers a wave in order, and this waits for them.
     __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0_keep_vm());
     asm volatile("" ::: "memory");
     if (j + NW < j1) {
-      stage(j + NW, buf ^ 1);
+      key0 = blocks.taken(j + NW);
+      stage(key0, buf ^ 1);
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(2 * CH));  // all but the loads just issued
     } else {
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));

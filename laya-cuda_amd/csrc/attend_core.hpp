@@ -38,16 +38,19 @@ __device__ __forceinline__ float halves_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ int rows_min(int v) {  // over 32 lanes; both halves of the wave hold the same rows
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v = min(v, __shfl_xor(v, d, kWave));
-  return __builtin_amdgcn_readfirstlane(v);
+// Over 32 rows; both halves of the wave hold the same ones.  Row rotations of 16 lanes, then two lanes by hand.
+template <int kBy>
+__device__ __forceinline__ int rotated16(int v) {
+  return __builtin_amdgcn_update_dpp(v, v, 0x120 + kBy, 0xf, 0xf, false);  // row_ror
 }
-__device__ __forceinline__ int rows_max(int v) {
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v = max(v, __shfl_xor(v, d, kWave));
-  return __builtin_amdgcn_readfirstlane(v);
+__device__ __forceinline__ int rows_min(int v) {
+  v = min(v, rotated16<8>(v));
+  v = min(v, rotated16<4>(v));
+  v = min(v, rotated16<2>(v));
+  v = min(v, rotated16<1>(v));
+  return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
+__device__ __forceinline__ int rows_max(int v) { return ~rows_min(~v); }
 
 // LDS rows of a staged block: kPitch elements, in 16-byte chunks whose index is XORed with a function of the row.  K is read 16
 // rows at one chunk (their 256-byte windows must hold 16 different positions), V four rows at four neighbouring chunks.
@@ -96,45 +99,70 @@ __device__ __forceinline__ Seen seen(const AttendArgs& a, const Sequence& s, int
   return r;
 }
 
-// What the 32 rows of a wave see together.  Rows past the sequence's last have no say.
+// What a wave's rows see together: keys behind the prefix that some row sees lie in [lo, hi), keys that every row sees hold
+// [all_lo, all_hi).  Queries first .. last; without bounds both ends grow with the query, so its two ends say it.
 struct Range {
-  int lo, hi;          // every seen key behind the prefix
-  int all_lo, all_hi;  // keys that all rows see
+  int lo, hi, all_lo, all_hi;
 };
-__device__ __forceinline__ Range wave_range(const Seen& s, bool valid) {
+__device__ __forceinline__ Range wave_range(const AttendArgs& a, const Sequence& s, const Seen& mine, bool valid, int first, int last) {
   Range r;
-  const bool any = valid && s.lo < s.hi;
-  r.lo = rows_min(any ? s.lo : INT_MAX);
-  r.hi = rows_max(any ? s.hi : 0);
-  r.all_lo = rows_max(valid ? s.lo : 0);
-  r.all_hi = rows_min(valid ? s.hi : INT_MAX);
+  if (a.bounds) {
+    const bool any = valid && mine.lo < mine.hi;
+    r.lo = rows_min(any ? mine.lo : INT_MAX);
+    r.hi = rows_max(any ? mine.hi : 0);
+    r.all_lo = rows_max(valid ? mine.lo : 0);
+    r.all_hi = rows_min(valid ? mine.hi : INT_MAX);
+  } else {
+    const int p = first + s.nk - s.nq, e = last + s.nk - s.nq;
+    r.lo = a.before >= 0 ? max(0, p - a.before) : 0;
+    r.hi = a.after >= 0 ? max(0, min(s.nk, e + a.after + 1)) : s.nk;
+    r.all_lo = a.before >= 0 ? max(0, e - a.before) : 0;
+    r.all_hi = a.after >= 0 ? min(s.nk, p + a.after + 1) : s.nk;
+  }
   return r;
 }
 
-// The blocks of KB keys that hold a seen key: those of the prefix, then those of a range behind it.
+// The blocks of KB keys that hold a seen key: those of the prefix, then those of a range behind it; and the order in which
+// they are taken, from the one that holds key `start` down, then up from it.
 template <int KB>
 struct Blocks {
   int first, second, count;  // blocks of the prefix; the range's first block; all
-  __device__ __forceinline__ Blocks(int prefix, int lo, int hi) {
+  int turn;                  // blocks up to the starting one, less 1
+  __device__ __forceinline__ Blocks(int prefix, int lo, int hi, int start) {
     first = (prefix + KB - 1) / KB;
     second = max(first, lo / KB);
     count = first + (lo < hi ? max(0, (hi + KB - 1) / KB - second) : 0);
+    const int b = max(start, 0) / KB;
+    turn = min(b < first ? b : max(first - 1, b - second + first), count - 1);
   }
   __device__ __forceinline__ int key(int j) const { return (j < first ? j : second + j - first) * KB; }
+  __device__ __forceinline__ int taken(int t) const { return key(t <= turn ? turn - t : t); }
 };
 
-// Buffer resource of the rows [key, min(key + KB, nk)) of one head: what lies behind them reads as zeros.
-template <typename T>
-__device__ __forceinline__ i32x4 block_resource(const T* head, long long row, int key, int rows, int dim) {
-  const uint64_t p = reinterpret_cast<uint64_t>(head + key * row);
-  i32x4 r;
-  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(p));
-  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32) & 0xffff);
-  r[2] = __builtin_amdgcn_readfirstlane(rows <= 0 ? 0 : static_cast<int>(((rows - 1) * row + dim) * 2));
-  r[3] = 0x00020000;
-  asm volatile("s_nop 4" : "+s"(r));  // a load may read an SGPR that a vector instruction wrote only five wait states later
-  return r;
-}
+// A head's rows as the blocks' loads take them.  What lies behind a block's last row reads as zeros.
+template <int KB>
+struct Source {
+  uint64_t base;
+  unsigned row;         // bytes
+  unsigned full, last;  // bytes of a whole block and of the sequence's last one
+  template <typename T>
+  __device__ __forceinline__ Source(const T* head, long long stride, int nk, int dim) {
+    base = reinterpret_cast<uint64_t>(head);
+    row = 2u * static_cast<unsigned>(stride);
+    full = (KB - 1) * row + 2u * dim;
+    last = (nk - 1) % KB * row + 2u * dim;
+  }
+  __device__ __forceinline__ i32x4 resource(int key, int nk) const {
+    const uint64_t p = base + static_cast<uint64_t>(static_cast<unsigned>(key)) * row;
+    i32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(p));
+    r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32) & 0xffff);
+    r[2] = __builtin_amdgcn_readfirstlane(key + KB <= nk ? full : last);
+    r[3] = 0x00020000;
+    asm volatile("s_nop 4" : "+s"(r));  // a load may read an SGPR that a vector instruction wrote only five wait states later
+    return r;
+  }
+};
 constexpr unsigned kNoChunk = 0x80000000u;  // an offset behind every resource (they span fewer than 2^31 bytes)
 
 typedef __attribute__((address_space(3))) const char* LdsBytes;
@@ -344,7 +372,7 @@ struct CarefulRow {
 #pragma unroll
     for (int i = 0; i < ND; ++i) sum[i] = 0.f;
     for (int j = j0; j < j1; ++j) {
-      const int first = blocks.key(j), key = first + lane;
+      const int first = blocks.taken(j), key = first + lane;
       const bool see = lane < KB && key < nk && ((key >= lo && key < hi) || key < prefix);
       float x = -INFINITY;
       if (see) {
