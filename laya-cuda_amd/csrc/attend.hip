@@ -191,34 +191,47 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
 }
 
 // Few rows: a workgroup owns 32 rows, the (token, head) pairs of the heads that share keys, and its waves split their keys into
-// blocks of 32, each wave with two stages of its own in LDS: while it works on one, the other's loads are on their way.  Long
-// contexts are shared by a.splits workgroups, whose sums join_kernel adds.
+// blocks of 32, each wave with a place of its own in LDS for a block of K and one of V.  The next K is on its way from the
+// scores to the next ones, the next V from one product to the next.  Long contexts are shared by a.splits workgroups, whose sums
+// join_kernel adds.
+template <int D>
+constexpr int split_waves() {
+  return D <= 128 ? 8 : 4;  // what 128 KB of LDS hold, or for heads of 64 half of it
+}
 template <typename T, int D, bool kCap, DistanceBias kBias>
-__global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 2 : 1))) void attend_split_kernel(AttendArgs a) {
-  constexpr int KB = 32, NW = D <= 128 ? 4 : 2, NT = 64 * NW, P = Block<D>::kPitch, kChunks = P / 8;
+__global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_split_kernel(
+    AttendArgs a) {
+  constexpr int KB = 32, NW = split_waves<D>(), NT = 64 * NW, P = Block<D>::kPitch, kChunks = P / 8;
   typedef Rows<T, D, KB, kCap, kBias> R;
   typedef typename R::T8 T8;
   typedef typename Vec4<T>::type T4;
-  constexpr int kStage = 2 * KB * P;  // elements: a block of K, one of V
+  constexpr int kPlace = 2 * KB * P;  // elements of a wave's place: a block of K, one of V
   constexpr int OP = D + 1;           // pitch of a row of sums (floats)
-  static_assert(NW * 2 * kStage * sizeof(T) >= NW * 32 * OP * sizeof(float), "the waves' sums fit the stages");
-  __shared__ __align__(16) T lds[NW * 2 * kStage];
+  constexpr size_t kPlaces = NW * kPlace * sizeof(T), kSums = NW * 32 * OP * sizeof(float);
+  __shared__ __align__(16) char lds[kPlaces > kSums ? kPlaces : kSums];
   __shared__ float s_reference[NW][32], s_total[NW][32];
   __shared__ int s_bad[32];
 
-  int id = blockIdx.x;
-  const int z = id % a.splits;
-  id /= a.splits;
-  const int tile = id % a.row_tiles;
-  id /= a.row_tiles;
-  const int kv = id % a.kv_heads, s = id / a.kv_heads;
+  // The divisions are scalar code of some 100 cycles each, before anything can be loaded.
+  int id = blockIdx.x, z = 0, tile = 0;
+  if (a.splits > 1) {
+    const int n = id / a.splits;
+    z = id - n * a.splits;
+    id = n;
+  }
+  if (a.row_tiles > 1) {
+    const int n = id / a.row_tiles;
+    tile = id - n * a.row_tiles;
+    id = n;
+  }
+  const int s = a.n_seq > 1 ? id / a.kv_heads : 0, kv = id - s * a.kv_heads;
   const Sequence sq = sequence(a, s);
-  const int n_rows = sq.nq * a.group;  // below 2^31: the host's check of max_q * group
+  const int n_rows = sq.nq * a.group;  // below 2^30: the host's check of max_q * group
   if (tile * 32 >= n_rows) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = tile * 32 + (lane & 31);
   const bool valid = row < n_rows;
-  const int i = valid ? row / a.group : 0, head = kv * a.group + (valid ? row - i * a.group : 0);
+  const int i = !valid ? 0 : a.group > 1 ? row / a.group : row, head = kv * a.group + (valid ? row - i * a.group : 0);
   const Seen me = valid ? seen(a, sq, i) : Seen{0, 0, 0};
   const int last = min(tile * 32 + 31, n_rows - 1) / a.group;
   const Range range = wave_range(a, sq, me, valid, tile * 32 / a.group, last);
@@ -231,25 +244,27 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
 
   constexpr int CH = KB * kChunks / 64, step = 64 / kChunks;
   const int r0 = lane / kChunks, c0 = lane % kChunks;
-  const unsigned stage0 = lds_address(lds + wave * 2 * kStage);
+  unsigned at_k[CH], at_v[CH];
+#pragma unroll
+  for (int m = 0; m < CH; ++m) {
+    const int r = r0 + m * step, ck = c0 ^ Block<D>::k_swizzle(r), cv = c0 ^ Block<D>::v_swizzle(r);
+    at_k[m] = ck * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.k_row) + 16u * ck : kNoChunk;
+    at_v[m] = cv * 8 < a.dim ? 2u * static_cast<unsigned>(r) * static_cast<unsigned>(a.v_row) + 16u * cv : kNoChunk;
+  }
   const Source<KB> from_k(K, a.k_row, sq.nk, a.dim), from_v(V, a.v_row, sq.nk, a.dim);
-  auto stage = [&](int key, int buf) __attribute__((always_inline)) {
-    const i32x4 rk = from_k.resource(key, sq.nk), rv = from_v.resource(key, sq.nk);
-    const unsigned to = stage0 + buf * static_cast<unsigned>(kStage * sizeof(T));
+  const unsigned mine = wave * static_cast<unsigned>(kPlace * sizeof(T));
+  const unsigned lds_k = lds_address(lds) + mine, lds_v = lds_k + KB * P * sizeof(T);
+  // A wave's LDS reads of a block are done before loads overwrite it.
+  auto load = [&](const Source<KB>& from, const unsigned (&at)[CH], unsigned to, int key) __attribute__((always_inline)) {
+    const i32x4 r = from.resource(key, sq.nk);
+    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0_keep_vm());
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int m = 0; m < CH; ++m) {
-      const int r = r0 + m * step, c = c0 ^ Block<D>::k_swizzle(r);
-      const unsigned at = c * 8 < a.dim ? static_cast<unsigned>(r) * from_k.row + 16u * c : kNoChunk;
-      lds_load16_buffer<true>(rk, at, 0u, to + m * 1024u);
-    }
-#pragma unroll
-    for (int m = 0; m < CH; ++m) {
-      const int r = r0 + m * step, c = c0 ^ Block<D>::v_swizzle(r);
-      const unsigned at = c * 8 < a.dim ? static_cast<unsigned>(r) * from_v.row + 16u * c : kNoChunk;
-      lds_load16_buffer<true>(rv, at, 0u, to + KB * P * 2u + m * 1024u);
-    }
+    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(r, at[m], 0u, to + m * 1024u);
   };
 
+  int j = j0 + wave, key0 = blocks.taken(j);
+  if (j < j1) load(from_k, at_k, lds_k, key0);
   R rows;
   rows.start(lane);
   rows.load_q(static_cast<const T*>(a.q) + (sq.q0 + i) * a.q_row + head * a.q_head, a.dim, valid);
@@ -259,32 +274,28 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
   rows.position = me.position;
   rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
   const float* table = kBias == DistanceBias::Table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr;
-
-  int j = j0 + wave;
-  int key0 = blocks.taken(j);
-  if (j < j1) stage(key0, 0);
-  for (int buf = 0; j < j1; j += NW, buf ^= 1) {
+  if (j < j1) load(from_v, at_v, lds_v, key0);
+  for (; j < j1; j += NW) {
     const int key = key0;
-    const unsigned mine = (wave * 2 + buf) * static_cast<unsigned>(kStage * sizeof(T));
-    // The other stage's reads ended before its loads start: LDS answers a wave in order, and this waits for them.
-    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0_keep_vm());
-    asm volatile("" ::: "memory");
-    if (j + NW < j1) {
-      key0 = blocks.taken(j + NW);
-      stage(key0, buf ^ 1);
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(2 * CH));  // all but the loads just issued
-    } else {
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));
-    }
-    asm volatile("" ::: "memory");
+    const bool more = j + NW < j1;
     f32x16 t[1];
     T8 p[2];
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(CH));  // all but this block's V
+    asm volatile("" ::: "memory");
     rows.scores((LdsBytes)(lds), mine, t);
+    if (more) {
+      key0 = blocks.taken(j + NW);
+      load(from_k, at_k, lds_k, key0);
+    }
     rows.change(a, t, key, table);
     if (!(key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi))) rows.hide(t, key);
     const float sum = rows.weights(a, t, p);
     rows.total += rows.move(a, t, p, sum);
+    if (more) __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(CH));  // all but the next block's K
+    else __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));
+    asm volatile("" ::: "memory");
     rows.weigh((LdsBytes)(lds) + KB * P * 2, mine, p);
+    if (more) load(from_v, at_v, lds_v, key0);
   }
 
   // The waves' sums join: sum_w 2^(m_w - M) O_w and sum_w 2^(m_w - M) l_w.
@@ -306,52 +317,45 @@ __global__ __launch_bounds__(D <= 128 ? 256 : 128) __attribute__((amdgpu_waves_p
       for (int r = 0; r < 16; ++r) mine[32 * d + 8 * (r >> 2) + 4 * rows.g + (r & 3)] = rows.o[d][r];
   }
   __syncthreads();
-  constexpr int DPT = D * 32 / NT;
-  static_assert(DPT % 4 == 0, "whole quads a thread");
   const long long slot = ((static_cast<long long>(s) * a.kv_heads + kv) * a.row_tiles + tile) * a.splits + z;
   float* part = a.parts + slot * 32 * a.dim;
   float* ml = a.parts + static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * a.splits * 32 * a.dim + slot * 64;
   T* out = static_cast<T*>(a.out);
-  {
-    const int mr = tid % 32, d0 = tid / 32 * DPT;
-    const int orow = tile * 32 + mr;
-    if (orow < n_rows && !s_bad[mr]) {
-      float m = kNothing;
+  const int mr = tid % 32, orow = tile * 32 + mr;  // NT is a multiple of 32: a thread's quads are of one row
+  if (orow < n_rows && !s_bad[mr]) {
+    float m = kNothing;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) m = fmaxf(m, s_reference[w][mr]);
-      float wt[NW], total = 0.f;
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, s_reference[w][mr]);
+    float wt[NW], total = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        wt[w] = __builtin_amdgcn_exp2f(s_reference[w][mr] - m);
-        total += wt[w] * s_total[w][mr];
+    for (int w = 0; w < NW; ++w) {
+      wt[w] = __builtin_amdgcn_exp2f(s_reference[w][mr] - m);
+      total += wt[w] * s_total[w][mr];
+    }
+    const int oi = orow / a.group, oh = kv * a.group + orow - oi * a.group;
+    T* to = out + (sq.q0 + oi) * a.out_row + oh * a.out_head;
+    const float inv = a.splits > 1 ? 1.f : total == 0.f ? 0.f : 1.0f / total;
+    for (int d = tid / 32 * 4; d < a.dim; d += NT / 32 * 4) {
+      f32x4 v;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) sum += wt[w] * so[(w * 32 + mr) * OP + d + x];
+        v[x] = sum * inv;
       }
-      const int oi = orow / a.group, oh = kv * a.group + orow - oi * a.group;
-      T* to = out + (sq.q0 + oi) * a.out_row + oh * a.out_head;
-      const float inv = a.splits > 1 ? 1.f : total == 0.f ? 0.f : 1.0f / total;
+      if (a.splits > 1) {
+        *reinterpret_cast<f32x4*>(part + mr * a.dim + d) = v;
+      } else {
+        T4 h;
 #pragma unroll
-      for (int e = 0; e < DPT; e += 4) {
-        if (d0 + e >= a.dim) continue;
-        f32x4 v;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          float sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < NW; ++w) sum += wt[w] * so[(w * 32 + mr) * OP + d0 + e + x];
-          v[x] = sum * inv;
-        }
-        if (a.splits > 1) {
-          *reinterpret_cast<f32x4*>(part + mr * a.dim + d0 + e) = v;
-        } else {
-          T4 h;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) h[x] = to_half<T>(v[x]);
-          *reinterpret_cast<T4*>(to + d0 + e) = h;
-        }
+        for (int x = 0; x < 4; ++x) h[x] = to_half<T>(v[x]);
+        *reinterpret_cast<T4*>(to + d) = h;
       }
-      if (a.splits > 1 && d0 == 0) {
-        ml[2 * mr] = m;
-        ml[2 * mr + 1] = total;
-      }
+    }
+    if (a.splits > 1 && tid < 32) {
+      ml[2 * mr] = m;
+      ml[2 * mr + 1] = total;
     }
   }
   for (int b = wave; b < 32; b += NW) {
@@ -381,7 +385,7 @@ template <typename T, int D, bool kCap, DistanceBias kBias>
 hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   if (split) {
     const unsigned grid = static_cast<unsigned>(static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * a.splits);
-    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(grid), dim3(D <= 128 ? 256 : 128), 0, stream, a);
+    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(grid), dim3(64 * split_waves<D>()), 0, stream, a);
     return hipGetLastError();
   }
   const int tiles = (a.max_q + 127) / 128;
@@ -426,44 +430,62 @@ template <> hipError_t launch_attend_dim<256>(const AttendArgs&, DType, Distance
 
 namespace {
 
-// A row's sums over the splits: weights 2^(m_z - M), then one division.  A wave a row; a lane a split, then a lane a dim.
+// A row's sums over the splits: weights 2^(m_z - M), then one division.  A workgroup a row: its four waves share the splits, in a
+// fixed order, a lane four dims; every load of a wave is on its way before the first sum.
+constexpr int kJoinWaves = 4, kJoinLoads = kMaxSplits / kJoinWaves;
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long long at = static_cast<long long>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long tiles = static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles;
-  const long long tile = at / 32;
-  const int r = static_cast<int>(at % 32);
-  if (tile >= tiles) return;
-  const int s = static_cast<int>(tile / (a.kv_heads * a.row_tiles)), w = static_cast<int>(tile % (a.kv_heads * a.row_tiles));
-  const int kv = w / a.row_tiles, row = w % a.row_tiles * 32 + r;
-  const int q0 = a.q_starts[s];
-  const int nq = q0 < 0 || q0 >= a.q_rows ? 0 : min(min(a.q_lengths[s], a.max_q), a.q_rows - q0);
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(AttendArgs a, int used) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x / used, r = blockIdx.x - tile * used;  // used: rows of a tile that any sequence has
+  const int per = a.kv_heads * a.row_tiles, tiles = a.n_seq * per;  // below 2^24
+  const int s = tile / per, w = tile - s * per;
+  const int kv = w / a.row_tiles, row = (w - kv * a.row_tiles) * 32 + r;
   const int i = row / a.group;
-  if (i >= nq) return;
-  const float* parts = a.parts + tile * a.splits * 32 * a.dim + r * a.dim;
-  const float2* ml = reinterpret_cast<const float2*>(a.parts + tiles * a.splits * 32 * a.dim) + tile * a.splits * 32 + r;
+  const int q0 = a.q_starts[s], nq = a.q_lengths[s];
+  if (q0 < 0 || q0 >= a.q_rows || i >= min(min(nq, a.max_q), a.q_rows - q0)) return;
+  const float* parts = a.parts + static_cast<long long>(tile) * a.splits * 32 * a.dim + r * a.dim;
+  const float2* ml = reinterpret_cast<const float2*>(a.parts + static_cast<long long>(tiles) * a.splits * 32 * a.dim) +
+                     static_cast<long long>(tile) * a.splits * 32 + r;
   float m = kNothing, l = 0.f;
   if (lane < a.splits) {
     const float2 x = ml[lane * 32];
     m = x.x;
     l = x.y;
   }
+  const bool mine = 4 * lane < a.dim;
+  f32x4 v[kJoinLoads];
+#pragma unroll
+  for (int n = 0; n < kJoinLoads; ++n) {
+    const int z = wave + kJoinWaves * n;
+    v[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (z < a.splits && mine) v[n] = *reinterpret_cast<const f32x4*>(parts + static_cast<long long>(z) * 32 * a.dim + 4 * lane);
+  }
   const float top = wave_max(m);
   const float weight = __builtin_amdgcn_exp2f(m - top);
   const float total = wave_sum(weight * l);
-  const float inv = total == 0.f ? 0.f : 1.0f / total;
-  float sum[kMaxAttendDim / 64] = {0.f, 0.f, 0.f, 0.f};
-  for (int z = 0; z < a.splits; ++z) {
-    const float f = __shfl(weight, z, kWave);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < kMaxAttendDim / 64; ++x)
-      if (lane + 64 * x < a.dim) sum[x] += f * parts[static_cast<long long>(z) * 32 * a.dim + lane + 64 * x];
+  for (int n = 0; n < kJoinLoads; ++n) {
+    const float f = __shfl(weight, wave + kJoinWaves * n, kWave);
+    if (wave + kJoinWaves * n < a.splits) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum[x] = __builtin_fmaf(f, v[n][x], sum[x]);
+    }
   }
-  T* out = static_cast<T*>(a.out) + (q0 + i) * a.out_row + (kv * a.group + row - i * a.group) * a.out_head;
+  __shared__ f32x4 others[kJoinWaves - 1][64];
+  if (wave) others[wave - 1][lane] = sum;
+  __syncthreads();
+  if (wave || !mine) return;
 #pragma unroll
-  for (int x = 0; x < kMaxAttendDim / 64; ++x)
-    if (lane + 64 * x < a.dim) out[lane + 64 * x] = to_half<T>(sum[x] * inv);
+  for (int n = 0; n < kJoinWaves - 1; ++n)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) sum[x] += others[n][lane][x];
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  typename Vec4<T>::type h;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) h[x] = to_half<T>(sum[x] * inv);
+  T* out = static_cast<T*>(a.out) + (q0 + i) * a.out_row + (kv * a.group + row - i * a.group) * a.out_head;
+  *reinterpret_cast<typename Vec4<T>::type*>(out + 4 * lane) = h;
 }
 
 // The run of equal ids around each row of a sequence.  A wave takes 64 rows: where ids change comes from one ballot, and what
@@ -533,9 +555,11 @@ AttendPlan attend_plan(const AttendArgs& a) {
   long long keys = a.max_k;
   if (a.before >= 0 && !a.prefix) keys = keys < static_cast<long long>(a.before) + a.max_q + 64 ? keys : static_cast<long long>(a.before) + a.max_q + 64;
   const long long base = static_cast<long long>(a.n_seq) * a.kv_heads * p.row_tiles;
-  const long long wanted = 1024 / (base > 0 ? base : 1), most = keys / 512;
-  long long n = wanted < most ? wanted : most;
-  p.splits = static_cast<int>(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
+  // As many workgroups as compute units, each with a block of keys for every wave at least; joining costs what two such
+  // rounds take, so two workgroups a tile are not worth it.
+  const long long wanted = 256 / (base > 0 ? base : 1), most = keys / 256;
+  const long long n = wanted < most ? wanted : most;
+  p.splits = static_cast<int>(n < 3 ? 1 : n > kMaxSplits ? kMaxSplits : n);
   if (p.splits > 1) p.workspace = base * p.splits * 32 * (a.dim + 2) * 4;
   return p;
 }
@@ -549,10 +573,10 @@ hipError_t launch_attend(const AttendArgs& args, DType t, DistanceBias bias, boo
                        : a.dim <= 128 ? launch_attend_dim<128>(a, t, bias, cap, plan.split, stream)
                                       : launch_attend_dim<256>(a, t, bias, cap, plan.split, stream);
   if (e != hipSuccess || plan.splits <= 1) return e;
-  const long long rows = static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * 32;
-  const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
-  if (t == DType::F16) LAYA_LAUNCH(join_kernel<f16>, grid, dim3(256), 0, stream, a);
-  else LAYA_LAUNCH(join_kernel<bf16>, grid, dim3(256), 0, stream, a);
+  const int used = a.row_tiles > 1 ? 32 : a.max_q * a.group;
+  const dim3 grid(static_cast<unsigned>(static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * used));
+  if (t == DType::F16) LAYA_LAUNCH(join_kernel<f16>, grid, dim3(64 * kJoinWaves), 0, stream, a, used);
+  else LAYA_LAUNCH(join_kernel<bf16>, grid, dim3(64 * kJoinWaves), 0, stream, a, used);
   return hipGetLastError();
 }
 

@@ -1724,7 +1724,7 @@ static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
                    static_cast<int64_t>(c->max_q) * a.group < (1LL << 30),
                "n_seq * heads * max_q: too large for one launch");
   *plan = attend_plan(a);
-  LAYA_REQUIRE(!plan->split || static_cast<int64_t>(c->n_seq) * c->kv_heads * plan->row_tiles * plan->splits < kMaxGroups,
+  LAYA_REQUIRE(!plan->split || static_cast<int64_t>(c->n_seq) * c->kv_heads * plan->row_tiles * plan->splits < kMaxGroups / 2,
                "n_seq * heads * max_q: too large for one launch");
   return a;
 }
