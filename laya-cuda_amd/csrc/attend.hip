@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
   if (lane == 0) wg_range[wave] = active ? range : Range{INT_MAX, 0, 0, INT_MAX};
   if constexpr (kBias == DistanceBias::Table) {
     const float* from = a.table + static_cast<size_t>(head) * (2 * a.span + 1);
-    for (int e = tid; e < 2 * (a.span + kPad) + 1; e += 256) stable[e] = from[max(0, min(2 * a.span, e - kPad))] * kLog2e;
+    for (int e = tid; e < 2 * (a.span + kPad) + 1; e += 256) stable[e] = from[max(0, min(2 * a.span, e - kPad))] * a.per_unit;
   }
   __syncthreads();
   Range wg = wg_range[0];
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
   rows.hi = me.hi;
   rows.prefix = sq.prefix;
   rows.position = me.position;
-  rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
+  rows.slope = kBias == DistanceBias::Slopes ? -a.slopes[head] * a.per_unit : 0.f;
   const LdsFloats table = (LdsFloats)(stable) + a.span + kPad;
 
   float far_left = 0.f, far_right = 0.f;
@@ -141,17 +141,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
       f32x16 t[R::KT];
       T8 p[2 * R::KT];
       rows.scores((LdsBytes)(sk[0]) + SB * h * P * 2, buffer, t);
-      if constexpr (kBias == DistanceBias::Table) {
-        // Steps wholly past the span on one side add that end's value; the table's LDS rows reach as far as the others need.
-        const bool left = key + SB - 1 - first_position <= -a.span, right = key - (first_position + 31) >= a.span;
-        if (left || right) rows.add(a, t, left ? far_left : far_right);
-        else rows.change(a, t, key, table);
+      float shift;
+      const int first = key - first_position;  // of the wave's first query to the step's first key
+      if (kBias == DistanceBias::Table && (first + SB - 1 <= -a.span || first - 31 >= a.span)) {
+        // Steps wholly past the span on one side have one bias; the table's LDS rows reach as far as the others need.
+        rows.capped(a, t);
+        shift = __builtin_fmaf(first < 0 ? far_left : far_right, a.unit, kCap ? a.cap : 0.f);
       } else {
-        rows.change(a, t, key, table);
+        shift = rows.change(a, t, key, table, first + SB - 1 <= 0 ? -1 : first - 31 >= 0 ? 1 : 0);
       }
       if (!whole) rows.hide(t, key);
-      const float sum = rows.weights(a, t, p);
-      rows.total += rows.move(a, t, p, sum);
+      const float sum = rows.weights(a, t, p, shift);
+      rows.total += rows.move(a, t, p, shift, sum);
       rows.weigh((LdsBytes)(sv[0]) + SB * h * P * 2, buffer, p);
     }
   }
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
   rows.hi = me.hi;
   rows.prefix = sq.prefix;
   rows.position = me.position;
-  rows.slope = kBias == DistanceBias::Slopes ? a.slopes[head] * kLog2e : 0.f;
+  rows.slope = kBias == DistanceBias::Slopes ? -a.slopes[head] * a.per_unit : 0.f;
   const float* table = kBias == DistanceBias::Table ? a.table + static_cast<size_t>(head) * (2 * a.span + 1) + a.span : nullptr;
   if (j < j1) load(from_v, at_v, lds_v, key0);
   for (; j < j1; j += NW) {
@@ -287,10 +288,10 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
       key0 = blocks.taken(j + NW);
       load(from_k, at_k, lds_k, key0);
     }
-    rows.change(a, t, key, table);
+    const float shift = rows.change(a, t, key, table, 0);
     if (!(key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi))) rows.hide(t, key);
-    const float sum = rows.weights(a, t, p);
-    rows.total += rows.move(a, t, p, sum);
+    const float sum = rows.weights(a, t, p, shift);
+    rows.total += rows.move(a, t, p, shift, sum);
     if (more) __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(CH));  // all but the next block's K
     else __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));
     asm volatile("" ::: "memory");
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
     const Seen m = seen(a, sq, oi);
     CarefulRow<T, D, KB, kCap, kBias> c;
     c.run(a, static_cast<const T*>(a.q) + (sq.q0 + oi) * a.q_row + oh * a.q_head, K, V, sq.nk, m.position, m.lo, m.hi, sq.prefix,
-          kBias == DistanceBias::Slopes ? a.slopes[oh] * kLog2e : 0.f,
+          kBias == DistanceBias::Slopes ? -a.slopes[oh] * a.per_unit : 0.f,
           a.table ? a.table + static_cast<size_t>(oh) * (2 * a.span + 1) + a.span : nullptr, blocks, j0, j1, lane);
     const float n = c.total == 0.f ? 0.f : 1.0f / c.total;
 #pragma unroll

@@ -18,8 +18,10 @@ struct AttendArgs {
   int heads, kv_heads, group, dim;  // group = heads / kv_heads
   int n_seq, max_q, max_k, q_rows, k_rows;
   const int32_t *q_starts, *q_lengths, *k_starts, *k_lengths;  // [n_seq]
-  float scale;           // of a raw product: to log2 units, or, capped, to twice the tanh's argument in log2 units
+  float scale;           // capped: of a raw product, to twice the tanh's argument in log2 units
   float cap;             // in log2 units
+  float unit;            // log2 units of a raw product, or, capped, of the tanh's reciprocal: -2 cap
+  float per_unit;        // log2(e) / unit: what a bias is multiplied with
   const float* slopes;   // [heads]
   const float* table;    // [heads][2 span + 1]
   int span;

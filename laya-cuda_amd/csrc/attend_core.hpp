@@ -19,7 +19,6 @@ namespace laya {
 
 constexpr float kNothing = -1e30f;    // the reference of a row that has seen no key; scores not above it count as hidden
 constexpr float kMostWeight = 8192.f;
-constexpr float kLog2e = 1.4426950408889634f;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -176,13 +175,12 @@ struct Rows {
   typedef short s16x8 __attribute__((ext_vector_type(8)));
   typedef Block<D> B;
   static constexpr int KS = D / 16, DT = D / 32, KT = KB / 32;
-  static constexpr bool kRaw = !kCap && kBias == DistanceBias::None;  // scores stay raw products until they become weights
 
   T8 q[KS];
   f32x16 o[DT];
   float reference, total;
   int lo, hi, prefix, position;
-  float slope;
+  float slope;  // in units of t
   int lane, g;
   unsigned k_at, v_at;  // byte offsets of this lane's first fragments
 
@@ -245,46 +243,52 @@ struct Rows {
   // Key of score r of tile kt of the block at `key`, less the lane's first.
   static constexpr int slot(int kt, int r) { return 32 * kt + 8 * (r >> 2) + (r & 3); }
 
-  // Raw products to log2 scores: cap and bias.  table: of this row's head, at distance 0; one in LDS is in log2 units and may
-  // be read up to a block and 32 rows past the span.
+  // A block's scores stand as t, of which the log2 score is a.unit t + shift: raw products, or, capped, the reciprocals in
+  // cap tanh(x) = cap - 2 cap / (1 + exp(2 x)), exact to 2^-22 of the cap; biases are added in units of t.  A weight's exponent is
+  // then one multiplication and addition away.  Slopes of a block to one side of every row are linear in the key: what they have in common
+  // goes into the shift.
+  // table: of this row's head, at distance 0; one in LDS is in units of t and may be read up to a block and 32 rows past the span.
+  // side: -1 and 1 where all keys lie before or behind all rows' positions (or at them), 0 where not.
   template <typename Table>
-  __device__ __forceinline__ void change(const AttendArgs& a, f32x16 (&s)[KT], int key, Table table) const {
-    constexpr bool kLdsTable = std::is_same<Table, LdsFloats>::value;
-    if constexpr (!kRaw) {
-      const int at = key + 4 * g - position;
+  __device__ __forceinline__ float change(const AttendArgs& a, f32x16 (&s)[KT], int key, Table table, int side) const {
+    capped(a, s);
+    float shift = kCap ? a.cap : 0.f;
+    const int at = key + 4 * g - position;
+    if constexpr (kBias == DistanceBias::Slopes) {
       const float from = static_cast<float>(at);
+      if (side) {
+        const float by = side < 0 ? -slope : slope;  // of |d| = -d or d
+        shift = __builtin_fmaf(from * by, a.unit, shift);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kt][r] += static_cast<float>(slot(kt, r)) * by;
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kt][r] = __builtin_fmaf(fabsf(from + static_cast<float>(slot(kt, r))), slope, s[kt][r]);
+      }
+    }
+    if constexpr (kBias == DistanceBias::Table) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          float x = s[kt][r];
-          if constexpr (kCap) {  // cap tanh(x) = cap - 2 cap / (1 + exp(2 x)); exact to 2^-22 of the cap
-            const float y = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f);
-            x = __builtin_fmaf(y, -2.0f * a.cap, a.cap);
-          }
-          float b = 0.f;
-          if constexpr (kBias == DistanceBias::Slopes) b = -slope * fabsf(from + static_cast<float>(slot(kt, r)));
-          if constexpr (kBias == DistanceBias::Table) {
-            const int d = at + slot(kt, r);
-            b = kLdsTable ? table[d] : table[max(-a.span, min(a.span, d))] * kLog2e;
-          }
-          s[kt][r] = kCap ? x + b : __builtin_fmaf(x, a.scale, b);
+          const int d = at + slot(kt, r);
+          if constexpr (std::is_same<Table, LdsFloats>::value) s[kt][r] += table[d];
+          else s[kt][r] = __builtin_fmaf(table[max(-a.span, min(a.span, d))], a.per_unit, s[kt][r]);
         }
     }
+    return shift;
   }
-
-  // The same with one bias for all keys.
-  __device__ __forceinline__ void add(const AttendArgs& a, f32x16 (&s)[KT], float b) const {
+  __device__ __forceinline__ void capped(const AttendArgs& a, f32x16 (&s)[KT]) const {
+    if constexpr (kCap) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = s[kt][r];
-        if constexpr (kCap)
-          s[kt][r] = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f), -2.0f * a.cap, a.cap) + b;
-        else
-          s[kt][r] = __builtin_fmaf(x, a.scale, b);
-      }
+        for (int r = 0; r < 16; ++r) s[kt][r] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kt][r] * a.scale) + 1.0f);
+    }
   }
 
   __device__ __forceinline__ void hide(f32x16 (&s)[KT], int key) const {
@@ -295,29 +299,27 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = at + slot(kt, r);
-        s[kt][r] = (static_cast<unsigned>(j - lo) < seen_keys || j < prefix) ? s[kt][r] : -INFINITY;
+        s[kt][r] = (static_cast<unsigned>(j - lo) < seen_keys || j < prefix) ? s[kt][r] : kCap ? INFINITY : -INFINITY;
       }
   }
 
-  __device__ __forceinline__ float block_max(const AttendArgs& a, const f32x16 (&s)[KT]) const {
-    float m = -INFINITY;
+  // The largest score: of the largest t, or of the smallest where the cap's unit is negative.
+  __device__ __forceinline__ float block_max(const AttendArgs& a, const f32x16 (&s)[KT], float shift) const {
+    float m = kCap ? INFINITY : -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, s[kt][r]);
-    m = halves_max(m);
-    return kRaw ? m * a.scale : m;
+      for (int r = 0; r < 16; ++r) m = kCap ? fminf(m, s[kt][r]) : fmaxf(m, s[kt][r]);
+    return halves_max(__builtin_fmaf(m, a.unit, shift));
   }
 
-  __device__ __forceinline__ float weights(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT]) const {
+  __device__ __forceinline__ float weights(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], float shift) const {
     float sum[2] = {0.f, 0.f};
+    const float base = shift - reference;
 #pragma unroll
     for (int c = 0; c < 2 * KT; ++c) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = s[c >> 1][8 * (c & 1) + e];
-        p[c][e] = to_half<T>(__builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(x, a.scale, -reference) : x - reference));
-      }
+      for (int e = 0; e < 8; ++e) p[c][e] = to_half<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 1][8 * (c & 1) + e], a.unit, base)));
       sum[0] = pair_sum(__builtin_shufflevector(p[c], p[c], 0, 1), sum[0]);
       sum[1] = pair_sum(__builtin_shufflevector(p[c], p[c], 2, 3), sum[1]);
       sum[0] = pair_sum(__builtin_shufflevector(p[c], p[c], 4, 5), sum[0]);
@@ -326,11 +328,10 @@ struct Rows {
     return sum[0] + sum[1];
   }
 
-  // Weights that are too large for the reference: it moves to the block's largest score.  Negative scales turn the order of raw
-  // scores round, so the caller's scale is not negative.
-  __device__ __forceinline__ float move(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], float sum) {
+  // Weights that are too large for the reference: it moves to the block's largest score.
+  __device__ __forceinline__ float move(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], float shift, float sum) {
     if (__builtin_amdgcn_ballot_w64(!(sum <= kMostWeight))) {
-      const float m = block_max(a, s);
+      const float m = block_max(a, s, shift);
       const float to = m > reference + 8.f ? m : reference;
       const float alpha = to == reference ? 1.f : __builtin_amdgcn_exp2f(reference - to);
       reference = to;
@@ -339,7 +340,7 @@ struct Rows {
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-      sum = weights(a, s, p);
+      sum = weights(a, s, p, shift);
     }
     return sum;
   }
@@ -383,10 +384,10 @@ struct CarefulRow {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x = __builtin_fmaf(to_float(kc[e]), to_float(qc[e]), x);
         }
-        x *= a.scale;
-        if constexpr (kCap) x = __builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f), -2.0f * a.cap, a.cap);
-        if constexpr (kBias == DistanceBias::Slopes) x -= slope * fabsf(static_cast<float>(key - position));
-        if constexpr (kBias == DistanceBias::Table) x += table[max(-a.span, min(a.span, key - position))] * kLog2e;
+        if constexpr (kCap) x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f);
+        if constexpr (kBias == DistanceBias::Slopes) x = __builtin_fmaf(fabsf(static_cast<float>(key - position)), slope, x);
+        if constexpr (kBias == DistanceBias::Table) x = __builtin_fmaf(table[max(-a.span, min(a.span, key - position))], a.per_unit, x);
+        x = __builtin_fmaf(x, a.unit, kCap ? a.cap : 0.f);
       }
       const float to = fmaxf(reference, wave_max(x));
       const float alpha = to == reference ? 1.f : __builtin_amdgcn_exp2f(reference - to);

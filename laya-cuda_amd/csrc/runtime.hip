@@ -1744,8 +1744,8 @@ int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_by
     AttendPlan plan;
     AttendArgs a = attend_sizes(call, &plan);
     const LayaAttend& c = *call;
-    LAYA_REQUIRE(c.scale >= 0.f && std::isfinite(c.scale) && (c.cap == 0.f || (c.cap >= 1e-30f && std::isfinite(c.cap))),
-                 "scale must not be negative, cap 0 or at least 1e-30, both finite");
+    LAYA_REQUIRE(c.scale >= 1e-10f && c.scale <= 1e10f && (c.cap == 0.f || (c.cap >= 1e-10f && c.cap <= 1e10f)),
+                 "scale must be 1e-10 to 1e10, cap 0 or as much");
     LAYA_REQUIRE(stride_ok(c.q_row) && stride_ok(c.q_head) && stride_ok(c.k_row) && stride_ok(c.k_head) && stride_ok(c.v_row) &&
                      stride_ok(c.v_head) && stride_ok(c.out_row) && stride_ok(c.out_head) &&
                      ((c.q_row | c.q_head | c.k_row | c.k_head | c.v_row | c.v_head | c.out_row | c.out_head) & 7) == 0,
@@ -1768,8 +1768,10 @@ int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_by
     a.v_row = c.v_row; a.v_head = c.v_head; a.out_row = c.out_row; a.out_head = c.out_head;
     a.q_starts = c.q_starts; a.q_lengths = c.q_lengths; a.k_starts = c.k_starts; a.k_lengths = c.k_lengths;
     constexpr float kLog2e = 1.4426950408889634f;
-    a.scale = c.cap > 0.f ? 2.0f * kLog2e * (c.scale / c.cap) : c.scale * kLog2e;
+    a.scale = 2.0f * kLog2e * (c.cap > 0.f ? c.scale / c.cap : 0.f);
     a.cap = c.cap * kLog2e;
+    a.unit = c.cap > 0.f ? -2.0f * a.cap : c.scale * kLog2e;
+    a.per_unit = kLog2e / a.unit;
     a.slopes = c.slopes; a.table = c.table; a.bounds = reinterpret_cast<const int2*>(c.bounds);
     a.parts = static_cast<float*>(workspace);
     const DistanceBias bias = c.slopes ? DistanceBias::Slopes : c.table ? DistanceBias::Table : DistanceBias::None;

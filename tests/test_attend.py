@@ -153,9 +153,9 @@ def test_attend_refusals():
     call("span", table=P, span=1025)
     call("too large", n_seq=1 << 23)
     call("too large", n_seq=1 << 12, max_q=1 << 20)
-    for bad in (dict(scale=-0.1), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.inf), dict(cap=math.nan),
-                dict(cap=1e-31)):
-        call("scale must not", **bad)
+    for bad in (dict(scale=-0.1), dict(scale=0.0), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.inf),
+                dict(cap=math.nan), dict(cap=1e-11)):
+        call("scale must be", **bad)
     for name in ("q_row", "k_head", "v_row", "out_head"):
         call("strides", **{name: 132})
         call("strides", **{name: -64})
