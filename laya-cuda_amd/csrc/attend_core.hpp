@@ -291,16 +291,20 @@ struct Rows {
     }
   }
 
+  // Scores of hidden keys: none.  A lane's keys of a step are bits of one word, and a score takes two instructions.
   __device__ __forceinline__ void hide(f32x16 (&s)[KT], int key) const {
-    const int at = key + 4 * g;
-    const unsigned seen_keys = static_cast<unsigned>(hi - lo);
+    static_assert(KT == 1, "32 keys a step");
+    const auto below = [&](int end) {  // keys before `end`
+      const int n = end - key;
+      return n <= 0 ? 0u : ~0u >> (32 - min(n, 32));
+    };
+    const unsigned hidden = ~((below(hi) & ~below(lo)) | below(prefix)) >> (4 * g);
+    constexpr int kNone = kCap ? 0x7f800000 : static_cast<int>(0xff800000);  // infinite, towards a score of -infinity
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = at + slot(kt, r);
-        s[kt][r] = (static_cast<unsigned>(j - lo) < seen_keys || j < prefix) ? s[kt][r] : kCap ? INFINITY : -INFINITY;
-      }
+    for (int r = 0; r < 16; ++r) {
+      const int mask = static_cast<int>(hidden << (31 - slot(0, r))) >> 31;
+      s[0][r] = __int_as_float((mask & kNone) | (~mask & __float_as_int(s[0][r])));
+    }
   }
 
   // The largest score: of the largest t, or of the smallest where the cap's unit is negative.
