@@ -201,19 +201,20 @@ constexpr int split_waves() {
 }
 template <typename T, int D, bool kCap, DistanceBias kBias>
 __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_split_kernel(
-    AttendArgs a) {
+    AttendArgs a, int units) {
   constexpr int KB = 32, NW = split_waves<D>(), NT = 64 * NW, P = Block<D>::kPitch, kChunks = P / 8;
   typedef Rows<T, D, KB, kCap, kBias> R;
   typedef typename R::T8 T8;
   typedef typename Vec4<T>::type T4;
   constexpr int kPlace = 2 * KB * P;  // elements of a wave's place: a block of K, one of V
-  constexpr int OP = D + 1;           // pitch of a row of sums (floats)
+  constexpr int OP = D + 4;           // pitch of a row of sums (floats): 16 rows' quads lie in 16 places of 256 bytes
   constexpr size_t kPlaces = NW * kPlace * sizeof(T), kSums = NW * 32 * OP * sizeof(float);
   __shared__ __align__(16) char lds[kPlaces > kSums ? kPlaces : kSums];
   __shared__ float s_reference[NW][32], s_total[NW][32];
   __shared__ int s_bad[32];
 
-  // The divisions are scalar code of some 100 cycles each, before anything can be loaded.
+  // Workgroup -> (sequence, key head, tile, split).  The divisions are scalar code of some 100 cycles each, before anything can be
+  // loaded.  Tiles of the same keys stay on one XCD, by the same rule as prompts.
   int id = blockIdx.x, z = 0, tile = 0;
   if (a.splits > 1) {
     const int n = id / a.splits;
@@ -221,9 +222,16 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
     id = n;
   }
   if (a.row_tiles > 1) {
-    const int n = id / a.row_tiles;
-    tile = id - n * a.row_tiles;
-    id = n;
+    if (units) {
+      const int y = id >> 3, at = y / a.row_tiles;
+      tile = y - at * a.row_tiles;
+      id = (id & 7) + 8 * at;
+      if (id >= units) return;
+    } else {
+      const int n = id / a.row_tiles;
+      tile = id - n * a.row_tiles;
+      id = n;
+    }
   }
   const int s = a.n_seq > 1 ? id / a.kv_heads : 0, kv = id - s * a.kv_heads;
   const Sequence sq = sequence(a, s);
@@ -311,11 +319,14 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
       s_total[wave][lane & 31] = total;
       if (valid && (bad >> lane & 1)) s_bad[lane] = 1;  // every writer writes 1
     }
-    float* mine = so + (wave * 32 + (lane & 31)) * OP;
+    float* mine = so + (wave * 32 + (lane & 31)) * OP + 4 * rows.g;
+    if (valid) {
 #pragma unroll
-    for (int d = 0; d < R::DT; ++d)
+      for (int d = 0; d < R::DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mine[32 * d + 8 * (r >> 2) + 4 * rows.g + (r & 3)] = rows.o[d][r];
+        for (int r = 0; r < 16; r += 4)
+          *reinterpret_cast<f32x4*>(mine + 32 * d + 2 * r) = f32x4{rows.o[d][r], rows.o[d][r + 1], rows.o[d][r + 2], rows.o[d][r + 3]};
+    }
   }
   __syncthreads();
   const long long slot = ((static_cast<long long>(s) * a.kv_heads + kv) * a.row_tiles + tile) * a.splits + z;
@@ -337,14 +348,15 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
     T* to = out + (sq.q0 + oi) * a.out_row + oh * a.out_head;
     const float inv = a.splits > 1 ? 1.f : total == 0.f ? 0.f : 1.0f / total;
     for (int d = tid / 32 * 4; d < a.dim; d += NT / 32 * 4) {
-      f32x4 v;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float sum = 0.f;
+      for (int w = 0; w < NW; ++w) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(so + (w * 32 + mr) * OP + d);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) sum += wt[w] * so[(w * 32 + mr) * OP + d + x];
-        v[x] = sum * inv;
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(wt[w], x[e], v[e]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= inv;
       if (a.splits > 1) {
         *reinterpret_cast<f32x4*>(part + mr * a.dim + d) = v;
       } else {
@@ -359,8 +371,11 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
       ml[2 * mr + 1] = total;
     }
   }
-  for (int b = wave; b < 32; b += NW) {
-    if (!s_bad[b]) continue;
+  unsigned bad = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(s_bad[lane & 31] != 0));
+  while (bad) {
+    const int b = __builtin_ctz(bad);
+    bad &= bad - 1;
+    if (b % NW != wave) continue;
     const int orow = tile * 32 + b, oi = orow / a.group, oh = kv * a.group + orow - oi * a.group;
     const Seen m = seen(a, sq, oi);
     CarefulRow<T, D, KB, kCap, kBias> c;
@@ -385,8 +400,12 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
 template <typename T, int D, bool kCap, DistanceBias kBias>
 hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   if (split) {
-    const unsigned grid = static_cast<unsigned>(static_cast<long long>(a.n_seq) * a.kv_heads * a.row_tiles * a.splits);
-    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(grid), dim3(64 * split_waves<D>()), 0, stream, a);
+    const long long units = static_cast<long long>(a.n_seq) * a.kv_heads, share = (units + 7) / 8;
+    // Evenly over the XCDs, or in one round on each however unevenly.
+    const bool kept = a.row_tiles > 1 && a.splits == 1 && (units % 8 == 0 || units >= 64 || share * a.row_tiles <= (D <= 64 ? 64 : 32));
+    const long long grid = (kept ? share * 8 : units) * a.row_tiles * a.splits;
+    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(64 * split_waves<D>()), 0, stream, a,
+                kept ? static_cast<int>(units) : 0);
     return hipGetLastError();
   }
   const int tiles = (a.max_q + 127) / 128;

@@ -352,11 +352,12 @@ struct Rows {
   // Rows (bits 0 to 31) whose sums are no numbers: a weight of 0 times an infinity or NaN in a hidden key's value, if nothing
   // the row sees is one.
   __device__ __forceinline__ unsigned not_numbers() const {
-    float x = total;
+    float sum[4] = {total, 0.f, 0.f, 0.f};  // NaN for a NaN or an infinity
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x = __builtin_fmaf(o[d][r], 0.f, x);  // NaN for a NaN or an infinity
+      for (int r = 0; r < 16; ++r) sum[r & 3] = __builtin_fmaf(o[d][r], 0.f, sum[r & 3]);
+    const float x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     const unsigned long long bad = __builtin_amdgcn_ballot_w64(x != x);
     return static_cast<unsigned>(bad | bad >> 32);
   }
