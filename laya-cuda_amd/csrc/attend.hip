@@ -39,7 +39,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
       pair = id - t * units;
     }
   }
-  const int s = pair / a.heads, head = pair - s * a.heads, kv = head / a.group;
+  const int s = pair / a.heads;
+  const int head = pair - s * a.heads, kv = head / a.group;
   const Sequence sq = sequence(a, s);
   const int row0 = tile * 128;
   if (row0 >= sq.nq) return;
@@ -402,7 +403,7 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   if (split) {
     const long long units = static_cast<long long>(a.n_seq) * a.kv_heads, share = (units + 7) / 8;
     // Evenly over the XCDs, or in one round on each however unevenly.
-    const bool kept = a.row_tiles > 1 && a.splits == 1 && (units % 8 == 0 || units >= 64 || share * a.row_tiles <= (D <= 64 ? 64 : 32));
+    const bool kept = a.row_tiles > 1 && a.splits == 1 && (share * 56 <= units * 8 || share * a.row_tiles <= (D <= 64 ? 64 : 32));
     const long long grid = (kept ? share * 8 : units) * a.row_tiles * a.splits;
     LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(64 * split_waves<D>()), 0, stream, a,
                 kept ? static_cast<int>(units) : 0);
@@ -410,8 +411,10 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   }
   const int tiles = (a.max_q + 127) / 128;
   const long long pairs = static_cast<long long>(a.n_seq) * a.heads, shared = static_cast<long long>(a.n_seq) * a.kv_heads;
-  // Heads that share keys on one XCD, or each head, where that fills the XCDs evenly; else every tile for itself.
-  int unit = shared % 8 == 0 || shared >= 64 ? a.group : pairs % 8 == 0 || pairs >= 64 ? 1 : 0;
+  // Heads that share keys on one XCD, or each head, where that leaves no XCD more than a seventh above the mean; else every
+  // tile for itself.
+  const auto even = [](long long n) { return (n + 7) / 8 * 56 <= n * 8; };
+  const int unit = even(shared) ? a.group : even(pairs) ? 1 : 0;
   const long long units = unit ? pairs / unit : pairs;
   const long long grid = unit ? (units + 7) / 8 * 8 * unit * tiles : pairs * tiles;
   LAYA_LAUNCH((attend_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a, tiles, unit,
