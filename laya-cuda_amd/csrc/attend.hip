@@ -11,10 +11,12 @@ namespace laya {
 
 namespace {
 
+constexpr int kPad = 96;  // distances past a bias table's span that the scores of a block near its ends reach: its 64 keys and 32 rows
+
 // Prompts: a workgroup of four waves owns 128 queries of one head, and blocks of 64 keys pass through LDS, shared by the waves
 // and double-buffered.  A wave works on them 32 keys at a time and skips those that none of its rows sees.
 template <typename T, int D, bool kCap, DistanceBias kBias>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3 : D <= 128 ? 2 : 1))) void attend_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
   constexpr int KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
   constexpr int SB = 32;  // keys of one step
@@ -53,8 +55,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3
   __shared__ __align__(16) T sk[2][KB * P];
   __shared__ __align__(16) T sv[2][KB * P];
   __shared__ Range wg_range[4];
-  constexpr int kPad = KB + 32;  // distances past the span that a block near its ends reaches
-  __shared__ float stable[kBias == DistanceBias::Table ? 2 * (kMaxSpan + kPad) + 1 : 1];
+  extern __shared__ float stable[];  // the head's bias table in units of t, 2 (span + kPad) + 1
 
   const Range range = wave_range(a, sq, me, valid, row0 + wave * 32, min(row0 + wave * 32 + 31, sq.nq - 1));
   if (lane == 0) wg_range[wave] = active ? range : Range{INT_MAX, 0, 0, INT_MAX};
@@ -417,7 +418,8 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   const int unit = even(shared) ? a.group : even(pairs) ? 1 : 0;
   const long long units = unit ? pairs / unit : pairs;
   const long long grid = unit ? (units + 7) / 8 * 8 * unit * tiles : pairs * tiles;
-  LAYA_LAUNCH((attend_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a, tiles, unit,
+  LAYA_LAUNCH((attend_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(256),
+              kBias == DistanceBias::Table ? (2 * (a.span + kPad) + 1) * sizeof(float) : 0, stream, a, tiles, unit,
               static_cast<int>(units));
   return hipGetLastError();
 }
