@@ -372,6 +372,10 @@ int laya_op_rotary(const void* x, int64_t x_row, int64_t x_head, void* out, int6
                    int dtype, const int32_t* positions, const double* turns, float amplitude, int layout,
                    int direction, int64_t rows, int heads, int dim, int rotated, void* stream);
 
+/* Kernels of laya_op_attend: the planner's choice; a workgroup for 128 queries of a head, for many rows; a workgroup or, over
+ * long keys, several for 32 rows, for few. */
+enum { LAYA_ATTEND_PLANNED = 0, LAYA_ATTEND_MANY = 1, LAYA_ATTEND_FEW = 2 };
+
 /* Ranges of a document mask: bounds[row] = (first, end) of the run of equal neighbouring ids that holds the row, counted from
  * its sequence's start.  documents [rows], bounds [rows][2], starts and lengths [n_seq] are device memory; a
  * sequence's rows are starts[s] .. starts[s] + lengths[s] - 1, cut to the array and to max_length; rows of no sequence are left
@@ -409,12 +413,13 @@ typedef struct LayaAttend {
   const float* table;     /* [heads][2 span + 1], or NULL; not both */
   int32_t span;
   int32_t before, after;
+  int32_t kernel;         /* a LAYA_ATTEND_* value */
   const int32_t* prefix;  /* [n_seq], or NULL */
   const int32_t* bounds;  /* [q_rows][2], or NULL */
 } LayaAttend;
 
 /* Bytes of workspace that laya_op_attend needs for this call: 0 unless long keys of few queries are shared by several
- * workgroups.  Depends on the sizes, before, and whether there is a prefix, not on pointers; -1 for sizes that are refused.  Host-only. */
+ * workgroups.  Depends on the sizes, before, after, kernel and whether there is a prefix, on no other pointer; -1 for sizes that are refused.  Host-only. */
 int64_t laya_attend_workspace(const LayaAttend* call);
 
 /* The attention described above, sums and softmax in fp32, weights rounded to dtype for the matrix unit, one rounding of the

@@ -39,7 +39,8 @@ struct AttendPlan {
   int row_tiles, splits;
   long long workspace;
 };
-AttendPlan attend_plan(const AttendArgs& a);
+enum AttendKernel : int { kAttendPlanned = 0, kAttendMany = 1, kAttendFew = 2 };
+AttendPlan attend_plan(const AttendArgs& a, int kernel);
 
 template <int D>  // the compiled head widths
 hipError_t launch_attend_dim(const AttendArgs& a, DType t, DistanceBias bias, bool cap, bool split, hipStream_t stream);

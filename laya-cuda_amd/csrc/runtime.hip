@@ -1712,6 +1712,7 @@ static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
                "rows, n_seq, max_q and max_k must not be negative, and below 2^30");
   LAYA_REQUIRE(c->before >= -1 && c->after >= -1 && c->before < kMaxPacked && c->after < kMaxPacked,
                "before and after must be -1 (no limit) or 0 to 2^30");
+  LAYA_REQUIRE(c->kernel >= LAYA_ATTEND_PLANNED && c->kernel <= LAYA_ATTEND_FEW, "kernel must be a LAYA_ATTEND_* value");
   LAYA_REQUIRE(!(c->slopes && c->table), "slopes or a table, not both");
   LAYA_REQUIRE(!c->table || (c->span >= 0 && c->span <= kMaxSpan), "span must be 0 to 1024");
   AttendArgs a{};
@@ -1723,7 +1724,7 @@ static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
   LAYA_REQUIRE(pairs < kMaxGroups && (static_cast<int64_t>(c->max_q) + 127) / 128 * (pairs + 8 * a.group) < kMaxGroups &&
                    static_cast<int64_t>(c->max_q) * a.group < (1LL << 30),
                "n_seq * heads * max_q: too large for one launch");
-  *plan = attend_plan(a);
+  *plan = attend_plan(a, c->kernel);
   LAYA_REQUIRE(!plan->split || static_cast<int64_t>(c->n_seq) * c->kv_heads * plan->row_tiles * plan->splits < kMaxGroups / 2,
                "n_seq * heads * max_q: too large for one launch");
   return a;

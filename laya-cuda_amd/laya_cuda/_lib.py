@@ -18,6 +18,7 @@ LAYER_NORM, RMS_NORM = 0, 1  # laya_op_norm8 kinds
 ACT_NONE, ACT_GELU, ACT_RELU, ACT_GEGLU, ACT_SWIGLU = range(5)  # laya_op_linear8 activations
 TILE_EXACT, TILE_FAST = -1, -2  # and its planned tiles
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1  # laya_op_rotary layouts
+ATTEND_PLANNED, ATTEND_MANY, ATTEND_FEW = range(3)  # laya_op_attend kernels
 FREQ_PLAIN, FREQ_LINEAR, FREQ_BASE, FREQ_PARTS = range(4)  # laya_rotary_frequencies kinds
 
 
@@ -50,7 +51,7 @@ class LayaAttend(ct.Structure):
                 + [(name, ct.c_int32) for name in ("heads", "kv_heads", "dim", "q_rows", "k_rows", "n_seq", "max_q", "max_k")]
                 + [(name, ct.c_void_p) for name in ("q_starts", "q_lengths", "k_starts", "k_lengths")]
                 + [("scale", ct.c_float), ("cap", ct.c_float), ("slopes", ct.c_void_p), ("table", ct.c_void_p),
-                   ("span", ct.c_int32), ("before", ct.c_int32), ("after", ct.c_int32), ("prefix", ct.c_void_p),
+                   ("span", ct.c_int32), ("before", ct.c_int32), ("after", ct.c_int32), ("kernel", ct.c_int32), ("prefix", ct.c_void_p),
                    ("bounds", ct.c_void_p)])
 
 

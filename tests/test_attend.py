@@ -125,7 +125,7 @@ def description(**change):
     values = dict(struct_bytes=ct.sizeof(_lib.LayaAttend), dtype=_lib.F16, q=P, k=P, v=P, out=P, q_row=256, q_head=64, k_row=128, k_head=64,
                   v_row=128, v_head=64, out_row=256, out_head=64, heads=4, kv_heads=2, dim=64, q_rows=100, k_rows=100, n_seq=2, max_q=50,
                   max_k=50, q_starts=P, q_lengths=P, k_starts=P, k_lengths=P, scale=0.125, cap=0.0, slopes=None, table=None, span=0,
-                  before=-1, after=-1, prefix=None, bounds=None)
+                  before=-1, after=-1, kernel=0, prefix=None, bounds=None)
     return _lib.LayaAttend(**{**values, **change})
 
 
@@ -148,6 +148,8 @@ def test_attend_refusals():
     for name in ("before", "after"):
         call("no limit", **{name: -2})
         call("no limit", **{name: 1 << 30})
+    for bad in (-1, 3):
+        call("kernel", kernel=bad)
     call("not both", slopes=P, table=P)
     call("span", table=P, span=-1)
     call("span", table=P, span=1025)
@@ -194,6 +196,8 @@ def test_workspaces():
     assert one == 2 * 64 * 32 * (64 + 2) * 4  # two key heads, 64 splits, 32 rows
     assert need(n_seq=1, max_q=1, max_k=1 << 17, before=100, after=0) == 0  # the window leaves little to share
     assert need(n_seq=1, max_q=1, max_k=1 << 17, before=100, after=0, prefix=P) == one
+    assert need(n_seq=1, max_q=1, max_k=1 << 17, kernel=_lib.ATTEND_FEW) == one
+    assert need(n_seq=1, max_q=1, max_k=1 << 17, kernel=_lib.ATTEND_MANY) == 0
 
 
 def test_reference_against_torch():

@@ -107,15 +107,22 @@ class Call:
 
 
 ODD = [1, 0, 63, 64, 65, 127, 128, 129, 31, 200, 33]
-MANY = ODD + [17] * 60  # enough (sequence, head) pairs for the prompts' kernel
+KERNELS = pytest.mark.parametrize("kernel", [_lib.ATTEND_MANY, _lib.ATTEND_FEW], ids=["many", "few"])
 BIASES = [("none", None, 0), ("slopes", "slopes", 0), ("table", "table", 20)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("dim", [8, 40, 64, 80, 96, 104, 128, 136, 256])
-@pytest.mark.parametrize("lengths", [ODD[:6], MANY], ids=["few", "many"])
-def test_widths(gpu, kind, dim, lengths):
-    Call(gpu, kind, lengths, 4, 2, dim).describe().run().check()
+@KERNELS
+def test_widths(gpu, kind, dim, kernel):
+    Call(gpu, kind, ODD, 4, 2, dim).describe(kernel=kernel).run().check()
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("n", [1, 60, 300])
+def test_planned(gpu, dim, n):
+    """The planner's choice, from few rows to more sequences than lanes and than one round of workgroups."""
+    Call(gpu, "bf16", ODD[:6] + [17] * n, 4, 4, dim, after=0).describe().run().check()
 
 
 @pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 128), ("f16", 96), ("bf16", 256)])
@@ -124,9 +131,9 @@ def test_widths(gpu, kind, dim, lengths):
 @pytest.mark.parametrize("masks", [dict(), dict(after=0), dict(before=37, after=5), dict(after=0, prefix=True),
                                    dict(prefix=True, documents=True), dict(documents=True, before=20)],
                          ids=["all", "causal", "window", "prefix", "documents", "near"])
-@pytest.mark.parametrize("lengths", [ODD, MANY], ids=["few", "many"])
-def test_masks_caps_and_biases(gpu, kind, dim, cap, bias, span, masks, lengths):
-    Call(gpu, kind, lengths, 4, 4, dim, cap=cap, bias=bias, span=span, **masks).describe().run().check()
+@KERNELS
+def test_masks_caps_and_biases(gpu, kind, dim, cap, bias, span, masks, kernel):
+    Call(gpu, kind, ODD, 4, 4, dim, cap=cap, bias=bias, span=span, **masks).describe(kernel=kernel).run().check()
 
 
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (7, 1), (8, 2), (40, 1), (12, 12)])
@@ -135,7 +142,9 @@ def test_masks_caps_and_biases(gpu, kind, dim, cap, bias, span, masks, lengths):
 def test_single_tokens(gpu, heads, kv_heads, queries, bias, span):
     keys = [queries, queries + 1, 31, 32, 33, 129, 1000, 64]
     c = Call(gpu, "f16", [queries] * 8, heads, kv_heads, 64, key_lengths=keys, after=0, bias=bias, span=span, cap=11.0)
-    c.describe().run().check()
+    for kernel in (_lib.ATTEND_PLANNED, _lib.ATTEND_FEW, _lib.ATTEND_MANY):
+        c.out.fill_(9.0)
+        c.describe(kernel=kernel).run().check()
 
 
 @pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 80), ("bf16", 128), ("f16", 256)])
@@ -143,7 +152,8 @@ def test_single_tokens(gpu, heads, kv_heads, queries, bias, span):
                          ids=["all", "causal", "window", "prefix"])
 @pytest.mark.parametrize("queries", [1, 7, 40])
 def test_long_keys_shared_by_workgroups(gpu, kind, dim, masks, queries):
-    c = Call(gpu, kind, [queries, queries, 1], 4, 2, dim, key_lengths=[9001, 4500, 70], bias="slopes", **masks).describe()
+    c = Call(gpu, kind, [queries, queries, 1], 4, 2, dim, key_lengths=[9001, 4500, 70], bias="slopes", **masks)
+    c.describe(kernel=_lib.ATTEND_FEW)
     if not masks or "before" not in masks or "prefix" in masks or masks["before"] > 1024:
         assert c.workspace is not None
     c.run().check()
@@ -156,47 +166,46 @@ def test_long_keys_shared_by_workgroups(gpu, kind, dim, masks, queries):
 
 @pytest.mark.parametrize("queries,keys,masks", [(300, 1000, dict(after=0)), (100, 40, dict(after=0)), (257, 513, dict(before=64, after=0)),
                                                 (130, 0, dict()), (64, 2000, dict(after=3))])
-@pytest.mark.parametrize("many", [False, True])
-def test_queries_and_keys_of_different_lengths(gpu, queries, keys, masks, many):
+@KERNELS
+def test_queries_and_keys_of_different_lengths(gpu, queries, keys, masks, kernel):
     """Later pieces of prompts; more queries than keys (the first see nothing); no keys at all."""
-    n = 40 if many else 1
-    Call(gpu, "bf16", [queries] + [11] * n, 8, 4, 64, key_lengths=[keys] + [23] * n, bias="table", span=64, **masks).describe().run().check()
+    c = Call(gpu, "bf16", [queries] + [11] * 9, 8, 4, 64, key_lengths=[keys] + [23] * 9, bias="table", span=64, **masks)
+    c.describe(kernel=kernel).run().check()
 
 
 @pytest.mark.parametrize("span", [0, 1, 32, 500, 1024])
-@pytest.mark.parametrize("many", [False, True])
-def test_table_spans(gpu, span, many):
-    lengths = [700, 3, 130] + [5] * (60 if many else 0)
-    Call(gpu, "f16", lengths, 6, 6, 64, bias="table", span=span).describe().run().check()
-    Call(gpu, "bf16", lengths, 6, 3, 256, bias="table", span=span, cap=20.0, after=0).describe().run().check()
+@KERNELS
+def test_table_spans(gpu, span, kernel):
+    Call(gpu, "f16", [700, 3, 130], 6, 6, 64, bias="table", span=span).describe(kernel=kernel).run().check()
+    Call(gpu, "bf16", [700, 3, 130], 6, 3, 256, bias="table", span=span, cap=20.0, after=0).describe(kernel=kernel).run().check()
 
 
-@pytest.mark.parametrize("lengths", [[200, 70], [200, 70] + [20] * 60], ids=["few", "many"])
-def test_rows_without_keys_are_zeros(gpu, lengths):
-    c = Call(gpu, "f16", lengths, 4, 2, 64, documents=True)
+@KERNELS
+def test_rows_without_keys_are_zeros(gpu, kernel):
+    c = Call(gpu, "f16", [200, 70], 4, 2, 64, documents=True)
     c.bounds[c.q0[0] + 10:c.q0[0] + 150] = [50, 50]
     c.bounds[c.q0[0] + 3] = [2 ** 31 - 1, -2 ** 31]
     c.bounds[c.q0[0] + 4] = [-5, 10 ** 9]  # cut to the keys
-    c.describe().run().check()
+    c.describe(kernel=kernel).run().check()
     assert not c.out[c.q0[0] + 10:c.q0[0] + 150, :, :64].any()
 
 
-@pytest.mark.parametrize("lengths", [[150, 90], [150, 90] + [20] * 60], ids=["few", "many"])
-def test_biases_of_the_lowest_value_hide(gpu, lengths):
-    c = Call(gpu, "bf16", lengths, 4, 4, 64, bias="table", span=100)
+@KERNELS
+def test_biases_of_the_lowest_value_hide(gpu, kernel):
+    c = Call(gpu, "bf16", [150, 90], 4, 4, 64, bias="table", span=100)
     c.table[:, :90] = np.finfo(np.float32).min
     c.table[1, 95:] = np.finfo(np.float32).min
     c.table[2, :] = -np.inf
     c.table[3, :] = np.finfo(np.float32).min  # a head that sees nothing
-    c.describe().run().check()
+    c.describe(kernel=kernel).run().check()
     assert not c.out[c.q0[0]:c.q0[0] + 150, 2:, :64].any()
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("cap", [0.0, 9.0])
-@pytest.mark.parametrize("queries,keys", [([200, 90], [200, 90]), ([200, 90] + [20] * 60, [200, 90] + [20] * 60), ([1, 3], [5000, 300])],
-                         ids=["few", "many", "step"])
-def test_hidden_keys_may_hold_anything(gpu, bad, cap, queries, keys):
+@pytest.mark.parametrize("queries,keys", [([200, 90], [200, 90]), ([1, 3], [5000, 300])], ids=["prompt", "step"])
+@KERNELS
+def test_hidden_keys_may_hold_anything(gpu, bad, cap, queries, keys, kernel):
     """Not finite keys and values at places that some rows see and others do not: rows that do not see them are as if they were
     not there; rows that see a NaN are NaN."""
     c = Call(gpu, "f16", queries, 4, 2, 64, key_lengths=keys, after=0, before=60, cap=cap, bias="slopes")
@@ -204,7 +213,7 @@ def test_hidden_keys_may_hold_anything(gpu, bad, cap, queries, keys):
     c.kv[c.k0[0] + keys[0] - 80, 1, 7] = bad       # keys behind some rows' windows
     c.kv[c.k0[0] + keys[0] - 90, 3, :64] = bad
     c.kv[c.k0[1]:c.k0[1] + 20, :, :64] = bad
-    c.describe().run()
+    c.describe(kernel=kernel).run()
     torch().cuda.synchronize()
     got = c.out.double().cpu().numpy()
     want, bound = c.expected()
@@ -218,9 +227,9 @@ def test_hidden_keys_may_hold_anything(gpu, bad, cap, queries, keys):
 
 def test_starts_and_lengths_are_cut_to_the_arrays(gpu):
     """Sequences that begin or end outside the arrays, or are longer than the call says: cut, and those that begin outside are none."""
-    for many in (0, 60):
-        c = Call(gpu, "f16", [100, 50, 60, 70] + [20] * many, 4, 2, 64, after=-1)
-        c.describe()
+    for kernel in (_lib.ATTEND_MANY, _lib.ATTEND_FEW):
+        c = Call(gpu, "f16", [100, 50, 60, 70], 4, 2, 64, after=-1)
+        c.describe(kernel=kernel)
         c.nq[3], c.nk[3] = 10 ** 9, 10 ** 9      # cut to max_q and max_k, and at the arrays' ends
         d = c.kept
         d["nq"].copy_(c.up(c.nq))
