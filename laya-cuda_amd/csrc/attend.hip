@@ -15,12 +15,12 @@ namespace {
 
 constexpr int kPad = 96;  // distances past a bias table's span that the scores of a block near its ends reach: its 64 keys and 32 rows
 
-// Prompts: a workgroup of four waves owns 128 queries of one head, and blocks of 64 keys pass through LDS, shared by the waves
+// Prompts: a workgroup of NW waves owns 32 NW queries of one head, and blocks of 64 keys pass through LDS, shared by the waves
 // and double-buffered.  A wave works on them 32 keys at a time and skips those that none of its rows sees.
-template <typename T, int D, bool kCap, DistanceBias kBias>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_kernel(
+template <typename T, int D, bool kCap, DistanceBias kBias, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
-  constexpr int KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
+  constexpr int NT = 64 * NW, TR = 32 * NW, KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
   constexpr int SB = 32;  // keys of one step
   typedef Rows<T, D, SB, kCap, kBias> R;
   typedef typename R::T8 T8;
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4
   const int s = pair / a.heads;
   const int head = pair - s * a.heads, kv = head / a.group;
   const Sequence sq = sequence(a, s);
-  const int row0 = tile * 128;
+  const int row0 = tile * TR;
   if (row0 >= sq.nq) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = row0 + wave * 32 + (lane & 31);
@@ -56,26 +56,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4
 
   __shared__ __align__(16) T sk[2][KB * P];
   __shared__ __align__(16) T sv[2][KB * P];
-  __shared__ Range wg_range[4];
+  __shared__ Range wg_range[NW];
   extern __shared__ float stable[];  // the head's bias table in units of t, 2 (span + kPad) + 1
 
   const Range range = wave_range(a, sq, me, valid, row0 + wave * 32, min(row0 + wave * 32 + 31, sq.nq - 1));
   if (lane == 0) wg_range[wave] = active ? range : Range{INT_MAX, 0, 0, INT_MAX};
   if constexpr (kBias == DistanceBias::Table) {
     const float* from = a.table + static_cast<size_t>(head) * (2 * a.span + 1);
-    for (int e = tid; e < 2 * (a.span + kPad) + 1; e += 256) stable[e] = from[max(0, min(2 * a.span, e - kPad))] * a.per_unit;
+    for (int e = tid; e < 2 * (a.span + kPad) + 1; e += NT) stable[e] = from[max(0, min(2 * a.span, e - kPad))] * a.per_unit;
   }
   __syncthreads();
   Range wg = wg_range[0];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
+  for (int w = 1; w < NW; ++w) {
     wg.lo = min(wg.lo, wg_range[w].lo);
     wg.hi = max(wg.hi, wg_range[w].hi);
     wg.all_lo = max(wg.all_lo, wg_range[w].all_lo);
     wg.all_hi = min(wg.all_hi, wg_range[w].all_hi);
   }
   // With a bias the keys next to the queries come first: their scores are the largest as a rule, and references move once.
-  const int last_position = min(row0 + 127, sq.nq - 1) + sq.nk - sq.nq;
+  const int last_position = min(row0 + TR - 1, sq.nq - 1) + sq.nk - sq.nq;
   const Blocks<KB> blocks(sq.prefix, __builtin_amdgcn_readfirstlane(wg.lo), __builtin_amdgcn_readfirstlane(wg.hi),
                           kBias == DistanceBias::None ? 0 : last_position);
   const int plain_lo = __builtin_amdgcn_readfirstlane(wg.all_lo), plain_hi = __builtin_amdgcn_readfirstlane(wg.all_hi) - KB;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4
   const T* Q = static_cast<const T*>(a.q) + (sq.q0 + (valid ? i : 0)) * a.q_row + head * a.q_head;
 
   // This thread's 16-byte chunks of a block: row r0 + step m, chunk index swizzled by the row.
-  constexpr int CH = KB * kChunks / 256, step = 256 / kChunks;
+  constexpr int CH = KB * kChunks / NT, step = NT / kChunks;
   const int r0 = tid / kChunks, c0 = tid % kChunks;
   unsigned at_k[CH], at_v[CH];
 #pragma unroll
@@ -101,9 +101,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4
   auto load = [&](int key, unsigned buffer) __attribute__((always_inline)) {
     const i32x4 rk = from_k.resource(key, sq.nk), rv = from_v.resource(key, sq.nk);
 #pragma unroll
-    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(rk, at_k[m], 0u, lds_k + buffer + 4096u * m);
+    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(rk, at_k[m], 0u, lds_k + buffer + NT * 16u * m);
 #pragma unroll
-    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(rv, at_v[m], 0u, lds_v + buffer + 4096u * m);
+    for (int m = 0; m < CH; ++m) lds_load16_buffer<true>(rv, at_v[m], 0u, lds_v + buffer + NT * 16u * m);
   };
 
   R rows;
@@ -401,6 +401,22 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
   }
 }
 
+template <typename T, int D, bool kCap, DistanceBias kBias, int NW>
+hipError_t launch_prompt(const AttendArgs& a, hipStream_t stream) {
+  const int tiles = (a.max_q + 32 * NW - 1) / (32 * NW);
+  const long long pairs = static_cast<long long>(a.n_seq) * a.heads, shared = static_cast<long long>(a.n_seq) * a.kv_heads;
+  // Heads that share keys on one XCD, or each head, where that leaves no XCD more than a seventh above the mean; else every
+  // tile for itself.
+  const auto even = [](long long n) { return (n + 7) / 8 * 56 <= n * 8; };
+  const int unit = even(shared) ? a.group : even(pairs) ? 1 : 0;
+  const long long units = unit ? pairs / unit : pairs;
+  const long long grid = unit ? (units + 7) / 8 * 8 * unit * tiles : pairs * tiles;
+  LAYA_LAUNCH((attend_kernel<T, D, kCap, kBias, NW>), dim3(static_cast<unsigned>(grid)), dim3(64 * NW),
+              kBias == DistanceBias::Table ? (2 * (a.span + kPad) + 1) * sizeof(float) : 0, stream, a, tiles, unit,
+              static_cast<int>(units));
+  return hipGetLastError();
+}
+
 template <typename T, int D, bool kCap, DistanceBias kBias>
 hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   if (split) {
@@ -412,18 +428,14 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
                 kept ? static_cast<int>(units) : 0);
     return hipGetLastError();
   }
-  const int tiles = (a.max_q + 127) / 128;
-  const long long pairs = static_cast<long long>(a.n_seq) * a.heads, shared = static_cast<long long>(a.n_seq) * a.kv_heads;
-  // Heads that share keys on one XCD, or each head, where that leaves no XCD more than a seventh above the mean; else every
-  // tile for itself.
-  const auto even = [](long long n) { return (n + 7) / 8 * 56 <= n * 8; };
-  const int unit = even(shared) ? a.group : even(pairs) ? 1 : 0;
-  const long long units = unit ? pairs / unit : pairs;
-  const long long grid = unit ? (units + 7) / 8 * 8 * unit * tiles : pairs * tiles;
-  LAYA_LAUNCH((attend_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(256),
-              kBias == DistanceBias::Table ? (2 * (a.span + kPad) + 1) * sizeof(float) : 0, stream, a, tiles, unit,
-              static_cast<int>(units));
-  return hipGetLastError();
+  // Eight waves take half the loads of four, but share one barrier on a CU: they gain where K and V outgrow the caches (16,384
+  // causal tokens of 8 heads of 128 562 and 522 us, 2 x 8,192 of 16 heads of 96 437 and 396) and for heads of 80 and 96 at any length
+  // (1,571 tokens 187 and 169), and lose where rows are few or ragged (32 of up to 2,000 of 128 291 and 307, 2,048 of 32 heads 57 and 64).
+  if constexpr (D == 96 || D == 128) {
+    const long long tiles8 = (a.max_q + 255) / 256 * static_cast<long long>(a.n_seq) * a.heads;
+    if (tiles8 >= 512 && (D == 96 || a.max_q >= 4096)) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
+  }
+  return launch_prompt<T, D, kCap, kBias, 4>(a, stream);
 }
 
 template <typename T, int D>

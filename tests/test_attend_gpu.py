@@ -136,6 +136,28 @@ def test_masks_caps_and_biases(gpu, kind, dim, cap, bias, span, masks, kernel):
     Call(gpu, kind, ODD, 4, 4, dim, cap=cap, bias=bias, span=span, **masks).describe(kernel=kernel).run().check()
 
 
+@pytest.mark.parametrize("kind,dim,lengths,heads", [("f16", 80, [300, 17, 257] + [5] * 60, 8), ("bf16", 96, [256] + [1] * 70, 8), ("bf16", 128, [4097, 300], 20)])
+@pytest.mark.parametrize("cap,bias,span", [(0.0, None, 0), (9.0, "table", 30), (0.0, "slopes", 0)])
+def test_tiles_of_256_queries(gpu, kind, dim, lengths, heads, cap, bias, span):
+    """Sizes that take eight waves a workgroup: 512 and more tiles of 256 queries, of heads of 80 and 96, or of 4,096 queries."""
+    c = Call(gpu, kind, lengths, heads, heads if dim < 128 else 1, dim, after=0, before=900, cap=cap, bias=bias, span=span, prefix=dim != 96)
+    c.describe(kernel=_lib.ATTEND_MANY)
+    assert (max(lengths) + 255) // 256 * len(lengths) * heads >= 512 or dim == 128
+    c.run()
+    if dim < 128:
+        c.check()
+        return
+    torch().cuda.synchronize()  # two heads of the long ones against 64 bits
+    got = c.out.double().cpu().numpy()
+    q, kv = c.q.double().cpu().numpy(), c.kv.double().cpu().numpy()
+    for h in (0, heads - 1):
+        rows, keys = slice(c.q0[0], c.q0[0] + lengths[0]), slice(c.k0[0], c.k0[0] + lengths[0])
+        want, bound = A.attend(q[rows, h:h + 1, :dim], kv[keys, :1, :dim], kv[keys, 1:, :dim], c.scale, c.cap,
+                               None if c.slopes is None else c.slopes[h:h + 1], None if c.table is None else c.table[h:h + 1], 900, 0,
+                               c.prefix[0], None, kind)
+        assert (np.abs(got[rows, h:h + 1, :dim] - want) <= bound).all()
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (7, 1), (8, 2), (40, 1), (12, 12)])
 @pytest.mark.parametrize("queries", [1, 2, 5])
 @pytest.mark.parametrize("bias,span", [b[1:] for b in BIASES], ids=[b[0] for b in BIASES])
