@@ -15,11 +15,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kUnits = 4;  // units a thread has in flight
 
-// cos and sin of 2 pi turn.  The nearest quarter turn goes first, in 64 bits: what is left, at most an eighth, rounds to fp32
-// within 2^-28 of a turn.
-__device__ __forceinline__ float2 cos_sin(double turn) {
-  const double quarter = rint(turn * 4.0);
-  const float rest = static_cast<float>(2.0 * turn - 0.5 * quarter);  // in half turns, at most 1/4
+// cos and sin of 2 pi position turns.  The nearest quarter turn goes first, in 64 bits and with one rounding: what is left, at
+// most an eighth, rounds to fp32 within 2^-28 of a turn.
+__device__ __forceinline__ float2 cos_sin(double position, double turns) {
+  const double quarter = rint(position * turns * 4.0);
+  const float rest = static_cast<float>(2.0 * fma(position, turns, -0.25 * quarter));  // in half turns, at most 1/4
   const float s = sinpif(rest), c = cospif(rest);
   const int q = static_cast<int>(quarter - 4.0 * floor(quarter * 0.25));
   const float x = q & 1 ? -s : c, y = q & 1 ? c : s;
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     if (!made) {
       for (int i = threadIdx.x; i < rows * pairs; i += kThreads) {
         const int r = i / pairs;
-        const float2 cs = cos_sin(a.positions[row0 + r] * a.turns[i - r * pairs]);
+        const float2 cs = cos_sin(a.positions[row0 + r], a.turns[i - r * pairs]);
         table[i] = make_float2(cs.x * a.amplitude, cs.y * a.amplitude * a.direction);
       }
       __syncthreads();

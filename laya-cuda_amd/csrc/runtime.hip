@@ -1628,6 +1628,16 @@ int laya_op_linear8(const void* x, const void* x_scales, const void* w, const vo
 constexpr int kMaxRotaryDim = 8192, kMaxRotaryRow = 1 << 20;
 constexpr int64_t kMaxRotaryRows = 1LL << 23, kMaxStride = 1LL << 40;
 static bool stride_ok(int64_t s) { return s >= 0 && s < kMaxStride; }
+// Rows of heads whose offsets fit 64 bits with room to spare, and, of an output, whose values lie apart: the rows' heads between
+// the rows, or the heads' rows between the heads.
+static bool span_ok(int64_t rows, int64_t row, int64_t heads, int64_t head) {
+  return (rows < 2 || row <= kMaxSpan8 / rows) && (heads < 2 || head <= kMaxSpan8 / heads);
+}
+static bool apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+  if (heads < 2) return rows < 2 || row >= dim;
+  if (rows < 2) return head >= dim;
+  return (head >= dim && row >= head * (heads - 1) + dim) || (row >= dim && head >= row * (rows - 1) + dim);
+}
 
 int laya_rotary_frequencies(int kind, double theta, int rotated, double factor, double original, double low, double high,
                             double* host_turns) {
@@ -1666,7 +1676,8 @@ int laya_op_rotary(const void* x, int64_t x_row, int64_t x_head, void* out, int6
     LAYA_REQUIRE(rotated >= 2 && rotated <= dim && rotated % 2 == 0, "rotated must be even, from 2 to dim");
     LAYA_REQUIRE(rows >= 0 && rows <= kMaxRotaryRows, "rows: 0 to 2^23");
     LAYA_REQUIRE(stride_ok(x_row) && stride_ok(x_head) && stride_ok(out_row) && stride_ok(out_head), "strides must be 0 to 2^40");
-    LAYA_REQUIRE((heads == 1 || out_head >= dim) && (rows < 2 || out_row >= dim), "out's rows and heads must not overlap");
+    LAYA_REQUIRE(span_ok(rows, x_row, heads, x_head) && span_ok(rows, out_row, heads, out_head), "strides: values that span at most 2^50 elements");
+    LAYA_REQUIRE(apart(rows, out_row, heads, out_head, dim), "out's rows and heads must not overlap");
     if (rows == 0) return;
     LAYA_REQUIRE(x && out && positions && turns, "x, out, positions and turns are required");
     LAYA_REQUIRE(aligned_to(x, type_size(dtype)) && aligned_to(out, type_size(dtype)) && aligned_to(positions, 4) && aligned_to(turns, 8),
@@ -1753,7 +1764,10 @@ int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_by
                  "strides must be multiples of 8 elements from 0 to 2^40");
     LAYA_REQUIRE(c.k_row >= c.dim && c.v_row >= c.dim && c.k_row < (1 << 23) && c.v_row < (1 << 23),
                  "rows of k and v must be dim to 2^23 elements apart");
-    LAYA_REQUIRE((c.heads == 1 || c.out_head >= c.dim) && (c.q_rows < 2 || c.out_row >= c.dim), "out's rows and heads must not overlap");
+    LAYA_REQUIRE(span_ok(c.q_rows, c.q_row, c.heads, c.q_head) && span_ok(c.q_rows, c.out_row, c.heads, c.out_head) &&
+                     span_ok(c.k_rows, c.k_row, c.kv_heads, c.k_head) && span_ok(c.k_rows, c.v_row, c.kv_heads, c.v_head),
+                 "strides: values that span at most 2^50 elements");
+    LAYA_REQUIRE(apart(c.q_rows, c.out_row, c.heads, c.out_head, c.dim), "out's rows and heads must not overlap");
     if (c.n_seq == 0 || c.max_q == 0 || c.q_rows == 0) return;
     LAYA_REQUIRE(c.q && c.out && c.q_starts && c.q_lengths && c.k_starts && c.k_lengths && (c.k_rows == 0 || (c.k && c.v)),
                  "q, k, v, out, starts and lengths are required");

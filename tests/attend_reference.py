@@ -69,10 +69,10 @@ def attend(q, k, v, scale, cap=0.0, slopes=None, table=None, before=-1, after=-1
 
 
 def rotate(x, positions, turns, amplitude=1.0, interleaved=False, direction=1):
-    """x [rows][heads][dim] in 64 bits, turned; angles reduced exactly where a position times a frequency fits 64 bits."""
+    """x [rows][heads][dim] in 64 bits, turned; a position times a frequency in 64 bits of mantissa before whole turns go."""
     r = 2 * len(turns)
-    turn = np.asarray(positions, np.float64)[:, None] * np.asarray(turns, np.float64)
-    angle = 2 * np.pi * (turn - np.rint(turn))[:, None]
+    turn = np.asarray(positions, np.longdouble)[:, None] * np.asarray(turns, np.longdouble)
+    angle = 2 * np.pi * (turn - np.rint(turn)).astype(np.float64)[:, None]
     c, s = np.cos(angle) * amplitude, np.sin(angle) * amplitude * direction
     a, b = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2), slice(r // 2, r))
     out = np.array(x, np.float64)

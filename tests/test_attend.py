@@ -92,8 +92,10 @@ def test_rotary_refusals():
         call("rows", rows=bad)
     for bad in (dict(x_row=-1), dict(x_head=1 << 40), dict(out_row=-64)):
         call("strides", **bad)
-    call("must not overlap", out_head=63)
-    call("must not overlap", out_row=63)
+    call("2^50", x_row=1 << 39, rows=1 << 20)
+    call("2^50", x_head=(1 << 40) - 64, heads=1 << 14)
+    for bad in (dict(out_head=63), dict(out_row=63), dict(out_row=255), dict(out_row=64), dict(out_row=64, out_head=191)):
+        call("must not overlap", **bad)
     for name in ("x", "out", "positions", "turns"):
         call("are required", **{name: None})
     call("aligned to their", x=ODD)
@@ -164,8 +166,10 @@ def test_attend_refusals():
         call("strides", **{name: 1 << 40})
     call("rows of k and v", k_row=56)
     call("rows of k and v", v_row=1 << 23)
-    call("must not overlap", out_head=56)
-    call("must not overlap", out_row=56)
+    call("2^50", q_row=(1 << 40) - 64, q_rows=1 << 20)
+    call("2^50", k_head=(1 << 40) - 64, heads=1 << 14, kv_heads=1 << 13, n_seq=1)
+    for bad in (dict(out_head=56), dict(out_row=56), dict(out_row=248), dict(out_row=64), dict(out_row=64, out_head=64 * 99)):
+        call("must not overlap", **bad)
     for name in ("q", "k", "v", "out", "q_starts", "q_lengths", "k_starts", "k_lengths"):
         call("are required", **{name: None})
     for name in ("q", "k", "v", "out"):

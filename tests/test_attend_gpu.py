@@ -291,6 +291,14 @@ def test_a_cache_past_32_bits(gpu):
         assert (np.abs(got[c.q0[0]:c.q0[0] + queries, :, :dim] - want) <= bound).all()
 
 
+def test_no_keys_at_all(gpu):
+    """An empty cache: no pointers, zeros."""
+    for kernel in (_lib.ATTEND_PLANNED, _lib.ATTEND_MANY, _lib.ATTEND_FEW):
+        c = Call(gpu, "f16", [40, 1], 4, 2, 64, key_lengths=[0, 0])
+        c.describe(k=None, v=None, k_rows=0, max_k=0, kernel=kernel).run().check()
+        assert not c.out[c.q0[0]:c.q0[0] + 40, :, :64].any()
+
+
 def test_head_major_planes(gpu):
     """The strides of [heads][rows][dim]."""
     t = torch()
