@@ -125,6 +125,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
   }
   const int first_position = __builtin_amdgcn_readfirstlane(me.position);
   unsigned buffer = 0;
+  bool fresh = true;  // no step done
   for (int j = 0; j < nb; ++j, buffer ^= kBuffer) {
     publish_stage<waitcnt_vm(0)>();
     const int now = key0;
@@ -155,6 +156,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
         shift = rows.change(a, t, key, table, first + SB - 1 <= 0 ? -1 : first - 31 >= 0 ? 1 : 0);
       }
       if (!whole) rows.hide(t, key);
+      if (fresh) rows.open(a, t, shift);
+      fresh = false;
       const float sum = rows.weights(a, t, p, shift);
       rows.total += rows.move(a, t, p, shift, sum);
       rows.weigh((LdsBytes)(sv[0]) + SB * h * P * 2, buffer, p);
@@ -302,6 +305,7 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
     }
     const float shift = rows.change(a, t, key, table, 0);
     if (!(key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi))) rows.hide(t, key);
+    if (j < j0 + NW) rows.open(a, t, shift);
     const float sum = rows.weights(a, t, p, shift);
     rows.total += rows.move(a, t, p, shift, sum);
     if (more) __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(CH));  // all but the next block's K

@@ -302,7 +302,7 @@ struct Rows {
     constexpr int kNone = kCap ? 0x7f800000 : static_cast<int>(0xff800000);  // infinite, towards a score of -infinity
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int mask = static_cast<int>(hidden << (31 - slot(0, r))) >> 31;
+      const int mask = __builtin_amdgcn_sbfe(static_cast<int>(hidden), slot(0, r), 1);
       s[0][r] = __int_as_float((mask & kNone) | (~mask & __float_as_int(s[0][r])));
     }
   }
@@ -330,6 +330,11 @@ struct Rows {
       sum[1] = pair_sum(__builtin_shufflevector(p[c], p[c], 6, 7), sum[1]);
     }
     return sum[0] + sum[1];
+  }
+
+  // The first block of a wave: its largest score is the reference, before any weight is made.
+  __device__ __forceinline__ void open(const AttendArgs& a, const f32x16 (&s)[KT], float shift) {
+    reference = fmaxf(kNothing, block_max(a, s, shift));
   }
 
   // Weights that are too large for the reference: it moves to the block's largest score.
