@@ -16,7 +16,17 @@ namespace {
 constexpr int kPad = 96;  // distances past a bias table's span that the scores of a block near its ends reach: its 64 keys and 32 rows
 
 // Prompts: a workgroup of NW waves owns 32 NW queries of one head, and blocks of 64 keys pass through LDS, shared by the waves
-// and double-buffered.  A wave works on them 32 keys at a time and skips those that none of its rows sees.
+// and double-buffered.  A wave works on them 32 keys at a time (scores, weights, products with V: one pass over the keys with the
+// running reference and total) and skips those that none of its rows sees.
+//
+// What bounds it: the card's power and the vector instructions beside the matrix ones.  64 x 1,024 tokens of 16 heads of 64 run
+// 350 us (785 TFLOP/s) at 1.91 of 2.4 GHz with the matrix cores busy 38% of the cycles and vector instructions 58%; with zeros for
+// inputs 280 us.  Copies without the exponentials, the loads or one of the products run 320, 315 and 290 us.  16,384
+// causal tokens of 8 heads of 128: 520 us, 1.06 PFLOP/s, the matrix cores 44%.
+// Why 32 keys a step in one straight line, with no more than 101 registers for heads of 64: four such workgroups share a CU.  64 keys a
+// step took 373 us where this took 361, scores of the next step under the softmax of this one 388 against 352, two row groups a
+// wave (half the LDS reads) 354 against 349 for heads of 64 and 1,535 against 1,069 for 128, three buffers 382 against 344, blocks of 32
+// keys 394 against 350, raised priorities for either phase or by slot nothing.
 template <typename T, int D, bool kCap, DistanceBias kBias, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
@@ -201,7 +211,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
 // Few rows: a workgroup owns 32 rows, the (token, head) pairs of the heads that share keys, and its waves split their keys into
 // blocks of 32, each wave with a place of its own in LDS for a block of K and one of V.  The next K is on its way from the
 // scores to the next ones, the next V from one product to the next.  Long contexts are shared by a.splits workgroups, whose sums
-// join_kernel adds.
+// join_kernel adds in a fixed order.
+//
+// What bounds it: over long caches their bytes (4 tokens over 131,072 keys of 8 heads of 128: 381 us and 4 to join, 5.6 TB/s where a copy
+// reaches 4.8; 48 ragged ones over up to 4,100 keys of 16 heads of 64: 97 us, 4.6 TB/s), over short ones a launch and five dependent
+// steps (kernel arguments, lengths, keys, sums in LDS, output): 500 keys 6.8 us, of which an empty kernel takes 2.2.
+// Why eight waves with one place each, not four with two: as many bytes on their way, and half the rounds (30,000 keys of 8 heads
+// 69 -> 29 us with as many workgroups as compute units, 500 keys 9.5 -> 8.3).
 template <int D>
 constexpr int split_waves() {
   return D <= 128 ? 8 : 4;  // what 128 KB of LDS hold, or for heads of 64 half of it
@@ -473,7 +489,8 @@ template <> hipError_t launch_attend_dim<256>(const AttendArgs&, DType, Distance
 
 namespace {
 
-// A row's sums over the splits: weights 2^(m_z - M), then one division.  A workgroup a row: its four waves share the splits, in a
+// A row's sums over the splits: weights 2^(m_z - M), then one division.  4 us for 128 rows of 8 splits and 23 in a loop of dependent
+// loads.  A workgroup a row: its four waves share the splits, in a
 // fixed order, a lane four dims; every load of a wave is on its way before the first sum.
 constexpr int kJoinWaves = 4, kJoinLoads = kMaxSplits / kJoinWaves;
 template <typename T>
@@ -531,7 +548,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(AttendArgs a, int
   *reinterpret_cast<typename Vec4<T>::type*>(out + 4 * lane) = h;
 }
 
-// The run of equal ids around each row of a sequence.  A wave takes 64 rows: where ids change comes from one ballot, and what
+// The run of equal ids around each row of a sequence.  Two dependent loads and a launch: 65,536 rows 6 us.  A wave takes 64 rows: where ids change comes from one ballot, and what
 // begins before or ends behind them is looked for 512 rows at a time.
 __global__ __launch_bounds__(256) void document_bounds_kernel(BoundsArgs a, int groups) {
   const int s = blockIdx.x / groups, lane = threadIdx.x & 63;
