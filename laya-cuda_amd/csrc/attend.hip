@@ -28,7 +28,7 @@ constexpr int kPad = 96;  // distances past a bias table's span that the scores 
 // wave (half the LDS reads) 354 against 349 for heads of 64 and 1,535 against 1,069 for 128, three buffers 382 against 344, blocks of 32
 // keys 394 against 350, raised priorities for either phase or by slot nothing.
 template <typename T, int D, bool kCap, DistanceBias kBias, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : D <= 128 ? 2 : 1))) void attend_kernel(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : 2))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
   constexpr int NT = 64 * NW, TR = 32 * NW, KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
   constexpr int SB = 32;  // keys of one step
@@ -448,14 +448,16 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
                 kept ? static_cast<int>(units) : 0);
     return hipGetLastError();
   }
-  // Eight waves take half the loads of four, but share one barrier on a CU: they gain where K and V outgrow the caches (16,384
+  // Eight waves take half the loads of four, but share one barrier on a CU.  Above 128 LDS holds one workgroup, and they are two a SIMD
+  // instead of one (4 x 4,096 causal tokens of 16 heads of 256 890 and 632 us, of 192 786 and 440).  Below they gain where K and V outgrow the caches (16,384
   // causal tokens of 8 heads of 128 562 and 522 us, 2 x 8,192 of 16 heads of 96 437 and 396) and for heads of 80 and 96 at any length
   // (1,571 tokens 187 and 169), and lose where rows are few or ragged (32 of up to 2,000 of 128 291 and 307, 2,048 of 32 heads 57 and 64).
+  if constexpr (D > 128) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
   if constexpr (D == 96 || D == 128) {
     const long long tiles8 = (a.max_q + 255) / 256 * static_cast<long long>(a.n_seq) * a.heads;
     if (tiles8 >= 512 && (D == 96 || a.max_q >= 4096)) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
   }
-  return launch_prompt<T, D, kCap, kBias, 4>(a, stream);
+  if constexpr (D <= 128) return launch_prompt<T, D, kCap, kBias, 4>(a, stream);
 }
 
 template <typename T, int D>
@@ -485,6 +487,8 @@ hipError_t launch_attend_dim<LAYA_ATTEND_DIM>(const AttendArgs& a, DType t, Dist
 template <> hipError_t launch_attend_dim<64>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
 template <> hipError_t launch_attend_dim<96>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
 template <> hipError_t launch_attend_dim<128>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
+template <> hipError_t launch_attend_dim<160>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
+template <> hipError_t launch_attend_dim<192>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
 template <> hipError_t launch_attend_dim<256>(const AttendArgs&, DType, DistanceBias, bool, bool, hipStream_t);
 
 namespace {
@@ -624,7 +628,7 @@ AttendPlan attend_plan(const AttendArgs& a, int kernel) {
   const double n = std::floor(std::min(256.0 / std::max(base, 1.0), most / 256.0));
   if (n >= 3) p.splits = static_cast<int>(std::min<double>(n, kMaxSplits));
   const double prompt = static_cast<double>((a.max_q + 127) / 128) * a.n_seq * a.heads / 256.0;  // workgroups a CU
-  const double wide = a.dim <= 64 ? 1 : a.dim <= 128 ? 2 : 4;
+  const double wide = a.dim <= 64 ? 1 : a.dim <= 128 ? 2 : a.dim / 64.0;
   const double prompt_us = 5.5 + (prompt > 1 ? mean : most) / 64 * (wide == 1 ? std::max(1.0, 0.55 + 0.5 * prompt) : wide / 2 * std::max(1.4, 0.3 + prompt));
   const double split_us = 5 + (p.splits > 1 ? 3 : 0) + std::max(1.0, base * p.splits / 256) * wide * (2 + 0.1 * mean / p.splits / 32);
   p.split = kernel == kAttendPlanned ? split_us < prompt_us : kernel == kAttendFew;
@@ -640,6 +644,8 @@ hipError_t launch_attend(const AttendArgs& args, DType t, DistanceBias bias, boo
   const hipError_t e = a.dim <= 64    ? launch_attend_dim<64>(a, t, bias, cap, plan.split, stream)
                        : a.dim <= 96  ? launch_attend_dim<96>(a, t, bias, cap, plan.split, stream)
                        : a.dim <= 128 ? launch_attend_dim<128>(a, t, bias, cap, plan.split, stream)
+                       : a.dim <= 160 ? launch_attend_dim<160>(a, t, bias, cap, plan.split, stream)
+                       : a.dim <= 192 ? launch_attend_dim<192>(a, t, bias, cap, plan.split, stream)
                                       : launch_attend_dim<256>(a, t, bias, cap, plan.split, stream);
   if (e != hipSuccess || plan.splits <= 1) return e;
   const int used = a.row_tiles > 1 ? 32 : a.max_q * a.group;

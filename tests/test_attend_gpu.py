@@ -112,7 +112,7 @@ BIASES = [("none", None, 0), ("slopes", "slopes", 0), ("table", "table", 20)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("dim", [8, 40, 64, 80, 96, 104, 128, 136, 256])
+@pytest.mark.parametrize("dim", [8, 40, 64, 80, 96, 104, 128, 136, 160, 168, 192, 200, 256])
 @KERNELS
 def test_widths(gpu, kind, dim, kernel):
     Call(gpu, kind, ODD, 4, 2, dim).describe(kernel=kernel).run().check()
@@ -125,7 +125,7 @@ def test_planned(gpu, dim, n):
     Call(gpu, "bf16", ODD[:6] + [17] * n, 4, 4, dim, after=0).describe().run().check()
 
 
-@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 128), ("f16", 96), ("bf16", 256)])
+@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 128), ("f16", 96), ("bf16", 256), ("f16", 192)])
 @pytest.mark.parametrize("cap", [0.0, 7.0])
 @pytest.mark.parametrize("bias,span", [b[1:] for b in BIASES], ids=[b[0] for b in BIASES])
 @pytest.mark.parametrize("masks", [dict(), dict(after=0), dict(before=37, after=5), dict(after=0, prefix=True),
@@ -169,7 +169,7 @@ def test_single_tokens(gpu, heads, kv_heads, queries, bias, span):
         c.describe(kernel=kernel).run().check()
 
 
-@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 80), ("bf16", 128), ("f16", 256)])
+@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 80), ("bf16", 128), ("f16", 256), ("f16", 152)])
 @pytest.mark.parametrize("masks", [dict(), dict(after=0), dict(after=0, before=3000), dict(after=0, before=700, prefix=True)],
                          ids=["all", "causal", "window", "prefix"])
 @pytest.mark.parametrize("queries", [1, 7, 40])
