@@ -28,7 +28,7 @@ constexpr int kPad = 96;  // distances past a bias table's span that the scores 
 // wave (half the LDS reads) 354 against 349 for heads of 64 and 1,535 against 1,069 for 128, three buffers 382 against 344, blocks of 32
 // keys 394 against 350, raised priorities for either phase or by slot nothing.
 template <typename T, int D, bool kCap, DistanceBias kBias, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 4 : 2))) void attend_kernel(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 || (D == 96 && NW == 8) ? 4 : 2))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
   constexpr int NT = 64 * NW, TR = 32 * NW, KB = 64, P = Block<D>::kPitch, kChunks = P / 8;
   constexpr int SB = 32;  // keys of one step
@@ -64,8 +64,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
   const bool active = row0 + wave * 32 < sq.nq;  // waves past the last query only stage keys
   const Seen me = valid ? seen(a, sq, i) : Seen{i + sq.nk - sq.nq, 0, 0};
 
-  __shared__ __align__(16) T sk[2][KB * P];
-  __shared__ __align__(16) T sv[2][KB * P];
+  __shared__ __align__(16) T skv[4][KB * P];  // two buffers of K, two of V
   __shared__ Range wg_range[NW];
   extern __shared__ float stable[];  // the head's bias table in units of t, 2 (span + kPad) + 1
 
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
   }
   const Source<KB> from_k(K, a.k_row, sq.nk, a.dim), from_v(V, a.v_row, sq.nk, a.dim);
   constexpr unsigned kBuffer = KB * P * sizeof(T);
-  const unsigned lds_k = lds_address(sk[0]) + wave * 1024u, lds_v = lds_address(sv[0]) + wave * 1024u;
+  const unsigned lds_k = lds_address(skv[0]) + wave * 1024u, lds_v = lds_address(skv[2]) + wave * 1024u;
   auto load = [&](int key, unsigned buffer) __attribute__((always_inline)) {
     const i32x4 rk = from_k.resource(key, sq.nk), rv = from_v.resource(key, sq.nk);
 #pragma unroll
@@ -155,7 +154,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
       }
       f32x16 t[R::KT];
       T8 p[2 * R::KT];
-      rows.scores((LdsBytes)(sk[0]) + SB * h * P * 2, buffer, t);
+      rows.scores((LdsBytes)(skv[0]), buffer + SB * h * P * 2u, t);
       float shift;
       const int first = key - first_position;  // of the wave's first query to the step's first key
       if (kBias == DistanceBias::Table && (first + SB - 1 <= -a.span || first - 31 >= a.span)) {
@@ -170,7 +169,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
       fresh = false;
       const float sum = rows.weights(a, t, p, shift);
       rows.total += rows.move(a, t, p, shift, sum);
-      rows.weigh((LdsBytes)(sv[0]) + SB * h * P * 2, buffer, p);
+      rows.weigh((LdsBytes)(skv[2]), buffer + SB * h * P * 2u, p);
     }
   }
   if (!active) return;
@@ -449,7 +448,7 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
     return hipGetLastError();
   }
   // Eight waves take half the loads of four, but share one barrier on a CU.  Above 128 LDS holds one workgroup, and they are two a SIMD
-  // instead of one (4 x 4,096 causal tokens of 16 heads of 256 890 and 632 us, of 192 786 and 440).  Below they gain where K and V outgrow the caches (16,384
+  // instead of one (4 x 4,096 causal tokens of 16 heads of 256 865 and 529 us, of 192 786 and 421).  Below they gain where K and V outgrow the caches (16,384
   // causal tokens of 8 heads of 128 562 and 522 us, 2 x 8,192 of 16 heads of 96 437 and 396) and for heads of 80 and 96 at any length
   // (1,571 tokens 187 and 169), and lose where rows are few or ragged (32 of up to 2,000 of 128 291 and 307, 2,048 of 32 heads 57 and 64).
   if constexpr (D > 128) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
