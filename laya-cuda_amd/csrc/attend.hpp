@@ -64,7 +64,8 @@ struct RotaryArgs {
   long long rows;
   int heads, dim, rotated;
   bool interleaved, in_place;
-  int rows_each;             // rows a workgroup (the launcher's)
+  int rows_each;             // rows a workgroup, and the inverses of a row's and a head's units (the launcher's)
+  float row_inverse, head_inverse;
 };
 hipError_t launch_rotary(const RotaryArgs& a, DType t, hipStream_t stream);
 

@@ -15,7 +15,13 @@ namespace laya {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;  // units a thread has in flight
+// Units a thread has in flight.  Units of 4 bytes and less take more of them for the bytes on their way (heads of 98 in bf16 at
+// eight 94 us for 103, of 80 turning 20 values 75 for 90); units of 8 lose by it (heads of 72: 58 us for 54).
+constexpr int in_flight(int bytes) { return bytes > 4 ? 4 : 8; }
+
+// n / d from d's rounded inverse: n + 1/2 is exact and the quotient off by at most 2^-23 of itself, less than the 1 / (2 d)
+// that lies between it and an integer while n < 2^22.  A workgroup's units are at most a row's 2^20 values.
+__device__ __forceinline__ int over(int n, float inverse) { return static_cast<int>((static_cast<float>(n) + 0.5f) * inverse); }
 
 // cos and sin of 2 pi position turns.  The nearest quarter turn goes first, in 64 bits and with one rounding: what is left, at
 // most an eighth, rounds to fp32 within 2^-28 of a turn.
@@ -34,10 +40,12 @@ struct alignas(sizeof(T) * V) Pack {
 };
 
 // A unit is V pairs (half layout: V values of either half) or V values in a row (interleaved pairs, or values behind the rotated
-// ones, which have no pair).  V: 16 bytes where strides, sizes and addresses allow it, else one pair or value.
+// ones, which have no pair).  V: the most, up to 16 bytes, that strides, sizes and addresses are multiples of: 67 million values in
+// bf16, half layout, at 16 bytes 5.4 TB/s (heads of 64), 8 4.9 (72), 4 4.3 (100), 2 2.8 (98: halves of 49).
 template <typename T, int V, bool kHalf>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 table[];  // [rows][pairs], cosine and sine times the amplitude
+  constexpr int kUnits = in_flight(V * sizeof(T));
   constexpr int kSide = kHalf ? 1 : (V > 1 ? V : 2);  // values a turning unit takes at one place
   const int pairs = a.rotated / 2;
   const int turning = kHalf ? pairs / V : a.rotated / kSide;      // units of a head that turn
@@ -59,8 +67,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
       const int u = first + k * kThreads + static_cast<int>(threadIdx.x);
       pair[k] = -2;
       if (u < units) {
-        const int r = u / per_row, w = u - r * per_row;
-        const int h = w / per_head, c = w - h * per_head;
+        const int r = over(u, a.row_inverse), w = u - r * per_row;
+        const int h = over(w, a.head_inverse), c = w - h * per_head;
         const bool turns = c < turning;
         const int at = turns ? c * (kHalf ? V : kSide) : a.rotated + (c - turning) * V;
         const T* src = x + (row0 + r) * a.x_row + h * a.x_head + at;
@@ -107,22 +115,24 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   }
 }
 
-template <typename T>
-bool whole(const RotaryArgs& a) {
-  constexpr long long V = 16 / sizeof(T);
-  const auto fits = [](long long n) { return n % V == 0; };
-  return fits(a.x_row) && fits(a.x_head) && fits(a.out_row) && fits(a.out_head) && fits(a.dim) &&
-         fits(a.interleaved ? a.rotated : a.rotated / 2) && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 &&
-         (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+// Whether units of V values fit: whole numbers of them, at addresses of their own size.
+template <typename T, int V>
+bool fits(const RotaryArgs& a) {
+  const int size = a.interleaved ? a.rotated : a.rotated / 2;
+  return ((a.x_row | a.x_head | a.out_row | a.out_head | a.dim | size) & (V - 1)) == 0 &&
+         ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out)) & (V * sizeof(T) - 1)) == 0;
 }
 
 template <typename T, int V, bool kHalf>
 hipError_t launch_v(RotaryArgs a, hipStream_t stream) {
   const int pairs = a.rotated / 2;
-  const int per_row = ((kHalf ? pairs / V : a.rotated / (V > 1 ? V : 2)) + (a.in_place ? 0 : (a.dim - a.rotated) / V)) * a.heads;
+  const int per_head = (kHalf ? pairs / V : a.rotated / (V > 1 ? V : 2)) + (a.in_place ? 0 : (a.dim - a.rotated) / V);
+  const int per_row = per_head * a.heads;
+  a.row_inverse = 1.0f / static_cast<float>(per_row);
+  a.head_inverse = 1.0f / static_cast<float>(per_head);
   // Rows a workgroup: one batch of units, whose tables fit the 32 KB of LDS that leave a CU five workgroups.  With few rows
   // one each, its units over as many workgroups as hold them (each makes the row's table again).
-  const int batch = kThreads * kUnits;
+  const int batch = kThreads * in_flight(V * sizeof(T));
   long long each = batch / per_row;
   if (each > 32768 / (8 * pairs)) each = 32768 / (8 * pairs);
   if (each > a.rows / 1024) each = a.rows / 1024;
@@ -137,20 +147,21 @@ hipError_t launch_v(RotaryArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, int V>
 hipError_t launch_t(const RotaryArgs& a, hipStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  if (whole<T>(a)) return a.interleaved ? launch_v<T, V, false>(a, stream) : launch_v<T, V, true>(a, stream);
-  return a.interleaved ? launch_v<T, 1, false>(a, stream) : launch_v<T, 1, true>(a, stream);
+  if constexpr (V > 1) {
+    if (!fits<T, V>(a)) return launch_t<T, V / 2>(a, stream);
+  }
+  return a.interleaved ? launch_v<T, V, false>(a, stream) : launch_v<T, V, true>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_rotary(const RotaryArgs& a, DType t, hipStream_t stream) {
   switch (t) {
-    case DType::F32: return launch_t<float>(a, stream);
-    case DType::F16: return launch_t<f16>(a, stream);
-    default: return launch_t<bf16>(a, stream);
+    case DType::F32: return launch_t<float, 4>(a, stream);
+    case DType::F16: return launch_t<f16, 8>(a, stream);
+    default: return launch_t<bf16, 8>(a, stream);
   }
 }
 

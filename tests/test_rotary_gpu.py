@@ -68,6 +68,12 @@ CASES = [  # rows, heads, dim, rotated, far, row, head, offset
     (5, 1, 8192, 8192, 100, None, None, 0),
     (2, 300, 96, 96, 70000, None, None, 0),            # more units a row than a workgroup takes at once
     (2000, 40, 64, 64, 70000, None, None, 0),
+    (300, 17, 72, 72, 1000, None, None, 0),            # halves of 36: a narrower unit for each power of two that divides
+    (300, 12, 100, 100, 1000, None, None, 0),          # of 50
+    (300, 13, 98, 98, 1000, None, None, 0),            # of 49
+    (300, 16, 80, 20, 1000, None, None, 2),            # of 10, at an address off 8 bytes
+    (3, 4, 200, 104, 1000, 812, 204, 4),               # strides of whole 4 values only
+    (3, 128, 8192, 8192, 1000, None, None, 1),         # a row of 2^20 values, one by one
 ]
 
 
