@@ -424,11 +424,12 @@ int64_t laya_attend_workspace(const LayaAttend* call);
 
 /* The attention described above, sums and softmax in fp32, weights rounded to dtype for the matrix unit, one rounding of the
  * output.  Lengths of zero are fine.  dim a multiple of 8 up to 256, heads a multiple of kv_heads; q, k, v and out and
- * their strides on whole 16 bytes, row strides of k and v at least dim and below 2^23; scale from 1e-10 to 1e10, cap 0 or as much;
- * span 0 to 1024 with a table; rows, max_q, max_k, before and after below 2^30, heads at most 2^16, and n_seq * heads * max_q at
- * most about 2^31 (one launch; the kernel for few rows, where it is named, takes about 2^28).  workspace: device memory, 16-byte aligned, of the
- * bytes that laya_attend_workspace tells (NULL for 0), written before it is read; calls that may run at
- * the same time, captured ones too, take different ones.  Equal calls give equal bits. */
+ * their strides on whole 16 bytes, row strides of k and v at least dim and below 2^23; scale from 1e-10 to 1e10; cap 0 or
+ * 1e-10 to 1024 (a capped score is exact to 2^-20 of the cap); span 0 to 1024 with a table; rows, max_q, max_k, before and after
+ * below 2^30, heads at most 2^16, and n_seq * heads * max_q, max_q counted as whole 128 (256 for heads above 64), at most about
+ * 2^31 (one launch; the kernel for few rows, where it is named, takes about 2^28).  workspace: device memory, 16-byte aligned,
+ * of the bytes that laya_attend_workspace tells (NULL for 0), written before it is read; calls that may run at the same time,
+ * captured ones too, take different ones.  Equal calls give equal bits. */
 int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

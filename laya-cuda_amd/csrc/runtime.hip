@@ -1732,7 +1732,9 @@ static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
   a.before = c->before; a.after = c->after; a.span = c->table ? c->span : 0;
   a.prefix = c->prefix;
   const int64_t pairs = static_cast<int64_t>(c->n_seq) * c->heads;
-  LAYA_REQUIRE(pairs < kMaxGroups && (static_cast<int64_t>(c->max_q) + 127) / 128 * (pairs + 8 * a.group) < kMaxGroups &&
+  // Workgroups of 256 threads; heads above 64 may run as half as many tiles of twice the threads.
+  const int64_t tile = c->dim > 64 ? 256 : 128;
+  LAYA_REQUIRE(pairs < kMaxGroups && (c->max_q + tile - 1) / tile * (tile / 128) * (pairs + 8 * a.group) < kMaxGroups &&
                    static_cast<int64_t>(c->max_q) * a.group < (1LL << 30),
                "n_seq * heads * max_q: too large for one launch");
   *plan = attend_plan(a, c->kernel);
@@ -1756,8 +1758,8 @@ int laya_op_attend(const LayaAttend* call, void* workspace, int64_t workspace_by
     AttendPlan plan;
     AttendArgs a = attend_sizes(call, &plan);
     const LayaAttend& c = *call;
-    LAYA_REQUIRE(c.scale >= 1e-10f && c.scale <= 1e10f && (c.cap == 0.f || (c.cap >= 1e-10f && c.cap <= 1e10f)),
-                 "scale must be 1e-10 to 1e10, cap 0 or as much");
+    LAYA_REQUIRE(c.scale >= 1e-10f && c.scale <= 1e10f && (c.cap == 0.f || (c.cap >= 1e-10f && c.cap <= 1024.f)),
+                 "scale must be 1e-10 to 1e10, cap 0 or 1e-10 to 1024");
     LAYA_REQUIRE(stride_ok(c.q_row) && stride_ok(c.q_head) && stride_ok(c.k_row) && stride_ok(c.k_head) && stride_ok(c.v_row) &&
                      stride_ok(c.v_head) && stride_ok(c.out_row) && stride_ok(c.out_head) &&
                      ((c.q_row | c.q_head | c.k_row | c.k_head | c.v_row | c.v_head | c.out_row | c.out_head) & 7) == 0,

@@ -157,8 +157,9 @@ def test_attend_refusals():
     call("span", table=P, span=1025)
     call("too large", n_seq=1 << 23)
     call("too large", n_seq=1 << 12, max_q=1 << 20)
+    call("too large", n_seq=1 << 21, heads=4, kv_heads=4, dim=96, max_q=1, kernel=_lib.ATTEND_MANY)  # 2^23 workgroups of 512 threads
     for bad in (dict(scale=-0.1), dict(scale=0.0), dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.inf),
-                dict(cap=math.nan), dict(cap=1e-11)):
+                dict(cap=math.nan), dict(cap=1e-11), dict(cap=1025.0)):
         call("scale must be", **bad)
     for name in ("q_row", "k_head", "v_row", "out_head"):
         call("strides", **{name: 132})

@@ -202,6 +202,13 @@ def test_table_spans(gpu, span, kernel):
     Call(gpu, "bf16", [700, 3, 130], 6, 3, 256, bias="table", span=span, cap=20.0, after=0).describe(kernel=kernel).run().check()
 
 
+@pytest.mark.parametrize("cap", [1e-10, 0.01, 200.0, 1024.0])
+@KERNELS
+def test_smallest_and_largest_caps(gpu, cap, kernel):
+    for kind, bias in (("f16", None), ("bf16", "slopes")):
+        Call(gpu, kind, [300, 7], 4, 2, 64, bias=bias, cap=cap, after=0).describe(kernel=kernel).run().check()
+
+
 @KERNELS
 def test_rows_without_keys_are_zeros(gpu, kernel):
     c = Call(gpu, "f16", [200, 70], 4, 2, 64, documents=True)
