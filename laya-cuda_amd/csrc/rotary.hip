@@ -42,14 +42,16 @@ struct alignas(sizeof(T) * V) Pack {
 // A unit is V pairs (half layout: V values of either half) or V values in a row (interleaved pairs, or values behind the rotated
 // ones, which have no pair).  V: the most, up to 16 bytes, that strides, sizes and addresses are multiples of: 67 million values in
 // bf16, half layout, at 16 bytes 5.4 TB/s (heads of 64), 8 4.9 (72), 4 4.3 (100), 2 2.8 (98: halves of 49).
+// An interleaved unit may hold both, pairs that turn and values that do not: 114 turned of 128 81 us as units of 4 bytes, 50 as whole ones.
 template <typename T, int V, bool kHalf>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 table[];  // [rows][pairs], cosine and sine times the amplitude
   constexpr int kUnits = in_flight(V * sizeof(T));
   constexpr int kSide = kHalf ? 1 : (V > 1 ? V : 2);  // values a turning unit takes at one place
   const int pairs = a.rotated / 2;
-  const int turning = kHalf ? pairs / V : a.rotated / kSide;      // units of a head that turn
-  const int copied = a.in_place ? 0 : (a.dim - a.rotated) / V;    // and that are copied
+  const int turning = kHalf ? pairs / V : (a.rotated + kSide - 1) / kSide;  // units of a head that turn
+  const int turned = kHalf ? a.rotated : turning * kSide;                   // and the values they hold
+  const int copied = a.in_place ? 0 : (a.dim - turned) / V;                 // units that are copied
   const int per_head = turning + copied, per_row = per_head * a.heads;
   const long long row0 = static_cast<long long>(blockIdx.x) * a.rows_each;
   const int rows = static_cast<int>(min(static_cast<long long>(a.rows_each), a.rows - row0));
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         const int r = over(u, a.row_inverse), w = u - r * per_row;
         const int h = over(w, a.head_inverse), c = w - h * per_head;
         const bool turns = c < turning;
-        const int at = turns ? c * (kHalf ? V : kSide) : a.rotated + (c - turning) * V;
+        const int at = turns ? c * (kHalf ? V : kSide) : turned + (c - turning) * V;
         const T* src = x + (row0 + r) * a.x_row + h * a.x_head + at;
         to[k] = (row0 + r) * a.out_row + h * a.out_head + at;
         local[k] = r * pairs;
@@ -103,6 +105,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         } else {
 #pragma unroll
           for (int e = 0; e < V; e += 2) {
+            if (V > 2 && 2 * pair[k] + e >= a.rotated) break;  // copied
             const float u = to_float(p[k].v[e]), w = to_float(p[k].v[e + 1]);
             p[k].v[e] = to_half<T>(__builtin_fmaf(u, cs[e / 2].x, -(w * cs[e / 2].y)));
             p[k].v[e + 1] = to_half<T>(__builtin_fmaf(u, cs[e / 2].y, w * cs[e / 2].x));
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // Whether units of V values fit: whole numbers of them, at addresses of their own size.
 template <typename T, int V>
 bool fits(const RotaryArgs& a) {
-  const int size = a.interleaved ? a.rotated : a.rotated / 2;
+  const int size = a.interleaved ? 0 : a.rotated / 2;
   return ((a.x_row | a.x_head | a.out_row | a.out_head | a.dim | size) & (V - 1)) == 0 &&
          ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out)) & (V * sizeof(T) - 1)) == 0;
 }
@@ -126,7 +129,8 @@ bool fits(const RotaryArgs& a) {
 template <typename T, int V, bool kHalf>
 hipError_t launch_v(RotaryArgs a, hipStream_t stream) {
   const int pairs = a.rotated / 2;
-  const int per_head = (kHalf ? pairs / V : a.rotated / (V > 1 ? V : 2)) + (a.in_place ? 0 : (a.dim - a.rotated) / V);
+  const int side = V > 1 ? V : 2, turning = kHalf ? pairs / V : (a.rotated + side - 1) / side;
+  const int per_head = turning + (a.in_place ? 0 : (a.dim - (kHalf ? a.rotated : turning * side)) / V);
   const int per_row = per_head * a.heads;
   a.row_inverse = 1.0f / static_cast<float>(per_row);
   a.head_inverse = 1.0f / static_cast<float>(per_head);
