@@ -42,11 +42,14 @@ struct alignas(sizeof(T) * V) Pack {
 // A unit is V pairs (half layout: V values of either half) or V values in a row (interleaved pairs, or values behind the rotated
 // ones, which have no pair).  V: the most, up to 16 bytes, that strides, sizes and addresses are multiples of: 67 million values in
 // bf16, half layout, at 16 bytes 5.4 TB/s (heads of 64), 8 4.9 (72), 4 4.3 (100), 2 2.8 (98: halves of 49).
+// Units below 16 bytes take their indices from inverses, vector instructions being what they wait for; for whole ones that was slower
+// (65,536 rows of 32 heads of 64 in bf16 118 us where divisions take 111).
 // An interleaved unit may hold both, pairs that turn and values that do not: 114 turned of 128 81 us as units of 4 bytes, 50 as whole ones.
 template <typename T, int V, bool kHalf>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 table[];  // [rows][pairs], cosine and sine times the amplitude
   constexpr int kUnits = in_flight(V * sizeof(T));
+  constexpr bool kSmall = V * sizeof(T) < 16;
   constexpr int kSide = kHalf ? 1 : (V > 1 ? V : 2);  // values a turning unit takes at one place
   const int pairs = a.rotated / 2;
   const int turning = kHalf ? pairs / V : (a.rotated + kSide - 1) / kSide;  // units of a head that turn
@@ -69,8 +72,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
       const int u = first + k * kThreads + static_cast<int>(threadIdx.x);
       pair[k] = -2;
       if (u < units) {
-        const int r = over(u, a.row_inverse), w = u - r * per_row;
-        const int h = over(w, a.head_inverse), c = w - h * per_head;
+        const int r = kSmall ? over(u, a.row_inverse) : u / per_row, w = u - r * per_row;
+        const int h = kSmall ? over(w, a.head_inverse) : w / per_head, c = w - h * per_head;
         const bool turns = c < turning;
         const int at = turns ? c * (kHalf ? V : kSide) : turned + (c - turning) * V;
         const T* src = x + (row0 + r) * a.x_row + h * a.x_head + at;
