@@ -3,8 +3,6 @@
 // Compiled once for each head width (LAYA_ATTEND_DIM), and once without for what is no kernel of a width.
 #include "attend_core.hpp"
 
-#include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 namespace laya {
@@ -439,12 +437,8 @@ hipError_t launch_prompt(const AttendArgs& a, hipStream_t stream) {
 template <typename T, int D, bool kCap, DistanceBias kBias>
 hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   if (split) {
-    const long long units = static_cast<long long>(a.n_seq) * a.kv_heads, share = (units + 7) / 8;
-    // Evenly over the XCDs, or in one round on each however unevenly.
-    const bool kept = a.row_tiles > 1 && a.splits == 1 && (share * 56 <= units * 8 || share * a.row_tiles <= (D <= 64 ? 64 : 32));
-    const long long grid = (kept ? share * 8 : units) * a.row_tiles * a.splits;
-    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid)), dim3(64 * split_waves<D>()), 0, stream, a,
-                kept ? static_cast<int>(units) : 0);
+    const FewGrid grid = few_grid(a, a.row_tiles, a.splits);
+    LAYA_LAUNCH((attend_split_kernel<T, D, kCap, kBias>), dim3(static_cast<unsigned>(grid.groups)), dim3(64 * split_waves<D>()), 0, stream, a, grid.units);
     return hipGetLastError();
   }
   // Eight waves take half the loads of four, but share one barrier on a CU.  Above 128 LDS holds one workgroup, and they are two a SIMD
@@ -606,35 +600,6 @@ __global__ __launch_bounds__(256) void document_bounds_kernel(BoundsArgs a, int 
 }
 
 }  // namespace
-
-// Which kernel: by what either takes, in us, as fitted to both on 18 calls of one to 64 sequences, 48 to 1,000 queries and 64 to
-// 8,000 keys.  A prompt's workgroup takes its blocks one after the other (1.0 us each for heads of 64 with one on a CU, 1.5 with
-// two; 1.4 for heads of 128); a tile of few rows shares them among eight waves, at 2 us (4) for each tile that a CU has and 0.1 us
-// (0.2) a block of 32.  The prompts' kernel, the other: 512 tokens of 12 heads of 64 14.9 and 8.4 us, 4 such 13.0 and 16.5, 1,024 of 16
-// heads 20.2 and 15.0, 2 x 2,048 52.6 and 71.2; 512 of 32 heads of 128 behind 8,000 keys 171 and 96, 1,000 causal ones 29 and 41.
-AttendPlan attend_plan(const AttendArgs& a, int kernel) {
-  AttendPlan p{};
-  const long long few = static_cast<long long>(a.max_q) * a.group;
-  p.row_tiles = static_cast<int>((few + 31) / 32);
-  p.splits = 1;
-  // Keys that a tile's queries see: at most, and on average where later queries see more.
-  double most = a.max_k;
-  if (a.before >= 0 && !a.prefix) most = std::min(most, a.before + (a.after >= 0 ? a.after : a.max_k) + 96.0);
-  const double mean = a.after >= 0 && a.max_k == most ? most - 0.5 * std::min(a.max_q, a.max_k) : most;
-  const double base = static_cast<double>(a.n_seq) * a.kv_heads * p.row_tiles;
-  // As many workgroups as compute units, each with a block of keys for every wave at least; joining costs what two such
-  // rounds take, so two workgroups a tile are not worth it.
-  const double n = std::floor(std::min(256.0 / std::max(base, 1.0), most / 256.0));
-  if (n >= 3) p.splits = static_cast<int>(std::min<double>(n, kMaxSplits));
-  const double prompt = static_cast<double>((a.max_q + 127) / 128) * a.n_seq * a.heads / 256.0;  // workgroups a CU
-  const double wide = a.dim <= 64 ? 1 : a.dim <= 128 ? 2 : a.dim / 64.0;
-  const double prompt_us = 5.5 + (prompt > 1 ? mean : most) / 64 * (wide == 1 ? std::max(1.0, 0.55 + 0.5 * prompt) : wide / 2 * std::max(1.4, 0.3 + prompt));
-  const double split_us = 5 + (p.splits > 1 ? 3 : 0) + std::max(1.0, base * p.splits / 256) * wide * (2 + 0.1 * mean / p.splits / 32);
-  p.split = kernel == kAttendPlanned ? split_us < prompt_us : kernel == kAttendFew;
-  if (!p.split) p.splits = 1;
-  if (p.splits > 1) p.workspace = static_cast<long long>(base) * p.splits * 32 * (a.dim + 2) * 4;
-  return p;
-}
 
 hipError_t launch_attend(const AttendArgs& args, DType t, DistanceBias bias, bool cap, const AttendPlan& plan, hipStream_t stream) {
   AttendArgs a = args;

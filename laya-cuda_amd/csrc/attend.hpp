@@ -1,22 +1,21 @@
 // Attention over packed sequences with key ranges, capped scores and distance biases: arguments and plan.
 #pragma once
 
+#include "attend_plan.hpp"
 #include "kernels.hpp"
 
 namespace laya {
 
 constexpr int kMaxSpan = 1024;     // of a bias table: its head's row lies in LDS
 constexpr int kMaxAttendDim = 256;
-constexpr int kMaxSplits = 64;     // of a sequence's keys over workgroups: one lane each when they are joined
 
 enum class DistanceBias : int { None = 0, Slopes = 1, Table = 2 };
 
-struct AttendArgs {
+struct AttendArgs : AttendSizes {
   const void *q, *k, *v;
   void* out;
   long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
-  int heads, kv_heads, group, dim;  // group = heads / kv_heads
-  int n_seq, max_q, max_k, q_rows, k_rows;
+  int q_rows, k_rows;
   const int32_t *q_starts, *q_lengths, *k_starts, *k_lengths;  // [n_seq]
   float scale;           // capped: of a raw product, to twice the tanh's argument in log2 units
   float cap;             // in log2 units
@@ -25,22 +24,12 @@ struct AttendArgs {
   const float* slopes;   // [heads]
   const float* table;    // [heads][2 span + 1]
   int span;
-  int before, after;     // -1: no limit
   const int32_t* prefix; // [n_seq] or null
   const int2* bounds;    // [q_rows] (first, end) or null
   // Split plan: row tiles of 32 (token, head) rows, and how many workgroups share a tile's keys.
   int row_tiles, splits;
   float* parts;          // [n_seq][kv_heads][row_tiles][splits][32][dim] sums, then as many [32][2] of reference and total
 };
-
-// The launch of a call: which kernel, and for the split one its row tiles and splits; workspace in bytes.
-struct AttendPlan {
-  bool split;
-  int row_tiles, splits;
-  long long workspace;
-};
-enum AttendKernel : int { kAttendPlanned = 0, kAttendMany = 1, kAttendFew = 2 };
-AttendPlan attend_plan(const AttendArgs& a, int kernel);
 
 template <int D>  // the compiled head widths
 hipError_t launch_attend_dim(const AttendArgs& a, DType t, DistanceBias bias, bool cap, bool split, hipStream_t stream);

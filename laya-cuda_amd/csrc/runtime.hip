@@ -1730,7 +1730,7 @@ static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
   a.heads = c->heads; a.kv_heads = c->kv_heads; a.group = c->heads / c->kv_heads; a.dim = c->dim;
   a.q_rows = c->q_rows; a.k_rows = c->k_rows; a.n_seq = c->n_seq; a.max_q = c->max_q; a.max_k = c->max_k;
   a.before = c->before; a.after = c->after; a.span = c->table ? c->span : 0;
-  a.prefix = c->prefix;
+  a.prefix = c->prefix; a.prefixed = c->prefix != nullptr;
   const int64_t pairs = static_cast<int64_t>(c->n_seq) * c->heads;
   // Workgroups of 256 threads; heads above 64 may run as half as many tiles of twice the threads.
   const int64_t tile = c->dim > 64 ? 256 : 128;
@@ -1738,7 +1738,7 @@ static AttendArgs attend_sizes(const LayaAttend* c, AttendPlan* plan) {
                    static_cast<int64_t>(c->max_q) * a.group < (1LL << 30),
                "n_seq * heads * max_q: too large for one launch");
   *plan = attend_plan(a, c->kernel);
-  LAYA_REQUIRE(!plan->split || static_cast<int64_t>(c->n_seq) * c->kv_heads * plan->row_tiles * plan->splits < kMaxGroups / 2,
+  LAYA_REQUIRE(!plan->split || few_grid(a, plan->row_tiles, plan->splits).groups < kMaxGroups / 2,
                "n_seq * heads * max_q: too large for one launch");
   return a;
 }
