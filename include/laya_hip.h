@@ -379,7 +379,8 @@ enum { LAYA_ATTEND_PLANNED = 0, LAYA_ATTEND_MANY = 1, LAYA_ATTEND_FEW = 2 };
 /* Ranges of a document mask: bounds[row] = (first, end) of the run of equal neighbouring ids that holds the row, counted from
  * its sequence's start.  documents [rows], bounds [rows][2], starts and lengths [n_seq] are device memory; a
  * sequence's rows are starts[s] .. starts[s] + lengths[s] - 1, cut to the array and to max_length; rows of no sequence are left
- * as they were.  One call serves every layer and head of a batch. */
+ * as they were.  Sequences must not share rows.  Work is linear in the rows; max_length above 4,096 takes three launches for one.  One
+ * call serves every layer and head of a batch. */
 int laya_op_document_bounds(const int32_t* documents, const int32_t* starts, const int32_t* lengths, int n_seq,
                             int64_t rows, int max_length, int32_t* bounds, void* stream);
 

@@ -545,39 +545,55 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(AttendArgs a, int
   *reinterpret_cast<typename Vec4<T>::type*>(out + 4 * lane) = h;
 }
 
-// The run of equal ids around each row of a sequence.  Two dependent loads and a launch: 65,536 rows 6 us.  A wave takes 64 rows: where ids change comes from one ballot, and what
-// begins before or ends behind them is looked for 512 rows at a time.
+// The run of equal ids around each row of a sequence, a wave for 64 rows.  Where ids change comes from one ballot.  What begins before
+// those rows or ends behind them is looked for from there, 512 rows at a time (kOpen false): one launch, but where one document
+// fills a sequence of n rows its n / 64 waves take n / 512 steps each.  Or it is left open (kOpen true) for the two kernels below,
+// so that each row is read and written a fixed number of times.  65,536 rows, documents of 200 and documents that fill their sequences, looked
+// for and left open: in sequences of 1,024 4.4 and 4.8 us, 8.4 and 8.5; of 4,096 4.6 and 10.7, 8.6 and 8.5; of 16,384 4.5 and 34.7, 9.0 and 9.0;
+// in one 4.6 and 130, 12.3 and 12.3.  One document of 2^20 rows 117 us, of 2^24 2.1 ms.
+struct Run {
+  int start, n;  // of a sequence, cut to the array
+};
+__device__ __forceinline__ Run run_of(const BoundsArgs& a, int s) {
+  const int start = __builtin_amdgcn_readfirstlane(a.starts[s]), n = __builtin_amdgcn_readfirstlane(a.lengths[s]);
+  return {start, start < 0 || start >= a.rows ? 0 : max(0, min(min(n, a.max_length), a.rows - start))};
+}
+constexpr int kLookedFor = 4096;  // rows of the longest sequences whose runs are looked for
+constexpr int kOpenFirst = -1, kOpenEnd = INT_MAX;  // a run that begins, or ends, outside its 64 rows
+
+template <bool kOpen>
 __global__ __launch_bounds__(256) void document_bounds_kernel(BoundsArgs a, int groups) {
-  const int s = blockIdx.x / groups, lane = threadIdx.x & 63;
-  const int start = __builtin_amdgcn_readfirstlane(a.starts[s]);
-  int n = __builtin_amdgcn_readfirstlane(a.lengths[s]);
-  n = start < 0 || start >= a.rows ? 0 : max(0, min(min(n, a.max_length), a.rows - start));
+  const int lane = threadIdx.x & 63;
+  const Run run = run_of(a, blockIdx.x / groups);
+  const int n = run.n;
   const int i0 = (static_cast<int>(blockIdx.x % groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64;
   if (i0 >= n) return;
-  const int32_t* ids = a.documents + start;
+  const int32_t* ids = a.documents + run.start;
   const int i = i0 + lane, last = min(n, i0 + 64) - 1;
   const int mine = ids[min(i, n - 1)], before = ids[max(0, min(i, n - 1) - 1)];
   const unsigned long long begins = __builtin_amdgcn_ballot_w64(i < n && (i == 0 || mine != before));
   // First row of the run that row i0 lies in, and the end of the one that row `last` lies in.
-  int first = i0, end = last + 1;
-  if (!(begins & 1)) {
-    const int id = __builtin_amdgcn_readfirstlane(mine);
-    for (first = 0;;) {  // ends where a row differs, or before row 0
-      int found = -1;
-      const int from = i0 - 1 - first;  // rows above it are of the run
-      for (int c = 7; c >= 0; --c) {
-        const int at = from - 64 * c - lane;
-        const unsigned long long other = __builtin_amdgcn_ballot_w64(at < 0 || ids[max(at, 0)] != id);
-        if (other) found = 64 * c + __builtin_ctzll(other);
+  int first = kOpenFirst, end = kOpenEnd;
+  if constexpr (kOpen) {
+    if (last + 1 == n || ids[last + 1] != ids[last]) end = last + 1;
+  } else {
+    if (!(begins & 1)) {
+      const int id = __builtin_amdgcn_readfirstlane(mine);
+      for (first = 0;;) {  // ends where a row differs, or before row 0
+        int found = -1;
+        const int from = i0 - 1 - first;  // rows above it are of the run
+        for (int c = 7; c >= 0; --c) {
+          const int at = from - 64 * c - lane;
+          const unsigned long long other = __builtin_amdgcn_ballot_w64(at < 0 || ids[max(at, 0)] != id);
+          if (other) found = 64 * c + __builtin_ctzll(other);
+        }
+        if (found >= 0) {
+          first = from - found + 1;
+          break;
+        }
+        first += 512;
       }
-      if (found >= 0) {
-        first = from - found + 1;
-        break;
-      }
-      first += 512;
     }
-  }
-  {
     const int id = __builtin_amdgcn_readfirstlane(ids[last]);
     for (int gone = 0;; gone += 512) {
       int found = -1;
@@ -596,7 +612,65 @@ __global__ __launch_bounds__(256) void document_bounds_kernel(BoundsArgs a, int 
   const unsigned long long upto = begins & (~0ull >> (63 - lane)), behind = lane == 63 ? 0 : begins >> (lane + 1);
   const int lo = upto ? i0 + 63 - __builtin_clzll(upto) : first;
   const int hi = behind ? i + 1 + __builtin_ctzll(behind) : end;
-  a.bounds[start + i] = make_int2(lo, hi);
+  a.bounds[run.start + i] = make_int2(lo, hi);
+}
+
+// Over a workgroup, in the order of its threads: the largest of what threads before this one hold, and of what all hold.
+constexpr int kCarryThreads = 1024;
+__device__ __forceinline__ int2 largest_before(int v) {
+  __shared__ int waves[kCarryThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int by = 1; by < 64; by *= 2) {
+    const int other = __shfl_up(v, by, kWave);
+    if (lane >= by) v = max(v, other);
+  }
+  if (lane == 63) waves[wave] = v;
+  const int own = __shfl_up(v, 1, kWave);
+  __syncthreads();
+  int before = INT_MIN, all = INT_MIN;
+  for (int w = 0; w < kCarryThreads / 64; ++w) {
+    if (w < wave) before = max(before, waves[w]);
+    all = max(all, waves[w]);
+  }
+  __syncthreads();
+  return make_int2(lane ? max(before, own) : before, all);
+}
+
+// What is open goes from each 64 rows to the next: a workgroup a sequence, 65,536 rows a step.  A group's last row has the first row
+// of the run that leaves it (open: as the group before), so the run that enters a group begins at the largest such row before it; ends
+// likewise, from the back, as negated rows.  The group's first row takes the one, its last row the other.
+__global__ __launch_bounds__(kCarryThreads) void document_carry_kernel(BoundsArgs a) {
+  const Run run = run_of(a, blockIdx.x);
+  int2* bounds = a.bounds + run.start;
+  const int groups = (run.n + 63) / 64;
+  int first = kOpenFirst;
+  for (int base = 0; base < groups; base += kCarryThreads) {
+    const int g = base + threadIdx.x, at = 64 * g;
+    const int2 r = largest_before(g < groups ? bounds[min(at + 63, run.n - 1)].x : kOpenFirst);
+    if (g < groups && bounds[at].x == kOpenFirst) bounds[at].x = max(first, r.x);
+    first = max(first, r.y);
+  }
+  int end = -kOpenEnd;
+  for (int base = 0; base < groups; base += kCarryThreads) {
+    const int g = groups - 1 - base - static_cast<int>(threadIdx.x), at = 64 * g;
+    const int2 r = largest_before(g >= 0 ? -bounds[at].y : -kOpenEnd);
+    const int last = min(at + 63, run.n - 1);
+    if (g >= 0 && bounds[last].y == kOpenEnd) bounds[last].y = -max(end, r.x);
+    end = max(end, r.y);
+  }
+}
+
+__global__ __launch_bounds__(256) void document_fill_kernel(BoundsArgs a, int groups) {
+  const int lane = threadIdx.x & 63;
+  const Run run = run_of(a, blockIdx.x / groups);
+  const int i0 = (static_cast<int>(blockIdx.x % groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64;
+  if (i0 >= run.n) return;
+  const int rows = min(64, run.n - i0);
+  int2* row = a.bounds + run.start + i0 + min(lane, rows - 1);
+  const int2 mine = *row;
+  const int first = __builtin_amdgcn_readfirstlane(mine.x), end = __builtin_amdgcn_readlane(mine.y, rows - 1);
+  if (lane < rows && (mine.x == kOpenFirst || mine.y == kOpenEnd))
+    *row = make_int2(mine.x == kOpenFirst ? first : mine.x, mine.y == kOpenEnd ? end : mine.y);
 }
 
 }  // namespace
@@ -621,7 +695,14 @@ hipError_t launch_attend(const AttendArgs& args, DType t, DistanceBias bias, boo
 
 hipError_t launch_document_bounds(const BoundsArgs& a, hipStream_t stream) {
   const int groups = (a.max_length + 255) / 256;
-  LAYA_LAUNCH(document_bounds_kernel, dim3(static_cast<unsigned>(static_cast<long long>(groups) * a.n_seq)), dim3(256), 0, stream, a, groups);
+  const dim3 grid(static_cast<unsigned>(static_cast<long long>(groups) * a.n_seq));
+  if (a.max_length <= kLookedFor) {
+    LAYA_LAUNCH(document_bounds_kernel<false>, grid, dim3(256), 0, stream, a, groups);
+  } else {
+    LAYA_LAUNCH(document_bounds_kernel<true>, grid, dim3(256), 0, stream, a, groups);
+    LAYA_LAUNCH(document_carry_kernel, dim3(a.n_seq), dim3(kCarryThreads), 0, stream, a);
+    LAYA_LAUNCH(document_fill_kernel, grid, dim3(256), 0, stream, a, groups);
+  }
   return hipGetLastError();
 }
 
