@@ -153,12 +153,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
       f32x16 t[R::KT];
       T8 p[2 * R::KT];
       rows.scores((LdsBytes)(skv[0]), buffer + SB * h * P * 2u, t);
-      float shift;
+      typename R::Shift shift;
       const int first = key - first_position;  // of the wave's first query to the step's first key
       if (kBias == DistanceBias::Table && (first + SB - 1 <= -a.span || first - 31 >= a.span)) {
         // Steps wholly past the span on one side have one bias; the table's LDS rows reach as far as the others need.
         rows.capped(a, t);
-        shift = __builtin_fmaf(first < 0 ? far_left : far_right, a.unit, kCap ? a.cap : 0.f);
+        shift = {first < 0 ? far_left : far_right, kCap ? a.cap : 0.f};
       } else {
         shift = rows.change(a, t, key, table, first + SB - 1 <= 0 ? -1 : first - 31 >= 0 ? 1 : 0);
       }
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
       key0 = blocks.taken(j + NW);
       load(from_k, at_k, lds_k, key0);
     }
-    const float shift = rows.change(a, t, key, table, 0);
+    const typename R::Shift shift = rows.change(a, t, key, table, 0);
     if (!(key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi))) rows.hide(t, key);
     if (j < j0 + NW) rows.open(a, t, shift);
     const float sum = rows.weights(a, t, p, shift);

@@ -243,22 +243,26 @@ struct Rows {
   // Key of score r of tile kt of the block at `key`, less the lane's first.
   static constexpr int slot(int kt, int r) { return 32 * kt + 8 * (r >> 2) + (r & 3); }
 
-  // A block's scores stand as t, of which the log2 score is a.unit t + shift: raw products, or, capped, the reciprocals in
-  // cap tanh(x) = cap - 2 cap / (1 + exp(2 x)), exact to 2^-22 of the cap; biases are added in units of t.  A weight's exponent is
-  // then one multiplication and addition away.  Slopes of a block to one side of every row are linear in the key: what they have in common
-  // goes into the shift.
+  // A block's scores stand as t, of which the log2 score is a.unit (t + shift.bias) + shift.rest: raw products, or, capped, the
+  // reciprocals in cap tanh(x) = cap - 2 cap / (1 + exp(2 x)), exact to 2^-20 of the cap; biases are added in units of t.  A weight's exponent
+  // is then one multiplication and addition away.  Slopes of a block to one side of every row are linear in the key: what they have in
+  // common goes into the shift.  Equal scores must come out equal however large their bias is, whether it was added to t or stands in the shift: the product
+  // with a.unit is not rounded by itself, and under a table capped scores are centred before their bias comes.
   // table: of this row's head, at distance 0; one in LDS is in units of t and may be read up to a block and 32 rows past the span.
   // side: -1 and 1 where all keys lie before or behind all rows' positions (or at them), 0 where not.
+  struct Shift {
+    float bias, rest;
+  };
   template <typename Table>
-  __device__ __forceinline__ float change(const AttendArgs& a, f32x16 (&s)[KT], int key, Table table, int side) const {
+  __device__ __forceinline__ Shift change(const AttendArgs& a, f32x16 (&s)[KT], int key, Table table, int side) const {
     capped(a, s);
-    float shift = kCap ? a.cap : 0.f;
+    Shift shift{0.f, kCap ? a.cap : 0.f};
     const int at = key + 4 * g - position;
     if constexpr (kBias == DistanceBias::Slopes) {
       const float from = static_cast<float>(at);
       if (side) {
         const float by = side < 0 ? -slope : slope;  // of |d| = -d or d
-        shift = __builtin_fmaf(from * by, a.unit, shift);
+        shift.bias = from * by;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -271,13 +275,15 @@ struct Rows {
       }
     }
     if constexpr (kBias == DistanceBias::Table) {
+      shift.rest = 0.f;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int d = at + slot(kt, r);
-          if constexpr (std::is_same<Table, LdsFloats>::value) s[kt][r] += table[d];
-          else s[kt][r] = __builtin_fmaf(table[max(-a.span, min(a.span, d))], a.per_unit, s[kt][r]);
+          const float t = kCap ? s[kt][r] - 0.5f : s[kt][r];
+          if constexpr (std::is_same<Table, LdsFloats>::value) s[kt][r] = t + table[d];
+          else s[kt][r] = __builtin_fmaf(table[max(-a.span, min(a.span, d))], a.per_unit, t);
         }
     }
     return shift;
@@ -308,18 +314,19 @@ struct Rows {
   }
 
   // The largest score: of the largest t, or of the smallest where the cap's unit is negative.
-  __device__ __forceinline__ float block_max(const AttendArgs& a, const f32x16 (&s)[KT], float shift) const {
+  __device__ __forceinline__ float block_max(const AttendArgs& a, const f32x16 (&s)[KT], Shift shift) const {
     float m = kCap ? INFINITY : -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = kCap ? fminf(m, s[kt][r]) : fmaxf(m, s[kt][r]);
-    return halves_max(__builtin_fmaf(m, a.unit, shift));
+    return halves_max(__builtin_fmaf(m + shift.bias, a.unit, shift.rest));
   }
 
-  __device__ __forceinline__ float weights(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], float shift) const {
+  __device__ __forceinline__ float weights(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], Shift shift) const {
     float sum[2] = {0.f, 0.f};
-    const float base = shift - reference;
+    float base = __builtin_fmaf(shift.bias, a.unit, -reference);
+    if constexpr (kCap) base += shift.rest;
 #pragma unroll
     for (int c = 0; c < 2 * KT; ++c) {
 #pragma unroll
@@ -333,12 +340,12 @@ struct Rows {
   }
 
   // The first block of a wave: its largest score is the reference, before any weight is made.
-  __device__ __forceinline__ void open(const AttendArgs& a, const f32x16 (&s)[KT], float shift) {
+  __device__ __forceinline__ void open(const AttendArgs& a, const f32x16 (&s)[KT], Shift shift) {
     reference = fmaxf(kNothing, block_max(a, s, shift));
   }
 
   // Weights that are too large for the reference: it moves to the block's largest score.
-  __device__ __forceinline__ float move(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], float shift, float sum) {
+  __device__ __forceinline__ float move(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], Shift shift, float sum) {
     if (__builtin_amdgcn_ballot_w64(!(sum <= kMostWeight))) {
       const float m = block_max(a, s, shift);
       const float to = m > reference + 8.f ? m : reference;
@@ -394,10 +401,10 @@ struct CarefulRow {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x = __builtin_fmaf(to_float(kc[e]), to_float(qc[e]), x);
         }
-        if constexpr (kCap) x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f);
+        if constexpr (kCap) x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f) - 0.5f;
         if constexpr (kBias == DistanceBias::Slopes) x = __builtin_fmaf(fabsf(static_cast<float>(key - position)), slope, x);
         if constexpr (kBias == DistanceBias::Table) x = __builtin_fmaf(table[max(-a.span, min(a.span, key - position))], a.per_unit, x);
-        x = __builtin_fmaf(x, a.unit, kCap ? a.cap : 0.f);
+        x *= a.unit;
       }
       const float to = fmaxf(reference, wave_max(x));
       const float alpha = to == reference ? 1.f : __builtin_amdgcn_exp2f(reference - to);
