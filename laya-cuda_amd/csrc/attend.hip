@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
 
   T* out = static_cast<T*>(a.out) + head * a.out_head;
   const unsigned live = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(valid));
-  unsigned bad = rows.not_numbers() & live;
+  unsigned bad = rows.doubtful() & live;
   const float total = halves_sum(rows.total);
   const float inv = total == 0.f ? 0.f : 1.0f / total;
   if (valid && !(bad >> (lane & 31) & 1)) {
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
   __syncthreads();  // every wave is done with its stages
   float* so = reinterpret_cast<float*>(lds);
   {
-    const unsigned bad = rows.not_numbers();
+    const unsigned bad = rows.doubtful();
     const float total = halves_sum(rows.total);
     if (rows.g == 0) {
       s_reference[wave][lane & 31] = rows.reference;

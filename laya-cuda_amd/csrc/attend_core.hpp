@@ -19,6 +19,7 @@ namespace laya {
 
 constexpr float kNothing = -1e30f;    // the reference of a row that has seen no key; scores not above it count as hidden
 constexpr float kMostWeight = 8192.f;
+constexpr float kLargest = 4194304.f;  // references up to here are rounded by at most 1/4, which all of a row's weights share
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -361,21 +362,23 @@ struct Rows {
     return sum;
   }
 
-  // Rows (bits 0 to 31) whose sums are no numbers: a weight of 0 times an infinity or NaN in a hidden key's value, if nothing
-  // the row sees is one.
-  __device__ __forceinline__ unsigned not_numbers() const {
+  // Rows (bits 0 to 31) to be done again by themselves: those whose sums are no numbers (a weight of 0 times an infinity or NaN in a
+  // hidden key's value, if nothing the row sees is one), and those whose scores are so large that a reference's own rounding is no longer
+  // small: at 2^30 it is up to 2^5, and weights of e^-22 in the place of 1 round to 0 in fp16.
+  __device__ __forceinline__ unsigned doubtful() const {
     float sum[4] = {total, 0.f, 0.f, 0.f};  // NaN for a NaN or an infinity
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum[r & 3] = __builtin_fmaf(o[d][r], 0.f, sum[r & 3]);
     const float x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    const unsigned long long bad = __builtin_amdgcn_ballot_w64(x != x);
+    const bool large = fabsf(reference) > kLargest && reference > kNothing;
+    const unsigned long long bad = __builtin_amdgcn_ballot_w64(x != x || large);
     return static_cast<unsigned>(bad | bad >> 32);
   }
 };
 
-// One row by itself, hidden keys never touched: what a wave does for a row whose sums are no numbers.  Blocks [j0, j1) of
+// One row by itself, hidden keys never touched and the reference taken from each rounded score: what a wave does for a doubtful row.  Blocks [j0, j1) of
 // the row's tile; lane l holds dims l, l + 64, ...
 template <typename T, int D, int KB, bool kCap, DistanceBias kBias>
 struct CarefulRow {

@@ -33,7 +33,7 @@ def compare(c, table=None):
 
 
 @KINDS
-@pytest.mark.parametrize("bias", [1e3, -1e6, 1.7e7])
+@pytest.mark.parametrize("bias", [1e3, -1e6, 1.7e7, -1e9, 1.1e9, -7.3e9, -1e12, 3e20, -5e29])
 @pytest.mark.parametrize("cap", [0.0, 9.0])
 @pytest.mark.parametrize("masks", [dict(), dict(after=0), dict(before=9, after=40)], ids=["all", "causal", "window"])
 @KERNELS
@@ -60,7 +60,7 @@ def test_masks_by_bias_beside_keys_that_are_seen(gpu, kind, dim, bias, kernel):
 
 
 @KINDS
-@pytest.mark.parametrize("scale", [1.0, 1e4, 1e6])
+@pytest.mark.parametrize("scale", [1.0, 1e4, 1e7, 1e10])
 @pytest.mark.parametrize("cap", [0.0, 1024.0])
 @KERNELS
 def test_scales_that_leave_the_largest_scores(gpu, kind, dim, scale, cap, kernel):
