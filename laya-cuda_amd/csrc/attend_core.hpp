@@ -17,7 +17,7 @@
 
 namespace laya {
 
-constexpr float kNothing = -1e30f;    // the reference of a row that has seen no key; scores not above it count as hidden
+constexpr float kNothing = -1.4426950e30f;  // of a row that has seen no key, its reference: a score of -1e30; scores not above it count as hidden
 constexpr float kMostWeight = 8192.f;
 constexpr float kLargest = 4194304.f;  // references up to here are rounded by at most 1/4, which all of a row's weights share
 

@@ -89,3 +89,14 @@ def test_steep_slopes_leave_the_nearest_key(gpu, kind, dim, slope, kernel):
         got = c.out[c.q0[s]:c.q0[s] + c.nq[s], :, :dim]
         want = c.kv[c.k0[s]:c.k0[s] + c.nk[s], 2:, :dim].repeat_interleave(2, 1)
         assert torch().equal(got, want)
+
+
+@KINDS
+@KERNELS
+def test_scores_below_1e30_hide_and_others_do_not(gpu, kind, dim, kernel):
+    for bias, hides in ((-0.99e30, False), (-1.01e30, True)):
+        c = Call(gpu, kind, ODD, 4, 2, dim, bias="table", span=20)
+        c.q[..., :dim] = 0
+        c.table[:] = bias
+        c.describe(kernel=kernel).run()
+        compare(c, np.full_like(c.table, -np.inf) if hides else np.zeros_like(c.table))
