@@ -405,7 +405,8 @@ struct CarefulRow {
           for (int e = 0; e < 8; ++e) x = __builtin_fmaf(to_float(kc[e]), to_float(qc[e]), x);
         }
         if constexpr (kCap) x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.scale) + 1.0f) - 0.5f;
-        if constexpr (kBias == DistanceBias::Slopes) x = __builtin_fmaf(fabsf(static_cast<float>(key - position)), slope, x);
+        // A slope past the type's range in units of a raw score is infinite here, and 0 times it no number, which is what brings the row here.
+        if constexpr (kBias == DistanceBias::Slopes) x = key == position ? x : __builtin_fmaf(fabsf(static_cast<float>(key - position)), slope, x);
         if constexpr (kBias == DistanceBias::Table) x = __builtin_fmaf(table[max(-a.span, min(a.span, key - position))], a.per_unit, x);
         x *= a.unit;
       }

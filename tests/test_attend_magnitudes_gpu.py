@@ -100,3 +100,18 @@ def test_scores_below_1e30_hide_and_others_do_not(gpu, kind, dim, kernel):
         c.table[:] = bias
         c.describe(kernel=kernel).run()
         compare(c, np.full_like(c.table, -np.inf) if hides else np.zeros_like(c.table))
+
+
+@KINDS
+@pytest.mark.parametrize("slope", [4e37, 3.4e38])
+@pytest.mark.parametrize("scale,cap", [(None, 0.0), (1e-6, 0.0), (None, 30.0)])
+@KERNELS
+def test_slopes_of_the_largest_values(gpu, kind, dim, slope, scale, cap, kernel):
+    """Slopes past the type's range in units of a raw score: 0 at the query's own key, and every other key hidden."""
+    c = Call(gpu, kind, ODD + [300], 4, 2, dim, bias="slopes", before=200, after=70, scale=scale, cap=cap)
+    c.slopes[:] = slope
+    c.describe(kernel=kernel).run()
+    torch().cuda.synchronize()
+    for s in range(len(c.nq)):
+        got = c.out[c.q0[s]:c.q0[s] + c.nq[s], :, :dim]
+        assert torch().equal(got, c.kv[c.k0[s]:c.k0[s] + c.nk[s], 2:, :dim].repeat_interleave(2, 1))
