@@ -372,8 +372,8 @@ int laya_op_rotary(const void* x, int64_t x_row, int64_t x_head, void* out, int6
                    int dtype, const int32_t* positions, const double* turns, float amplitude, int layout,
                    int direction, int64_t rows, int heads, int dim, int rotated, void* stream);
 
-/* Kernels of laya_op_attend: the planner's choice; a workgroup for 128 queries of a head, for many rows; a workgroup or, over
- * long keys, several for 32 rows, for few. */
+/* Kernels of laya_op_attend: the planner's choice; a workgroup for 128 queries of a head (256 of heads above 128 and, of those above
+ * 64, in long prompts), for many rows; a workgroup or, over long keys, several for 32 rows, for few. */
 enum { LAYA_ATTEND_PLANNED = 0, LAYA_ATTEND_MANY = 1, LAYA_ATTEND_FEW = 2 };
 
 /* Ranges of a document mask: bounds[row] = (first, end) of the run of equal neighbouring ids that holds the row, counted from
@@ -393,7 +393,8 @@ int laya_op_document_bounds(const int32_t* documents, const int32_t* starts, con
  *   t = scale q . k;  t = cap tanh(t / cap) if cap > 0;  t -= slopes[h] |j - p|  or  t += table[h][clamp(j - p, -span, span) + span];
  *   out = sum of softmax(t) v over the keys seen.
  * A query that sees no key, or whose scores are all below -1e30 (biases of a type's lowest value hide keys), gets zeros; what lies in
- * hidden keys, NaNs and infinities too, does not matter.  out's rows of no query are left as they were. */
+ * hidden keys, NaNs and infinities too, does not matter.  Other entries of a table are at most 1e27
+ * in size.  Rows whose largest score passes 2^21 in size go a path some 200 times as slow, one by one.  out's rows of no query are left as they were.  Sequences may share keys, not queries. */
 typedef struct LayaAttend {
   uint32_t struct_bytes;  /* sizeof(LayaAttend) */
   int32_t dtype;          /* LAYA_F16 or LAYA_BF16: q, k, v, out */
@@ -426,8 +427,8 @@ int64_t laya_attend_workspace(const LayaAttend* call);
 /* The attention described above, sums and softmax in fp32, weights rounded to dtype for the matrix unit, one rounding of the
  * output.  Lengths of zero are fine.  dim a multiple of 8 up to 256, heads a multiple of kv_heads; q, k, v and out and
  * their strides on whole 16 bytes, row strides of k and v at least dim and below 2^23; scale from 1e-10 to 1e10; cap 0 or
- * 1e-10 to 1024 (a capped score is exact to 2^-20 of the cap); span 0 to 1024 with a table; rows, max_q, max_k, before and after
- * below 2^30, heads at most 2^16, and n_seq * heads * max_q, max_q counted as whole 128 (256 for heads above 64), at most about
+ * 1e-10 to 1024 (a capped score is exact to 2^-20 of the cap: from 512 on half a step of an fp16 weight and more); span 0 to
+ * 1024 with a table; rows, max_q, max_k, before and after below 2^30, heads at most 2^16, and n_seq * heads * max_q, max_q counted as whole 128 (256 for heads above 64), at most about
  * 2^31 (one launch; the kernel for few rows, where it is named, takes about 2^28).  workspace: device memory, 16-byte aligned,
  * of the bytes that laya_attend_workspace tells (NULL for 0), written before it is read; calls that may run at the same time,
  * captured ones too, take different ones.  Equal calls give equal bits. */

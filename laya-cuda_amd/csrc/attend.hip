@@ -18,13 +18,14 @@ constexpr int kPad = 96;  // distances past a bias table's span that the scores 
 // running reference and total) and skips those that none of its rows sees.
 //
 // What bounds it: the card's power and the vector instructions beside the matrix ones.  64 x 1,024 tokens of 16 heads of 64 run
-// 350 us (785 TFLOP/s) at 1.91 of 2.4 GHz with the matrix cores busy 38% of the cycles and vector instructions 58%; with zeros for
+// 350 us (785 TFLOP/s; boxes differ, 316 to 362) at 1.91 of 2.4 GHz with the matrix cores busy 38% of the cycles and vector instructions 58%; with zeros for
 // inputs 280 us.  Copies without the exponentials, the loads or one of the products run 320, 315 and 290 us.  16,384
-// causal tokens of 8 heads of 128: 520 us, 1.06 PFLOP/s, the matrix cores 44%.
+// causal tokens of 8 heads of 128: 511 to 545 us, 1.01 to 1.08 PFLOP/s, the matrix cores 44%.
 // Why 32 keys a step in one straight line, with no more than 101 registers for heads of 64: four such workgroups share a CU.  64 keys a
 // step took 373 us where this took 361, scores of the next step under the softmax of this one 388 against 352, two row groups a
 // wave (half the LDS reads) 354 against 349 for heads of 64 and 1,535 against 1,069 for 128, three buffers 382 against 344, blocks of 32
-// keys 394 against 350, raised priorities for either phase or by slot nothing.
+// keys 394 against 350, raised priorities for either phase or by slot nothing.  Tiles of 64 queries, two waves: 488 against 338, documents 314
+// against 239, ragged requests with a bias table 121 against 83, 1,571 tokens behind a window of heads of 80 64 against 41.
 template <typename T, int D, bool kCap, DistanceBias kBias, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64 || (D == 96 && NW == 8) ? 4 : 2))) void attend_kernel(
     AttendArgs a, int tiles, int unit, int units) {
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
 }
 
 // Few rows: a workgroup owns 32 rows, the (token, head) pairs of the heads that share keys, and its waves split their keys into
-// blocks of 32, each wave with a place of its own in LDS for a block of K and one of V.  The next K is on its way from the
+// blocks of 32 (eight waves, four for heads above 128), each wave with a place of its own in LDS for a block of K and one of V.  The next K is on its way from the
 // scores to the next ones, the next V from one product to the next.  Long contexts are shared by a.splits workgroups, whose sums
 // join_kernel adds in a fixed order.
 //
@@ -448,7 +449,7 @@ hipError_t launch_kind(const AttendArgs& a, bool split, hipStream_t stream) {
   if constexpr (D > 128) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
   if constexpr (D == 96 || D == 128) {
     const long long tiles8 = (a.max_q + 255) / 256 * static_cast<long long>(a.n_seq) * a.heads;
-    if (tiles8 >= 512 && (D == 96 || a.max_q >= 4096)) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
+    if (tiles8 >= 2 * kPlannedUnits && (D == 96 || a.max_q >= 4096)) return launch_prompt<T, D, kCap, kBias, 8>(a, stream);
   }
   if constexpr (D <= 128) return launch_prompt<T, D, kCap, kBias, 4>(a, stream);
 }

@@ -6,8 +6,8 @@
 // once, so HBM is the bound.  A workgroup takes a few rows: every thread loads its values first, and while they are on their way
 // the workgroup makes the rows' cosines and sines once for all heads, in LDS.  The angle is reduced to an eighth of a turn in
 // 64 bits (a position of a million at 32 bits would be off by 0.06 radians), the sine and cosine of the rest are fp32.
-// 65,536 rows of 32 heads of 64 in bf16: 101 us, 5.3 TB/s (a copy of 4 GiB 4.8; part of it stays in the last-level cache), vector
-// instructions 31% of the cycles; 131,072 rows of 10 heads of 128, 124 us.
+// 65,536 rows of 32 heads of 64 in bf16: 111 us in a row of such calls, 101 the shortest, 4.8 and 5.3 TB/s (a copy of 4 GiB 4.8; part of it stays in
+// the last-level cache), vector instructions 32% of the cycles; 131,072 rows of 10 heads of 128, 131 us and 123.
 #include "attend.hpp"
 
 namespace laya {
