@@ -132,6 +132,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
     far_right = stable[2 * (a.span + kPad)];
   }
   const int first_position = __builtin_amdgcn_readfirstlane(me.position);
+  const bool steep = kBias == DistanceBias::Slopes && !(fabsf(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(rows.slope))) * a.unit) <= kSteepest);
   unsigned buffer = 0;
   bool fresh = true;  // no step done
   for (int j = 0; j < nb; ++j, buffer ^= kBuffer) {
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
         rows.capped(a, t);
         shift = {first < 0 ? far_left : far_right, kCap ? a.cap : 0.f};
       } else {
-        shift = rows.change(a, t, key, table, first + SB - 1 <= 0 ? -1 : first - 31 >= 0 ? 1 : 0);
+        shift = rows.change(a, t, key, table, steep ? 0 : first + SB - 1 <= 0 ? -1 : first - 31 >= 0 ? 1 : 0);
       }
       if (!whole) rows.hide(t, key);
       if (fresh) rows.open(a, t, shift);

@@ -20,6 +20,9 @@ namespace laya {
 constexpr float kNothing = -1.4426950e30f;  // of a row that has seen no key, its reference: a score of -1e30; scores not above it count as hidden
 constexpr float kMostWeight = 8192.f;
 constexpr float kLargest = 4194304.f;  // references up to here are rounded by at most 1/4, which all of a row's weights share
+// Of a slope, in log2 units a key, that a step's shift may stand for: a score then loses 2^-24 of 31 keys' bias, 1e-4.  From 1e7 on a query's own key in such
+// a step came out with a weight of 0.
+constexpr float kSteepest = 64.f;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

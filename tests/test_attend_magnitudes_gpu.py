@@ -115,3 +115,21 @@ def test_slopes_of_the_largest_values(gpu, kind, dim, slope, scale, cap, kernel)
     for s in range(len(c.nq)):
         got = c.out[c.q0[s]:c.q0[s] + c.nq[s], :, :dim]
         assert torch().equal(got, c.kv[c.k0[s]:c.k0[s] + c.nk[s], 2:, :dim].repeat_interleave(2, 1))
+
+
+@KINDS
+@pytest.mark.parametrize("slope", [40.0, 1e3, 3.3e6, 1e9, 1.7e12, 1e30])
+@pytest.mark.parametrize("ahead", [1, 17, 31, 100])
+@KERNELS
+def test_steep_slopes_at_any_place_of_a_step(gpu, kind, dim, slope, ahead, kernel):
+    """Queries behind a cache: their own keys lie anywhere in a step of 32.  The next key weighs e^-40 or less."""
+    lengths = [1, 33, 130, 64]
+    c = Call(gpu, kind, lengths, 4, 2, dim, key_lengths=[n + ahead for n in lengths], bias="slopes", after=0)
+    c.slopes[:] = slope
+    c.describe(kernel=kernel).run()
+    torch().cuda.synchronize()
+    for s, n in enumerate(lengths):
+        got = c.out[c.q0[s]:c.q0[s] + n, :, :dim].double()
+        want = c.kv[c.k0[s] + ahead:c.k0[s] + ahead + n, 2:, :dim].repeat_interleave(2, 1).double()
+        # A score is at most 30 here: e^-10 of a value of at most 6, a hundred of them, where the slope is 40; else nothing.
+        assert ((got - want).abs() <= (0.03 if slope == 40.0 else 0.0)).all()
