@@ -394,7 +394,7 @@ int laya_op_document_bounds(const int32_t* documents, const int32_t* starts, con
  *   out = sum of softmax(t) v over the keys seen.
  * A query that sees no key, or whose scores are all below -1e30 (biases of a type's lowest value hide keys), gets zeros; what lies in
  * hidden keys, NaNs and infinities too, does not matter.  Other entries of a table are at most 1e27
- * in size.  Rows whose largest score passes 2^21 in size go a path some 200 times as slow, one by one.  out's rows of no query are left as they were.  Sequences may share keys, not queries. */
+ * in size.  out's rows of no query are left as they were.  Sequences may share keys, not queries. */
 typedef struct LayaAttend {
   uint32_t struct_bytes;  /* sizeof(LayaAttend) */
   int32_t dtype;          /* LAYA_F16 or LAYA_BF16: q, k, v, out */

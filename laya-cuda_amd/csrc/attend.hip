@@ -167,8 +167,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
       if (!whole) rows.hide(t, key);
       if (fresh) rows.open(a, t, shift);
       fresh = false;
-      const float sum = rows.weights(a, t, p, shift);
-      rows.total += rows.move(a, t, p, shift, sum);
+      rows.total += rows.weigh_step(a, t, p, shift);
       rows.weigh((LdsBytes)(skv[2]), buffer + SB * h * P * 2u, p);
     }
   }
@@ -176,8 +175,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D <= 64
 
   T* out = static_cast<T*>(a.out) + head * a.out_head;
   const unsigned live = static_cast<unsigned>(__builtin_amdgcn_ballot_w64(valid));
-  unsigned bad = rows.doubtful() & live;
   const float total = halves_sum(rows.total);
+  unsigned bad = rows.doubtful(total) & live;
   const float inv = total == 0.f ? 0.f : 1.0f / total;
   if (valid && !(bad >> (lane & 31) & 1)) {
     T* row = out + (sq.q0 + i) * a.out_row;
@@ -321,8 +320,7 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
     const typename R::Shift shift = rows.change(a, t, key, table, 0);
     if (!(key + KB <= sq.prefix || (key >= range.all_lo && key + KB <= range.all_hi))) rows.hide(t, key);
     if (j < j0 + NW) rows.open(a, t, shift);
-    const float sum = rows.weights(a, t, p, shift);
-    rows.total += rows.move(a, t, p, shift, sum);
+    rows.total += rows.weigh_step(a, t, p, shift);
     if (more) __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(CH));  // all but the next block's K
     else __builtin_amdgcn_s_waitcnt(waitcnt_vm_only(0));
     asm volatile("" ::: "memory");
@@ -335,8 +333,8 @@ __global__ __launch_bounds__(64 * split_waves<D>()) __attribute__((amdgpu_waves_
   __syncthreads();  // every wave is done with its stages
   float* so = reinterpret_cast<float*>(lds);
   {
-    const unsigned bad = rows.doubtful();
     const float total = halves_sum(rows.total);
+    const unsigned bad = rows.doubtful(total);
     if (rows.g == 0) {
       s_reference[wave][lane & 31] = rows.reference;
       s_total[wave][lane & 31] = total;

@@ -8,7 +8,9 @@
 //
 // Scores live in log2 units.  A row's reference starts at kNothing and moves to a block's largest score only when the lane's
 // weights pass 2^13 in sum (each is at most that, so fp16 holds it): most blocks need no maximum.  Weights are rounded to 16 bits
-// for the matrix unit, and the normaliser sums the rounded ones.
+// for the matrix unit, and the normaliser sums the rounded ones.  Rows of references beyond 2^22 (biases of -1e9 as masks, where nothing else is
+// seen yet) take another way to their weights, so that they cost the same: 16 x 1,024 tokens of 16 heads of 64 under a table that hides what lies behind each
+// query by -1e9 108 us, by -1e4 118.
 #pragma once
 
 #include "attend.hpp"
@@ -183,6 +185,8 @@ struct Rows {
   T8 q[KS];
   f32x16 o[DT];
   float reference, total;
+  float top;   // what the reference was rounded from: in units of t, capped ones centred
+  bool large;  // of the wave: some row's reference is larger than kLargest
   int lo, hi, prefix, position;
   float slope;  // in units of t
   int lane, g;
@@ -197,6 +201,8 @@ struct Rows {
     v_at = 2u * static_cast<unsigned>(row * B::kPitch + ((chunk ^ B::v_swizzle(row)) << 3) + (l & 1) * 4);
     reference = kNothing;
     total = 0.f;
+    top = 0.f;
+    large = false;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -317,24 +323,37 @@ struct Rows {
     }
   }
 
-  // The largest score: of the largest t, or of the smallest where the cap's unit is negative.
-  __device__ __forceinline__ float block_max(const AttendArgs& a, const f32x16 (&s)[KT], Shift shift) const {
+  // The largest score, in units of t, capped ones centred: of the largest t, or of the smallest where the cap's unit is negative.
+  __device__ __forceinline__ float block_top(const f32x16 (&s)[KT], Shift shift) const {
     float m = kCap ? INFINITY : -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = kCap ? fminf(m, s[kt][r]) : fmaxf(m, s[kt][r]);
-    return halves_max(__builtin_fmaf(m + shift.bias, a.unit, shift.rest));
+    m = m - centre(shift) + shift.bias;
+    return kCap ? -halves_max(-m) : halves_max(m);
   }
+  __device__ __forceinline__ static float centre(Shift shift) { return kCap && shift.rest != 0.f ? 0.5f : 0.f; }
+  __device__ __forceinline__ bool is_large() const { return fabsf(reference) > kLargest && reference > kNothing; }
 
+  // kLarge: rows of large references subtract what those were rounded from, in units of t, which equal scores have in common to the last bit; a
+  // rounded one is off by whole powers of two from 2^24 on, which would take every weight to 0 or past the type.
+  template <bool kLarge>
   __device__ __forceinline__ float weights(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], Shift shift) const {
     float sum[2] = {0.f, 0.f};
-    float base = __builtin_fmaf(shift.bias, a.unit, -reference);
+    float base = __builtin_fmaf(shift.bias, a.unit, -reference), from = 0.f;
     if constexpr (kCap) base += shift.rest;
+    if (kLarge && is_large()) {
+      base = 0.f;
+      from = top - shift.bias + centre(shift);
+    }
 #pragma unroll
     for (int c = 0; c < 2 * KT; ++c) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[c][e] = to_half<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 1][8 * (c & 1) + e], a.unit, base)));
+      for (int e = 0; e < 8; ++e) {
+        const float t = s[c >> 1][8 * (c & 1) + e];
+        p[c][e] = to_half<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(kLarge ? t - from : t, a.unit, base)));
+      }
       sum[0] = pair_sum(__builtin_shufflevector(p[c], p[c], 0, 1), sum[0]);
       sum[1] = pair_sum(__builtin_shufflevector(p[c], p[c], 2, 3), sum[1]);
       sum[0] = pair_sum(__builtin_shufflevector(p[c], p[c], 4, 5), sum[0]);
@@ -345,38 +364,47 @@ struct Rows {
 
   // The first block of a wave: its largest score is the reference, before any weight is made.
   __device__ __forceinline__ void open(const AttendArgs& a, const f32x16 (&s)[KT], Shift shift) {
-    reference = fmaxf(kNothing, block_max(a, s, shift));
+    top = block_top(s, shift);
+    reference = fmaxf(kNothing, top * a.unit);
+    large = __builtin_amdgcn_ballot_w64(is_large()) != 0;
   }
 
-  // Weights that are too large for the reference: it moves to the block's largest score.
-  __device__ __forceinline__ float move(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], Shift shift, float sum) {
+  // A step's weights and their sum.  Where they are too large for the reference, it moves to the step's largest score.
+  __device__ __forceinline__ float weigh_step(const AttendArgs& a, const f32x16 (&s)[KT], T8 (&p)[2 * KT], Shift shift) {
+    float sum = INFINITY;
+    if (!large) sum = weights<false>(a, s, p, shift);
     if (__builtin_amdgcn_ballot_w64(!(sum <= kMostWeight))) {
-      const float m = block_max(a, s, shift);
-      const float to = m > reference + 8.f ? m : reference;
-      const float alpha = to == reference ? 1.f : __builtin_amdgcn_exp2f(reference - to);
-      reference = to;
+      const float t = block_top(s, shift), m = t * a.unit;
+      const bool was_large = is_large();
+      const bool moves = was_large && fabsf(m) > kLargest ? (kCap ? t < top : t > top) : m > reference + 8.f;
+      const float by = was_large ? (top - t) * a.unit : reference - m;
+      const float alpha = moves ? __builtin_amdgcn_exp2f(by) : 1.f;
+      if (moves) {
+        reference = m;
+        top = t;
+      }
+      large = __builtin_amdgcn_ballot_w64(is_large()) != 0;
       total *= alpha;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-      sum = weights(a, s, p, shift);
+      sum = weights<true>(a, s, p, shift);
     }
     return sum;
   }
 
   // Rows (bits 0 to 31) to be done again by themselves: those whose sums are no numbers (a weight of 0 times an infinity or NaN in a
-  // hidden key's value, if nothing the row sees is one), and those whose scores are so large that a reference's own rounding is no longer
-  // small: at 2^30 it is up to 2^5, and weights of e^-22 in the place of 1 round to 0 in fp16.
-  __device__ __forceinline__ unsigned doubtful() const {
+  // hidden key's value, if nothing the row sees is one), and those whose weights are all too small, where biases of more than 2^24 in several steps' shifts
+  // were rounded apart.
+  __device__ __forceinline__ unsigned doubtful(float row_total) const {
     float sum[4] = {total, 0.f, 0.f, 0.f};  // NaN for a NaN or an infinity
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum[r & 3] = __builtin_fmaf(o[d][r], 0.f, sum[r & 3]);
     const float x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    const bool large = fabsf(reference) > kLargest && reference > kNothing;
-    const unsigned long long bad = __builtin_amdgcn_ballot_w64(x != x || large);
+    const unsigned long long bad = __builtin_amdgcn_ballot_w64(x != x || (row_total < 0.5f && reference > kNothing));
     return static_cast<unsigned>(bad | bad >> 32);
   }
 };

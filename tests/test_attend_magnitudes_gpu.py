@@ -118,6 +118,27 @@ def test_slopes_of_the_largest_values(gpu, kind, dim, slope, scale, cap, kernel)
 
 
 @KINDS
+@pytest.mark.parametrize("bias", [-1e6, -1e9, -7.3e9, -1e12])
+@pytest.mark.parametrize("cap", [0.0, 9.0])
+def test_biases_of_long_keys_shared_by_workgroups(gpu, kind, dim, bias, cap):
+    """A mask by bias over all but the nearest keys, and one bias for every key, of contexts that several workgroups share."""
+    for everywhere in (False, True):
+        c = Call(gpu, kind, [1, 3, 40], 4, 2, dim, key_lengths=[9001, 4500, 70], bias="table", span=20, after=0, cap=cap)
+        if everywhere:
+            c.q[..., :dim] = 0
+            c.table[:] = bias
+        else:
+            c.table[:, :9] = bias
+        c.describe(kernel=_lib.ATTEND_FEW).run()
+        assert c.workspace is not None
+        if everywhere:
+            compare(c, np.zeros_like(c.table))
+        else:
+            c.table[:, :9] = -np.inf
+            c.check()
+
+
+@KINDS
 @pytest.mark.parametrize("slope", [40.0, 1e3, 3.3e6, 1e9, 1.7e12, 1e30])
 @pytest.mark.parametrize("ahead", [1, 17, 31, 100])
 @KERNELS
