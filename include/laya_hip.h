@@ -364,9 +364,9 @@ int laya_rotary_frequencies(int kind, double theta, int rotated, double factor, 
 /* out = x with each head's first `rotated` values turned by their row's position: with the angle 2 pi positions[row] turns[i]
  * of pair i, (a, b) -> amplitude (a cos - b sin, a sin + b cos); direction -1 turns back (the gradient of direction 1, and
  * its inverse where amplitude is 1).  Values rotated .. dim - 1 are copied.  dtype LAYA_F32/F16/BF16; positions
- * int32, of either sign; turns as laya_rotary_frequencies makes them.  Angles are exact to 2^-27 of a turn at any position,
- * arithmetic is fp32, and the output rounds once.  out may be x itself with the same strides, else it overlaps nothing; what lies
- * between rows and heads is left as it was.  rotated even, 2 <= rotated <= dim <= 8192, heads * dim <= 2^20, rows <= 2^23,
+ * int32, of either sign; turns as laya_rotary_frequencies makes them.  Angles are exact to 2^-27 of a turn at any position (turns up to
+ * 2^20 in size), arithmetic is fp32, and the output rounds once.  out may be x itself with the same strides, else it overlaps nothing;
+ * what lies between rows and heads is left as it was.  rotated even, 2 <= rotated <= dim <= 8192, heads * dim <= 2^20, rows <= 2^23,
  * strides not negative and below 2^40, over at most 2^50 elements.  Whole 16 bytes of halves, strides and addresses are fastest. */
 int laya_op_rotary(const void* x, int64_t x_row, int64_t x_head, void* out, int64_t out_row, int64_t out_head,
                    int dtype, const int32_t* positions, const double* turns, float amplitude, int layout,
