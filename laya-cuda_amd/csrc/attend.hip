@@ -18,10 +18,10 @@ constexpr int kPad = 96;  // distances past a bias table's span that the scores 
 // running reference and total) and skips those that none of its rows sees.
 //
 // What bounds it: the card's power and the vector instructions beside the matrix ones.  64 x 1,024 tokens of 16 heads of 64 run
-// 350 us (785 TFLOP/s; boxes differ, 316 to 362) at 1.91 of 2.4 GHz with the matrix cores busy 38% of the cycles and vector instructions 58%; with zeros for
+// 350 us (785 TFLOP/s; boxes differ, 316 to 362) at 1.91 of 2.4 GHz with the matrix cores busy 41% of the cycles and vector instructions 62%; with zeros for
 // inputs 280 us.  Copies without the exponentials, the loads or one of the products run 320, 315 and 290 us.  16,384
-// causal tokens of 8 heads of 128: 511 to 545 us, 1.01 to 1.08 PFLOP/s, the matrix cores 44%.
-// Why 32 keys a step in one straight line, with no more than 101 registers for heads of 64: four such workgroups share a CU.  64 keys a
+// causal tokens of 8 heads of 128: 511 to 545 us, 1.01 to 1.08 PFLOP/s, the matrix cores 46%.
+// Why 32 keys a step in one straight line, with 102 to 114 registers for heads of 64: four such workgroups share a CU (up to 128).  64 keys a
 // step took 373 us where this took 361, scores of the next step under the softmax of this one 388 against 352, two row groups a
 // wave (half the LDS reads) 354 against 349 for heads of 64 and 1,535 against 1,069 for 128, three buffers 382 against 344, blocks of 32
 // keys 394 against 350, raised priorities for either phase or by slot nothing.  Tiles of 64 queries, two waves: 488 against 338, documents 314
